@@ -149,6 +149,109 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
                                     const uint32_t* write_index, float scale, void* workspace,
                                     size_t workspace_bytes, void* stream, char* err, size_t errlen);
 
+/* paged_chunk_attention -- paged_decode_attention for more than one new token a
+ * request (the store and the causal flash attention of
+ * unlimited_ocr_max/decoder.py:425-437): a chunk of new tokens of each of
+ * `requests` requests, appended to its cached rows.
+ *   out, q, k_new, v_new fp32 [tokens, heads, head_dim] (post-RoPE), head_dim 128;
+ *   the rows of q, k_new and v_new are row_stride floats apart (a multiple of 4).
+ *   chunk_offsets int32 [requests + 1], ascending: request n's chunk is token rows
+ *   [chunk_offsets[n], chunk_offsets[n+1]), which may be empty; cache_lengths uint32
+ *   [requests]: its rows c_n in the cache before the chunk; lookup uint32
+ *   [requests, lookup_cols] (all device).  kv_blocks as for paged_decode_attention.
+ *   attend_max (host): the largest c_n + chunk length.
+ * Token i of chunk n is logical row c_n + i: its k_new / v_new are stored there, then
+ *   out = sum_{r <= c_n + i} softmax_r(scale * q . k_r) v_r.
+ * Rows of out that no chunk holds are left as they were, as is every row of the
+ * pool that is no new token's.  Device metadata is clamped as there: a row past what
+ * the lookup row addresses is neither stored nor attended, nor is one past attend_max
+ * attended.  Two requests may share pages that no chunk writes.  fp32 throughout.
+ * workspace may be NULL (the library's own) or at least
+ * uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max) bytes, 16-byte
+ * aligned; calls that overlap in time must not share one (nor, with NULL, a stream's
+ * own one across captured graphs).  out must not overlap the inputs. */
+size_t uocr_paged_chunk_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max);
+int uocr_paged_chunk_attention(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
+                               int64_t heads, int64_t head_dim, int64_t row_stride, float* kv_blocks, int64_t pages,
+                               int64_t layers, int64_t page_size, int64_t layer, const uint32_t* lookup,
+                               int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
+                               const int32_t* chunk_offsets, int64_t attend_max, float scale, void* workspace,
+                               size_t workspace_bytes, void* stream, char* err, size_t errlen);
+
+/* paged_chunk_attention_qkv -- Attention._rope of q and k
+ * (unlimited_ocr_max/decoder.py:459-462) and paged_chunk_attention in one call: q / k_new / v_new are the
+ * thirds of one fused projection's output, qkv [tokens, 3, heads, head_dim] with rows
+ * row_stride floats apart, q and k_new before RoPE; the stored k rows have the
+ * bits of uocr_rope.  positions int32 [tokens] (clamped into the tables), cos_table /
+ * sin_table fp32 [table_rows, head_dim]. */
+int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens, int64_t heads, int64_t head_dim,
+                                   int64_t row_stride, const int32_t* positions, const float* cos_table,
+                                   const float* sin_table, int64_t table_rows, int64_t table_dim, float* kv_blocks,
+                                   int64_t pages, int64_t layers, int64_t page_size, int64_t layer,
+                                   const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                                   const uint32_t* cache_lengths, const int32_t* chunk_offsets, int64_t attend_max,
+                                   float scale, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                                   size_t errlen);
+
+/* ---------------------------------------------------------------------------
+ * The pages of the pool (the page lists of KvPagePool, unlimited_ocr_max/
+ * kv_cache.py:210-335, which the reference keeps on the host), on the device, so
+ * that a serving loop moves requests without waiting for it.
+ *   kv_blocks fp32 [pages, 2, layers, page_size, heads, head_dim], heads * head_dim a
+ *   multiple of 4; the last page is the null page, which is nobody's.
+ *   lookup uint32 [requests, lookup_cols]: entry c is the page of logical rows
+ *   [c P, c P + P); an entry that is not below pages - 1 is unset, and unset entries are
+ *   written as pages - 1.  ref_counts int32 [pages]: how many entries name the page;
+ *   a page with a count <= 0 is free.  The table outputs may be their inputs (in
+ *   place) and must not overlap them otherwise.  Each result is the same whatever the
+ *   timing: pages are taken from the lowest free one up, in (row, column) order.
+ *   missing int32 [1]: the entries that found no free page (they stay unset).
+ *   A workspace is NULL (the library's own) or of the size asked for, 16-byte aligned;
+ *   calls that overlap in time must not share one.
+ * ------------------------------------------------------------------------- */
+
+/* copy_pages -- page dst[i] = page src[i], k and v of all layers, i < count, as if one
+ * after the other (a page may be in both lists, and more than once); with rows
+ * (int32 [count], may be NULL), the first rows[i] rows of each layer only.  A pair
+ * with an id outside [0, pages) is skipped.  All lists on the device. */
+int uocr_copy_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
+                    int64_t head_dim, const int32_t* src, const int32_t* dst, const int32_t* rows, int64_t count,
+                    void* stream, char* err, size_t errlen);
+
+/* fork_pages -- child row children[i] becomes a continuation of parent row parents[i],
+ * i < count, all of them as the tables were before the call.  Of the parent's pages that
+ * hold its rows [0, lengths[i]), those wholly below shared_rows[i] are shared (their
+ * counts rise), the others are copied, the rows below the length only, to pages that were free before the
+ * call; the child's other entries are unset and its old pages released.  A pair whose child is its parent
+ * leaves the row as it is; one with a row outside [0, requests) is skipped; of several pairs with one child the
+ * last counts. */
+size_t uocr_fork_pages_workspace_bytes(int64_t pages, int64_t requests, int64_t lookup_cols, int64_t count);
+int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
+                    int64_t head_dim, int32_t* ref_counts_out, const int32_t* ref_counts, uint32_t* lookup_out,
+                    const uint32_t* lookup, int64_t requests, int64_t lookup_cols, const int32_t* parents,
+                    const int32_t* children, const int32_t* lengths, const int32_t* shared_rows, int64_t count,
+                    int32_t* missing, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                    size_t errlen);
+
+/* resize_pages -- every row gets the pages of lengths[n] logical rows (int32
+ * [requests]; 0: none): entries past them are released, then unset ones below
+ * are taken, the pages just released among the free ones. */
+size_t uocr_resize_pages_workspace_bytes(int64_t pages);
+int uocr_resize_pages(int32_t* ref_counts_out, const int32_t* ref_counts, int64_t pages, int64_t page_size,
+                      uint32_t* lookup_out, const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                      const int32_t* lengths, int32_t* missing, void* workspace, size_t workspace_bytes, void* stream,
+                      char* err, size_t errlen);
+
+/* compact_pages -- the L pages in use become pages [0, L): those at or past L move, in
+ * ascending order, to the free ones below L in ascending order; counts and lookup
+ * entries follow.  remap int32 [pages]: where each page is now (-1: it was free).  An
+ * entry that names a free page is unset. */
+size_t uocr_compact_pages_workspace_bytes(int64_t pages);
+int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
+                       int64_t head_dim, int32_t* ref_counts_out, const int32_t* ref_counts, uint32_t* lookup_out,
+                       const uint32_t* lookup, int64_t requests, int64_t lookup_cols, int32_t* remap, void* workspace,
+                       size_t workspace_bytes, void* stream, char* err, size_t errlen);
+
 /* rms_norm -- replaces RmsNorm.__call__ (unlimited_ocr_max/decoder.py:252-261,
  * ops.rms_norm with gamma cast to fp32) and, given `residual`, the residual add
  * before it (DecoderLayer.decode, decoder.py:702-709).

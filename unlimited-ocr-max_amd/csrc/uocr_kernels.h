@@ -267,6 +267,59 @@ struct PagedAttention {
 size_t attn_workspace_bytes(int64_t rows, int heads, int max_attend);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s);
 
+// ---- attention of a chunk of new tokens over the page pool (chunk.hip) ----
+
+struct ChunkAttention {
+  float* out;            // [tokens, heads, D]
+  const float* q;        // rows in_stride floats apart
+  const float* k_new;
+  const float* v_new;
+  float* kv_blocks;      // [pages, 2, layers, page_size, heads, D]
+  int pages, layers, page_size, heads, head_dim, layer;
+  const uint32_t* lookup;         // [requests, lookup_cols]
+  int lookup_cols;
+  const uint32_t* cache_lengths;  // [requests]: rows before the chunk
+  const int32_t* chunk_offsets;   // [requests + 1]: the token rows of each chunk
+  int64_t tokens, requests;
+  int attend_max;                 // the most rows a token attends (host)
+  float scale;
+  void* workspace;                // chunk_workspace_bytes(tokens, requests, heads, attend_max)
+  int64_t in_stride;
+  const int32_t* positions;       // null: q, k_new come rotated; else rotated here at these positions
+  const float* cos_table;         // [table_rows, head_dim]
+  const float* sin_table;
+  int table_rows;
+};
+size_t chunk_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max);
+hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s);
+
+// ---- the pages of the pool (pages.hip) ----
+
+struct PagePool {
+  float* kv_blocks;  // [pages, 2, layers, page_size, slot floats], or null where no page moves
+  int pages, layers, page_size;
+  int slot;          // floats per slot: heads * head_dim, a multiple of 4
+};
+struct PageTables {
+  const int32_t* counts;    // [pages]
+  int32_t* counts_out;      // may be counts
+  const uint32_t* lookup;   // [requests, cols]
+  uint32_t* lookup_out;     // may be lookup
+  int requests, cols;
+};
+hipError_t launch_copy_pages(const PagePool& p, const int32_t* src, const int32_t* dst, const int32_t* rows,
+                             int count, hipStream_t s);
+size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count);
+hipError_t launch_fork_pages(const PagePool& p, const PageTables& t, const int32_t* parents, const int32_t* children,
+                             const int32_t* lengths, const int32_t* shared_rows, int count, int32_t* missing,
+                             void* workspace, hipStream_t s);
+size_t resize_workspace_bytes(int64_t pages);
+hipError_t launch_resize_pages(const PagePool& p, const PageTables& t, const int32_t* lengths, int32_t* missing,
+                               void* workspace, hipStream_t s);
+size_t compact_workspace_bytes(int64_t pages);
+hipError_t launch_compact_pages(const PagePool& p, const PageTables& t, int32_t* remap, void* workspace,
+                                hipStream_t s);
+
 // ---- the persistent decode layer (decode.hip) ----
 
 constexpr int kFusedWaves = 12;  // waves per workgroup, one workgroup per CU (168 VGPRs a lane)

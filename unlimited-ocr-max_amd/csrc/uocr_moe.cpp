@@ -775,6 +775,280 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
                               errlen);
 }
 
+// ------------------------------------------------------------------ paged chunk attention
+
+// Whether [a, a + an) and [b, b + bn) (bytes) share a byte.
+static bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + bn && y < x + an;
+}
+
+// own_workspace allocates host memory too: nothing is thrown through the C entries.
+static int chunk_workspace(const char* op, void* workspace, size_t workspace_bytes, size_t need, hipStream_t stream,
+                           void** out, char* err, size_t errlen) {
+  *out = nullptr;
+  if (!aligned16(workspace)) return fail(err, errlen, "%s: workspace must be 16-byte aligned", op);
+  if (need == 0) return 0;
+  try {
+    return resolve_workspace(op, workspace, workspace_bytes, need, stream, out, err, errlen);
+  } catch (...) {
+    return fail(err, errlen, "%s: out of host memory", op);
+  }
+}
+
+size_t uocr_paged_chunk_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max) {
+  if (tokens < 0 || tokens > INT32_MAX || requests < 0 || requests > INT32_MAX || heads < 1 || heads > 65535 ||
+      attend_max < 1 || attend_max > INT32_MAX)
+    return 0;
+  return chunk_workspace_bytes(tokens, requests, (int)heads, (int)attend_max);
+}
+
+// The checks and launch of both chunk attention entries.
+static int paged_chunk_call(const char* op, float* out, const float* q, const float* k_new, const float* v_new,
+                            int64_t in_stride, const int32_t* positions, const float* cos_table,
+                            const float* sin_table, int64_t table_rows, int64_t tokens, int64_t heads,
+                            int64_t head_dim, float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size,
+                            int64_t layer, const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                            const uint32_t* cache_lengths, const int32_t* chunk_offsets, int64_t attend_max,
+                            float scale, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                            size_t errlen) {
+  if (head_dim != 128) return fail(err, errlen, "%s: head_dim must be 128, got %lld", op, (long long)head_dim);
+  if (page_size < kAttnSplitRows || page_size % kAttnSplitRows || page_size > INT32_MAX)
+    return fail(err, errlen, "%s: page_size must be a positive multiple of %d", op, kAttnSplitRows);
+  if (pages < 1 || layers < 1 || layers > INT32_MAX || layer < 0 || layer >= layers)
+    return fail(err, errlen, "%s: layer %lld is not in the pool's %lld layers", op, (long long)layer,
+                (long long)layers);
+  if (pages > INT32_MAX) return fail(err, errlen, "%s: more than 2^31 pages", op);
+  if (heads < 1 || heads > 65535) return fail(err, errlen, "%s: heads must be in [1, 65535]", op);
+  if (tokens < 0 || requests < 0 || requests > 65535 || tokens > (1 << 25) / heads)
+    return fail(err, errlen, "%s: requests must be in [0, 65535] and tokens * heads in [0, 2^25]", op);
+  if (lookup_cols < 1 || lookup_cols > INT32_MAX / page_size)
+    return fail(err, errlen, "%s: bad lookup table width %lld", op, (long long)lookup_cols);
+  if (attend_max < 1 || attend_max > lookup_cols * page_size)
+    return fail(err, errlen, "%s: attend_max %lld is not in [1, %lld], the rows the lookup table addresses", op,
+                (long long)attend_max, (long long)(lookup_cols * page_size));
+  if (in_stride < heads * head_dim)
+    return fail(err, errlen, "%s: input rows %lld floats apart overlap rows of %lld", op, (long long)in_stride,
+                (long long)(heads * head_dim));
+  if (tokens == 0 || requests == 0) return 0;
+  if (!out || !q || !k_new || !v_new || !kv_blocks || !lookup || !cache_lengths || !chunk_offsets)
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  if (!aligned16(out) || !aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(kv_blocks) ||
+      in_stride % 4)
+    return fail(err, errlen, "%s: q, k_new, v_new, out and kv_blocks must be 16-byte aligned", op);
+  const size_t row = (size_t)(heads * head_dim) * sizeof(float);
+  const size_t in_bytes = (size_t)(tokens - 1) * in_stride * sizeof(float) + row;
+  for (const float* in : {q, k_new, v_new})
+    if (overlap(out, (size_t)tokens * row, in, in_bytes))
+      return fail(err, errlen, "%s: out must not overlap the inputs", op);
+  const hipStream_t s = (hipStream_t)stream;
+  void* ws = nullptr;
+  if (chunk_workspace(op, workspace, workspace_bytes,
+                      chunk_workspace_bytes(tokens, requests, (int)heads, (int)attend_max), s, &ws, err, errlen))
+    return 1;
+  ChunkAttention p{};
+  p.out = out;
+  p.q = q;
+  p.k_new = k_new;
+  p.v_new = v_new;
+  p.kv_blocks = kv_blocks;
+  p.pages = (int)pages;
+  p.layers = (int)layers;
+  p.page_size = (int)page_size;
+  p.heads = (int)heads;
+  p.head_dim = (int)head_dim;
+  p.layer = (int)layer;
+  p.lookup = lookup;
+  p.lookup_cols = (int)lookup_cols;
+  p.cache_lengths = cache_lengths;
+  p.chunk_offsets = chunk_offsets;
+  p.tokens = tokens;
+  p.requests = requests;
+  p.attend_max = (int)attend_max;
+  p.scale = scale;
+  p.workspace = ws;
+  p.in_stride = in_stride;
+  p.positions = positions;
+  p.cos_table = cos_table;
+  p.sin_table = sin_table;
+  p.table_rows = (int)table_rows;
+  const hipError_t e = launch_chunk_attention(p, s);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+int uocr_paged_chunk_attention(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
+                               int64_t heads, int64_t head_dim, int64_t row_stride, float* kv_blocks, int64_t pages,
+                               int64_t layers, int64_t page_size, int64_t layer, const uint32_t* lookup,
+                               int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
+                               const int32_t* chunk_offsets, int64_t attend_max, float scale, void* workspace,
+                               size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  return paged_chunk_call("paged_chunk_attention", out, q, k_new, v_new, row_stride, nullptr, nullptr, nullptr, 0,
+                          tokens, heads, head_dim, kv_blocks, pages, layers, page_size, layer, lookup, requests,
+                          lookup_cols, cache_lengths, chunk_offsets, attend_max, scale, workspace, workspace_bytes,
+                          stream, err, errlen);
+}
+
+int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens, int64_t heads, int64_t head_dim,
+                                   int64_t row_stride, const int32_t* positions, const float* cos_table,
+                                   const float* sin_table, int64_t table_rows, int64_t table_dim, float* kv_blocks,
+                                   int64_t pages, int64_t layers, int64_t page_size, int64_t layer,
+                                   const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                                   const uint32_t* cache_lengths, const int32_t* chunk_offsets, int64_t attend_max,
+                                   float scale, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                                   size_t errlen) {
+  const char* op = "paged_chunk_attention_qkv";
+  if (table_dim != head_dim)
+    return fail(err, errlen, "%s: the cos/sin tables are %lld wide, not head_dim %lld", op, (long long)table_dim,
+                (long long)head_dim);
+  if (table_rows < 1 || table_rows > INT32_MAX) return fail(err, errlen, "%s: bad cos/sin table", op);
+  if (heads < 1 || heads > 65535) return fail(err, errlen, "%s: heads must be in [1, 65535]", op);
+  if (row_stride < 3 * heads * head_dim)
+    return fail(err, errlen, "%s: qkv rows %lld floats apart overlap rows of %lld", op, (long long)row_stride,
+                (long long)(3 * heads * head_dim));
+  if (tokens > 0 && requests > 0 && (!qkv || !positions || !cos_table || !sin_table))
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  const float* k = qkv ? qkv + heads * head_dim : nullptr;
+  const float* v = qkv ? qkv + 2 * heads * head_dim : nullptr;
+  return paged_chunk_call(op, out, qkv, k, v, row_stride, positions, cos_table, sin_table, table_rows, tokens, heads,
+                          head_dim, kv_blocks, pages, layers, page_size, layer, lookup, requests, lookup_cols,
+                          cache_lengths, chunk_offsets, attend_max, scale, workspace, workspace_bytes, stream, err,
+                          errlen);
+}
+
+// ------------------------------------------------------------------ the pages of the pool
+
+static int page_pool(const char* op, PagePool& p, float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size,
+                     int64_t heads, int64_t head_dim, char* err, size_t errlen) {
+  if (pages < 1 || pages > INT32_MAX || layers < 1 || layers > INT32_MAX / 2 || page_size < 1 ||
+      page_size > INT32_MAX || heads < 1 || head_dim < 1 || heads > INT32_MAX / head_dim ||
+      layers * 2 * page_size > INT64_MAX / 16 / (heads * head_dim) / pages)
+    return fail(err, errlen, "%s: bad pool [%lld, 2, %lld, %lld, %lld, %lld]", op, (long long)pages,
+                (long long)layers, (long long)page_size, (long long)heads, (long long)head_dim);
+  if (heads * head_dim % 4) return fail(err, errlen, "%s: heads * head_dim must be a multiple of 4", op);
+  if (!aligned16(kv_blocks)) return fail(err, errlen, "%s: kv_blocks must be 16-byte aligned", op);
+  p.kv_blocks = kv_blocks;
+  p.pages = (int)pages;
+  p.layers = (int)layers;
+  p.page_size = (int)page_size;
+  p.slot = (int)(heads * head_dim);
+  return 0;
+}
+
+static int page_tables(const char* op, PageTables& t, int32_t* counts_out, const int32_t* counts, int64_t pages,
+                       uint32_t* lookup_out, const uint32_t* lookup, int64_t requests, int64_t cols, char* err,
+                       size_t errlen) {
+  if (requests < 0 || cols < 1 || cols > INT32_MAX || requests > INT32_MAX / cols)
+    return fail(err, errlen, "%s: bad lookup table [%lld, %lld]", op, (long long)requests, (long long)cols);
+  if (!counts_out || !counts || (requests > 0 && (!lookup_out || !lookup)))
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  const size_t cb = (size_t)pages * 4, lb = (size_t)(requests * cols) * 4;
+  if ((counts_out != counts && overlap(counts_out, cb, counts, cb)) ||
+      (lookup_out != lookup && overlap(lookup_out, lb, lookup, lb)) || overlap(counts_out, cb, lookup_out, lb) ||
+      overlap(counts_out, cb, lookup, lb) || overlap(lookup_out, lb, counts, cb))
+    return fail(err, errlen, "%s: an output must be its input or not overlap an input", op);
+  t.counts = counts;
+  t.counts_out = counts_out;
+  t.lookup = lookup;
+  t.lookup_out = lookup_out;
+  t.requests = (int)requests;
+  t.cols = (int)cols;
+  return 0;
+}
+
+int uocr_copy_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
+                    int64_t head_dim, const int32_t* src, const int32_t* dst, const int32_t* rows, int64_t count,
+                    void* stream, char* err, size_t errlen) {
+  const char* op = "copy_pages";
+  PagePool p{};
+  if (page_pool(op, p, kv_blocks, pages, layers, page_size, heads, head_dim, err, errlen)) return 1;
+  if (count < 0 || count > INT32_MAX) return fail(err, errlen, "%s: bad number of pairs %lld", op, (long long)count);
+  if (count == 0) return 0;
+  if (!kv_blocks || !src || !dst) return fail(err, errlen, "%s: a tensor is missing", op);
+  const hipError_t e = launch_copy_pages(p, src, dst, rows, (int)count, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+size_t uocr_fork_pages_workspace_bytes(int64_t pages, int64_t requests, int64_t lookup_cols, int64_t count) {
+  if (pages < 1 || pages > INT32_MAX || requests < 0 || requests > INT32_MAX || count < 0 || lookup_cols < 1 ||
+      lookup_cols > INT32_MAX || count > INT32_MAX / lookup_cols)
+    return 0;
+  return fork_workspace_bytes(pages, requests, lookup_cols, count);
+}
+
+int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
+                    int64_t head_dim, int32_t* ref_counts_out, const int32_t* ref_counts, uint32_t* lookup_out,
+                    const uint32_t* lookup, int64_t requests, int64_t lookup_cols, const int32_t* parents,
+                    const int32_t* children, const int32_t* lengths, const int32_t* shared_rows, int64_t count,
+                    int32_t* missing, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                    size_t errlen) {
+  const char* op = "fork_pages";
+  PagePool p{};
+  PageTables t{};
+  if (page_pool(op, p, kv_blocks, pages, layers, page_size, heads, head_dim, err, errlen) ||
+      page_tables(op, t, ref_counts_out, ref_counts, pages, lookup_out, lookup, requests, lookup_cols, err, errlen))
+    return 1;
+  if (count < 0 || count > INT32_MAX / lookup_cols)
+    return fail(err, errlen, "%s: bad number of pairs %lld", op, (long long)count);
+  if (!kv_blocks || !missing || (count > 0 && (!parents || !children || !lengths || !shared_rows)))
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  void* ws = nullptr;
+  if (chunk_workspace(op, workspace, workspace_bytes, fork_workspace_bytes(pages, requests, lookup_cols, count),
+                      (hipStream_t)stream, &ws, err, errlen))
+    return 1;
+  const hipError_t e = launch_fork_pages(p, t, parents, children, lengths, shared_rows, (int)count, missing, ws,
+                                         (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+size_t uocr_resize_pages_workspace_bytes(int64_t pages) {
+  return pages < 1 || pages > INT32_MAX ? 0 : resize_workspace_bytes(pages);
+}
+
+int uocr_resize_pages(int32_t* ref_counts_out, const int32_t* ref_counts, int64_t pages, int64_t page_size,
+                      uint32_t* lookup_out, const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                      const int32_t* lengths, int32_t* missing, void* workspace, size_t workspace_bytes, void* stream,
+                      char* err, size_t errlen) {
+  const char* op = "resize_pages";
+  if (pages < 1 || pages > INT32_MAX || page_size < 1 || page_size > INT32_MAX)
+    return fail(err, errlen, "%s: bad pool of %lld pages of %lld rows", op, (long long)pages, (long long)page_size);
+  PagePool p{};
+  p.pages = (int)pages;
+  p.page_size = (int)page_size;
+  PageTables t{};
+  if (page_tables(op, t, ref_counts_out, ref_counts, pages, lookup_out, lookup, requests, lookup_cols, err, errlen))
+    return 1;
+  if (!missing || (requests > 0 && !lengths)) return fail(err, errlen, "%s: a tensor is missing", op);
+  void* ws = nullptr;
+  if (chunk_workspace(op, workspace, workspace_bytes, resize_workspace_bytes(pages), (hipStream_t)stream, &ws, err,
+                      errlen))
+    return 1;
+  const hipError_t e = launch_resize_pages(p, t, lengths, missing, ws, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+size_t uocr_compact_pages_workspace_bytes(int64_t pages) {
+  return pages < 1 || pages > INT32_MAX ? 0 : compact_workspace_bytes(pages);
+}
+
+int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
+                       int64_t head_dim, int32_t* ref_counts_out, const int32_t* ref_counts, uint32_t* lookup_out,
+                       const uint32_t* lookup, int64_t requests, int64_t lookup_cols, int32_t* remap, void* workspace,
+                       size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  const char* op = "compact_pages";
+  PagePool p{};
+  PageTables t{};
+  if (page_pool(op, p, kv_blocks, pages, layers, page_size, heads, head_dim, err, errlen) ||
+      page_tables(op, t, ref_counts_out, ref_counts, pages, lookup_out, lookup, requests, lookup_cols, err, errlen))
+    return 1;
+  if (!kv_blocks || !remap) return fail(err, errlen, "%s: a tensor is missing", op);
+  void* ws = nullptr;
+  if (chunk_workspace(op, workspace, workspace_bytes, compact_workspace_bytes(pages), (hipStream_t)stream, &ws, err,
+                      errlen))
+    return 1;
+  const hipError_t e = launch_compact_pages(p, t, remap, ws, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
 // ------------------------------------------------------------------ the MoE block
 
 static int check_layer(const char* op, const uocr_moe_layer* L, int64_t hidden, char* err, size_t errlen) {

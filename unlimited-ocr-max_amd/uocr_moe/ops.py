@@ -17,7 +17,9 @@ ngram_block            logits f32 [B,V], history i32 [B,W], ngram i32 [1]   f32 
 =====================  ===================================================  ==================
 
 :func:`paged_decode_attention` (decoder.py:425-437) takes its page pool and
-step metadata as a :class:`PagedKv`.
+step metadata as a :class:`PagedKv`, :func:`paged_chunk_attention` (several new
+tokens a request) as a :class:`PagedChunk`; :func:`copy_pages`, :func:`fork_pages`,
+:func:`resize_pages` and :func:`compact_pages` move the pool's pages.
 
 :func:`custom` dispatches by symbol like ``ops.custom(symbol, values=...)``.
 Inputs must be GPU tensors; non-contiguous views are packed first (the
@@ -424,6 +426,258 @@ def paged_decode_attention_qkv(qkv, positions, cos_table, sin_table, *, heads: i
               lookup.shape[1], attend.data_ptr(), int(kv.attend_max), write.data_ptr(), float(scale), ws, ws_bytes,
               _stream(qkv))
     return out
+
+
+@dataclass(frozen=True)
+class PagedChunk:
+    """The page pool and the metadata of a call that appends a chunk of new tokens to each of ``N`` requests.
+
+    ``kv_blocks`` and ``lookup_table`` ``[N, cols]`` as in :class:`PagedKv`; ``cache_lengths`` ``[N]`` (int32 or
+    uint32), each request's rows in the cache before its chunk; ``chunk_offsets`` int32 ``[N + 1]``, ascending:
+    request ``n``'s chunk is token rows ``chunk_offsets[n]`` up to ``chunk_offsets[n + 1]`` (none: an empty
+    chunk); ``attend_max`` the largest sum of the two, a host int.
+    """
+
+    kv_blocks: torch.Tensor
+    lookup_table: torch.Tensor
+    cache_lengths: torch.Tensor
+    chunk_offsets: torch.Tensor
+    attend_max: int
+
+
+def _pool(op: str, blocks) -> torch.Tensor:
+    """A page pool: written in place, so it must be contiguous."""
+    if not isinstance(blocks, torch.Tensor) or blocks.dtype != torch.float32 or blocks.dim() != 6 or \
+            not blocks.is_cuda or not blocks.is_contiguous() or blocks.shape[1] != 2:
+        raise ValueError(f"{op}: kv_blocks must be a contiguous f32 [pages, 2, layers, page_size, heads, head_dim] "
+                         "GPU tensor (it is written in place)")
+    return blocks
+
+
+def _workspace(op: str, t: torch.Tensor | None, nbytes: int, like: torch.Tensor) -> torch.Tensor | None:
+    """The caller's workspace, or one from torch's allocator (stream-ordered; a captured graph's own)."""
+    if t is None:
+        return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{op}: workspace must be a contiguous GPU tensor")
+    return t
+
+
+def _nbytes(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _on_device(op: str, name: str, *args, tensors) -> None:
+    """Calls entry ``name`` with ``args`` and the current stream of the tensors' device, made current for the
+    launch; tensors of several devices are refused."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{op}: the tensors are on different devices")
+    if dev == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _chunk_call(op: str, name: str, inputs: tuple, tokens: int, heads: int, head_dim: int, kv: PagedChunk,
+                layer_idx: int, scale: float, out, workspace, like: torch.Tensor, tensors: list) -> torch.Tensor:
+    blocks = _pool(op, kv.kv_blocks)
+    pages, _, layers, page_size, bh, bd = blocks.shape
+    if (bh, bd) != (heads, head_dim):
+        raise ValueError(f"{op}: kv_blocks {tuple(blocks.shape)} does not hold {heads} heads of {head_dim}")
+    lookup = _u32(op, "lookup_table", kv.lookup_table, 2)
+    cached = _u32(op, "cache_lengths", kv.cache_lengths, 1)
+    offsets = _gpu(op, "chunk_offsets", kv.chunk_offsets, torch.int32, 1)
+    requests = lookup.shape[0]
+    if cached.shape[0] != requests or offsets.shape[0] != requests + 1:
+        raise ValueError(f"{op}: the chunks' metadata is not for {requests} requests")
+    if out is None:
+        out = like.new_empty((tokens, heads, head_dim))
+    out = _out(op, "out", out, torch.float32, 3)
+    if tuple(out.shape) != (tokens, heads, head_dim):
+        raise ValueError(f"{op}: out must be {(tokens, heads, head_dim)}, got {tuple(out.shape)}")
+    attend_max = int(kv.attend_max)
+    ws = _workspace(op, workspace, _lib.load().uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max),
+                    like)
+    _on_device(op, name, out.data_ptr(), *inputs, blocks.data_ptr(), pages, layers, page_size, int(layer_idx),
+               lookup.data_ptr(), requests, lookup.shape[1], cached.data_ptr(), offsets.data_ptr(), attend_max,
+               float(scale), _ptr(ws), _nbytes(ws), tensors=[*tensors, out, blocks, lookup, cached, offsets, ws])
+    return out
+
+
+def paged_chunk_attention(q, k_new, v_new, *, kv: PagedChunk, layer_idx: int, scale: float,
+                          out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_decode_attention` for a chunk of new tokens of each request (a prompt, a piece of one, the
+    tokens of a draft): stores the chunk's k/v after the request's cached rows, then attends each token over
+    the request's rows up to its own (unlimited_ocr_max/decoder.py:425-437).
+
+    ``q`` / ``k_new`` / ``v_new`` are post-RoPE f32 ``[tokens, heads, head_dim]``, the requests' chunks one after
+    the other (rows may be strided); returns ``[tokens, heads, head_dim]``.  Rows that no chunk holds are not
+    written: those of ``out`` keep what they held, those of a new result are not set.  ``kv.kv_blocks`` is
+    written in place.
+    """
+    op = "paged_chunk_attention"
+    q = _rows_view(op, "q", q)
+    # rows of one stride: views of unlike ones are packed
+    views = [_rows_view(op, name, t) for name, t in (("k_new", k_new), ("v_new", v_new))]
+    if any(t.shape != q.shape for t in views):
+        raise ValueError(f"{op}: q, k_new and v_new disagree on shape: {tuple(q.shape)}, {tuple(views[0].shape)}, "
+                         f"{tuple(views[1].shape)}")
+    tokens, heads, head_dim = q.shape
+    stride = q.stride(0)
+    if any(t.stride(0) != stride or t.data_ptr() % 16 for t in (q, *views)) or stride % 4 or stride < heads * head_dim:
+        q, views = _packed(q), [_packed(t) for t in views]
+        stride = heads * head_dim
+    k, v = views
+    return _chunk_call(op, "uocr_paged_chunk_attention", (q.data_ptr(), k.data_ptr(), v.data_ptr(), tokens, heads,
+                                                          head_dim, stride),
+                       tokens, heads, head_dim, kv, layer_idx, scale, out, workspace, q, [q, k, v])
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """A packed copy at a 16-byte boundary (``t`` itself if it is one)."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def paged_chunk_attention_qkv(qkv, positions, cos_table, sin_table, *, heads: int, kv: PagedChunk, layer_idx: int,
+                              scale: float, out: torch.Tensor | None = None,
+                              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`rope` of q and k followed by :func:`paged_chunk_attention`: ``qkv [tokens, 3 * heads * head_dim]``
+    (q, k, v side by side, q and k before RoPE; rows may be strided) is one fused projection's output,
+    ``positions`` int32 ``[tokens]`` (unlimited_ocr_max/decoder.py:459-462 with :425-437).  The stored k rows
+    have the bits of :func:`rope`."""
+    op = "paged_chunk_attention_qkv"
+    if not isinstance(qkv, torch.Tensor) or qkv.dtype != torch.float32 or qkv.dim() != 2 or not qkv.is_cuda:
+        raise ValueError(f"{op}: qkv must be an fp32 [tokens, 3 * heads * head_dim] GPU tensor")
+    tokens, width = qkv.shape
+    if heads < 1 or width % (3 * heads):
+        raise ValueError(f"{op}: qkv width {width} is not 3 x {heads} heads")
+    if qkv.stride(1) != 1 or qkv.stride(0) < width or qkv.stride(0) % 4 or qkv.data_ptr() % 16:
+        qkv = _packed(qkv)
+    head_dim = width // (3 * heads)
+    positions = _gpu(op, "positions", positions, torch.int32, 1)
+    cos_table = _gpu(op, "cos_table", cos_table, torch.float32, 2)
+    sin_table = _gpu(op, "sin_table", sin_table, torch.float32, 2)
+    if positions.shape[0] != tokens or cos_table.shape != sin_table.shape:
+        raise ValueError(f"{op}: positions or the cos/sin tables do not fit {tokens} tokens")
+    return _chunk_call(op, "uocr_paged_chunk_attention_qkv",
+                       (qkv.data_ptr(), tokens, heads, head_dim, max(qkv.stride(0), width), positions.data_ptr(),
+                        cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0], cos_table.shape[1]),
+                       tokens, heads, head_dim, kv, layer_idx, scale, out, workspace, qkv,
+                       [qkv, positions, cos_table, sin_table])
+
+
+def copy_pages(kv_blocks, src, dst, *, rows=None) -> torch.Tensor:
+    """Page ``dst[i]`` of the pool = page ``src[i]``, k and v of all layers, as if one pair after the other: a page
+    may be in both lists, and more than once.  ``src``, ``dst`` int32 ``[n]`` on the GPU; with ``rows`` (int32
+    ``[n]``) only each layer's first ``rows[i]`` rows.  Pairs with an id outside the pool are skipped.
+    Returns ``kv_blocks``, written in place."""
+    op = "copy_pages"
+    blocks = _pool(op, kv_blocks)
+    src = _gpu(op, "src", src, torch.int32, 1)
+    dst = _gpu(op, "dst", dst, torch.int32, 1)
+    rows = None if rows is None else _gpu(op, "rows", rows, torch.int32, 1)
+    if dst.shape != src.shape or (rows is not None and rows.shape != src.shape):
+        raise ValueError(f"{op}: src, dst and rows must have one length")
+    pages, _, layers, page_size, heads, head_dim = blocks.shape
+    _on_device(op, "uocr_copy_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim, src.data_ptr(),
+               dst.data_ptr(), _ptr(rows), src.shape[0], tensors=[blocks, src, dst, rows])
+    return blocks
+
+
+def _tables(op: str, ref_counts, lookup_table, out_ref_counts, out_lookup) -> tuple:
+    """The page tables and their outputs: (counts, lookup, counts out, lookup out, the caller's lookup out)."""
+    counts = _gpu(op, "ref_counts", ref_counts, torch.int32, 1)
+    lookup = _u32(op, "lookup_table", lookup_table, 2)
+    out_ref_counts = torch.empty_like(counts) if out_ref_counts is None else \
+        _out(op, "out_ref_counts", out_ref_counts, torch.int32, 1)
+    if out_lookup is None:
+        out_lookup = torch.empty(lookup.shape, dtype=lookup_table.dtype, device=lookup.device)
+    if out_ref_counts.shape != counts.shape or out_lookup.shape != lookup.shape or not out_lookup.is_contiguous():
+        raise ValueError(f"{op}: out_ref_counts and out_lookup must be contiguous and shaped as their inputs")
+    return counts, lookup, out_ref_counts, _u32(op, "out_lookup", out_lookup, 2), out_lookup
+
+
+def fork_pages(kv_blocks, ref_counts, lookup_table, parents, children, lengths, shared_rows, *,
+               out_ref_counts: torch.Tensor | None = None, out_lookup: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Row ``children[i]`` of the lookup table becomes a continuation of row ``parents[i]`` (another sample of one
+    prompt, a beam that follows another), all pairs as the tables were before the call.
+
+    Of the parent's pages that hold its rows ``[0, lengths[i])`` those wholly below ``shared_rows[i]`` are
+    shared, the others copied (their rows below the length) to pages that were free before the call; the
+    child's old pages are released.  Rows that either will write again, such as a ring's, must lie at or past
+    ``shared_rows``.  A pair of one row with itself leaves it as it is; of several pairs with one child the last
+    counts; pairs with a row outside the table are skipped.  ``ref_counts`` int32 ``[pages]`` counts the entries
+    that name each page (0: free; the last page, the null page, is never taken); the lists are int32 ``[n]`` on
+    the GPU.  Returns ``(lookup_table, ref_counts, missing)``: new tables (``out_*`` may be the inputs), and int32
+    ``[1]`` the number of entries that found no free page and stay unset.  ``kv_blocks`` is written in place, in
+    free pages only."""
+    op = "fork_pages"
+    blocks = _pool(op, kv_blocks)
+    pages, _, layers, page_size, heads, head_dim = blocks.shape
+    counts, lookup, new_counts, new_lookup, result = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
+    if counts.shape[0] != pages:
+        raise ValueError(f"{op}: ref_counts is for {counts.shape[0]} pages, the pool has {pages}")
+    lists = [_gpu(op, name, t, torch.int32, 1) for name, t in
+             (("parents", parents), ("children", children), ("lengths", lengths), ("shared_rows", shared_rows))]
+    n = lists[0].shape[0]
+    if any(t.shape[0] != n for t in lists):
+        raise ValueError(f"{op}: parents, children, lengths and shared_rows must have one length")
+    requests, cols = lookup.shape
+    ws = _workspace(op, workspace, _lib.load().uocr_fork_pages_workspace_bytes(pages, requests, cols, n), blocks)
+    missing = torch.empty(1, dtype=torch.int32, device=blocks.device)
+    _on_device(op, "uocr_fork_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim,
+               new_counts.data_ptr(), counts.data_ptr(), new_lookup.data_ptr(), lookup.data_ptr(), requests, cols,
+               *(t.data_ptr() for t in lists), n, missing.data_ptr(), _ptr(ws), _nbytes(ws),
+               tensors=[blocks, counts, lookup, new_counts, new_lookup, *lists, ws])
+    return result, new_counts, missing
+
+
+def resize_pages(ref_counts, lookup_table, lengths, *, page_size: int, out_ref_counts: torch.Tensor | None = None,
+                 out_lookup: torch.Tensor | None = None, workspace: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gives every request the pages of ``lengths[n]`` rows (int32 ``[N]`` on the GPU; 0 ends it): entries past them
+    are released, then unset ones below are taken from the lowest free page up, in (request, column) order, the
+    pages just released among the free ones.  Tables and result as for :func:`fork_pages`; no page's rows move."""
+    op = "resize_pages"
+    counts, lookup, new_counts, new_lookup, result = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
+    lengths = _gpu(op, "lengths", lengths, torch.int32, 1)
+    requests, cols = lookup.shape
+    if lengths.shape[0] != requests:
+        raise ValueError(f"{op}: {lengths.shape[0]} lengths for {requests} requests")
+    pages = counts.shape[0]
+    ws = _workspace(op, workspace, _lib.load().uocr_resize_pages_workspace_bytes(pages), counts)
+    missing = torch.empty(1, dtype=torch.int32, device=counts.device)
+    _on_device(op, "uocr_resize_pages", new_counts.data_ptr(), counts.data_ptr(), pages, int(page_size),
+               new_lookup.data_ptr(), lookup.data_ptr(), requests, cols, lengths.data_ptr(), missing.data_ptr(),
+               _ptr(ws), _nbytes(ws), tensors=[counts, lookup, new_counts, new_lookup, lengths, ws])
+    return result, new_counts, missing
+
+
+def compact_pages(kv_blocks, ref_counts, lookup_table, *, out_ref_counts: torch.Tensor | None = None,
+                  out_lookup: torch.Tensor | None = None, workspace: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moves the ``L`` pages in use to the front of the pool: those at or past ``L`` go, in ascending order, to the
+    free ones below ``L`` in ascending order (the fewest copies).  Returns ``(lookup_table, ref_counts, remap)``:
+    the tables as for :func:`fork_pages`, and int32 ``[pages]`` where each page is now (-1: it was free).
+    ``kv_blocks`` is written in place, in free pages only."""
+    op = "compact_pages"
+    blocks = _pool(op, kv_blocks)
+    pages, _, layers, page_size, heads, head_dim = blocks.shape
+    counts, lookup, new_counts, new_lookup, result = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
+    if counts.shape[0] != pages:
+        raise ValueError(f"{op}: ref_counts is for {counts.shape[0]} pages, the pool has {pages}")
+    requests, cols = lookup.shape
+    ws = _workspace(op, workspace, _lib.load().uocr_compact_pages_workspace_bytes(pages), blocks)
+    remap = torch.empty(pages, dtype=torch.int32, device=blocks.device)
+    _on_device(op, "uocr_compact_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim,
+               new_counts.data_ptr(), counts.data_ptr(), new_lookup.data_ptr(), lookup.data_ptr(), requests, cols,
+               remap.data_ptr(), _ptr(ws), _nbytes(ws),
+               tensors=[blocks, counts, lookup, new_counts, new_lookup, ws])
+    return result, new_counts, remap
 
 
 _OPS = {
