@@ -154,7 +154,8 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
  * unlimited_ocr_max/decoder.py:425-437): a chunk of new tokens of each of
  * `requests` requests, appended to its cached rows.
  *   out, q, k_new, v_new fp32 [tokens, heads, head_dim] (post-RoPE), head_dim 128;
- *   the rows of q, k_new and v_new are row_stride floats apart (a multiple of 4).
+ *   the rows of q, k_new and v_new are row_stride floats apart (a multiple of 4 below
+ *   2^25).
  *   chunk_offsets int32 [requests + 1], ascending: request n's chunk is token rows
  *   [chunk_offsets[n], chunk_offsets[n+1]), which may be empty; cache_lengths uint32
  *   [requests]: its rows c_n in the cache before the chunk; lookup uint32
@@ -183,7 +184,7 @@ int uocr_paged_chunk_attention(float* out, const float* q, const float* k_new, c
  * thirds of one fused projection's output, qkv [tokens, 3, heads, head_dim] with rows
  * row_stride floats apart, q and k_new before RoPE; the stored k rows have the
  * bits of uocr_rope.  positions int32 [tokens] (clamped into the tables), cos_table /
- * sin_table fp32 [table_rows, head_dim]. */
+ * sin_table fp32 [table_rows, head_dim], 16-byte aligned. */
 int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens, int64_t heads, int64_t head_dim,
                                    int64_t row_stride, const int32_t* positions, const float* cos_table,
                                    const float* sin_table, int64_t table_rows, int64_t table_dim, float* kv_blocks,

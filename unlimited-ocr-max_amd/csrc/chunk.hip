@@ -8,9 +8,10 @@
 // are stored there, and it attends rows [0, c_n + i]:
 //   out = sum_r softmax_r(scale * q.k_r) v_r      (fp32, D = 128).
 //
-// k_chunk_store writes the new rows into the pool (rotating q and k first where
-// they come unrotated; the rotated q waits in out), so the attention reads every
-// row from the pool.
+// k_chunk_store writes the new rows into the pool, and rotated queries into out, before k_chunk_tiles, which reads
+// every row from there.  (Queries rotated by the tiles as they are read: 10 us more for 8 prompts of up to 512.)  In
+// k_chunk_few a new row is read from the inputs (rotated by whoever reads it, where it comes unrotated) and stored by
+// the workgroup whose queries its token is among; nothing else in the launch reads that pool row.
 //
 // k_chunk_tiles (256 queries a workgroup) and k_chunk_few (32) run the two products on the fp16 matrix instruction,
 // each operand as a pair of halves, and keep a running maximum and sum of every query (below).
@@ -45,21 +46,38 @@ struct ChunkArgs {
   int64_t in_stride;  // floats between rows of q / k_new / v_new
 };
 
-// The request whose chunk holds token t, its first token and its cached rows; false
-// where none does.  Offsets are device data: whatever they hold, the request is in range.
-__device__ __forceinline__ bool request_of(const ChunkArgs& a, int t, int& n, int& first, int64_t& row) {
-  int lo = 0, hi = a.requests;  // the last n < requests with off[n] <= t (an empty chunk's offset is its successor's)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (ldg(a.offsets + mid) <= t) lo = mid;
-    else hi = mid;
+// A request's chunk: its token rows [first, end) and its cached rows.
+struct Chunk {
+  int n, first, end, cached;
+};
+// The last request n with floor(off[n] / 2^log2) + (n if `numbered`) <= key, found by the whole wave: 64 probes at a
+// time, whose last round brings the request's metadata along.  Offsets are device data: whatever they hold, the
+// request is one of them.
+__device__ __forceinline__ Chunk find_chunk(const ChunkArgs& a, int log2, bool numbered, int64_t key) {
+  const int lane = lane_id();
+  const auto below = [&](int off, int i) { return (int64_t)(off >> log2) + (numbered ? i : 0) <= key; };
+  int lo = 0, hi = a.requests;
+  while (hi - lo > 64) {
+    const int step = (hi - lo + 63) / 64, i = lo + lane * step;
+    const bool b = i < hi && below(ldg(a.offsets + min(i, hi - 1)), i);
+    lo = min(lo + (max(1, __popcll(__ballot(b))) - 1) * step, hi - 1);
+    hi = min(hi, lo + step);
   }
-  n = lo;
-  first = ldg(a.offsets + n);
-  if (first < 0 || first > t || ldg(a.offsets + n + 1) <= t) return false;
-  const uint32_t cached = min(ldg(a.cache_lengths + n), (uint32_t)a.max_rows);
-  row = (int64_t)cached + (t - first);
-  return true;
+  const int i = min(lo + lane, hi - 1);
+  const int off = ldg(a.offsets + i), next = ldg(a.offsets + i + 1);
+  const uint32_t cached = min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
+  const int at = __builtin_amdgcn_readfirstlane(max(1, __popcll(__ballot(lo + lane < hi && below(off, i)))) - 1);
+  Chunk c;
+  c.n = __builtin_amdgcn_readfirstlane(lo) + at;
+  c.first = __builtin_amdgcn_readlane(off, at);
+  c.end = min(__builtin_amdgcn_readlane(next, at), a.tokens);
+  c.cached = __builtin_amdgcn_readlane((int)cached, at);
+  return c;
+}
+// The chunk that holds token t (wave-uniform); false where none does.
+__device__ __forceinline__ bool chunk_of(const ChunkArgs& a, int t, Chunk& c) {
+  c = find_chunk(a, 0, false, t);
+  return c.first >= 0 && c.first <= t && t < c.end;
 }
 
 __device__ __forceinline__ float* row_ptr(const ChunkArgs& a, int n, int h, int r, int kv) {
@@ -68,43 +86,71 @@ __device__ __forceinline__ float* row_ptr(const ChunkArgs& a, int n, int h, int 
          (int64_t)(r % a.P) * a.slot_stride + (int64_t)h * kD;
 }
 
-// Thread (token, head, d < 64): the pair (d, d + 64) of k and v into the pool, and, given
-// positions, of q into out, q and k rotated with k_rope's arithmetic (each product and the
-// sum rounded, no contraction).
-__global__ void __launch_bounds__(256) k_chunk_store(ChunkArgs a, float* __restrict__ out, const float* q,
-                                                     const float* k_new, const float* v_new,
-                                                     const int32_t* __restrict__ positions,
-                                                     const float* __restrict__ cos_t,
-                                                     const float* __restrict__ sin_t, int table_rows) {
+// RoPE's tables (positions null: q and k come rotated).
+struct Rope {
+  const int32_t* positions;
+  const float* cos_t;
+  const float* sin_t;
+  int table_rows;
+};
+
+// Element d of the rotated row x, and four pairs of such: k_rope's arithmetic.
+__device__ __forceinline__ float rotated(const float* x, const float* c, const float* s, int d) {
 #pragma clang fp contract(off)
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int d = (int)(i % 64);
-  const int64_t th = i / 64;  // token * heads + head
-  if (th >= (int64_t)a.tokens * a.heads) return;
-  const int t = (int)(th / a.heads), h = (int)(th % a.heads);
-  int n, first;
-  int64_t row;
-  if (!request_of(a, t, n, first, row)) return;
-  const int64_t src = (int64_t)t * a.in_stride + (int64_t)h * kD;
-  float kl = ldg(k_new + src + d), kh = ldg(k_new + src + d + 64);
-  const float vl = ldg(v_new + src + d), vh = ldg(v_new + src + d + 64);
-  if (positions != nullptr) {
-    const int pos = min(max(ldg(positions + t), 0), table_rows - 1);
-    const float cl = ldg(cos_t + (int64_t)pos * kD + d), ch = ldg(cos_t + (int64_t)pos * kD + d + 64);
-    const float sl = ldg(sin_t + (int64_t)pos * kD + d), sh = ldg(sin_t + (int64_t)pos * kD + d + 64);
-    const float l = kl, u = kh;
-    kl = l * cl + (-u) * sl;
-    kh = u * ch + l * sh;
-    const float ql = ldg(q + src + d), qu = ldg(q + src + d + 64);
-    out[th * kD + d] = ql * cl + (-qu) * sl;
-    out[th * kD + d + 64] = qu * ch + ql * sh;
+  return d < 64 ? ldg(x + d) * ldg(c + d) + (-ldg(x + d + 64)) * ldg(s + d)
+                : ldg(x + d) * ldg(c + d) + ldg(x + d - 64) * ldg(s + d);
+}
+__device__ __forceinline__ void rotate4(f32x4& lo, f32x4& hi, f32x4 cl, f32x4 ch, f32x4 sl, f32x4 sh) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float l = lo[e], u = hi[e];
+    lo[e] = l * cl[e] + (-u) * sl[e];
+    hi[e] = u * ch[e] + l * sh[e];
   }
+}
+
+// The tensors whose rows are in_stride floats apart.
+struct Inputs {
+  const float* q;
+  const float* k_new;
+  const float* v_new;
+};
+
+// Lane d < 64 of a wave: the pair (d, d + 64) of token t's k and v of one head into the pool.
+__device__ __forceinline__ void store_pair(const ChunkArgs& a, const Rope& rope, const Inputs& in, const Chunk& c, int t,
+                                           int h, int d) {
+  const int64_t src = (int64_t)t * a.in_stride + (int64_t)h * kD, row = (int64_t)c.cached + (t - c.first);
   if (row >= a.max_rows) return;  // past what the lookup row addresses: not stored
-  float* kp = row_ptr(a, n, h, (int)row, 0);
-  kp[d] = kl;
-  kp[d + 64] = kh;
-  kp[a.kv_stride + d] = vl;
-  kp[a.kv_stride + d + 64] = vh;
+  const float* k = in.k_new + src;
+  float* kp = row_ptr(a, c.n, h, (int)row, 0) + d;
+  if (rope.positions != nullptr) {
+    const int64_t at = (int64_t)min(max(ldg(rope.positions + t), 0), rope.table_rows - 1) * kD;
+    kp[0] = rotated(k, rope.cos_t + at, rope.sin_t + at, d);
+    kp[64] = rotated(k, rope.cos_t + at, rope.sin_t + at, d + 64);
+  } else {
+    kp[0] = ldg(k + d);
+    kp[64] = ldg(k + d + 64);
+  }
+  kp[a.kv_stride] = ldg(in.v_new + src + d);
+  kp[a.kv_stride + 64] = ldg(in.v_new + src + d + 64);
+}
+
+// One wave per (token, head).
+__global__ void __launch_bounds__(256) k_chunk_store(ChunkArgs a, Rope rope, Inputs in, float* out) {
+  const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  if (th >= (int64_t)a.tokens * a.heads) return;
+  const int t = (int)(th / a.heads);
+  Chunk c;
+  if (!chunk_of(a, t, c)) return;
+  const int h = (int)(th % a.heads), d = lane_id();
+  if (rope.positions != nullptr) {
+    const int64_t at = (int64_t)min(max(ldg(rope.positions + t), 0), rope.table_rows - 1) * kD;
+    const float* q = in.q + (int64_t)t * a.in_stride + (int64_t)h * kD;
+    out[th * kD + d] = rotated(q, rope.cos_t + at, rope.sin_t + at, d);
+    out[th * kD + d + 64] = rotated(q, rope.cos_t + at, rope.sin_t + at, d + 64);
+  }
+  store_pair(a, rope, in, c, t, h, d);
 }
 
 // ------------------------------------------------------------------ fp32 products on the fp16 matrix instruction
@@ -215,6 +261,15 @@ struct Queries {
   f32x16 o[4];
 };
 
+__device__ __forceinline__ void start_queries(Queries& w, float scale, int limit) {
+  w.unit = __builtin_fabsf(scale) * 1.44269504f;
+  w.limit = limit;
+  w.m = -kInf;
+  w.l = 0.0f;
+  w.ev = w.most = kMinExp;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w.o[u] = f32x16{};
+}
 __device__ __forceinline__ void load_queries(Queries& w, _Float16* qlo, const float* row, float scale, int limit) {
   const int h = lane_id() >> 5;
   f32x4 x[16];
@@ -241,13 +296,7 @@ __device__ __forceinline__ void load_queries(Queries& w, _Float16* qlo, const fl
     w.hi[t] = halves(hi);
     *(f16x8*)(qlo + t * kFrag + lane_id() * 8) = halves(lo);
   }
-  w.unit = __builtin_fabsf(scale) * 1.44269504f;
-  w.limit = limit;
-  w.m = -kInf;
-  w.l = 0.0f;
-  w.ev = w.most = kMinExp;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) w.o[u] = f32x16{};
+  start_queries(w, scale, limit);
 }
 
 // Brings a lane's unit to where values of exponent eb can be added: at or above it, and not more
@@ -277,10 +326,37 @@ __device__ __forceinline__ float move_max(Queries& w, float mx) {
   return w.m == -kInf ? 0.0f : w.m;
 }
 
+// What the slow path reads: a block's rows from the pool, and from old_rows on from the inputs.
+struct SlowRows {
+  const float* k;  // the block's first row
+  const float* q;  // this lane's query
+  int64_t kv_stride, slot_stride, in_stride;
+  const float* k_new;  // as if the block's first row were new
+  const float* v_new;
+  int old_rows;  // of the block
+  const Rope* rope;
+  int64_t q_pos, row_pos;  // the query's token, and the block's first row's
+  __device__ __forceinline__ const float* table(const float* t, int64_t token) const {
+    return t + (int64_t)min(max(ldg(rope->positions + token), 0), rope->table_rows - 1) * kD;
+  }
+  __device__ __forceinline__ float q_at(int d) const {
+    if (rope == nullptr || rope->positions == nullptr) return ldg(q + d);
+    return rotated(q, table(rope->cos_t, q_pos), table(rope->sin_t, q_pos), d);
+  }
+  __device__ __forceinline__ float k_at(int key, int d) const {
+    if (key < old_rows) return ldg(k + key * slot_stride + d);
+    const float* x = k_new + key * in_stride;
+    if (rope->positions == nullptr) return ldg(x + d);
+    return rotated(x, table(rope->cos_t, row_pos + key), table(rope->sin_t, row_pos + key), d);
+  }
+  __device__ __forceinline__ const float* v_row(int key) const {
+    return key < old_rows ? k + kv_stride + key * slot_stride : v_new + key * in_stride;
+  }
+};
+
 // A block that the fp16 pairs cannot hold (a value that is not finite, or rows of unlike sizes beside
 // hidden ones), in fp32 and one key at a time.  stash: 32 floats a lane.
-__device__ __forceinline__ void slow_block(Queries& w, const float* q, float scale, const float* k,
-                                           int64_t kv_stride, int64_t slot_stride, int live, float* stash) {
+__device__ __forceinline__ void slow_block(Queries& w, const SlowRows& rows, float scale, int live, float* stash) {
   const int h = lane_id() >> 5;
   float y[16], mx = -kInf;
 #pragma unroll 1
@@ -289,7 +365,7 @@ __device__ __forceinline__ void slow_block(Queries& w, const float* q, float sca
     float s = 0.0f;
     if (key < live) {
 #pragma unroll 1
-      for (int d = 0; d < kD; ++d) s = __builtin_fmaf(ldg(q + d), ldg(k + (int64_t)key * slot_stride + d), s);
+      for (int d = 0; d < kD; ++d) s = __builtin_fmaf(rows.q_at(d), rows.k_at(key, d), s);
     }
     stash[r * kWave] = key < live ? s * scale * 1.44269504f : -kInf;
   }
@@ -307,11 +383,10 @@ __device__ __forceinline__ void slow_block(Queries& w, const float* q, float sca
     stash[(8 * (r / 4) + r % 4) * kWave] = h == 0 ? p : theirs;  // by key, for this lane's query
     stash[(8 * (r / 4) + 4 + r % 4) * kWave] = h == 0 ? theirs : p;
   }
-  const float* v = k + kv_stride;
   uint32_t most = 0;  // of the attended rows' finite values
 #pragma unroll 1
   for (int i = 0; i < live * 64; ++i) {
-    const uint32_t x = __float_as_uint(ldg(v + (int64_t)(i / 64) * slot_stride + 64 * h + i % 64)) & 0x7fffffffu;
+    const uint32_t x = __float_as_uint(ldg(rows.v_row(i / 64) + 64 * h + i % 64)) & 0x7fffffffu;
     if (x < 0x7f800000u) most = max(most, x);
   }
   most = max(most, other<32>(most));
@@ -320,9 +395,10 @@ __device__ __forceinline__ void slow_block(Queries& w, const float* q, float sca
 #pragma unroll 1
   for (int key = 0; key < live; ++key) {
     const float p = stash[key * kWave];
+    const float* v = rows.v_row(key) + 16 * h;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const f32x4 x = *(const UOCR_GLOBAL f32x4*)(v + (int64_t)key * slot_stride + 4 * (8 * (i / 4) + 4 * h + i % 4));
+      const f32x4 x = *(const UOCR_GLOBAL f32x4*)(v + 32 * (i / 4) + 4 * (i % 4));
 #pragma unroll
       for (int u = 0; u < 4; ++u) w.o[u][i] = __builtin_fmaf(p, x[u] * down, w.o[u][i]);
     }
@@ -452,31 +528,35 @@ __device__ __forceinline__ void apart_weights(Queries& w, f32x16& s, const int* 
 
 // ------------------------------------------------------------------ tiles of queries
 
-// The query tiles of all chunks, numbered without a sum over the requests: tile j of request
-// n is slot floor(off[n] / rows) + n + j, which no other tile is.
-struct QueryTile {
-  int n, first, end;  // the request, its first token and the one behind its last
-  int t0;             // the tile's first token
-  int cached;
+// The query tiles of all chunks.  Of up to 64 requests they are numbered one after the other: a lane per request, and a
+// sum over the lanes.  Of more, without a sum: tile j of request n is slot floor(off[n] / rows) + n + j, which no other
+// tile is, with slots left out.  (Those in between, where every request fills its last tile: every other workgroup
+// is empty, the others meet on half of the shader engines, and 8 chunks of 256 over 1000 rows took 138 us for 78.)
+struct QueryTile : Chunk {
+  int t0;  // the tile's first token
 };
 __device__ __forceinline__ bool query_tile(const ChunkArgs& a, int rows_log2, int slot, QueryTile& q) {
-  // the last n with floor(off[n] / rows) + n <= slot: 64 probes at a time
-  int lo = 0, hi = a.requests;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64, i = lo + lane_id() * step;
-    const bool below = i < hi && (ldg(a.offsets + min(i, hi - 1)) >> rows_log2) + (int64_t)i <= slot;
-    const int found = max(1, __popcll(__ballot(below)));
-    lo = min(lo + (found - 1) * step, hi - 1);
-    hi = min(hi, lo + step);
+  int64_t j;
+  if (a.requests <= 64) {
+    const int i = min(lane_id(), a.requests - 1);
+    const int off = ldg(a.offsets + i), next = min(ldg(a.offsets + i + 1), a.tokens);
+    const uint32_t cached = min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
+    const bool some = lane_id() < a.requests && off >= 0 && off < next;
+    const int tiles = some ? ((next - off - 1) >> rows_log2) + 1 : 0, behind = wave_scan_i(tiles);
+    const int at = __popcll(__ballot(behind <= slot));  // the first whose tiles reach past the slot
+    if (at >= a.requests) return false;
+    q.n = at;
+    q.first = __builtin_amdgcn_readlane(off, at);
+    q.end = __builtin_amdgcn_readlane(next, at);
+    q.cached = __builtin_amdgcn_readlane((int)cached, at);
+    j = slot - (__builtin_amdgcn_readlane(behind, at) - __builtin_amdgcn_readlane(tiles, at));
+  } else {
+    (Chunk&)q = find_chunk(a, rows_log2, true, slot);
+    j = (int64_t)slot - ((int64_t)(q.first >> rows_log2) + q.n);
   }
-  q.n = __builtin_amdgcn_readfirstlane(lo);
-  q.first = ldc(a.offsets + q.n);
-  q.end = min(ldc(a.offsets + q.n + 1), a.tokens);
-  const int64_t j = (int64_t)slot - ((int64_t)(q.first >> rows_log2) + q.n);
-  if (q.first < 0 || j < 0 || ((int64_t)q.first + (j << rows_log2)) >= q.end) return false;
-  q.t0 = q.first + (int)(j << rows_log2);
-  q.cached = (int)min(ldc(a.cache_lengths + q.n), (uint32_t)a.max_rows);
-  return true;
+  const int64_t t0 = (int64_t)q.first + (j << rows_log2);
+  q.t0 = (int)t0;
+  return q.first >= 0 && j >= 0 && t0 < q.end;
 }
 // Rows that token t of the request attends.
 __device__ __forceinline__ int rows_of(const ChunkArgs& a, const QueryTile& q, int t) {
@@ -523,25 +603,24 @@ struct Stage {
   float m, up;
   uint32_t bits;
   int e, word;
-  uint32_t at;  // this lane's offset in bytes from the block's first row
 
   __device__ __forceinline__ static int row_in_group(int lane) { return kValues ? 4 * (lane >> 5) : lane & 7; }
   __device__ __forceinline__ static uint32_t column(int lane) { return 16u * (kValues ? lane & 31 : lane >> 3); }
-  // 32 rows are below 2^31 bytes: 32 bits of offset a lane, from a scalar base
-  __device__ __forceinline__ void load(const float* base, int64_t kv_stride, uint32_t row_bytes, int group, int last,
-                                       int lane) {
-    const char* from = (const char*)(kValues ? base + kv_stride : base);
+  // 32 rows are below 2^32 bytes: 32 bits of offset a lane, from a scalar base.  Rows past the last are its
+  // copies, zeroed before they are converted.
+  __device__ __forceinline__ void load(const float* from, uint32_t row_bytes, int group, int last, int lane) {
+    const int row = 8 * group + row_in_group(lane);
     if (last >= kBlock - 1) {
+      const uint32_t at = (uint32_t)row * row_bytes + column(lane);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        x[j] = kValues ? *(const UOCR_GLOBAL f32x4*)(from + (at + j * row_bytes))
-                       : *(const UOCR_GLOBAL f32x4*)(from + at + 128 * j);
-    } else {  // rows past the last are its copies, zeroed before they are converted
+        x[j] = kValues ? *(const UOCR_GLOBAL f32x4*)((const char*)from + (at + j * row_bytes))
+                       : *(const UOCR_GLOBAL f32x4*)((const char*)from + at + 128 * j);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = min(8 * group + row_in_group(lane) + (kValues ? j : 0), last);
-        x[j] = *(const UOCR_GLOBAL f32x4*)(from + ((uint32_t)row * row_bytes + column(lane) + (kValues ? 0u : 128u * j)));
-      }
+      for (int j = 0; j < 4; ++j)
+        x[j] = *(const UOCR_GLOBAL f32x4*)((const char*)from + ((uint32_t)min(row + (kValues ? j : 0), last) * row_bytes +
+                                                                column(lane) + (kValues ? 0u : 128u * j)));
     }
   }
   __device__ __forceinline__ void clear_past(int group, int last, int lane) {
@@ -676,8 +755,8 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
   Stage<true> v[2];
   const auto load = [&](int i, int at) {  // block i into buffer `at`
     const int last = end - 1 - (begin + i * kBlock);
-    k[at].load(rows.base, kv_stride, row_bytes, group, last, lane);
-    v[at].load(rows.base, kv_stride, row_bytes, group, last, lane);
+    k[at].load(rows.base, row_bytes, group, last, lane);
+    v[at].load(rows.base + kv_stride, row_bytes, group, last, lane);
   };
   const auto measure = [&](auto& x, int i) {
     const int key0 = begin + i * kBlock, last = end - 1 - key0;
@@ -699,11 +778,6 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
       for (int j = 0; j < 4; ++j) x.convert(j, at);
     }
   };
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    k[j].at = (uint32_t)(8 * group + k[j].row_in_group(lane)) * row_bytes + k[j].column(lane);
-    v[j].at = (uint32_t)(8 * group + v[j].row_in_group(lane)) * row_bytes + v[j].column(lane);
-  }
   rows.start(begin);
   load(0, 0);
   if (blocks > 1) {
@@ -726,7 +800,7 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     load(2, 0);
   }
   lds_barrier();
-  const int plain = (min(end, shown) - begin) / kBlock;  // blocks whose rows every query sees
+  const int full = (end - begin) / kBlock;
   int v_buf = 1;
   const auto step = [&](int i, int at) {  // block i + 1, from buffer `at`, in the interval of block i
     if (i + 1 < blocks) {
@@ -735,7 +809,8 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
       if (group == 0) sh.apart[(i + 3) & 3] = 0;  // of block i - 1, which all have read, for block i + 3
       k[at].largest();
       v[at].largest();
-      if (i + 1 < plain && k[at].fits(kunit) && v[at].fits(vunit)) {
+      // (at the walk's scale a hidden row costs the others nothing, whatever its size)
+      if (i + 1 < full && k[at].fits(kunit) && v[at].fits(vunit)) {
         k[at].up = pow2_of(141 - kunit);
         v[at].up = pow2_of(141 - vunit);
         sh.meta[(i + 1) & 3][group] = 0;
@@ -817,8 +892,8 @@ __device__ __forceinline__ void attend_walk(Queries& w, int begin, int end, bool
 }
 
 __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3)
-    k_chunk_tiles(ChunkArgs a, float* out, const float* q, int64_t q_stride, float scale, float* part, float* weights,
-                  int slots, int split_rows, int splits) {
+    k_chunk_tiles(ChunkArgs a, const float* q, int64_t q_stride, float* out, float scale, float* part, float* weights, int slots,
+                  int split_rows, int splits) {
   __shared__ __align__(16) _Float16 lds[kLdsHalves];
   __shared__ __align__(16) Shared sh;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
@@ -831,39 +906,42 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3)
   const int t_last = min(qt.t0 + 32 * kTileWaves, qt.end) - 1;
   const int all_rows = rows_of(a, qt, t_last);
   const int begin = split * split_rows, end = min(begin + split_rows, all_rows);
-  if (begin >= end) return;
   const int shown = rows_of(a, qt, qt.t0);  // rows past these are hidden from some query
   RowWalk rows{a.pool + a.layer_off + (int64_t)head * kD, a.lookup + (int64_t)qt.n * a.lookup_cols, a.page_stride,
                a.slot_stride, a.P, a.pages - 1, end, nullptr, nullptr, 0};
   if (wave >= kTileWaves) {
-    convert_walk(rows, a.kv_stride, begin, shown, wave - kTileWaves, lds, sh);
+    if (begin < end) convert_walk(rows, a.kv_stride, begin, shown, wave - kTileWaves, lds, sh);
     return;
   }
+  if (begin >= end) return;
   for (int i = (int)threadIdx.x; i < kMaxSplitRows / kBlock / 32; i += 64 * kTileWaves) sh.slow[i] = 0;
-  const int my_t = min(qt.t0 + 32 * wave + (lane & 31), t_last);
   const bool idle = qt.t0 + 32 * wave > t_last;  // a wave without queries
   Queries w;
   _Float16* qlo = lds + 2 * kKHalves + 3 * kVHalves + wave * kQHalves;
-  load_queries(w, qlo, q + (int64_t)my_t * q_stride + (int64_t)head * kD, scale, min(rows_of(a, qt, my_t), end));
+  const auto my_token = [&](int lane) { return min(qt.t0 + 32 * wave + (lane & 31), t_last); };
+  const auto my_query = [&](int t) { return q + (int64_t)t * q_stride + (int64_t)head * kD; };
+  load_queries(w, qlo, my_query(my_token(lane)), scale, min(rows_of(a, qt, my_token(lane)), end));
   attend_walk(w, begin, end, idle, wave >= kTileWaves / 2, lds, qlo, sh);
   if (idle) return;
-  float* stash = (float*)lds + wave * 32 * kWave + lane;
+  const int now = lane_now(), my_t = my_token(now);  // not kept through the walk
+  float* stash = (float*)lds + wave * 32 * kWave + now;
 #pragma unroll 1
   for (int i = 0; i < (end - begin + kBlock - 1) / kBlock; ++i) {
     const int k0 = begin + i * kBlock;
     if ((sh.slow[i / 32] >> (i % 32) & 1) == 0 || __ballot(w.limit > k0) == 0) continue;
-    slow_block(w, q + (int64_t)my_t * q_stride + (int64_t)head * kD, scale, rows.at(k0), a.kv_stride, a.slot_stride,
-               min(w.limit - k0, kBlock), stash);
+    const SlowRows from{rows.at(k0), my_query(my_t), a.kv_stride, a.slot_stride, 0, nullptr, nullptr, kBlock, nullptr, 0,
+                        0};
+    slow_block(w, from, scale, min(w.limit - k0, kBlock), stash);
   }
-  const bool live = qt.t0 + 32 * wave + (lane & 31) <= t_last;
+  const bool live = qt.t0 + 32 * wave + (now & 31) <= t_last;
   store_queries(w, a, my_t, live, head, split, all_rows <= split_rows, out, part, weights);
 }
 
-// k_chunk_few: 32 queries a workgroup, whose 4 waves take the rows' blocks in turn, each straight from memory into
-// the operands' lanes (keys: lane (row l % 32, columns 8 i + 4 (l / 32)); values: lane (columns 4 (l % 32) on, rows
+// k_chunk_few: 32 queries a workgroup, whose 4 waves take the rows' blocks in turn, each straight from memory into the
+// operands' lanes (keys: lane (row l % 32, columns 8 i + 4 (l / 32)); values: lane (columns 4 (l % 32) on, rows
 // 16 t + 8 (j / 4) + 4 (l / 32) + j % 4)), and join their sums in LDS.
 constexpr int kFewWaves = 4;
-constexpr int kFewLog2 = 5;             // queries of a workgroup
+constexpr int kFewLog2 = 5;  // queries of a workgroup
 constexpr int kFewSplitRows = kFewWaves * 64 * kBlock;  // a wave notes its slow blocks in 64 bits
 
 // 32 rows of keys or values on their way from memory to the operands of one wave.
@@ -885,11 +963,12 @@ __device__ __forceinline__ uint32_t wave_largest(float m) {
 }
 // The scale of a block whose lanes' largest are m: the walk's if that fits (unit 0: there is none yet, and the
 // block sets it).
-__device__ __forceinline__ int few_scale(float m, int& unit, bool& finite) {
+__device__ __forceinline__ int few_scale(float m, int& unit, bool& finite, bool& own) {
   if (unit != 0) {
     const float most = pow2_of(min(unit + 1, kMaxExp) - 127), least = pow2_of(max(unit - kBelow, 1) - 127);
     if (__ballot(!(m < most)) == 0 && __ballot(m >= least) != 0) return unit;
   }
+  own = true;
   const uint32_t bits = wave_largest(m);
   finite = finite && bits < 0x7f800000u;
   const int e = clamp_exp(bits);
@@ -899,11 +978,12 @@ __device__ __forceinline__ int few_scale(float m, int& unit, bool& finite) {
 }
 
 __global__ void __launch_bounds__(64 * kFewWaves, 2)
-    k_chunk_few(ChunkArgs a, float* out, const float* q, int64_t q_stride, float scale, float* part, float* weights,
-                int slots, int split_rows, int splits) {
-  __shared__ __align__(16) float sums[kFewWaves][32 * kD];  // a wave's sums, before that its slow path's stash,
-  _Float16* const qs = (_Float16*)sums;  // and first the queries' operands, [part][step][lane][8]
+    k_chunk_few(ChunkArgs a, Rope rope, Inputs in, float* out, float scale, float* part, float* weights, int slots,
+                int split_rows, int splits) {
+  __shared__ __align__(16) float sums[kFewWaves][32 * kD];  // the waves' sums, before that their slow paths' stash,
+  _Float16* const qs = (_Float16*)sums;             // and first the queries' operands, [part][step][lane][8]
   __shared__ float peak[kFewWaves][32], total[kFewWaves][32];
+  __shared__ int q_exp[32];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = lane >> 5;
   const int per = (int)(gridDim.x / 8), item = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
   if (item >= slots * a.heads * splits) return;
@@ -913,15 +993,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
   const int t_last = min(qt.t0 + 32, qt.end) - 1;
   const int all_rows = rows_of(a, qt, t_last);
   const int begin = split * split_rows, end = min(begin + split_rows, all_rows);
+  if (split == 0)  // new rows that none attends
+    for (int t = qt.t0 + wave; t <= t_last; t += kFewWaves)
+      if ((int64_t)qt.cached + (t - qt.first) >= a.attend_max) store_pair(a, rope, in, qt, t, head, lane);
   if (begin >= end) return;
   const int shown = rows_of(a, qt, qt.t0);
-  const int my_t = min(qt.t0 + (lane & 31), t_last);
-  const float* my_q = q + (int64_t)my_t * q_stride + (int64_t)head * kD;
-  Queries w;
-  load_queries(w, qs + kQHalves, my_q, scale, min(rows_of(a, qt, my_t), end));  // every wave the same values
-#pragma unroll
-  for (int t = 0; t < 8; ++t) *(f16x8*)(qs + t * kFrag + lane * 8) = w.hi[t];
-  __syncthreads();
   const float* pool = a.pool + a.layer_off + (int64_t)head * kD;
   const uint32_t* lookup = a.lookup + (int64_t)qt.n * a.lookup_cols;
   const uint32_t row_bytes = (uint32_t)a.slot_stride * 4u;
@@ -929,37 +1005,135 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
     return pool + (int64_t)min(ldc(lookup + row / a.P), (uint32_t)(a.pages - 1)) * a.page_stride +
            (int64_t)(row % a.P) * a.slot_stride;
   };
-  int kunit = 0, vunit = 0;
-  uint64_t slow = 0;
+  // rows from old_rows on are the inputs', those from my_rows on this workgroup's to store
+  const int old_rows = qt.cached, my_rows = qt.cached + (qt.t0 - qt.first);
+  const auto token_of = [&](int row) { return (int64_t)(qt.first + (row - qt.cached)); };
   FewStage k, v;
-  const auto load_k = [&](int key0, int lane) {
-    const int h = lane >> 5;
-    const char* from = (const char*)row_base(key0);
-    const uint32_t at = (uint32_t)min(lane & 31, end - 1 - key0) * row_bytes + 16u * h;
+  int row_pos = 0;  // the position of this lane's key row, where it is a new one
+  const auto load_k = [&](const float* base, int key0, int lane) {
+    const int row = min(lane & 31, end - 1 - key0), h = lane >> 5;
+    const char* from = (const char*)base + ((uint32_t)row * row_bytes + 16u * h);
+    if (key0 + kBlock > old_rows) {
+      if (key0 + row >= old_rows)
+        from = (const char*)(in.k_new + token_of(key0 + row) * a.in_stride + (int64_t)head * kD + 4 * h);
+      if (rope.positions != nullptr) row_pos = ldg(rope.positions + max(token_of(key0 + row), (int64_t)0));
+    }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) k.x[i] = *(const UOCR_GLOBAL f32x4*)(from + at + 32 * i);
+    for (int i = 0; i < 16; ++i) k.x[i] = *(const UOCR_GLOBAL f32x4*)(from + 32 * i);
   };
-  const auto load_v = [&](int key0, int lane) {
-    const int h = lane >> 5;
-    const char* from = (const char*)(row_base(key0) + a.kv_stride);
+  const auto v_row = [](int j, int h) { return 16 * (j / 8) + 8 * (j / 4 % 2) + 4 * h + j % 4; };
+  const auto load_v = [&](const float* base, int key0, int lane) {
+    const char* from = (const char*)(base + a.kv_stride);
     const int last = end - 1 - key0;
+    if (key0 + kBlock <= old_rows) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = min(16 * (i / 8) + 8 * (i / 4 % 2) + 4 * h + i % 4, last);
-      v.x[i] = *(const UOCR_GLOBAL f32x4*)(from + ((uint32_t)row * row_bytes + 16u * (lane & 31)));
+      for (int j = 0; j < 16; ++j)
+        v.x[j] = *(const UOCR_GLOBAL f32x4*)(from + ((uint32_t)min(v_row(j, lane >> 5), last) * row_bytes +
+                                                     16u * (lane & 31)));
+    } else {
+      const float* news = in.v_new + token_of(key0) * a.in_stride + (int64_t)head * kD;
+      const uint32_t new_bytes = (uint32_t)a.in_stride * 4u;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int row = min(v_row(j, lane >> 5), last);
+        const bool old = key0 + row < old_rows;
+        v.x[j] = *(const UOCR_GLOBAL f32x4*)((old ? from : (const char*)news) +
+                                             ((uint64_t)((uint32_t)row * (uint64_t)(old ? row_bytes : new_bytes)) +
+                                              16u * (lane & 31)));
+      }
     }
   };
-  const int first = begin + wave * kBlock;
-  if (first < end) {
-    load_k(first, lane);
-    load_v(first, lane);
+  // The new rows of a block: keys rotated, this tile's own rows stored.
+  const auto take_new = [&](int key0, int lane) {
+    const int h = lane >> 5, row = key0 + (lane & 31);
+    float* to = const_cast<float*>(row_base(key0));
+    if (rope.positions != nullptr && row >= old_rows && row < end) {
+      const int pos = min(max(row_pos, 0), rope.table_rows - 1);
+      const float* ct = rope.cos_t + (int64_t)pos * kD + 4 * h;
+      const float* st = rope.sin_t + (int64_t)pos * kD + 4 * h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        rotate4(k.x[i], k.x[i + 8], *(const UOCR_GLOBAL f32x4*)(ct + 8 * i), *(const UOCR_GLOBAL f32x4*)(ct + 8 * i + 64),
+                *(const UOCR_GLOBAL f32x4*)(st + 8 * i), *(const UOCR_GLOBAL f32x4*)(st + 8 * i + 64));
+    }
+    if (row >= my_rows && row < end) {
+      float* p = to + (int64_t)(lane & 31) * a.slot_stride + 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) *(UOCR_GLOBAL f32x4*)(p + 8 * i) = k.x[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int r = v_row(j, h);
+      if (key0 + r >= my_rows && key0 + r < end)
+        *(UOCR_GLOBAL f32x4*)(to + a.kv_stride + (int64_t)r * a.slot_stride + 4 * (lane & 31)) = v.x[j];
+    }
+  };
+  // The blocks are dealt from the last one, which has the new rows: their latencies begin first.  What does not wait
+  // for one another is asked for together: the first block's page, the queries and their positions; then the rows
+  // and the tables.
+  const int first = begin + ((end - begin + kBlock - 1) / kBlock - 1 - wave) * kBlock;
+  {
+    constexpr int R = 32 / kFewWaves, kPieces = 16 / kFewWaves, kStep = kD / kPieces;
+    const float* base = first >= begin ? row_base(first) : pool;
+    // the queries' operands: each wave 32 / kFewWaves of them, lane (query l % R, columns kStep i + 4 (l / R))
+    const int row = wave * R + lane % R, col = 4 * (lane / R), t = min(qt.t0 + row, t_last);
+    const float* src = in.q + (int64_t)t * a.in_stride + (int64_t)head * kD + col;
+    int pos = 0;
+    if (rope.positions != nullptr) pos = ldg(rope.positions + t);
+    f32x4 x[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) x[i] = *(const UOCR_GLOBAL f32x4*)(src + kStep * i);
+    __builtin_amdgcn_sched_barrier(0);
+    if (first >= begin) {
+      load_k(base, first, lane);
+      load_v(base, first, lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (rope.positions != nullptr) {
+      pos = min(max(pos, 0), rope.table_rows - 1);
+      const float* ct = rope.cos_t + (int64_t)pos * kD + col;
+      const float* st = rope.sin_t + (int64_t)pos * kD + col;
+#pragma unroll
+      for (int i = 0; i < kPieces / 2; ++i)
+        rotate4(x[i], x[i + kPieces / 2], *(const UOCR_GLOBAL f32x4*)(ct + kStep * i),
+                *(const UOCR_GLOBAL f32x4*)(ct + kStep * i + 64), *(const UOCR_GLOBAL f32x4*)(st + kStep * i),
+                *(const UOCR_GLOBAL f32x4*)(st + kStep * i + 64));
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) m = amax3(amax3(m, x[i].x, x[i].y), x[i].z, x[i].w);
+    uint32_t bits = __float_as_uint(m);  // a query's lanes are R apart
+    bits = max(bits, other<32>(bits));
+    bits = max(bits, other<16>(bits));
+    bits = max(bits, ror<8>(bits));
+    const int e = clamp_exp(bits);
+    q_exp[row] = e;
+    const float up = __builtin_copysignf(pow2_of(141 - e), scale);  // the scale's sign goes into the query
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int d = kStep * i + col;
+      const f32x4 y = x[i] * up;
+      uint32_t l0, l1;
+      const uint32_t h0 = split2(y.x, y.y, l0), h1 = split2(y.z, y.w, l1);
+      _Float16* at = qs + (d / 16) * kFrag + ((d / 4 % 2) * 32 + row) * 8 + (d / 8 % 2) * 4;
+      *(u32x2*)at = u32x2{h0, h1};
+      *(u32x2*)(at + kQHalves) = u32x2{l0, l1};
+    }
   }
+  __syncthreads();
+  Queries w;
+  w.exp = q_exp[lane & 31];
+  const int my_t = min(qt.t0 + (lane & 31), t_last);
+  start_queries(w, scale, min(rows_of(a, qt, my_t), end));
+  int kunit = 0, vunit = 0;
+  uint64_t slow = 0;
 #pragma unroll 1
-  for (int key0 = first, i = 0; key0 < end; key0 += kFewWaves * kBlock, ++i) {
+  for (int key0 = first, i = 0; key0 >= begin; key0 -= kFewWaves * kBlock, ++i) {
     const int lane = lane_now(), h = lane >> 5;
-    const int last = end - 1 - key0, next = key0 + kFewWaves * kBlock;
+    const int last = end - 1 - key0, next = key0 - kFewWaves * kBlock;
     int live = w.limit - key0;
-    bool finite = true;
+    bool finite = true, own = false;
+    if (key0 + kBlock > old_rows) take_new(key0, lane);
     if (last < kBlock - 1) {  // rows past the last were its copies
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -968,7 +1142,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
       }
     }
     const float km = k.largest();
-    const int ek = few_scale(km, kunit, finite);
+    const int ek = few_scale(km, kunit, finite, own);
     f32x16 s = {};
     const float kup = pow2_of(141 - ek);
 #pragma unroll
@@ -989,8 +1163,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
       s = mfma(halves(hi), qh, s);
     }
     const float vm = v.largest();
-    const int ev = few_scale(vm, vunit, finite);
-    if (key0 + kBlock > shown) {
+    int ev = few_scale(vm, vunit, finite, own);
+    if (own && key0 + kBlock > shown) {
       // rows hidden from some query: what they hold must not cost the others their bits
       const auto apart = [](uint32_t least, int e) {
         least = min(least, other<32>(least));
@@ -1013,10 +1187,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
     if (!finite) {  // left to the slow path
       slow |= 1ull << i;
       live = 0;
+      ev = __builtin_amdgcn_readfirstlane(w.ev);
 #pragma unroll
       for (int j = 0; j < 16; ++j) v.x[j] = f32x4{};
     }
-    if (next < end) load_k(next, lane);
+    const float* next_base = next >= begin ? row_base(next) : pool;
+    if (next >= begin) load_k(next_base, next, lane);
     const float c = scale_of(w, ek);
     hide(s, live, lane);
     const float lift = (float)kLift - move_max(w, largest_of(s) * c);
@@ -1047,14 +1223,18 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
         w.o[u] = mfma(halves(lo), p.hi[t], w.o[u]);
         w.o[u] = mfma(halves(hi), p.hi[t], w.o[u]);
       }
-    if (next < end) load_v(next, lane);
+    if (next >= begin) load_v(next_base, next, lane);
   }
   __syncthreads();
+#pragma unroll 1
   for (int i = 0; slow != 0; ++i, slow >>= 1) {
-    const int key0 = first + i * kFewWaves * kBlock;
-    if ((slow & 1) != 0)
-      slow_block(w, my_q, scale, row_base(key0), a.kv_stride, a.slot_stride, min(w.limit - key0, kBlock),
-                 sums[wave] + lane);
+    if ((slow & 1) == 0) continue;
+    const int key0 = first - i * kFewWaves * kBlock;
+    const int64_t token = token_of(key0), new0 = token * a.in_stride + (int64_t)head * kD;
+    const SlowRows from{row_base(key0), in.q + (int64_t)my_t * a.in_stride + (int64_t)head * kD, a.kv_stride,
+                        a.slot_stride, a.in_stride, in.k_new + new0, in.v_new + new0, old_rows - key0,
+                        &rope, my_t, token};
+    slow_block(w, from, scale, min(w.limit - key0, kBlock), sums[0] + wave * 32 * kWave + lane);
   }
   // the waves' sums at one maximum, in the values' own unit
   const float l = w.l + other32(w.l);
@@ -1073,15 +1253,16 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
     sum += mj == -kInf ? lj : lj * __builtin_amdgcn_exp2f(mj - m);  // lj: 0, or NaN
   }
   const float f = (w.m == -kInf ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(w.m - m)) / sum;
-  // column 4 r' + u of query l % 32, rows of 128 floats whose 16-byte pieces are rotated by the query
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int piece = 8 * (r / 4) + 4 * h + r % 4;
+  // query l % 32, a row of 128 floats whose 16-byte pieces are rotated by the query
+  const auto at = [&](int r) { return (lane & 31) * kD + 4 * ((8 * (r / 4) + 4 * h + r % 4 + lane) & 31); };
+  const auto mine = [&](int r) {
     f32x4 y;
 #pragma unroll
     for (int u = 0; u < 4; ++u) y[u] = __builtin_ldexpf(w.o[u][r] * f, w.ev - 141);
-    *(f32x4*)(sums[wave] + (lane & 31) * kD + 4 * ((piece + lane) & 31)) = y;
-  }
+    return y;
+  };
+#pragma unroll
+  for (int r = 0; r < 16; ++r) *(f32x4*)(sums[wave] + at(r)) = mine(r);
   __syncthreads();
   const bool whole = all_rows <= split_rows;
   const int64_t stride = (int64_t)a.tokens * a.heads;
@@ -1089,10 +1270,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
   for (int j = 0; j < 32 * 32 / (64 * kFewWaves); ++j) {
     const int i = j * 64 * kFewWaves + (int)threadIdx.x, query = i / 32, piece = i % 32;
     if (qt.t0 + query > t_last) continue;
-    const int at = query * kD + 4 * ((piece + query) & 31);
-    f32x4 y = *(const f32x4*)(sums[0] + at);
+    const int from = query * kD + 4 * ((piece + query) & 31);
+    f32x4 y = *(const f32x4*)(sums[0] + from);
 #pragma unroll
-    for (int k2 = 1; k2 < kFewWaves; ++k2) y += *(const f32x4*)(sums[k2] + at);
+    for (int k2 = 1; k2 < kFewWaves; ++k2) y += *(const f32x4*)(sums[k2] + from);
     const int64_t th = (int64_t)(qt.t0 + query) * a.heads + head;
     *(UOCR_GLOBAL f32x4*)((whole ? out + th * kD : part + (split * stride + th) * kD) + 4 * piece) = y;
   }
@@ -1105,37 +1286,56 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
 // hold normalised sums, so a split weighs what its weights sum to.
 __global__ void __launch_bounds__(256) k_chunk_join(ChunkArgs a, float* out, const float* __restrict__ part,
                                                     const float* __restrict__ weights, int rows_log2, int split_rows) {
-  const int64_t th = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   if (th >= (int64_t)a.tokens * a.heads) return;
   const int t = (int)(th / a.heads), lane = lane_id();
-  int n, first;
-  int64_t row;
-  if (!request_of(a, t, n, first, row)) return;
-  const int end = min(ldg(a.offsets + n + 1), a.tokens);
-  const int t_last = min(first + ((((t - first) >> rows_log2) + 1) << rows_log2), end) - 1;  // of its tile
-  const int splits = ((int)min(row + (t_last - t) + 1, (int64_t)a.attend_max) + split_rows - 1) / split_rows;
+  QueryTile q;
+  if (!chunk_of(a, t, q)) return;
+  const int t_last = min(q.first + ((((t - q.first) >> rows_log2) + 1) << rows_log2), q.end) - 1;  // of its tile
+  const int splits = (rows_of(a, q, t_last) + split_rows - 1) / split_rows;
   if (splits == 1) return;  // written by its tile
   const int64_t stride = (int64_t)a.tokens * a.heads;
-  float m = -kInf;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, ldg(weights + s * stride + th));
-  float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float ws = ldg(weights + s * stride + th);
-    if (ws == -kInf) continue;
-    const float f = __builtin_amdgcn_exp2f(ws - m);
-    const float* p = part + (s * stride + th) * kD + 2 * lane;
-    l += f;
-    o0 = __builtin_fmaf(f, ldg(p), o0);
-    o1 = __builtin_fmaf(f, ldg(p + 1), o1);
+  float m = -kInf, l = 0.0f;
+  f32x2 o = {0.0f, 0.0f};
+  constexpr int kAtOnce = 8;  // splits read together
+  for (int s0 = 0; s0 < splits; s0 += kAtOnce) {
+    float ws[kAtOnce], mn = m;
+    f32x2 p[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int64_t at = (int64_t)min(s0 + j, splits - 1) * stride + th;
+      ws[j] = ldc(weights + at);
+      p[j] = *(const UOCR_GLOBAL f32x2*)(part + at * kD + 2 * lane);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) mn = fmaxf(mn, ws[j]);
+    if (mn == -kInf) mn = 0.0f;
+    const float keep = __builtin_amdgcn_exp2f(m - mn);
+    l *= keep;
+    o *= keep;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (s0 + j >= splits || ws[j] == -kInf) continue;  // a split without a weight has no sum
+      const float f = __builtin_amdgcn_exp2f(ws[j] - mn);
+      l += f;
+      o.x = __builtin_fmaf(f, p[j].x, o.x);
+      o.y = __builtin_fmaf(f, p[j].y, o.y);
+    }
+    m = mn;
   }
-  out[th * kD + 2 * lane] = o0 / l;
-  out[th * kD + 2 * lane + 1] = o1 / l;
+  *(UOCR_GLOBAL f32x2*)(out + th * kD + 2 * lane) = o / l;
 }
 
 }  // namespace
 
 // How a call's rows are cut: tiles of 256 or of 32 queries, and splits of their rows where the tiles alone do not fill
-// the device.
+// the device.  A tile of 256 has a CU to itself and converts each row once for all its queries, but a short chunk
+// leaves most of it empty, and few tiles leave most CUs without one; tiles of 32 convert and read each row eight times
+// as often.  Measured, 10 heads, tiles of 256 / tiles of 32, in us: one request of 256 tokens 37 / 27, of 512 54 / 47,
+// of 1024 87 / 111, of 2048 110 / 229; of 256 tokens over 2000 cached rows 88 / 48, of 512 95 / 82, of 256 over 14000
+// 167 / 131, of 512 over 14000 144 / 259; four requests of 256 43 / 38, of 512 62 / 76; eight of 32 tokens over 1000
+// rows 66 / 42, of 128 79 / 72, of 256 108 / 122; eight of 64 24 / 20, of 256 50 / 58, of 512 75 / 129.
 namespace {
 constexpr int kCus = 256;
 struct Cut {
@@ -1144,14 +1344,15 @@ struct Cut {
 };
 Cut cut_of(int64_t tokens, int64_t requests, int heads, int attend_max) {
   Cut c{};
-  c.few = requests > 0 && tokens / requests < 128;
+  c.few = requests > 0 && (tokens / requests < 128 || (tokens < 1024 && tokens * attend_max < (int64_t)1 << 22));
   c.rows_log2 = c.few ? kFewLog2 : kTileLog2;
-  c.slots = (int)((tokens >> c.rows_log2) + requests);
-  const int64_t full = std::max<int64_t>(1, (tokens + (1 << c.rows_log2) - 1) >> c.rows_log2) * heads;
-  const int most = c.few ? kFewSplitRows : kMaxSplitRows, least = c.few ? 2 * kFewWaves * kBlock : 1024;
-  const int64_t wanted = std::max<int64_t>(1, (c.few ? 2 : 1) * kCus / full);
-  const int64_t rows = (attend_max + wanted - 1) / wanted;
-  c.split_rows = (int)std::min<int64_t>(most, std::max<int64_t>(least, (rows + 127) / 128 * 128));
+  const int64_t rows = (int64_t)1 << c.rows_log2;
+  c.slots = (int)(tokens / rows + requests);
+  // about as many tiles as there are: of each request's last one half is queries
+  const int64_t tiles = std::max(requests, (tokens + rows - 1) / rows + (requests - 1) / 2);
+  const int64_t fill = std::max<int64_t>(1, (c.few ? 2 * kCus : kCus) / std::max<int64_t>(1, tiles * heads));
+  const int64_t least = c.few ? 4 * kBlock : 1024, most = c.few ? kFewSplitRows : kMaxSplitRows;
+  c.split_rows = (int)std::min(most, std::max(least, (attend_max / fill + 127) / 128 * 128));
   c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
   return c;
 }
@@ -1183,26 +1384,26 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
   a.tokens = (int)p.tokens;
   a.attend_max = p.attend_max;
   a.in_stride = p.in_stride;
-  const int64_t pairs = p.tokens * p.heads;
-  UOCR_LAUNCH("chunk_store", k_chunk_store, dim3((unsigned)((pairs * 64 + 255) / 256)), dim3(256), 0, s, a, p.out,
-              p.q, p.k_new, p.v_new, p.positions, p.cos_table, p.sin_table, p.table_rows);
-  const bool rotated = p.positions != nullptr;
-  const float* q = rotated ? p.out : p.q;
-  const int64_t q_stride = rotated ? (int64_t)p.heads * kD : p.in_stride;
+  const Rope rope{p.positions, p.cos_table, p.sin_table, p.table_rows};
   const Cut c = cut_of(p.tokens, p.requests, p.heads, p.attend_max);
+  const int64_t pairs = p.tokens * p.heads, items = (int64_t)c.slots * p.heads * c.splits;
+  const dim3 by_pair((unsigned)((pairs + 3) / 4)), grid((unsigned)((items + 7) / 8 * 8));
+  const Inputs in{p.q, p.k_new, p.v_new};
   float* part = (float*)p.workspace;
-  float* weights = part + (int64_t)c.splits * p.tokens * p.heads * kD;
-  const int64_t items = (int64_t)c.slots * p.heads * c.splits;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8));
-  if (c.few)
-    UOCR_LAUNCH("chunk_few", k_chunk_few, grid, dim3(64 * kFewWaves), 0, s, a, p.out, q, q_stride, p.scale, part, weights,
+  float* weights = part + (int64_t)c.splits * pairs * kD;
+  if (!c.few) {
+    UOCR_LAUNCH("chunk_store", k_chunk_store, by_pair, dim3(256), 0, s, a, rope, in, p.out);
+    const bool rotated_q = p.positions != nullptr;  // they wait in out
+    UOCR_LAUNCH("chunk_tiles", k_chunk_tiles, grid, dim3(64 * (kTileWaves + kStageWaves)), 0, s, a,
+                rotated_q ? p.out : p.q, rotated_q ? (int64_t)p.heads * kD : p.in_stride, p.out, p.scale, part, weights,
                 c.slots, c.split_rows, c.splits);
-  else
-    UOCR_LAUNCH("chunk_tiles", k_chunk_tiles, grid, dim3(64 * (kTileWaves + kStageWaves)), 0, s, a, p.out, q, q_stride,
-                p.scale, part, weights, c.slots, c.split_rows, c.splits);
+  } else {
+    UOCR_LAUNCH("chunk_few", k_chunk_few, grid, dim3(64 * kFewWaves), 0, s, a, rope, in, p.out, p.scale, part, weights,
+                c.slots, c.split_rows, c.splits);
+  }
   if (c.splits > 1)
-    UOCR_LAUNCH("chunk_join", k_chunk_join, dim3((unsigned)((p.tokens * p.heads + 3) / 4)), dim3(256), 0, s, a, p.out,
-                part, weights, c.rows_log2, c.split_rows);
+    UOCR_LAUNCH("chunk_join", k_chunk_join, by_pair, dim3(256), 0, s, a, p.out, part, weights, c.rows_log2,
+                c.split_rows);
   return hipGetLastError();
 }
 

@@ -836,6 +836,9 @@ static int paged_chunk_call(const char* op, float* out, const float* q, const fl
   if (!aligned16(out) || !aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(kv_blocks) ||
       in_stride % 4)
     return fail(err, errlen, "%s: q, k_new, v_new, out and kv_blocks must be 16-byte aligned", op);
+  if (!aligned16(cos_table) || !aligned16(sin_table))
+    return fail(err, errlen, "%s: the cos/sin tables must be 16-byte aligned", op);
+  if (in_stride >= (int64_t)1 << 25) return fail(err, errlen, "%s: input rows must be less than 2^25 floats apart", op);
   const size_t row = (size_t)(heads * head_dim) * sizeof(float);
   const size_t in_bytes = (size_t)(tokens - 1) * in_stride * sizeof(float) + row;
   for (const float* in : {q, k_new, v_new})

@@ -527,13 +527,18 @@ def paged_chunk_attention(q, k_new, v_new, *, kv: PagedChunk, layer_idx: int, sc
                          f"{tuple(views[1].shape)}")
     tokens, heads, head_dim = q.shape
     stride = q.stride(0)
-    if any(t.stride(0) != stride or t.data_ptr() % 16 for t in (q, *views)) or stride % 4 or stride < heads * head_dim:
+    if any(t.stride(0) != stride or t.data_ptr() % 16 for t in (q, *views)) or stride % 4 or \
+            not heads * head_dim <= stride < _CHUNK_STRIDE:
         q, views = _packed(q), [_packed(t) for t in views]
         stride = heads * head_dim
     k, v = views
     return _chunk_call(op, "uocr_paged_chunk_attention", (q.data_ptr(), k.data_ptr(), v.data_ptr(), tokens, heads,
                                                           head_dim, stride),
                        tokens, heads, head_dim, kv, layer_idx, scale, out, workspace, q, [q, k, v])
+
+
+#: Input rows must be fewer floats apart than this (rows further apart are packed).
+_CHUNK_STRIDE = 1 << 25
 
 
 def _packed(t: torch.Tensor) -> torch.Tensor:
@@ -554,12 +559,13 @@ def paged_chunk_attention_qkv(qkv, positions, cos_table, sin_table, *, heads: in
     tokens, width = qkv.shape
     if heads < 1 or width % (3 * heads):
         raise ValueError(f"{op}: qkv width {width} is not 3 x {heads} heads")
-    if qkv.stride(1) != 1 or qkv.stride(0) < width or qkv.stride(0) % 4 or qkv.data_ptr() % 16:
+    if qkv.stride(1) != 1 or not width <= qkv.stride(0) < _CHUNK_STRIDE or qkv.stride(0) % 4 or qkv.data_ptr() % 16:
         qkv = _packed(qkv)
     head_dim = width // (3 * heads)
     positions = _gpu(op, "positions", positions, torch.int32, 1)
     cos_table = _gpu(op, "cos_table", cos_table, torch.float32, 2)
     sin_table = _gpu(op, "sin_table", sin_table, torch.float32, 2)
+    cos_table, sin_table = _packed(cos_table), _packed(sin_table)
     if positions.shape[0] != tokens or cos_table.shape != sin_table.shape:
         raise ValueError(f"{op}: positions or the cos/sin tables do not fit {tokens} tokens")
     return _chunk_call(op, "uocr_paged_chunk_attention_qkv",
