@@ -107,7 +107,8 @@ def test_table_operators_refuse_bad_tables() -> None:
     assert resize(lookup_out=2 * FAKE + 44) == overlapping
     assert resize(lookup_out=FAKE + 32) == overlapping
     assert resize(ws=8) == op + "workspace must be 16-byte aligned"
-    assert resize(ws=16, ws_bytes=35) == op + "workspace of 35 bytes is smaller than the 36 needed"
+    assert resize(pages=20000, lookup_out=4 * FAKE, lookup=4 * FAKE, ws=16, ws_bytes=79999) == \
+        op + "workspace of 79999 bytes is smaller than the 80000 needed"
 
     def fork(pool=5 * FAKE, count=2, lists=3 * FAKE, missing=4 * FAKE, ws=16, ws_bytes=0):
         return _err("uocr_fork_pages", pool, 9, 2, 128, 10, 128, FAKE, FAKE, 2 * FAKE, 2 * FAKE, 3, 4, lists, lists, lists,
@@ -129,7 +130,8 @@ def test_workspace_sizes_of_bad_shapes_are_zero() -> None:
     assert lib.uocr_paged_chunk_workspace_bytes(4, 1, 10, 0) == 0
     assert lib.uocr_fork_pages_workspace_bytes(9, 3, 0, 2) == 0
     assert lib.uocr_resize_pages_workspace_bytes(0) == 0
-    assert lib.uocr_resize_pages_workspace_bytes(9) == 36
+    assert lib.uocr_resize_pages_workspace_bytes(9) == 0  # in LDS
+    assert lib.uocr_resize_pages_workspace_bytes(20000) == 80000
     assert lib.uocr_compact_pages_workspace_bytes(-1) == 0
 
 

@@ -9,8 +9,10 @@
 //
 // The table kernels are one workgroup each: a fork, a resize and a compaction are scans
 // over the counts and the table in a fixed order, so that which page an entry gets does
-// not depend on timing.  What they decide to copy goes, as (source, destination, rows)
+// not depend on timing.  Each output may be its input.  What they decide to copy goes, as (source, destination, rows)
 // triples, to a second launch over the whole device.
+#include <algorithm>
+
 #include "uocr_device.h"
 #include "uocr_kernels.h"
 
@@ -20,223 +22,356 @@ namespace {
 
 constexpr int kTableThreads = 1024;
 constexpr int kTableWaves = kTableThreads / kWave;
+constexpr int kPer = 16;                     // elements of a thread at a time: their loads are under way together
+constexpr int kRound = kPer * kTableThreads;
 constexpr int kCopyThreads = 256;
 constexpr int kSegment = 4 * kCopyThreads;  // float4s of one plane that a workgroup copies at a time
 
-// The rank of this thread among the workgroup's threads whose flag is set, and their number.
-__device__ __forceinline__ int block_rank(bool flag, int* totals, int& all) {
-  const uint64_t set = __ballot(flag);
-  if (lane_id() == 0) totals[threadIdx.x / kWave] = __popcll(set);
-  __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kTableWaves; ++w) {
-    before += w < (int)threadIdx.x / kWave ? totals[w] : 0;
-    all += totals[w];
-  }
-  __syncthreads();
-  return before + lanes_below(set);
+// Up to these sizes counts, lists and the rest of a table kernel's state are in LDS (145 KB of 160), else in memory.
+constexpr int kLdsPages = kRound, kLdsRows = 4096;
+
+// n / d of 0 <= n < 2^31 and 1 <= d < 2^31: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), m d - 2^(31+s) is
+// below d <= 2^s, so n m / 2^(31+s) is less than 1 / d above n / d.
+struct Divide {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t)(uint32_t)n * m >> shift); }
+};
+Divide divide_by(int d) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return {(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
 }
 
-// Counts change by atomics, which act past the CU's L1: they are read the same way.
+// f(u, e) for this thread's elements e < n of the round that starts at e0.
+template <typename F>
+__device__ __forceinline__ void each(int64_t e0, int64_t n, F f) {
+#pragma unroll
+  for (int u = 0; u < kPer; ++u)
+    if (e0 + u * kTableThreads < n) {
+      const int64_t e = e0 + u * kTableThreads + threadIdx.x;
+      if (e < n) f(u, (int)e);
+    }
+}
+
+// Of every element of a round whose flag (bit u) is set, how many before it are (in element order), and their number.
+__device__ __forceinline__ void ranks(uint32_t flags, int (&rank)[kPer], int* totals, int& all) {
+  const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  uint64_t set[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    set[u] = __ballot(flags >> u & 1);
+    if (lane_id() == 0) totals[u * kTableWaves + w] = __popcll(set[u]);
+  }
+  __syncthreads();
+  // element order is that of the totals: lane l sums those of 4l .. 4l+3
+  const int4 t = *(const int4*)(totals + 4 * lane_id());
+  const int sum = t.x + t.y + t.z + t.w, upto = wave_scan_i(sum);
+  const int at = upto - sum + (w % 4 > 0 ? t.x : 0) + (w % 4 > 1 ? t.y : 0) + (w % 4 > 2 ? t.z : 0);
+  all = __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+  for (int u = 0; u < kPer; ++u)
+    rank[u] = __builtin_amdgcn_readlane(at, u * kTableWaves / 4 + w / 4) + lanes_below(set[u]);
+  __syncthreads();
+}
+static_assert(kPer * kTableWaves == 4 * kWave, "a lane sums four totals");
+
+// Counts in memory change by atomics, which act past the CU's L1: they are read the same way.
+template <bool kLds>
 __device__ __forceinline__ int32_t count_of(int32_t* c) {
+  if constexpr (kLds) return *c;
   return __hip_atomic_load(c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+template <bool kLds>
 __device__ __forceinline__ void set_count(int32_t* c, int32_t v) {
-  __hip_atomic_store(c, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if constexpr (kLds)
+    *c = v;
+  else
+    __hip_atomic_store(c, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+template <bool kLds>
 __device__ __forceinline__ void release(int32_t* c) {  // never below zero
-  int32_t old = count_of(c);
-  while (old > 0 && !__hip_atomic_compare_exchange_strong(c, &old, old - 1, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                                          __HIP_MEMORY_SCOPE_AGENT)) {
+  constexpr int kScope = kLds ? __HIP_MEMORY_SCOPE_WORKGROUP : __HIP_MEMORY_SCOPE_AGENT;
+  int32_t old = __hip_atomic_load(c, __ATOMIC_RELAXED, kScope);
+  while (old > 0 && !__hip_atomic_compare_exchange_strong(c, &old, old - 1, __ATOMIC_RELAXED, __ATOMIC_RELAXED, kScope)) {
+  }
+}
+
+// The call's counts to where they are worked on (in memory: counts_out, which may hold them already).
+template <bool kLds>
+__device__ __forceinline__ void load_counts(const PageTables& t, int pages, int32_t* counts) {
+  if (!kLds && counts == t.counts) return;
+  for (int64_t p0 = 0; p0 < pages; p0 += kRound) {
+    int32_t v[kPer];
+    each(p0, pages, [&](int u, int p) { v[u] = ldg(t.counts + p); });
+    each(p0, pages, [&](int u, int p) { set_count<kLds>(counts + p, v[u]); });
   }
 }
 
 // The free pages in ascending order into `list`; returns their number (to every thread).
+template <bool kLds>
 __device__ __forceinline__ int list_free(int32_t* counts, int null, int32_t* list, int* totals) {
   int found = 0;
-  for (int p0 = 0; p0 < null; p0 += kTableThreads) {
-    const int p = p0 + (int)threadIdx.x;
-    const bool free = p < null && count_of(counts + p) <= 0;
-    int all;
-    const int rank = block_rank(free, totals, all);
-    if (free) list[found + rank] = p;
+  for (int64_t p0 = 0; p0 < null; p0 += kRound) {
+    uint32_t free = 0;
+    each(p0, null, [&](int u, int p) { free |= (uint32_t)(count_of<kLds>(counts + p) <= 0) << u; });
+    int rank[kPer], all;
+    ranks(free, rank, totals, all);
+    each(p0, null, [&](int u, int p) {
+      if (free >> u & 1) list[found + rank[u]] = p;
+    });
     found += all;
   }
+  __syncthreads();
   return found;
 }
 
-__device__ __forceinline__ int pages_for(int32_t rows, int P, int cols) {
-  return rows <= 0 ? 0 : min((rows - 1) / P + 1, cols);
+__device__ __forceinline__ int pages_for(int32_t rows, const Divide& by_page, int cols) {
+  return rows <= 0 ? 0 : min(by_page(rows - 1) + 1, cols);
 }
 
 // Every request gets exactly the pages of its length: entries past them are released,
 // then missing ones are taken, in (request, column) order, from the free pages in
 // ascending order (the released ones among them).
-__global__ void __launch_bounds__(kTableThreads) k_resize(PageTables t, int pages, int P,
+//
+// One scan over the counts and one over the entries, of 16384 elements each at a time; what bounds it is latency: a
+// trip to memory for the counts, lengths and entries together, and one for the results.  256 requests of 32 pages in a
+// pool of 6001: RESIZE_FIG.
+template <bool kLds>
+__global__ void __launch_bounds__(kTableThreads) k_resize(PageTables t, int pages, Divide by_page, Divide by_cols,
                                                           const int32_t* __restrict__ lengths, int32_t* missing,
-                                                          int32_t* list) {
-  __shared__ int totals[kTableWaves];
-  const int null = pages - 1, tid = (int)threadIdx.x;
+                                                          int32_t* list_mem) {
+  __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
+  __shared__ int32_t lds_counts[kLds ? kLdsPages : 1], lds_list[kLds ? kLdsPages : 1], lds_need[kLdsRows];
+  int32_t* counts = kLds ? lds_counts : t.counts_out;
+  int32_t* list = kLds ? lds_list : list_mem;
+  const int null = pages - 1;
   const int64_t entries = (int64_t)t.requests * t.cols;
-  if (t.counts_out != t.counts)
-    for (int p = tid; p < pages; p += kTableThreads) set_count(t.counts_out + p, t.counts[p]);
+  const bool once = entries <= kRound;
+  uint32_t old[kPer];
+  if (once) each(0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
+  const bool listed = t.requests <= kLdsRows;
+  if (listed)
+    for (int n = (int)threadIdx.x; n < t.requests; n += kTableThreads)
+      lds_need[n] = pages_for(ldg(lengths + n), by_page, t.cols);
+  load_counts<kLds>(t, pages, counts);
   __syncthreads();
-  for (int64_t e = tid; e < entries; e += kTableThreads) {
-    const uint32_t page = t.lookup[e];
-    const bool set = page < (uint32_t)null;
-    const bool need = (int)(e % t.cols) < pages_for(lengths[e / t.cols], P, t.cols);
-    if (set && !need) release(t.counts_out + page);
-    t.lookup_out[e] = set && need ? page : (uint32_t)null;
+  // whether an entry lies below its request's length
+  auto needed = [&](int e) {
+    const int n = by_cols(e);
+    return e - n * t.cols < (listed ? lds_need[n] : pages_for(ldg(lengths + n), by_page, t.cols));
+  };
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound) {
+    if (!once) each(e0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
+    each(e0, entries, [&](int u, int e) {
+      if (old[u] < (uint32_t)null && !needed(e)) release<kLds>(counts + old[u]);
+    });
   }
   __syncthreads();
-  const int free = list_free(t.counts_out, null, list, totals);
-  __syncthreads();
+  const int free = list_free<kLds>(counts, null, list, totals);
   int taken = 0;
-  for (int64_t e0 = 0; e0 < entries; e0 += kTableThreads) {
-    const int64_t e = e0 + tid;
-    // this thread wrote the entry above
-    const bool want = e < entries && t.lookup_out[e] == (uint32_t)null &&
-                      (int)(e % t.cols) < pages_for(lengths[e / t.cols], P, t.cols);
-    int all;
-    const int rank = taken + block_rank(want, totals, all);
-    if (want && rank < free) {
-      t.lookup_out[e] = (uint32_t)list[rank];
-      set_count(t.counts_out + list[rank], 1);
-    }
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound) {
+    if (!once) each(e0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
+    uint32_t want = 0;
+    each(e0, entries, [&](int u, int e) {
+      const bool need = needed(e), set = old[u] < (uint32_t)null;
+      want |= (uint32_t)(need && !set) << u;
+      if (!need || !set) old[u] = (uint32_t)null;
+    });
+    int rank[kPer], all;
+    ranks(want, rank, totals, all);
+    each(e0, entries, [&](int u, int e) {
+      const int r = taken + rank[u];
+      if ((want >> u & 1) && r < free) {
+        old[u] = (uint32_t)list[r];
+        set_count<kLds>(counts + old[u], 1);
+      }
+      t.lookup_out[e] = old[u];
+    });
     taken += all;
   }
-  if (tid == 0) missing[0] = max(0, taken - free);
+  if (threadIdx.x == 0) missing[0] = max(0, taken - free);
+  if constexpr (kLds) {
+    __syncthreads();
+    each(0, pages, [&](int, int p) { t.counts_out[p] = counts[p]; });
+  }
 }
 
 struct ForkScratch {
   int32_t* moves;   // [0]: pages to copy
+  int32_t* plan;    // [3 * count * cols]: source, destination, rows
+  int32_t* fresh;   // [count * cols]: the children's new entries
   int32_t* winner;  // [requests]: the last pair whose child the row is
   int32_t* list;    // [pages]: the free pages
-  int32_t* fresh;   // [count * cols]: the children's new entries
-  int32_t* plan;    // [3 * count * cols]: source, destination, rows
 };
-
-__device__ __forceinline__ bool fork_pair(const PageTables& t, const ForkScratch& w, const int32_t* parents,
-                                          const int32_t* children, int c, int& parent, int& child) {
-  parent = parents[c];
-  child = children[c];
-  return (uint32_t)parent < (uint32_t)t.requests && (uint32_t)child < (uint32_t)t.requests && parent != child &&
-         w.winner[child] == c;
-}
 
 // Each child's row becomes its parent's, as the table was before the call: pages wholly
 // below shared_rows are shared, the others up to the length are copied to pages that were
 // free before the call, in (pair, column) order from the lowest; then the child's old
-// pages are released.
-__global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages, int P,
+// pages are released.  Bound by latency, as k_resize is.
+template <bool kLds>
+__global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages, int P, Divide by_page, Divide by_cols,
                                                         const int32_t* __restrict__ parents,
                                                         const int32_t* __restrict__ children,
                                                         const int32_t* __restrict__ lengths,
                                                         const int32_t* __restrict__ shared_rows, int count,
                                                         int32_t* missing, ForkScratch w) {
-  __shared__ int totals[kTableWaves];
+  __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
+  __shared__ int32_t lds_counts[kLds ? kLdsPages : 1], lds_list[kLds ? kLdsPages : 1], lds_winner[kLds ? kLdsRows : 1];
+  int32_t* counts = kLds ? lds_counts : t.counts_out;
+  int32_t* list = kLds ? lds_list : w.list;
+  int32_t* winner = kLds ? lds_winner : w.winner;
+  constexpr int kScope = kLds ? __HIP_MEMORY_SCOPE_WORKGROUP : __HIP_MEMORY_SCOPE_AGENT;
   const int null = pages - 1, tid = (int)threadIdx.x;
-  if (t.counts_out != t.counts)
-    for (int p = tid; p < pages; p += kTableThreads) set_count(t.counts_out + p, t.counts[p]);
   if (t.lookup_out != t.lookup)
-    for (int64_t e = tid; e < (int64_t)t.requests * t.cols; e += kTableThreads) t.lookup_out[e] = t.lookup[e];
-  for (int n = tid; n < t.requests; n += kTableThreads) set_count(w.winner + n, -1);
-  __syncthreads();
-  for (int c = tid; c < count; c += kTableThreads)
-    if ((uint32_t)children[c] < (uint32_t)t.requests)
-      __hip_atomic_fetch_max(w.winner + children[c], c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const int free = list_free(t.counts_out, null, w.list, totals);
-  __syncthreads();
-  const int64_t entries = (int64_t)count * t.cols;
-  int taken = 0;
-  for (int64_t e0 = 0; e0 < entries; e0 += kTableThreads) {
-    const int64_t e = e0 + tid;
-    const int c = (int)(min(e, entries - 1) / t.cols), col = (int)(e % t.cols);
-    int parent, child;
-    const bool pair = e < entries && fork_pair(t, w, parents, children, c, parent, child);
-    const uint32_t old = pair ? t.lookup[(int64_t)parent * t.cols + col] : (uint32_t)null;
-    const bool held = old < (uint32_t)null && col < pages_for(lengths[c], P, t.cols);
-    const bool share = held && col < max(shared_rows[c], 0) / P;
-    const bool copy = held && !share;
-    int all;
-    const int rank = taken + block_rank(copy, totals, all);
-    uint32_t page = share ? old : (uint32_t)null;
-    if (copy && rank < free) {
-      page = (uint32_t)w.list[rank];
-      w.plan[3 * (int64_t)rank] = (int32_t)old;
-      w.plan[3 * (int64_t)rank + 1] = (int32_t)page;
-      w.plan[3 * (int64_t)rank + 2] = min(P, lengths[c] - col * P);
-      set_count(t.counts_out + page, 1);
+    for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound) {
+      uint32_t v[kPer];
+      each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { v[u] = ldg(t.lookup + e); });
+      each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { t.lookup_out[e] = v[u]; });
     }
-    if (share) __hip_atomic_fetch_add(t.counts_out + page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (e < entries) w.fresh[e] = (int32_t)page;
+  load_counts<kLds>(t, pages, counts);
+  for (int n = tid; n < t.requests; n += kTableThreads) set_count<kLds>(winner + n, -1);
+  __syncthreads();
+  for (int c = tid; c < count; c += kTableThreads) {
+    const int child = ldg(children + c);
+    if ((uint32_t)child < (uint32_t)t.requests) __hip_atomic_fetch_max(winner + child, c, __ATOMIC_RELAXED, kScope);
+  }
+  const int free = list_free<kLds>(counts, null, list, totals);  // its barriers are the winners' too
+  const int64_t entries = (int64_t)count * t.cols;
+  const bool once = entries <= kRound;
+  auto child_of = [&](int c) {  // the pair's child, or -1 where the pair does not count
+    const int parent = ldg(parents + c), child = ldg(children + c);
+    return (uint32_t)parent < (uint32_t)t.requests && (uint32_t)child < (uint32_t)t.requests && parent != child &&
+                   count_of<kLds>(winner + child) == c
+               ? child
+               : -1;
+  };
+  int32_t page[kPer];
+  int taken = 0;
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound) {
+    uint32_t share = 0, copy = 0;
+    each(e0, entries, [&](int u, int e) {
+      const int c = by_cols(e), col = e - c * t.cols;
+      const uint32_t old = child_of(c) < 0 ? null : ldg(t.lookup + (int64_t)ldg(parents + c) * t.cols + col);
+      const bool held = old < (uint32_t)null && col < pages_for(ldg(lengths + c), by_page, t.cols);
+      const bool whole = col < by_page(max(ldg(shared_rows + c), 0));
+      share |= (uint32_t)(held && whole) << u;
+      copy |= (uint32_t)(held && !whole) << u;
+      page[u] = held ? (int32_t)old : null;
+    });
+    int rank[kPer], all;
+    ranks(copy, rank, totals, all);
+    each(e0, entries, [&](int u, int e) {
+      const int64_t r = taken + rank[u];
+      if (share >> u & 1) __hip_atomic_fetch_add(counts + page[u], 1, __ATOMIC_RELAXED, kScope);
+      if (copy >> u & 1) {
+        const int old = page[u], c = by_cols(e);
+        page[u] = null;
+        if (r < free) {
+          page[u] = list[r];
+          w.plan[3 * r] = old;
+          w.plan[3 * r + 1] = page[u];
+          w.plan[3 * r + 2] = min(P, ldg(lengths + c) - (e - c * t.cols) * P);
+          set_count<kLds>(counts + page[u], 1);
+        }
+      }
+      if (!once) w.fresh[e] = page[u];
+    });
     taken += all;
   }
-  __syncthreads();  // every new entry is counted before an old one is released
+  __syncthreads();  // every new entry is counted, and every row read, before an old one is released
   for (int64_t e = tid; e < entries; e += kTableThreads) {
-    const int c = (int)(e / t.cols), col = (int)(e % t.cols);
-    int parent, child;
-    if (!fork_pair(t, w, parents, children, c, parent, child)) continue;
-    const int64_t at = (int64_t)child * t.cols + col;
-    const uint32_t old = t.lookup[at];  // in place: this thread alone writes the entry
-    if (old < (uint32_t)null) release(t.counts_out + old);
-    t.lookup_out[at] = (uint32_t)w.fresh[e];
+    const int c = by_cols((int)e), child = child_of(c);
+    const uint32_t old = child < 0 ? null : ldg(t.lookup + (int64_t)child * t.cols + (e - c * t.cols));
+    if (old < (uint32_t)null) release<kLds>(counts + old);
   }
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound)
+    each(e0, entries, [&](int u, int e) {  // in place: the entries that this thread read above
+      const int c = by_cols(e), child = child_of(c);
+      int now = page[u];
+      if (!once) now = w.fresh[e];
+      if (child >= 0) t.lookup_out[(int64_t)child * t.cols + (e - c * t.cols)] = (uint32_t)now;
+    });
   if (tid == 0) {
     w.moves[0] = min(taken, free);
     missing[0] = max(0, taken - free);
   }
+  if constexpr (kLds) {
+    __syncthreads();
+    each(0, pages, [&](int, int p) { t.counts_out[p] = counts[p]; });
+  }
 }
 
 // The pages in use move to the front: with L of them, those at or past L go, in ascending
-// order, to the free ones below L in ascending order.
+// order, to the free ones below L in ascending order.  With b(p) the used pages below p,
+// the free page p < L is hole p - b(p), and the used page p >= L goes to hole b(p) - b(L).
+template <bool kLds>
 __global__ void __launch_bounds__(kTableThreads) k_compact(PageTables t, int pages, int P, int32_t* remap,
-                                                           int32_t* moves, int32_t* plan) {
-  __shared__ int totals[kTableWaves];
+                                                           int32_t* moves, int32_t* plan, int32_t* holes_mem) {
+  __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
+  __shared__ int32_t lds_remap[kLds ? kLdsPages : 1], lds_holes[kLds ? kLdsPages / 2 : 1];
+  __shared__ int below_live;
+  int32_t* holes = kLds ? lds_holes : holes_mem;
   const int null = pages - 1, tid = (int)threadIdx.x;
-  int live = 0;
-  for (int p0 = 0; p0 < null; p0 += kTableThreads) {
+  int32_t v[kPer];
+  int rank[kPer], live = 0;
+  uint32_t used = 0;
+  for (int64_t p0 = 0; p0 < null; p0 += kRound) {
+    used = 0;
+    each(p0, null, [&](int u, int p) { v[u] = ldg(t.counts + p); });
+    each(p0, null, [&](int u, int) { used |= (uint32_t)(v[u] > 0) << u; });
     int all;
-    block_rank(p0 + tid < null && t.counts[min(p0 + tid, null)] > 0, totals, all);
+    ranks(used, rank, totals, all);
     live += all;
   }
-  int from = 0, to = 0;
-  for (int p0 = 0; p0 < null; p0 += kTableThreads) {
-    const int p = p0 + tid;
-    const bool used = p < null && t.counts[min(p, null)] > 0;
-    const bool source = used && p >= live, hole = p < null && !used && p < live;
-    int n_from, n_to;
-    const int i = from + block_rank(source, totals, n_from), j = to + block_rank(hole, totals, n_to);
-    if (source) {
-      plan[3 * (int64_t)i] = p;
-      plan[3 * (int64_t)i + 2] = P;
+  int before = 0;
+  for (int64_t p0 = 0; p0 < null; p0 += kRound) {
+    if constexpr (!kLds) {  // else the round above was the only one
+      used = 0;
+      each(p0, null, [&](int u, int p) { v[u] = t.counts[p]; });
+      each(p0, null, [&](int u, int) { used |= (uint32_t)(v[u] > 0) << u; });
+      int all;
+      ranks(used, rank, totals, all);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) rank[u] += before;
+      before += all;
     }
-    if (hole) plan[3 * (int64_t)j + 1] = p;
-    if (p < null) remap[p] = used ? p : -1;
-    if (p < null && t.counts_out != t.counts) t.counts_out[p] = t.counts[p];
-    from += n_from;
-    to += n_to;
+    each(p0, null, [&](int u, int p) {
+      if (p == live) below_live = rank[u];
+      if (p < live && !(used >> u & 1)) holes[p - rank[u]] = p;
+    });
+    __syncthreads();
+    each(p0, null, [&](int u, int p) {
+      const bool in_use = used >> u & 1;
+      int now = in_use ? p : -1;
+      if (in_use && p >= live) {
+        const int64_t i = rank[u] - below_live;
+        now = holes[i];
+        plan[3 * i] = p;
+        plan[3 * i + 1] = now;
+        plan[3 * i + 2] = P;
+        t.counts_out[now] = v[u];
+        t.counts_out[p] = 0;
+      } else if ((in_use || p >= live) && t.counts_out != t.counts) {
+        t.counts_out[p] = v[u];
+      }
+      if constexpr (kLds) lds_remap[p] = now;
+      remap[p] = now;
+    });
   }
   if (tid == 0) {
     remap[null] = null;
     if (t.counts_out != t.counts) t.counts_out[null] = t.counts[null];
-    moves[0] = from;
+    moves[0] = live < null ? live - below_live : 0;
   }
   __syncthreads();
-  for (int i = tid; i < from; i += kTableThreads) {
-    const int src = plan[3 * (int64_t)i], dst = plan[3 * (int64_t)i + 1];
-    const int32_t held = t.counts[src];
-    remap[src] = dst;
-    t.counts_out[dst] = held;
-    t.counts_out[src] = 0;
-  }
-  __syncthreads();
-  for (int64_t e = tid; e < (int64_t)t.requests * t.cols; e += kTableThreads) {
-    const uint32_t page = t.lookup[e];
-    const int32_t now = page < (uint32_t)null ? remap[page] : null;
-    t.lookup_out[e] = (uint32_t)(now < 0 ? null : now);
+  for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound) {
+    uint32_t page[kPer];
+    each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { page[u] = ldg(t.lookup + e); });
+    each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) {
+      const int32_t now = page[u] >= (uint32_t)null ? null : kLds ? lds_remap[page[u]] : remap[page[u]];
+      t.lookup_out[e] = (uint32_t)(now < 0 ? null : now);
+    });
   }
 }
 
@@ -267,20 +402,24 @@ __global__ void __launch_bounds__(kCopyThreads) k_copy_plan(f32x4* pool, int pla
   }
 }
 
-// Copies in the order of the pairs: a thread does its elements of every pair, one pair
-// after the other, so a page may be both written and read.
-__global__ void __launch_bounds__(kCopyThreads) k_copy_pages(f32x4* pool, int pages, int planes, int P, int slot4,
-                                                             const int32_t* src, const int32_t* dst,
-                                                             const int32_t* rows, int count) {
-  const int64_t plane4 = (int64_t)P * slot4, page4 = planes * plane4;
-  const int64_t e = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
-  if (e >= page4) return;
-  const int slot = (int)(e % plane4 / slot4);
-  for (int i = 0; i < count; ++i) {
-    const int a = ldg(src + i), b = ldg(dst + i);
-    if ((uint32_t)a >= (uint32_t)pages || (uint32_t)b >= (uint32_t)pages) continue;
-    if (rows != nullptr && slot >= ldg(rows + i)) continue;
-    pool[b * page4 + e] = pool[a * page4 + e];
+// Copies in the order of the pairs: a thread does its element of every pair, one pair after the other, so a page may be
+// both written and read.  Bound by memory: 24 pages of 12 layers part filled 76.7 us, which is
+// 4.92 TB/s of reads and writes, what a plain copy reaches; one page 5.3 us.  More loads of a thread under way (two to
+// eight elements, or pairs that do not meet) are no faster or slower, 5.0 to 11.6 us
+// for one page, 75.8 to 151 us for 24, 11 to 52 us (here 9.7) for 24 of one layer: the waves of a CU are enough.
+__global__ void __launch_bounds__(kCopyThreads) k_copy_pages(f32x4* pool, int pages, int planes, int64_t plane4,
+                                                             int slot4, const int32_t* __restrict__ src,
+                                                             const int32_t* __restrict__ dst,
+                                                             const int32_t* __restrict__ rows, int count) {
+  const int64_t e = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x, page4 = planes * plane4;
+  for (int plane = (int)blockIdx.y; plane < planes; plane += (int)gridDim.y) {
+    UOCR_GLOBAL f32x4* at = (UOCR_GLOBAL f32x4*)pool + plane * plane4 + e;
+    for (int i = 0; i < count; ++i) {
+      const int a = ldc(src + i), b = ldc(dst + i);
+      if ((uint32_t)a >= (uint32_t)pages || (uint32_t)b >= (uint32_t)pages) continue;
+      const int64_t end = rows == nullptr ? plane4 : min(plane4, (int64_t)ldc(rows + i) * slot4);
+      if (e < end) at[b * page4] = at[a * page4];
+    }
   }
 }
 
@@ -294,51 +433,64 @@ hipError_t launch_plan(const PagePool& p, const int32_t* moves, const int32_t* p
 
 hipError_t launch_copy_pages(const PagePool& p, const int32_t* src, const int32_t* dst, const int32_t* rows,
                              int count, hipStream_t s) {
-  const int64_t page4 = (int64_t)2 * p.layers * p.page_size * (p.slot / 4);
   if (count == 0) return hipSuccess;
-  UOCR_LAUNCH("copy_pages", k_copy_pages, dim3((unsigned)((page4 + kCopyThreads - 1) / kCopyThreads)),
-              dim3(kCopyThreads), 0, s, (f32x4*)p.kv_blocks, p.pages, 2 * p.layers, p.page_size, p.slot / 4, src, dst,
-              rows, count);
+  const int64_t plane4 = (int64_t)p.page_size * (p.slot / 4);
+  const int planes = 2 * p.layers;
+  const dim3 grid((unsigned)((plane4 + kCopyThreads - 1) / kCopyThreads), (unsigned)std::min(planes, 65535));
+  UOCR_LAUNCH("copy_pages", k_copy_pages, grid, dim3(kCopyThreads), 0, s, (f32x4*)p.kv_blocks, p.pages, planes, plane4,
+              p.slot / 4, src, dst, rows, count);
   return hipGetLastError();
 }
 
+namespace {
+bool in_lds(int64_t pages, int64_t requests) { return pages <= kLdsPages && requests <= kLdsRows; }
+}  // namespace
+
 size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count) {
-  return sizeof(int32_t) * (4 + requests + pages + 4 * count * cols);
+  const int64_t entries = count * cols;
+  return sizeof(int32_t) * (4 + 3 * entries + (entries > kRound ? entries : 0) +
+                            (in_lds(pages, requests) ? 0 : requests + pages));
 }
 
 hipError_t launch_fork_pages(const PagePool& p, const PageTables& t, const int32_t* parents, const int32_t* children,
                              const int32_t* lengths, const int32_t* shared_rows, int count, int32_t* missing,
                              void* workspace, hipStream_t s) {
+  const int64_t entries = (int64_t)count * t.cols;
   ForkScratch w{};
   w.moves = (int32_t*)workspace;
-  w.winner = w.moves + 4;
+  w.plan = w.moves + 4;
+  w.fresh = w.plan + 3 * entries;
+  w.winner = w.fresh + (entries > kRound ? entries : 0);
   w.list = w.winner + t.requests;
-  w.fresh = w.list + p.pages;
-  w.plan = w.fresh + (int64_t)count * t.cols;
-  UOCR_LAUNCH("fork_tables", k_fork, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size, parents, children,
-              lengths, shared_rows, count, missing, w);
+  const auto kernel = in_lds(p.pages, t.requests) ? k_fork<true> : k_fork<false>;
+  UOCR_LAUNCH("fork_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size,
+              divide_by(p.page_size), divide_by(t.cols), parents, children, lengths, shared_rows, count, missing, w);
   if (count == 0) return hipGetLastError();
   return launch_plan(p, w.moves, w.plan, s);
 }
 
-size_t resize_workspace_bytes(int64_t pages) { return sizeof(int32_t) * pages; }
+size_t resize_workspace_bytes(int64_t pages) { return in_lds(pages, 0) ? 0 : sizeof(int32_t) * pages; }
 
 hipError_t launch_resize_pages(const PagePool& p, const PageTables& t, const int32_t* lengths, int32_t* missing,
                                void* workspace, hipStream_t s) {
-  UOCR_LAUNCH("resize_tables", k_resize, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size, lengths, missing,
-              (int32_t*)workspace);
+  const auto kernel = in_lds(p.pages, 0) ? k_resize<true> : k_resize<false>;
+  UOCR_LAUNCH("resize_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, divide_by(p.page_size),
+              divide_by(t.cols), lengths, missing, (int32_t*)workspace);
   return hipGetLastError();
 }
 
 // At most half of the pages move.
-size_t compact_workspace_bytes(int64_t pages) { return sizeof(int32_t) * (4 + 3 * (pages / 2 + 1)); }
+size_t compact_workspace_bytes(int64_t pages) {
+  return sizeof(int32_t) * (4 + (in_lds(pages, 0) ? 3 : 4) * (pages / 2 + 1));
+}
 
 hipError_t launch_compact_pages(const PagePool& p, const PageTables& t, int32_t* remap, void* workspace,
                                 hipStream_t s) {
   int32_t* moves = (int32_t*)workspace;
   int32_t* plan = moves + 4;
-  UOCR_LAUNCH("compact_tables", k_compact, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size, remap, moves,
-              plan);
+  const auto kernel = in_lds(p.pages, 0) ? k_compact<true> : k_compact<false>;
+  UOCR_LAUNCH("compact_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size, remap, moves,
+              plan, plan + 3 * ((int64_t)p.pages / 2 + 1));
   return launch_plan(p, moves, plan, s);
 }
 

@@ -223,7 +223,7 @@ def rms_norm(x, gamma, eps: float, *, residual=None, out: torch.Tensor | None = 
 
 def _rows_view(op: str, name: str, t, like=None) -> torch.Tensor:
     """A ``[rows, heads, D]`` fp32 GPU view whose heads and elements are packed (rows may be strided)."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 3 or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 3 or not t.is_cuda:
         raise ValueError(f"{op}: {name} must be an fp32 [rows, heads, head_dim] GPU tensor")
     if t.stride(2) != 1 or t.stride(1) != t.shape[2]:
         t = t.contiguous()
@@ -454,6 +454,12 @@ def _pool(op: str, blocks) -> torch.Tensor:
     return blocks
 
 
+def _ids(op: str, name: str, t: torch.Tensor, rank: int) -> torch.Tensor:
+    """An int32 or uint32 GPU tensor, as it is."""
+    return _gpu(op, name, t, torch.uint32 if isinstance(t, torch.Tensor) and t.dtype == torch.uint32 else torch.int32,
+                rank)
+
+
 def _workspace(op: str, t: torch.Tensor | None, nbytes: int, like: torch.Tensor) -> torch.Tensor | None:
     """The caller's workspace, or one from torch's allocator (stream-ordered; a captured graph's own)."""
     if t is None:
@@ -474,7 +480,7 @@ def _on_device(op: str, name: str, *args, tensors) -> None:
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{op}: the tensors are on different devices")
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
@@ -487,8 +493,8 @@ def _chunk_call(op: str, name: str, inputs: tuple, tokens: int, heads: int, head
     pages, _, layers, page_size, bh, bd = blocks.shape
     if (bh, bd) != (heads, head_dim):
         raise ValueError(f"{op}: kv_blocks {tuple(blocks.shape)} does not hold {heads} heads of {head_dim}")
-    lookup = _u32(op, "lookup_table", kv.lookup_table, 2)
-    cached = _u32(op, "cache_lengths", kv.cache_lengths, 1)
+    lookup = _ids(op, "lookup_table", kv.lookup_table, 2)
+    cached = _ids(op, "cache_lengths", kv.cache_lengths, 1)
     offsets = _gpu(op, "chunk_offsets", kv.chunk_offsets, torch.int32, 1)
     requests = lookup.shape[0]
     if cached.shape[0] != requests or offsets.shape[0] != requests + 1:
@@ -594,16 +600,20 @@ def copy_pages(kv_blocks, src, dst, *, rows=None) -> torch.Tensor:
 
 
 def _tables(op: str, ref_counts, lookup_table, out_ref_counts, out_lookup) -> tuple:
-    """The page tables and their outputs: (counts, lookup, counts out, lookup out, the caller's lookup out)."""
+    """The page tables and their outputs: (counts, lookup, counts out, lookup out)."""
     counts = _gpu(op, "ref_counts", ref_counts, torch.int32, 1)
-    lookup = _u32(op, "lookup_table", lookup_table, 2)
-    out_ref_counts = torch.empty_like(counts) if out_ref_counts is None else \
+    lookup = _ids(op, "lookup_table", lookup_table, 2)
+    if out_ref_counts is None:
+        out_ref_counts = torch.empty_like(counts)
+    else:
         _out(op, "out_ref_counts", out_ref_counts, torch.int32, 1)
     if out_lookup is None:
-        out_lookup = torch.empty(lookup.shape, dtype=lookup_table.dtype, device=lookup.device)
+        out_lookup = torch.empty_like(lookup)
+    else:
+        _ids(op, "out_lookup", out_lookup, 2)
     if out_ref_counts.shape != counts.shape or out_lookup.shape != lookup.shape or not out_lookup.is_contiguous():
         raise ValueError(f"{op}: out_ref_counts and out_lookup must be contiguous and shaped as their inputs")
-    return counts, lookup, out_ref_counts, _u32(op, "out_lookup", out_lookup, 2), out_lookup
+    return counts, lookup, out_ref_counts, out_lookup
 
 
 def fork_pages(kv_blocks, ref_counts, lookup_table, parents, children, lengths, shared_rows, *,
@@ -624,7 +634,7 @@ def fork_pages(kv_blocks, ref_counts, lookup_table, parents, children, lengths, 
     op = "fork_pages"
     blocks = _pool(op, kv_blocks)
     pages, _, layers, page_size, heads, head_dim = blocks.shape
-    counts, lookup, new_counts, new_lookup, result = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
+    counts, lookup, new_counts, new_lookup = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
     if counts.shape[0] != pages:
         raise ValueError(f"{op}: ref_counts is for {counts.shape[0]} pages, the pool has {pages}")
     lists = [_gpu(op, name, t, torch.int32, 1) for name, t in
@@ -634,12 +644,12 @@ def fork_pages(kv_blocks, ref_counts, lookup_table, parents, children, lengths, 
         raise ValueError(f"{op}: parents, children, lengths and shared_rows must have one length")
     requests, cols = lookup.shape
     ws = _workspace(op, workspace, _lib.load().uocr_fork_pages_workspace_bytes(pages, requests, cols, n), blocks)
-    missing = torch.empty(1, dtype=torch.int32, device=blocks.device)
+    missing = counts.new_empty(1)
     _on_device(op, "uocr_fork_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim,
                new_counts.data_ptr(), counts.data_ptr(), new_lookup.data_ptr(), lookup.data_ptr(), requests, cols,
                *(t.data_ptr() for t in lists), n, missing.data_ptr(), _ptr(ws), _nbytes(ws),
                tensors=[blocks, counts, lookup, new_counts, new_lookup, *lists, ws])
-    return result, new_counts, missing
+    return new_lookup, new_counts, missing
 
 
 def resize_pages(ref_counts, lookup_table, lengths, *, page_size: int, out_ref_counts: torch.Tensor | None = None,
@@ -649,18 +659,18 @@ def resize_pages(ref_counts, lookup_table, lengths, *, page_size: int, out_ref_c
     are released, then unset ones below are taken from the lowest free page up, in (request, column) order, the
     pages just released among the free ones.  Tables and result as for :func:`fork_pages`; no page's rows move."""
     op = "resize_pages"
-    counts, lookup, new_counts, new_lookup, result = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
+    counts, lookup, new_counts, new_lookup = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
     lengths = _gpu(op, "lengths", lengths, torch.int32, 1)
     requests, cols = lookup.shape
     if lengths.shape[0] != requests:
         raise ValueError(f"{op}: {lengths.shape[0]} lengths for {requests} requests")
     pages = counts.shape[0]
     ws = _workspace(op, workspace, _lib.load().uocr_resize_pages_workspace_bytes(pages), counts)
-    missing = torch.empty(1, dtype=torch.int32, device=counts.device)
+    missing = counts.new_empty(1)
     _on_device(op, "uocr_resize_pages", new_counts.data_ptr(), counts.data_ptr(), pages, int(page_size),
                new_lookup.data_ptr(), lookup.data_ptr(), requests, cols, lengths.data_ptr(), missing.data_ptr(),
                _ptr(ws), _nbytes(ws), tensors=[counts, lookup, new_counts, new_lookup, lengths, ws])
-    return result, new_counts, missing
+    return new_lookup, new_counts, missing
 
 
 def compact_pages(kv_blocks, ref_counts, lookup_table, *, out_ref_counts: torch.Tensor | None = None,
@@ -673,17 +683,17 @@ def compact_pages(kv_blocks, ref_counts, lookup_table, *, out_ref_counts: torch.
     op = "compact_pages"
     blocks = _pool(op, kv_blocks)
     pages, _, layers, page_size, heads, head_dim = blocks.shape
-    counts, lookup, new_counts, new_lookup, result = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
+    counts, lookup, new_counts, new_lookup = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
     if counts.shape[0] != pages:
         raise ValueError(f"{op}: ref_counts is for {counts.shape[0]} pages, the pool has {pages}")
     requests, cols = lookup.shape
     ws = _workspace(op, workspace, _lib.load().uocr_compact_pages_workspace_bytes(pages), blocks)
-    remap = torch.empty(pages, dtype=torch.int32, device=blocks.device)
+    remap = torch.empty_like(counts)
     _on_device(op, "uocr_compact_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim,
                new_counts.data_ptr(), counts.data_ptr(), new_lookup.data_ptr(), lookup.data_ptr(), requests, cols,
                remap.data_ptr(), _ptr(ws), _nbytes(ws),
                tensors=[blocks, counts, lookup, new_counts, new_lookup, ws])
-    return result, new_counts, remap
+    return new_lookup, new_counts, remap
 
 
 _OPS = {
