@@ -30,7 +30,7 @@ def rows_behind(monkeypatch):
     plain, qkv = u.paged_chunk_attention, u.paged_chunk_attention_qkv
 
     def behind(kv):
-        return 128 * max(8, len(kv.cache_lengths))
+        return max(128 * max(8, len(kv.cache_lengths)), 2 ** 19 // max(8, kv.attend_max) + 1)
 
     def call(run, q, heads, head_dim, kv, out):
         wide = torch.empty(q.shape[0], heads, head_dim, device=q.device) if out is None else out.clone()

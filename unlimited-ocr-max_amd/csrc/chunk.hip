@@ -528,39 +528,83 @@ __device__ __forceinline__ void apart_weights(Queries& w, f32x16& s, const int* 
 
 // ------------------------------------------------------------------ tiles of queries
 
-// The query tiles of all chunks.  Of up to 64 requests they are numbered one after the other: a lane per request, and a
-// sum over the lanes.  Of more, without a sum: tile j of request n is slot floor(off[n] / rows) + n + j, which no other
-// tile is, with slots left out.  (Those in between, where every request fills its last tile: every other workgroup
-// is empty, the others meet on half of the shader engines, and 8 chunks of 256 over 1000 rows took 138 us for 78.)
+// The pieces of a call: a tile of 2^rows_log2 queries of one request with one split of its rows and one head.  Of up to
+// 64 requests they are dealt one after the other, the longest first (a lane per request counts its pieces); else by
+// tile, where tile j of request n is slot floor(off[n] / rows) + n + j, which no other tile is, with slots and splits
+// left out.  Workgroups go round the XCDs: neighbours walk the same rows, and stay on one XCD, whose L2 then serves all
+// but the first.  Those without a piece are best dealt last: left between the others, 8 chunks of 256 over 1000 rows
+// took 138 us for 78 (every other workgroup was empty, and the others met on half of the shader engines), and two of
+// 1024 in splits of 256 took 84 us for 60 (some CUs had two pieces, others none).
 struct QueryTile : Chunk {
   int t0;  // the tile's first token
 };
-__device__ __forceinline__ bool query_tile(const ChunkArgs& a, int rows_log2, int slot, QueryTile& q) {
-  int64_t j;
-  if (a.requests <= 64) {
-    const int i = min(lane_id(), a.requests - 1);
-    const int off = ldg(a.offsets + i), next = min(ldg(a.offsets + i + 1), a.tokens);
-    const uint32_t cached = min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
-    const bool some = lane_id() < a.requests && off >= 0 && off < next;
-    const int tiles = some ? ((next - off - 1) >> rows_log2) + 1 : 0, behind = wave_scan_i(tiles);
-    const int at = __popcll(__ballot(behind <= slot));  // the first whose tiles reach past the slot
-    if (at >= a.requests) return false;
-    q.n = at;
-    q.first = __builtin_amdgcn_readlane(off, at);
-    q.end = __builtin_amdgcn_readlane(next, at);
-    q.cached = __builtin_amdgcn_readlane((int)cached, at);
-    j = slot - (__builtin_amdgcn_readlane(behind, at) - __builtin_amdgcn_readlane(tiles, at));
-  } else {
-    (Chunk&)q = find_chunk(a, rows_log2, true, slot);
-    j = (int64_t)slot - ((int64_t)(q.first >> rows_log2) + q.n);
-  }
-  const int64_t t0 = (int64_t)q.first + (j << rows_log2);
-  q.t0 = (int)t0;
-  return q.first >= 0 && j >= 0 && t0 < q.end;
-}
 // Rows that token t of the request attends.
 __device__ __forceinline__ int rows_of(const ChunkArgs& a, const QueryTile& q, int t) {
   return (int)min((int64_t)q.cached + (t - q.first) + 1, (int64_t)a.attend_max);
+}
+struct Cuts {
+  int rows_log2, slots, split_rows, splits;
+  Divide by_split, by_slots, by_splits;
+};
+struct Piece : QueryTile {
+  int head, split, t_last;  // t_last: the tile's last token
+};
+__device__ __forceinline__ bool find_piece(const ChunkArgs& a, const Cuts& c, Piece& q) {
+  const int turn = (int)(blockIdx.x / 8), xcd = (int)(blockIdx.x % 8), rows = 1 << c.rows_log2;
+  int j;
+  if (a.requests <= 64) {
+    const int i = min(lane_id(), a.requests - 1);
+    const int off = ldg(a.offsets + i), next = min(ldg(a.offsets + i + 1), a.tokens);
+    const int cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
+    const bool some = lane_id() < a.requests && off >= 0 && off < next;
+    const int tiles = some ? ((next - off - 1) >> c.rows_log2) + 1 : 0;
+    // splits of tile j: those of its last token's rows
+    const auto cuts = [&](int cached, int length, int j) {
+      const int64_t rows = (int64_t)cached + min((j + 1) << c.rows_log2, length);
+      return c.by_split((int)min(rows, (int64_t)a.attend_max) - 1) + 1;
+    };
+    int pieces = tiles;
+    if (c.splits > 1) {
+      pieces = 0;
+      for (int k = 0; __ballot(k < tiles) != 0; ++k)
+        if (k < tiles) pieces += cuts(cached, next - off, k);
+    }
+    const int upto = wave_scan_i(pieces), total = __builtin_amdgcn_readlane(upto, 63);
+    const int per = (total * a.heads + 7) / 8, item = xcd * per + turn;
+    if (turn >= per || item >= total * a.heads) return false;
+    q.head = item / total;
+    int left = item - q.head * total;
+    const int at = __popcll(__ballot(upto <= left));  // the request whose pieces reach past it
+    left -= __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(pieces, at);
+    q.n = at;
+    q.first = __builtin_amdgcn_readlane(off, at);
+    q.end = __builtin_amdgcn_readlane(next, at);
+    q.cached = (uint32_t)__builtin_amdgcn_readlane(cached, at);
+    j = __builtin_amdgcn_readlane(tiles, at) - 1;
+    if (c.splits > 1) {
+      for (; j > 0; --j) {
+        const int here = cuts((int)q.cached, q.end - q.first, j);
+        if (left < here) break;
+        left -= here;
+      }
+      q.split = left;
+    } else {
+      q.split = 0;
+      j -= left;
+    }
+  } else {
+    const int item = xcd * (int)(gridDim.x / 8) + turn;
+    if (item >= c.slots * a.heads * c.splits) return false;
+    const int by_tile = c.by_slots(item), slot = c.slots - 1 - (item - by_tile * c.slots);
+    q.head = c.by_splits(by_tile);
+    q.split = by_tile - q.head * c.splits;
+    (Chunk&)q = find_chunk(a, c.rows_log2, true, slot);
+    j = slot - ((q.first >> c.rows_log2) + q.n);
+    if (q.first < 0 || j < 0 || (int64_t)j << c.rows_log2 >= q.end - q.first) return false;
+  }
+  q.t0 = q.first + (j << c.rows_log2);
+  q.t_last = min(q.t0 + rows, q.end) - 1;
+  return true;
 }
 
 // Results of one wave: into out, or, where the rows of the tile are split, normalised into part with
@@ -892,18 +936,14 @@ __device__ __forceinline__ void attend_walk(Queries& w, int begin, int end, bool
 }
 
 __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3)
-    k_chunk_tiles(ChunkArgs a, const float* q, int64_t q_stride, float* out, float scale, float* part, float* weights, int slots,
-                  int split_rows, int splits) {
+    k_chunk_tiles(ChunkArgs a, const float* q, int64_t q_stride, float* out, float scale, float* part, float* weights,
+                  Cuts cuts) {
   __shared__ __align__(16) _Float16 lds[kLdsHalves];
   __shared__ __align__(16) Shared sh;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-  // neighbours in `item` walk the same rows: they go to one XCD, whose L2 then serves all but the first
-  const int per = (int)(gridDim.x / 8), item = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-  if (item >= slots * a.heads * splits) return;
-  const int slot = slots - 1 - item % slots, head = item / slots % a.heads, split = item / slots / a.heads;
-  QueryTile qt;
-  if (!query_tile(a, kTileLog2, slot, qt)) return;
-  const int t_last = min(qt.t0 + 32 * kTileWaves, qt.end) - 1;
+  Piece qt;
+  if (!find_piece(a, cuts, qt)) return;
+  const int head = qt.head, split = qt.split, t_last = qt.t_last, split_rows = cuts.split_rows;
   const int all_rows = rows_of(a, qt, t_last);
   const int begin = split * split_rows, end = min(begin + split_rows, all_rows);
   const int shown = rows_of(a, qt, qt.t0);  // rows past these are hidden from some query
@@ -978,19 +1018,16 @@ __device__ __forceinline__ int few_scale(float m, int& unit, bool& finite, bool&
 }
 
 __global__ void __launch_bounds__(64 * kFewWaves, 2)
-    k_chunk_few(ChunkArgs a, Rope rope, Inputs in, float* out, float scale, float* part, float* weights, int slots,
-                int split_rows, int splits) {
+    k_chunk_few(ChunkArgs a, Rope rope, Inputs in, float* out, float scale, float* part, float* weights,
+                Cuts cuts) {
   __shared__ __align__(16) float sums[kFewWaves][32 * kD];  // the waves' sums, before that their slow paths' stash,
   _Float16* const qs = (_Float16*)sums;             // and first the queries' operands, [part][step][lane][8]
   __shared__ float peak[kFewWaves][32], total[kFewWaves][32];
   __shared__ int q_exp[32];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = lane >> 5;
-  const int per = (int)(gridDim.x / 8), item = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-  if (item >= slots * a.heads * splits) return;
-  const int slot = slots - 1 - item % slots, head = item / slots % a.heads, split = item / slots / a.heads;
-  QueryTile qt;
-  if (!query_tile(a, kFewLog2, slot, qt)) return;
-  const int t_last = min(qt.t0 + 32, qt.end) - 1;
+  Piece qt;
+  if (!find_piece(a, cuts, qt)) return;
+  const int head = qt.head, split = qt.split, t_last = qt.t_last, split_rows = cuts.split_rows;
   const int all_rows = rows_of(a, qt, t_last);
   const int begin = split * split_rows, end = min(begin + split_rows, all_rows);
   if (split == 0)  // new rows that none attends
@@ -1331,29 +1368,40 @@ __global__ void __launch_bounds__(256) k_chunk_join(ChunkArgs a, float* out, con
 
 // How a call's rows are cut: tiles of 256 or of 32 queries, and splits of their rows where the tiles alone do not fill
 // the device.  A tile of 256 has a CU to itself and converts each row once for all its queries, but a short chunk
-// leaves most of it empty, and few tiles leave most CUs without one; tiles of 32 convert and read each row eight times
-// as often.  Measured, 10 heads, tiles of 256 / tiles of 32, in us: one request of 256 tokens 37 / 27, of 512 54 / 47,
-// of 1024 87 / 111, of 2048 110 / 229; of 256 tokens over 2000 cached rows 88 / 48, of 512 95 / 82, of 256 over 14000
-// 167 / 131, of 512 over 14000 144 / 259; four requests of 256 43 / 38, of 512 62 / 76; eight of 32 tokens over 1000
-// rows 66 / 42, of 128 79 / 72, of 256 108 / 122; eight of 64 24 / 20, of 256 50 / 58, of 512 75 / 129.
+// leaves most of it empty, and it has more to set up; tiles of 32 convert and read each row eight times as often.
+// Measured, 10 heads, tiles of 256 / tiles of 32, in us: one request of 256 tokens 33 / 24, of 512 41 / 30, of 1024
+// 50 / 69; of 256 tokens over 2000 cached rows 45 / 41, of 512 51 / 68, of 32 over 14000 48 / 42, of 64 52 / 55, of 128
+// 59 / 80, of 512 206 / 240; four of 128 tokens 24 / 19, of 512 57 / 69; eight of 32 over 1000 rows 35 / 28, of 64
+// 39 / 43, of 128 49 / 68; 64 of 33 over 300 81 / 72, of 64 107 / 90; 100 of 7 over 500 124 / 94.
+//
+// More splits than fill the device once make some CUs take two pieces while others wait: two requests of 1024 in
+// splits of 256 rows 60 us, of 1024 rows 86.  Tiles of 32 go two to a CU, and share it: 256, 384 and 512 pieces, eight
+// requests of 7 over 1150 rows 27 / 25 / 28 us, of 32 over 1000 33 / 28 / 28, one of 8 over 14000 37 / 39 / 40.
 namespace {
 constexpr int kCus = 256;
-struct Cut {
+struct Cut : Cuts {
   bool few;
-  int rows_log2, slots, split_rows, splits;
 };
 Cut cut_of(int64_t tokens, int64_t requests, int heads, int attend_max) {
   Cut c{};
-  c.few = requests > 0 && (tokens / requests < 128 || (tokens < 1024 && tokens * attend_max < (int64_t)1 << 22));
+  c.few = requests > 0 && (tokens / requests <= 64 || tokens * attend_max < 1 << 19);
   c.rows_log2 = c.few ? kFewLog2 : kTileLog2;
   const int64_t rows = (int64_t)1 << c.rows_log2;
-  c.slots = (int)(tokens / rows + requests);
-  // about as many tiles as there are: of each request's last one half is queries
-  const int64_t tiles = std::max(requests, (tokens + rows - 1) / rows + (requests - 1) / 2);
-  const int64_t fill = std::max<int64_t>(1, (c.few ? 2 * kCus : kCus) / std::max<int64_t>(1, tiles * heads));
-  const int64_t least = c.few ? 4 * kBlock : 1024, most = c.few ? kFewSplitRows : kMaxSplitRows;
-  c.split_rows = (int)std::min(most, std::max(least, (attend_max / fill + 127) / 128 * 128));
+  c.slots = (int)(requests > 64 ? tokens / rows + requests
+                                : tokens < requests ? tokens : (tokens - requests) / rows + requests);
+  // Of about so many tiles (half of a request's last one is queries) each attends on average the part f of attend_max,
+  // and has one split at least: tiles (1 - f + f splits) pieces.
+  const double tiles = (double)std::max(requests, (tokens + rows - 1) / rows + (requests - 1) / 2) * heads;
+  const double f = 1.0 - 0.5 * std::min(1.0, (double)tokens / ((double)std::max<int64_t>(1, requests) * attend_max));
+  const int64_t splits = std::max(1, (int)(((c.few ? kCus * 3 / 2 : kCus) / std::max(1.0, tiles) - (1.0 - f)) / f));
+  const int64_t least = c.few ? 4 * kBlock : 256, most = c.few ? kFewSplitRows : kMaxSplitRows;
+  c.split_rows = (int)std::min(most, std::max(least, ((attend_max + splits - 1) / splits + 127) / 128 * 128));
+  // two splits of 128 rows and their join take the time of one of 256, and a launch more
+  if (c.few && attend_max <= 2 * least) c.split_rows = (int)(2 * least);
   c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
+  c.by_split = divide_by(c.split_rows);
+  c.by_slots = divide_by(std::max(1, c.slots));
+  c.by_splits = divide_by(c.splits);
   return c;
 }
 }  // namespace
@@ -1396,10 +1444,10 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
     const bool rotated_q = p.positions != nullptr;  // they wait in out
     UOCR_LAUNCH("chunk_tiles", k_chunk_tiles, grid, dim3(64 * (kTileWaves + kStageWaves)), 0, s, a,
                 rotated_q ? p.out : p.q, rotated_q ? (int64_t)p.heads * kD : p.in_stride, p.out, p.scale, part, weights,
-                c.slots, c.split_rows, c.splits);
+                c);
   } else {
     UOCR_LAUNCH("chunk_few", k_chunk_few, grid, dim3(64 * kFewWaves), 0, s, a, rope, in, p.out, p.scale, part, weights,
-                c.slots, c.split_rows, c.splits);
+                c);
   }
   if (c.splits > 1)
     UOCR_LAUNCH("chunk_join", k_chunk_join, by_pair, dim3(256), 0, s, a, p.out, part, weights, c.rows_log2,

@@ -30,19 +30,6 @@ constexpr int kSegment = 4 * kCopyThreads;  // float4s of one plane that a workg
 // Up to these sizes counts, lists and the rest of a table kernel's state are in LDS (145 KB of 160), else in memory.
 constexpr int kLdsPages = kRound, kLdsRows = 4096;
 
-// n / d of 0 <= n < 2^31 and 1 <= d < 2^31: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), m d - 2^(31+s) is
-// below d <= 2^s, so n m / 2^(31+s) is less than 1 / d above n / d.
-struct Divide {
-  uint32_t m;
-  int shift;
-  __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t)(uint32_t)n * m >> shift); }
-};
-Divide divide_by(int d) {
-  int s = 0;
-  while (((int64_t)1 << s) < d) ++s;
-  return {(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
-}
-
 // f(u, e) for this thread's elements e < n of the round that starts at e0.
 template <typename F>
 __device__ __forceinline__ void each(int64_t e0, int64_t n, F f) {

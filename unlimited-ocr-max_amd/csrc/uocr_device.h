@@ -299,6 +299,19 @@ __device__ __forceinline__ int lanes_below(uint64_t m) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
 }
 
+// n / d of 0 <= n < 2^31 and 1 <= d < 2^31: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), m d - 2^(31+s) is
+// below d <= 2^s, so n m / 2^(31+s) is less than 1 / d above n / d.
+struct Divide {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t)(uint32_t)n * m >> shift); }
+};
+inline Divide divide_by(int d) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return {(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
+}
+
 __device__ __forceinline__ int clamp_expert(int32_t key, int E) {
   int e = key;
   e = e < 0 ? 0 : e;
