@@ -183,7 +183,8 @@ def test_copies_happen_in_order(src, dst) -> None:
 
 @pytest.mark.parametrize(("seed", "requests", "cols", "pages"), [
     (1, 1, 1, 2), (2, 1, 5, 9), (3, 7, 3, 40), (4, 64, 6, 200), (5, 200, 17, 3000), (6, 40, 40, 1100), (7, 5, 4, 1),
-    (8, 3000, 2, 4000), (9, 5000, 1, 6000), (10, 300, 60, 16384), (11, 90, 190, 16385), (12, 4100, 5, 21000)])
+    (8, 3000, 2, 4000), (9, 5000, 1, 6000), (10, 300, 60, 16384), (11, 90, 190, 16385), (12, 4100, 5, 21000),
+    (13, 128, 16, 2048), (14, 683, 3, 2048), (15, 50, 30, 2049)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_resize(seed, requests, cols, pages, in_place) -> None:
     u = _uocr()
@@ -260,7 +261,7 @@ def test_fork(seed, in_place) -> None:
 
 
 @pytest.mark.parametrize(("requests", "cols", "pages"), [
-    (4096, 2, 9000), (4097, 2, 9000), (70, 300, 16384), (60, 250, 16385), (90, 400, 30000)])
+    (4096, 2, 9000), (4097, 2, 9000), (70, 300, 16384), (60, 250, 16385), (90, 400, 30000), (64, 32, 2048), (65, 32, 2048)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_fork_of_many(requests, cols, pages, in_place) -> None:
     r = random.Random(requests + cols)
@@ -310,7 +311,8 @@ def _check_compact(pool, counts, table, in_place=False):
 
 @pytest.mark.parametrize(("seed", "requests", "cols", "pages"), [
     (1, 1, 1, 2), (2, 3, 2, 9), (3, 8, 5, 100), (4, 60, 4, 1025), (5, 60, 20, 2600), (6, 2, 3, 5000), (7, 1, 1, 1), (8, 40, 400, 16384),
-    (9, 500, 34, 16385), (10, 7, 5000, 40000)])
+    (9, 500, 34, 16385), (10, 7, 5000, 40000),
+    (11, 256, 8, 2048), (12, 64, 32, 2049)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_compact(seed, requests, cols, pages, in_place) -> None:
     table, counts = _scene(seed, requests, cols, pages)

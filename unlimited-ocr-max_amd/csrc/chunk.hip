@@ -1319,49 +1319,67 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
         sum == 0.0f ? -kInf : m + __builtin_amdgcn_logf(sum);
 }
 
-// Joins the splits of a token's rows: one wave per (token, head), two columns a lane.  The splits
-// hold normalised sums, so a split weighs what its weights sum to.
+// Joins the splits of a token's rows: a wave for four heads of a token, four columns a lane, half a wave a head.  The
+// splits hold normalised sums, so a split weighs what its weights sum to.  Bound by the trips to memory (metadata, then
+// the splits) for few tokens, JOIN_FEW; by the splits' bytes for many, JOIN_MANY.
+constexpr int kJoinHeads = 4;
 __global__ void __launch_bounds__(256) k_chunk_join(ChunkArgs a, float* out, const float* __restrict__ part,
-                                                    const float* __restrict__ weights, int rows_log2, int split_rows) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-  if (th >= (int64_t)a.tokens * a.heads) return;
-  const int t = (int)(th / a.heads), lane = lane_id();
+                                                    const float* __restrict__ weights, int rows_log2, Divide by_split) {
+  const int groups = (a.heads + kJoinHeads - 1) / kJoinHeads;
+  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int64_t t = w / groups;
+  if (t >= a.tokens) return;
   QueryTile q;
-  if (!chunk_of(a, t, q)) return;
-  const int t_last = min(q.first + ((((t - q.first) >> rows_log2) + 1) << rows_log2), q.end) - 1;  // of its tile
-  const int splits = (rows_of(a, q, t_last) + split_rows - 1) / split_rows;
+  if (!chunk_of(a, (int)t, q)) return;
+  const int t_last = min(q.first + (((((int)t - q.first) >> rows_log2) + 1) << rows_log2), q.end) - 1;  // of its tile
+  const int splits = by_split(rows_of(a, q, t_last) - 1) + 1;
   if (splits == 1) return;  // written by its tile
+  const int lane = lane_id(), h0 = (int)(w - t * groups) * kJoinHeads + lane / 32;
   const int64_t stride = (int64_t)a.tokens * a.heads;
-  float m = -kInf, l = 0.0f;
-  f32x2 o = {0.0f, 0.0f};
-  constexpr int kAtOnce = 8;  // splits read together
-  for (int s0 = 0; s0 < splits; s0 += kAtOnce) {
-    float ws[kAtOnce], mn = m;
-    f32x2 p[kAtOnce];
+  constexpr int kTwo = kJoinHeads / 2, kAtOnce = 4;  // heads of a lane, splits read together
+  float m[kTwo], l[kTwo];
+  f32x4 o[kTwo];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int64_t at = (int64_t)min(s0 + j, splits - 1) * stride + th;
-      ws[j] = ldc(weights + at);
-      p[j] = *(const UOCR_GLOBAL f32x2*)(part + at * kD + 2 * lane);
-    }
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) mn = fmaxf(mn, ws[j]);
-    if (mn == -kInf) mn = 0.0f;
-    const float keep = __builtin_amdgcn_exp2f(m - mn);
-    l *= keep;
-    o *= keep;
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      if (s0 + j >= splits || ws[j] == -kInf) continue;  // a split without a weight has no sum
-      const float f = __builtin_amdgcn_exp2f(ws[j] - mn);
-      l += f;
-      o.x = __builtin_fmaf(f, p[j].x, o.x);
-      o.y = __builtin_fmaf(f, p[j].y, o.y);
-    }
-    m = mn;
+  for (int u = 0; u < kTwo; ++u) {
+    m[u] = -kInf;
+    l[u] = 0.0f;
+    o[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  *(UOCR_GLOBAL f32x2*)(out + th * kD + 2 * lane) = o / l;
+  for (int s0 = 0; s0 < splits; s0 += kAtOnce) {
+    float ws[kTwo][kAtOnce];
+    f32x4 p[kTwo][kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kTwo; ++u)
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int64_t at = min(s0 + j, splits - 1) * stride + t * a.heads + min(h0 + 2 * u, a.heads - 1);
+        ws[u][j] = ldg(weights + at);
+        p[u][j] = *(const UOCR_GLOBAL f32x4*)(part + at * kD + 4 * (lane & 31));
+      }
+#pragma unroll
+    for (int u = 0; u < kTwo; ++u) {
+      float mn = m[u];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) mn = fmaxf(mn, ws[u][j]);
+      if (mn == -kInf) mn = 0.0f;
+      const float keep = __builtin_amdgcn_exp2f(m[u] - mn);
+      l[u] *= keep;
+      o[u] *= keep;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (s0 + j >= splits || ws[u][j] == -kInf) continue;  // a split without a weight has no sum
+        const float f = __builtin_amdgcn_exp2f(ws[u][j] - mn);
+        l[u] += f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[u][e] = __builtin_fmaf(f, p[u][j][e], o[u][e]);
+      }
+      m[u] = mn;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kTwo; ++u)
+    if (h0 + 2 * u < a.heads)
+      *(UOCR_GLOBAL f32x4*)(out + (t * a.heads + h0 + 2 * u) * kD + 4 * (lane & 31)) = o[u] / l[u];
 }
 
 }  // namespace
@@ -1435,6 +1453,7 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
   const Rope rope{p.positions, p.cos_table, p.sin_table, p.table_rows};
   const Cut c = cut_of(p.tokens, p.requests, p.heads, p.attend_max);
   const int64_t pairs = p.tokens * p.heads, items = (int64_t)c.slots * p.heads * c.splits;
+  const int64_t joins = p.tokens * ((p.heads + kJoinHeads - 1) / kJoinHeads);
   const dim3 by_pair((unsigned)((pairs + 3) / 4)), grid((unsigned)((items + 7) / 8 * 8));
   const Inputs in{p.q, p.k_new, p.v_new};
   float* part = (float*)p.workspace;
@@ -1450,8 +1469,8 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
                 c);
   }
   if (c.splits > 1)
-    UOCR_LAUNCH("chunk_join", k_chunk_join, by_pair, dim3(256), 0, s, a, p.out, part, weights, c.rows_log2,
-                c.split_rows);
+    UOCR_LAUNCH("chunk_join", k_chunk_join, dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, s, a, p.out, part, weights,
+                c.rows_log2, c.by_split);
   return hipGetLastError();
 }
 
