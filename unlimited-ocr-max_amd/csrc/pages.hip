@@ -22,19 +22,19 @@ namespace {
 
 constexpr int kTableThreads = 1024;
 constexpr int kTableWaves = kTableThreads / kWave;
-// Elements of a thread at a time (kPer), whose loads are under way together: few in small tables, where the code of the
-// others costs more than it does (a resize of 8 requests in 81 pages: 2 SMALL_FIG, 16 9.8 us).
-constexpr int kFew = 2, kMany = 16;
-template <int kPer>
+// Elements of a thread at a time, whose loads are under way together.  Few: each kernel's code is fetched cold, and more
+// of it costs more than more rounds do.  A resize of 8 requests in 81 pages / of 256 of 32 pages in 6001, in us: 2
+// 3.6 / 11.2, 4 4.1 / 10.8, 16 9.8 / 15.1.
+constexpr int kPer = 2;
 constexpr int kRound = kPer * kTableThreads;
 constexpr int kCopyThreads = 256;
 constexpr int kSegment = 4 * kCopyThreads;  // float4s of one plane that a workgroup copies at a time
 
 // Up to these sizes counts, lists and the rest of a table kernel's state are in LDS (145 KB of 160), else in memory.
-constexpr int kLdsPages = kRound<kMany>, kLdsRows = 4096;
+constexpr int kLdsPages = 16384, kLdsRows = 4096;
 
 // f(u, e) for this thread's elements e < n of the round that starts at e0.
-template <int kPer, typename F>
+template <typename F>
 __device__ __forceinline__ void each(int64_t e0, int64_t n, F f) {
 #pragma unroll
   for (int u = 0; u < kPer; ++u)
@@ -44,11 +44,10 @@ __device__ __forceinline__ void each(int64_t e0, int64_t n, F f) {
     }
 }
 
+static_assert(kPer * kTableWaves <= kWave, "a lane has a total");
+
 // Of every element of a round whose flag (bit u) is set, how many before it are (in element order), and their number.
-template <int kPer>
 __device__ __forceinline__ void ranks(uint32_t flags, int (&rank)[kPer], int* totals, int& all) {
-  constexpr int kMine = kPer * kTableWaves > kWave ? kPer * kTableWaves / kWave : 1;  // totals of a lane
-  static_assert(kMine == 1 || kMine == 4, "a lane reads its totals at once");
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), lane = lane_id();
   uint64_t set[kPer];
 #pragma unroll
@@ -58,21 +57,11 @@ __device__ __forceinline__ void ranks(uint32_t flags, int (&rank)[kPer], int* to
   }
   __syncthreads();
   // element order is that of the totals
-  int at, upto;
-  if constexpr (kMine == 4) {
-    const int4 t = *(const int4*)(totals + 4 * lane);
-    const int sum = t.x + t.y + t.z + t.w;
-    upto = wave_scan_i(sum);
-    at = upto - sum + (w % 4 > 0 ? t.x : 0) + (w % 4 > 1 ? t.y : 0) + (w % 4 > 2 ? t.z : 0);
-  } else {
-    const int t = lane < kPer * kTableWaves ? totals[lane] : 0;
-    upto = wave_scan_i(t);
-    at = upto - t;
-  }
+  const int mine = lane < kPer * kTableWaves ? totals[lane] : 0, upto = wave_scan_i(mine);
   all = __builtin_amdgcn_readlane(upto, 63);
 #pragma unroll
   for (int u = 0; u < kPer; ++u)
-    rank[u] = __builtin_amdgcn_readlane(at, (u * kTableWaves + w) / kMine) + lanes_below(set[u]);
+    rank[u] = __builtin_amdgcn_readlane(upto - mine, u * kTableWaves + w) + lanes_below(set[u]);
   __syncthreads();
 }
 
@@ -98,26 +87,26 @@ __device__ __forceinline__ void release(int32_t* c) {  // never below zero
 }
 
 // The call's counts to where they are worked on (in memory: counts_out, which may hold them already).
-template <int kPer, bool kLds>
+template <bool kLds>
 __device__ __forceinline__ void load_counts(const PageTables& t, int pages, int32_t* counts) {
   if (!kLds && counts == t.counts) return;
-  for (int64_t p0 = 0; p0 < pages; p0 += kRound<kPer>) {
+  for (int64_t p0 = 0; p0 < pages; p0 += kRound) {
     int32_t v[kPer];
-    each<kPer>(p0, pages, [&](int u, int p) { v[u] = ldg(t.counts + p); });
-    each<kPer>(p0, pages, [&](int u, int p) { set_count<kLds>(counts + p, v[u]); });
+    each(p0, pages, [&](int u, int p) { v[u] = ldg(t.counts + p); });
+    each(p0, pages, [&](int u, int p) { set_count<kLds>(counts + p, v[u]); });
   }
 }
 
 // The free pages in ascending order into `list`; returns their number (to every thread).
-template <int kPer, bool kLds>
+template <bool kLds>
 __device__ __forceinline__ int list_free(int32_t* counts, int null, int32_t* list, int* totals) {
   int found = 0;
-  for (int64_t p0 = 0; p0 < null; p0 += kRound<kPer>) {
+  for (int64_t p0 = 0; p0 < null; p0 += kRound) {
     uint32_t free = 0;
-    each<kPer>(p0, null, [&](int u, int p) { free |= (uint32_t)(count_of<kLds>(counts + p) <= 0) << u; });
+    each(p0, null, [&](int u, int p) { free |= (uint32_t)(count_of<kLds>(counts + p) <= 0) << u; });
     int rank[kPer], all;
     ranks(free, rank, totals, all);
-    each<kPer>(p0, null, [&](int u, int p) {
+    each(p0, null, [&](int u, int p) {
       if (free >> u & 1) list[found + rank[u]] = p;
     });
     found += all;
@@ -136,51 +125,51 @@ __device__ __forceinline__ int pages_for(int32_t rows, const Divide& by_page, in
 //
 // One scan over the counts and one over the entries, of 16384 elements each at a time; what bounds it is latency: a
 // trip to memory for the counts, lengths and entries together, and one for the results.  256 requests of 32 pages in a
-// pool of 6001: RESIZE_FIG.
-template <int kPer, bool kLds>
+// pool of 6001: 11.2 us on the device, of 8 requests in 81 pages 3.6.
+template <bool kLds>
 __global__ void __launch_bounds__(kTableThreads) k_resize(PageTables t, int pages, Divide by_page, Divide by_cols,
                                                           const int32_t* __restrict__ lengths, int32_t* missing,
                                                           int32_t* list_mem) {
   __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
-  __shared__ int32_t lds_counts[kLds ? kRound<kPer> : 1], lds_list[kLds ? kRound<kPer> : 1], lds_need[kLdsRows];
+  __shared__ int32_t lds_counts[kLds ? kLdsPages : 1], lds_list[kLds ? kLdsPages : 1], lds_need[kLdsRows];
   int32_t* counts = kLds ? lds_counts : t.counts_out;
   int32_t* list = kLds ? lds_list : list_mem;
   const int null = pages - 1;
   const int64_t entries = (int64_t)t.requests * t.cols;
-  const bool once = entries <= kRound<kPer>;
+  const bool once = entries <= kRound;
   uint32_t old[kPer];
-  if (once) each<kPer>(0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
+  if (once) each(0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
   const bool listed = t.requests <= kLdsRows;
   if (listed)
     for (int n = (int)threadIdx.x; n < t.requests; n += kTableThreads)
       lds_need[n] = pages_for(ldg(lengths + n), by_page, t.cols);
-  load_counts<kPer, kLds>(t, pages, counts);
+  load_counts<kLds>(t, pages, counts);
   __syncthreads();
   // whether an entry lies below its request's length
   auto needed = [&](int e) {
     const int n = by_cols(e);
     return e - n * t.cols < (listed ? lds_need[n] : pages_for(ldg(lengths + n), by_page, t.cols));
   };
-  for (int64_t e0 = 0; e0 < entries; e0 += kRound<kPer>) {
-    if (!once) each<kPer>(e0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
-    each<kPer>(e0, entries, [&](int u, int e) {
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound) {
+    if (!once) each(e0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
+    each(e0, entries, [&](int u, int e) {
       if (old[u] < (uint32_t)null && !needed(e)) release<kLds>(counts + old[u]);
     });
   }
   __syncthreads();
-  const int free = list_free<kPer, kLds>(counts, null, list, totals);
+  const int free = list_free<kLds>(counts, null, list, totals);
   int taken = 0;
-  for (int64_t e0 = 0; e0 < entries; e0 += kRound<kPer>) {
-    if (!once) each<kPer>(e0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound) {
+    if (!once) each(e0, entries, [&](int u, int e) { old[u] = ldg(t.lookup + e); });
     uint32_t want = 0;
-    each<kPer>(e0, entries, [&](int u, int e) {
+    each(e0, entries, [&](int u, int e) {
       const bool need = needed(e), set = old[u] < (uint32_t)null;
       want |= (uint32_t)(need && !set) << u;
       if (!need || !set) old[u] = (uint32_t)null;
     });
     int rank[kPer], all;
     ranks(want, rank, totals, all);
-    each<kPer>(e0, entries, [&](int u, int e) {
+    each(e0, entries, [&](int u, int e) {
       const int r = taken + rank[u];
       if ((want >> u & 1) && r < free) {
         old[u] = (uint32_t)list[r];
@@ -193,7 +182,7 @@ __global__ void __launch_bounds__(kTableThreads) k_resize(PageTables t, int page
   if (threadIdx.x == 0) missing[0] = max(0, taken - free);
   if constexpr (kLds) {
     __syncthreads();
-    each<kPer>(0, pages, [&](int, int p) { t.counts_out[p] = counts[p]; });
+    for (int p = (int)threadIdx.x; p < pages; p += kTableThreads) t.counts_out[p] = counts[p];
   }
 }
 
@@ -209,7 +198,7 @@ struct ForkScratch {
 // below shared_rows are shared, the others up to the length are copied to pages that were
 // free before the call, in (pair, column) order from the lowest; then the child's old
 // pages are released.  Bound by latency, as k_resize is.
-template <int kPer, bool kLds>
+template <bool kLds>
 __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages, int P, Divide by_page, Divide by_cols,
                                                         const int32_t* __restrict__ parents,
                                                         const int32_t* __restrict__ children,
@@ -217,28 +206,28 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
                                                         const int32_t* __restrict__ shared_rows, int count,
                                                         int32_t* missing, ForkScratch w) {
   __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
-  __shared__ int32_t lds_counts[kLds ? kRound<kPer> : 1], lds_list[kLds ? kRound<kPer> : 1], lds_winner[kLds ? kLdsRows : 1];
+  __shared__ int32_t lds_counts[kLds ? kLdsPages : 1], lds_list[kLds ? kLdsPages : 1], lds_winner[kLds ? kLdsRows : 1];
   int32_t* counts = kLds ? lds_counts : t.counts_out;
   int32_t* list = kLds ? lds_list : w.list;
   int32_t* winner = kLds ? lds_winner : w.winner;
   constexpr int kScope = kLds ? __HIP_MEMORY_SCOPE_WORKGROUP : __HIP_MEMORY_SCOPE_AGENT;
   const int null = pages - 1, tid = (int)threadIdx.x;
   if (t.lookup_out != t.lookup)
-    for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound<kPer>) {
+    for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound) {
       uint32_t v[kPer];
-      each<kPer>(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { v[u] = ldg(t.lookup + e); });
-      each<kPer>(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { t.lookup_out[e] = v[u]; });
+      each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { v[u] = ldg(t.lookup + e); });
+      each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { t.lookup_out[e] = v[u]; });
     }
-  load_counts<kPer, kLds>(t, pages, counts);
+  load_counts<kLds>(t, pages, counts);
   for (int n = tid; n < t.requests; n += kTableThreads) set_count<kLds>(winner + n, -1);
   __syncthreads();
   for (int c = tid; c < count; c += kTableThreads) {
     const int child = ldg(children + c);
     if ((uint32_t)child < (uint32_t)t.requests) __hip_atomic_fetch_max(winner + child, c, __ATOMIC_RELAXED, kScope);
   }
-  const int free = list_free<kPer, kLds>(counts, null, list, totals);  // its barriers are the winners' too
+  const int free = list_free<kLds>(counts, null, list, totals);  // its barriers are the winners' too
   const int64_t entries = (int64_t)count * t.cols;
-  const bool once = entries <= kRound<kPer>;
+  const bool once = entries <= kRound;
   auto child_of = [&](int c) {  // the pair's child, or -1 where the pair does not count
     const int parent = ldg(parents + c), child = ldg(children + c);
     return (uint32_t)parent < (uint32_t)t.requests && (uint32_t)child < (uint32_t)t.requests && parent != child &&
@@ -248,9 +237,9 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
   };
   int32_t page[kPer];
   int taken = 0;
-  for (int64_t e0 = 0; e0 < entries; e0 += kRound<kPer>) {
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound) {
     uint32_t share = 0, copy = 0;
-    each<kPer>(e0, entries, [&](int u, int e) {
+    each(e0, entries, [&](int u, int e) {
       const int c = by_cols(e), col = e - c * t.cols;
       const uint32_t old = child_of(c) < 0 ? null : ldg(t.lookup + (int64_t)ldg(parents + c) * t.cols + col);
       const bool held = old < (uint32_t)null && col < pages_for(ldg(lengths + c), by_page, t.cols);
@@ -261,7 +250,7 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
     });
     int rank[kPer], all;
     ranks(copy, rank, totals, all);
-    each<kPer>(e0, entries, [&](int u, int e) {
+    each(e0, entries, [&](int u, int e) {
       const int64_t r = taken + rank[u];
       if (share >> u & 1) __hip_atomic_fetch_add(counts + page[u], 1, __ATOMIC_RELAXED, kScope);
       if (copy >> u & 1) {
@@ -285,8 +274,8 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
     const uint32_t old = child < 0 ? null : ldg(t.lookup + (int64_t)child * t.cols + (e - c * t.cols));
     if (old < (uint32_t)null) release<kLds>(counts + old);
   }
-  for (int64_t e0 = 0; e0 < entries; e0 += kRound<kPer>)
-    each<kPer>(e0, entries, [&](int u, int e) {  // in place: the entries that this thread read above
+  for (int64_t e0 = 0; e0 < entries; e0 += kRound)
+    each(e0, entries, [&](int u, int e) {  // in place: the entries that this thread read above
       const int c = by_cols(e), child = child_of(c);
       int now = page[u];
       if (!once) now = w.fresh[e];
@@ -298,50 +287,50 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
   }
   if constexpr (kLds) {
     __syncthreads();
-    each<kPer>(0, pages, [&](int, int p) { t.counts_out[p] = counts[p]; });
+    for (int p = (int)threadIdx.x; p < pages; p += kTableThreads) t.counts_out[p] = counts[p];
   }
 }
 
 // The pages in use move to the front: with L of them, those at or past L go, in ascending
 // order, to the free ones below L in ascending order.  With b(p) the used pages below p,
 // the free page p < L is hole p - b(p), and the used page p >= L goes to hole b(p) - b(L).
-template <int kPer, bool kLds>
+template <bool kLds>
 __global__ void __launch_bounds__(kTableThreads) k_compact(PageTables t, int pages, int P, int32_t* remap,
                                                            int32_t* moves, int32_t* plan, int32_t* holes_mem) {
   __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
-  __shared__ int32_t lds_remap[kLds ? kRound<kPer> : 1], lds_holes[kLds ? kRound<kPer> / 2 : 1];
+  __shared__ int32_t lds_remap[kLds ? kLdsPages : 1], lds_holes[kLds ? kLdsPages / 2 : 1];
   __shared__ int below_live;
   int32_t* holes = kLds ? lds_holes : holes_mem;
   const int null = pages - 1, tid = (int)threadIdx.x;
   int32_t v[kPer];
   int rank[kPer], live = 0;
   uint32_t used = 0;
-  for (int64_t p0 = 0; p0 < null; p0 += kRound<kPer>) {
+  for (int64_t p0 = 0; p0 < null; p0 += kRound) {
     used = 0;
-    each<kPer>(p0, null, [&](int u, int p) { v[u] = ldg(t.counts + p); });
-    each<kPer>(p0, null, [&](int u, int) { used |= (uint32_t)(v[u] > 0) << u; });
+    each(p0, null, [&](int u, int p) { v[u] = ldg(t.counts + p); });
+    each(p0, null, [&](int u, int) { used |= (uint32_t)(v[u] > 0) << u; });
     int all;
     ranks(used, rank, totals, all);
     live += all;
   }
   int before = 0;
-  for (int64_t p0 = 0; p0 < null; p0 += kRound<kPer>) {
-    if constexpr (!kLds) {  // else the round above was the only one
+  for (int64_t p0 = 0; p0 < null; p0 += kRound) {
+    if (null > kRound) {  // else the round above was the only one
       used = 0;
-      each<kPer>(p0, null, [&](int u, int p) { v[u] = t.counts[p]; });
-      each<kPer>(p0, null, [&](int u, int) { used |= (uint32_t)(v[u] > 0) << u; });
+      each(p0, null, [&](int u, int p) { v[u] = t.counts[p]; });
+      each(p0, null, [&](int u, int) { used |= (uint32_t)(v[u] > 0) << u; });
       int all;
       ranks(used, rank, totals, all);
 #pragma unroll
       for (int u = 0; u < kPer; ++u) rank[u] += before;
       before += all;
     }
-    each<kPer>(p0, null, [&](int u, int p) {
+    each(p0, null, [&](int u, int p) {
       if (p == live) below_live = rank[u];
       if (p < live && !(used >> u & 1)) holes[p - rank[u]] = p;
     });
     __syncthreads();
-    each<kPer>(p0, null, [&](int u, int p) {
+    each(p0, null, [&](int u, int p) {
       const bool in_use = used >> u & 1;
       int now = in_use ? p : -1;
       if (in_use && p >= live) {
@@ -365,10 +354,10 @@ __global__ void __launch_bounds__(kTableThreads) k_compact(PageTables t, int pag
     moves[0] = live < null ? live - below_live : 0;
   }
   __syncthreads();
-  for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound<kPer>) {
+  for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound) {
     uint32_t page[kPer];
-    each<kPer>(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { page[u] = ldg(t.lookup + e); });
-    each<kPer>(e0, (int64_t)t.requests * t.cols, [&](int u, int e) {
+    each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { page[u] = ldg(t.lookup + e); });
+    each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) {
       const int32_t now = page[u] >= (uint32_t)null ? null : kLds ? lds_remap[page[u]] : remap[page[u]];
       t.lookup_out[e] = (uint32_t)(now < 0 ? null : now);
     });
@@ -444,14 +433,11 @@ hipError_t launch_copy_pages(const PagePool& p, const int32_t* src, const int32_
 
 namespace {
 bool in_lds(int64_t pages, int64_t requests) { return pages <= kLdsPages && requests <= kLdsRows; }
-bool small(const PagePool& p, const PageTables& t, int64_t rows) {
-  return p.pages <= kRound<kFew> && rows * t.cols <= kRound<kFew>;
-}
 }  // namespace
 
 size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count) {
   const int64_t entries = count * cols;
-  return sizeof(int32_t) * (4 + 3 * entries + (entries > kRound<kFew> ? entries : 0) +
+  return sizeof(int32_t) * (4 + 3 * entries + (entries > kRound ? entries : 0) +
                             (in_lds(pages, requests) ? 0 : requests + pages));
 }
 
@@ -463,10 +449,9 @@ hipError_t launch_fork_pages(const PagePool& p, const PageTables& t, const int32
   w.moves = (int32_t*)workspace;
   w.plan = w.moves + 4;
   w.fresh = w.plan + 3 * entries;
-  w.winner = w.fresh + (entries > kRound<kFew> ? entries : 0);
+  w.winner = w.fresh + (entries > kRound ? entries : 0);
   w.list = w.winner + t.requests;
-  const auto kernel = in_lds(p.pages, t.requests) ? small(p, t, count) ? k_fork<kFew, true> : k_fork<kMany, true>
-                                                  : k_fork<kMany, false>;
+  const auto kernel = in_lds(p.pages, t.requests) ? k_fork<true> : k_fork<false>;
   UOCR_LAUNCH("fork_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size,
               divide_by(p.page_size), divide_by(t.cols), parents, children, lengths, shared_rows, count, missing, w);
   if (count == 0) return hipGetLastError();
@@ -477,8 +462,7 @@ size_t resize_workspace_bytes(int64_t pages) { return in_lds(pages, 0) ? 0 : siz
 
 hipError_t launch_resize_pages(const PagePool& p, const PageTables& t, const int32_t* lengths, int32_t* missing,
                                void* workspace, hipStream_t s) {
-  const auto kernel = in_lds(p.pages, 0) ? small(p, t, t.requests) ? k_resize<kFew, true> : k_resize<kMany, true>
-                                         : k_resize<kMany, false>;
+  const auto kernel = in_lds(p.pages, 0) ? k_resize<true> : k_resize<false>;
   UOCR_LAUNCH("resize_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, divide_by(p.page_size),
               divide_by(t.cols), lengths, missing, (int32_t*)workspace);
   return hipGetLastError();
@@ -493,8 +477,7 @@ hipError_t launch_compact_pages(const PagePool& p, const PageTables& t, int32_t*
                                 hipStream_t s) {
   int32_t* moves = (int32_t*)workspace;
   int32_t* plan = moves + 4;
-  const auto kernel = in_lds(p.pages, 0) ? small(p, t, t.requests) ? k_compact<kFew, true> : k_compact<kMany, true>
-                                         : k_compact<kMany, false>;
+  const auto kernel = in_lds(p.pages, 0) ? k_compact<true> : k_compact<false>;
   UOCR_LAUNCH("compact_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size, remap, moves,
               plan, plan + 3 * ((int64_t)p.pages / 2 + 1));
   return launch_plan(p, moves, plan, s);
