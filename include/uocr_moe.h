@@ -166,7 +166,9 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
  * Rows of out that no chunk holds are left as they were, as is every row of the
  * pool that is no new token's.  Device metadata is clamped as there: a row past what
  * the lookup row addresses is neither stored nor attended, nor is one past attend_max
- * attended.  Two requests may share pages that no chunk writes.  fp32 throughout.
+ * attended.  Two requests may share pages that no chunk writes.  fp32 in and out;
+ * the products are of operands held to 22 bits (pairs of fp16) and summed in fp32, as
+ * are the softmax's maxima and sums.
  * workspace may be NULL (the library's own) or at least
  * uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max) bytes, 16-byte
  * aligned; calls that overlap in time must not share one (nor, with NULL, a stream's

@@ -136,7 +136,7 @@ __device__ __forceinline__ void store_pair(const ChunkArgs& a, const Rope& rope,
   kp[a.kv_stride + 64] = ldg(in.v_new + src + d + 64);
 }
 
-// One wave per (token, head).
+// One wave per (token, head).  Bound by memory: 8 prompts of up to 512 tokens, 100 MB read and written, 18 us.
 __global__ void __launch_bounds__(256) k_chunk_store(ChunkArgs a, Rope rope, Inputs in, float* out) {
   const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   if (th >= (int64_t)a.tokens * a.heads) return;
@@ -631,6 +631,13 @@ __device__ __forceinline__ void store_queries(const Queries& w, const ChunkArgs&
 // k_chunk_tiles: 8 waves of 32 queries each walk the rows together, a block of 32 at a time.  4 more bring the
 // rows, two blocks ahead, turn them into fp16 pairs and write them to LDS as the matrix operands they will
 // be, an operand's 64 lanes side by side.
+//
+// Bound by the matrix instruction and the power it draws: 2048 tokens over 14001 rows, 10 heads, are 158 GFLOP, three
+// times that as fp16 products, in 441 us: 1.07 PFLOP/s, where a large fp16 matrix product reaches 1.13 (and an fp32 one
+// 0.153, which would be 1031 us).  256 queries, since each row is converted once for all of them; the operands, 144 KB,
+// take a CU's LDS.  Waves that convert for themselves, without the four: 538 us; blocks of 64 rows: 716 (spills);
+// conversions between the matrix instructions: 588; both waves of a SIMD in step: 527; the new rows stored and rotated
+// here and not by k_chunk_store: 551, and 8 prompts 83 us for 68.
 constexpr int kTileWaves = 8;   // that attend
 constexpr int kStageWaves = 4;  // that convert: one a SIMD, beside two that attend
 constexpr int kTileLog2 = 8;    // queries of a workgroup
@@ -980,6 +987,11 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3)
 // k_chunk_few: 32 queries a workgroup, whose 4 waves take the rows' blocks in turn, each straight from memory into the
 // operands' lanes (keys: lane (row l % 32, columns 8 i + 4 (l / 32)); values: lane (columns 4 (l % 32) on, rows
 // 16 t + 8 (j / 4) + 4 (l / 32) + j % 4)), and join their sums in LDS.
+//
+// Bound by the trips to memory where there are few rows (metadata; queries, page and positions; rows and tables: 11 us
+// for 4 tokens over 300 rows) and by the rows' bytes where there are many: 8 requests of 7 over 1150 rows, 68 MB, in
+// 19 us, 3.6 TB/s.  No row goes by way of LDS, so two workgroups share a CU, and one's loads are under way while the
+// other multiplies.
 constexpr int kFewWaves = 4;
 constexpr int kFewLog2 = 5;  // queries of a workgroup
 constexpr int kFewSplitRows = kFewWaves * 64 * kBlock;  // a wave notes its slow blocks in 64 bits
@@ -1319,9 +1331,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
         sum == 0.0f ? -kInf : m + __builtin_amdgcn_logf(sum);
 }
 
-// Joins the splits of a token's rows: a wave for four heads of a token, four columns a lane, half a wave a head.  The
+// Joins the splits of a token's rows: a wave takes four heads of a token, four columns a lane, half a wave a head.  The
 // splits hold normalised sums, so a split weighs what its weights sum to.  Bound by the trips to memory (metadata, then
-// the splits) for few tokens, JOIN_FEW; by the splits' bytes for many, JOIN_MANY.
+// the splits): 3 us for 4 tokens, 6.0 us for 8 prompts of up to 512, 8.9 us for 2048 tokens of 3 splits (31 MB).  A wave
+// to each head looked the metadata up ten times as often: 10.3 and 15 us.
 constexpr int kJoinHeads = 4;
 __global__ void __launch_bounds__(256) k_chunk_join(ChunkArgs a, float* out, const float* __restrict__ part,
                                                     const float* __restrict__ weights, int rows_log2, Divide by_split) {
@@ -1455,6 +1468,7 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
   const int64_t pairs = p.tokens * p.heads, items = (int64_t)c.slots * p.heads * c.splits;
   const int64_t joins = p.tokens * ((p.heads + kJoinHeads - 1) / kJoinHeads);
   const dim3 by_pair((unsigned)((pairs + 3) / 4)), grid((unsigned)((items + 7) / 8 * 8));
+  if (items > INT32_MAX - 8) return hipErrorInvalidValue;
   const Inputs in{p.q, p.k_new, p.v_new};
   float* part = (float*)p.workspace;
   float* weights = part + (int64_t)c.splits * pairs * kD;
