@@ -160,7 +160,7 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
  *   [chunk_offsets[n], chunk_offsets[n+1]), which may be empty; cache_lengths uint32
  *   [requests]: its rows c_n in the cache before the chunk; lookup uint32
  *   [requests, lookup_cols] (all device).  kv_blocks as for paged_decode_attention.
- *   attend_max (host): the largest c_n + chunk length.
+ *   attend_max (host): the largest c_n + chunk length.  scale must be finite.
  * Token i of chunk n is logical row c_n + i: its k_new / v_new are stored there, then
  *   out = sum_{r <= c_n + i} softmax_r(scale * q . k_r) v_r.
  * Rows of out that no chunk holds are left as they were, as is every row of the

@@ -450,6 +450,53 @@ def test_repeats_streams_and_graphs_give_the_same_bits(chunks, cached) -> None:
     assert all(_same_bits(out, want) for _, out in graphs)
 
 
+@pytest.mark.parametrize("chunks", [(3, 2), (40, 90)])
+def test_a_graph_replayed_for_other_lengths(chunks) -> None:
+    """A serving loop's graph: captured once for the longest requests, replayed as the lengths, the offsets and the
+    pages change in place."""
+    u = _uocr()
+    s = Setup(37, list(chunks), [600, 300], heads=3)
+    s.attend_max = 700
+    q, k, v = s.qkv.unbind(1)
+    on = [x.to(DEV) for x in (q, k, v)]
+    pool = s.pool.to(DEV)
+    kv = s.kv(pool)
+    run = lambda out: u.paged_chunk_attention(*on, kv=kv, layer_idx=1, scale=SCALE, out=out)  # noqa: E731
+    out = torch.zeros_like(on[0])
+    run(out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        run(out)
+    total = sum(chunks)
+    for lengths, cached in ((chunks, (600, 300)), ((total, 0), (5, 9)), ((1, total - 1), (127, 128)),
+                            ((0, total), (0, 0)), (chunks, (0, 31))):
+        s.chunks, s.cached = list(lengths), list(cached)
+        s.offsets = torch.tensor([0, lengths[0], total], dtype=torch.int32)
+        kv.chunk_offsets.copy_(s.offsets)
+        kv.cache_lengths.copy_(torch.tensor(cached, dtype=torch.int32))
+        null = s.pool.shape[0] - 1
+        s.table = torch.where(s.table < null, (s.table + 1) % null, s.table)
+        kv.lookup_table.copy_(s.table)
+        pool.copy_(s.pool)
+        out.zero_()
+        g.replay()
+        assert _far(out.cpu(), s.want(1, q, k, v)) <= BAR, (lengths, cached)
+        assert _same_bits(pool.cpu(), s.stored(1, k, v)), (lengths, cached)
+        assert _same_bits(run(torch.zeros_like(out)), out), (lengths, cached)
+
+
+@pytest.mark.parametrize("chunk", [5, 70])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-30])
+def test_a_scale_of_nothing_is_the_mean(chunk, scale) -> None:
+    u = _uocr()
+    s = Setup(39, [chunk], [90])
+    q, k, v = s.qkv.unbind(1)
+    got = u.paged_chunk_attention(q.to(DEV), k.to(DEV), v.to(DEV), kv=s.kv(), layer_idx=0, scale=scale)
+    assert _far(got.cpu(), s.want(0, q, k, v, scale)) <= BAR
+
+
 def test_the_callers_workspace_and_the_wrappers_refusals() -> None:
     from uocr_moe import UocrError, _lib
 

@@ -204,6 +204,43 @@ def test_resize(seed, requests, cols, pages, in_place) -> None:
         assert torch.equal(gt, kept[0]) and torch.equal(gc, kept[1])
 
 
+@pytest.mark.parametrize("output", ["out_lookup", "out_ref_counts"])
+def test_one_table_in_place(output) -> None:
+    u = _uocr()
+    table, counts = _scene(3, 9, 4, 40)
+    pool = _pool(3, 40)
+    lists = [0, 1, 2], [5, 6, 7], [32, 9, 17], [8, 0, 16]
+    lengths = [8 * (i % 5) for i in range(9)]
+    for name in ("resize", "fork", "compact"):
+        gpu, gt, gc = pool.to(DEV), _ints(table), _ints(counts)
+        out = {output: gt if output == "out_lookup" else gc}
+        if name == "resize":
+            got, want = u.resize_pages(gc, gt, _ints(lengths), page_size=8, **out), resized(counts, table, lengths, 8)
+        elif name == "fork":
+            got = u.fork_pages(gpu, gc, gt, *map(_ints, lists), **out)
+            want = forked(pool, counts, table, *lists)[1:]
+        else:
+            got, want = u.compact_pages(gpu, gc, gt, **out), compacted(pool, counts, table)[1:]
+        assert got[0].tolist() == want[0] and got[1].tolist() == want[1], name
+        kept = (gc, counts) if output == "out_lookup" else (gt, table)
+        assert kept[0].tolist() == kept[1], name
+
+
+def test_tables_without_requests_and_forks_without_pairs() -> None:
+    u = _uocr()
+    none, counts = torch.zeros(0, 3, dtype=torch.int32, device=DEV), [0, 2, 0, 1, 0]
+    pool = _pool(4, 5)
+    lookup, got, missing = u.resize_pages(_ints(counts), none, none[:, 0].contiguous(), page_size=8)
+    assert lookup.shape == (0, 3) and got.tolist() == counts and missing.tolist() == [0]
+    gpu, table = pool.to(DEV), [[1, 3, 4]]
+    empty = torch.zeros(0, dtype=torch.int32, device=DEV)
+    lookup, got, missing = u.fork_pages(gpu, _ints(counts), _ints(table), empty, empty, empty, empty)
+    assert lookup.tolist() == table and got.tolist() == counts and missing.tolist() == [0] and _same_bits(gpu, pool)
+    lookup, got, remap = u.compact_pages(gpu, _ints(counts), none)
+    assert got.tolist() == [1, 2, 0, 0, 0] and remap.tolist() == [-1, 1, -1, 0, 4]
+    assert _same_bits(gpu[:2], pool[[3, 1]])
+
+
 def test_resize_runs_out_and_recovers() -> None:
     """Too few free pages: the first entries in (request, column) order get them; released pages are free at once; the
     lowest page goes first."""

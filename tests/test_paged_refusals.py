@@ -16,9 +16,9 @@ def _err(name: str, *args) -> str:
 
 
 def _chunk(tokens=4, heads=10, head_dim=128, stride=1280, pages=3, layers=2, page_size=128, layer=0, requests=1, cols=2,
-           attend_max=4, out=None, q=None, k=None, v=None, pool=None, table=None, ws=None, ws_bytes=0):
+           attend_max=4, out=None, q=None, k=None, v=None, pool=None, table=None, ws=None, ws_bytes=0, scale=1.0):
     return _err("uocr_paged_chunk_attention", out, q, k, v, tokens, heads, head_dim, stride, pool, pages, layers, page_size,
-                layer, table, requests, cols, table, table, attend_max, 1.0, ws, ws_bytes, None)
+                layer, table, requests, cols, table, table, attend_max, scale, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize(("kwargs", "message"), [
@@ -37,6 +37,8 @@ def _chunk(tokens=4, heads=10, head_dim=128, stride=1280, pages=3, layers=2, pag
     ({"cols": 1 << 24}, "bad lookup table width 16777216"),
     ({"attend_max": 257}, "attend_max 257 is not in [1, 256], the rows the lookup table addresses"),
     ({"attend_max": 0}, "attend_max 0 is not in [1, 256], the rows the lookup table addresses"),
+    ({"scale": float("inf")}, "scale must be finite"),
+    ({"scale": float("nan")}, "scale must be finite"),
     ({"stride": 1279}, "input rows 1279 floats apart overlap rows of 1280"),
     ({}, "a tensor is missing"),
 ])
@@ -52,12 +54,14 @@ def test_chunk_attention_refuses_unaligned_and_overlapping_tensors() -> None:
     # the last byte of k_new's last row, and the first of v_new
     assert _chunk(out=2 * FAKE + 4 * 1280 * 4 - 16, **far) == "paged_chunk_attention: out must not overlap the inputs"
     assert _chunk(out=3 * FAKE - 4 * 1280 * 4 + 16, **far) == "paged_chunk_attention: out must not overlap the inputs"
+    assert _chunk(out=4 * FAKE, stride=1 << 25, **far) == \
+        "paged_chunk_attention: input rows must be less than 2^25 floats apart"
     assert _chunk(out=4 * FAKE, ws=8, **far) == "paged_chunk_attention: workspace must be 16-byte aligned"
 
 
 def test_chunk_attention_qkv_refusals() -> None:
-    def call(stride=3840, table_rows=16, table_dim=128, heads=10, qkv=None, rest=None, out=None):
-        return _err("uocr_paged_chunk_attention_qkv", out, qkv, 4, heads, 128, stride, rest, rest, rest, table_rows,
+    def call(stride=3840, table_rows=16, table_dim=128, heads=10, qkv=None, rest=None, out=None, cos=None, sin=None):
+        return _err("uocr_paged_chunk_attention_qkv", out, qkv, 4, heads, 128, stride, rest, cos or rest, sin or rest, table_rows,
                     table_dim, rest, 3, 2, 128, 0, rest, 1, 2, rest, rest, 4, 1.0, None, 0, None)
 
     op = "paged_chunk_attention_qkv: "
@@ -66,6 +70,9 @@ def test_chunk_attention_qkv_refusals() -> None:
     assert call(heads=0) == op + "heads must be in [1, 65535]"
     assert call(stride=3839) == op + "qkv rows 3839 floats apart overlap rows of 3840"
     assert call() == op + "a tensor is missing"
+    for tables in ({"cos": 4 * FAKE + 4}, {"sin": 4 * FAKE + 8}):
+        assert call(qkv=FAKE, rest=2 * FAKE, out=3 * FAKE, **tables) == \
+            op + "the cos/sin tables must be 16-byte aligned"
     # out within qkv's rows
     assert call(qkv=FAKE, rest=2 * FAKE, out=FAKE + 3 * 3840 * 4) == op + "out must not overlap the inputs"
 

@@ -827,6 +827,7 @@ static int paged_chunk_call(const char* op, float* out, const float* q, const fl
   if (attend_max < 1 || attend_max > lookup_cols * page_size)
     return fail(err, errlen, "%s: attend_max %lld is not in [1, %lld], the rows the lookup table addresses", op,
                 (long long)attend_max, (long long)(lookup_cols * page_size));
+  if (!(scale - scale == 0.0f)) return fail(err, errlen, "%s: scale must be finite", op);
   if (in_stride < heads * head_dim)
     return fail(err, errlen, "%s: input rows %lld floats apart overlap rows of %lld", op, (long long)in_stride,
                 (long long)(heads * head_dim));
