@@ -209,7 +209,8 @@ int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens,
  *   place) and must not overlap them otherwise.  Each result is the same whatever the
  *   timing: pages are taken from the lowest free one up, in (row, column) order.
  *   missing int32 [1]: the entries that found no free page (they stay unset).
- *   A workspace is NULL (the library's own) or of the size asked for, 16-byte aligned;
+ *   A workspace is NULL (the library's own) or of the size asked for, 16-byte aligned
+ *   (in_place: whether a table output is its input; a call that needs 0 bytes reads none);
  *   calls that overlap in time must not share one.
  * ------------------------------------------------------------------------- */
 
@@ -228,7 +229,8 @@ int uocr_copy_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t pag
  * call; the child's other entries are unset and its old pages released.  A pair whose child is its parent
  * leaves the row as it is; one with a row outside [0, requests) is skipped; of several pairs with one child the
  * last counts. */
-size_t uocr_fork_pages_workspace_bytes(int64_t pages, int64_t requests, int64_t lookup_cols, int64_t count);
+size_t uocr_fork_pages_workspace_bytes(int64_t pages, int64_t requests, int64_t lookup_cols, int64_t count,
+                                       int64_t in_place);
 int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
                     int64_t head_dim, int32_t* ref_counts_out, const int32_t* ref_counts, uint32_t* lookup_out,
                     const uint32_t* lookup, int64_t requests, int64_t lookup_cols, const int32_t* parents,
@@ -249,7 +251,7 @@ int uocr_resize_pages(int32_t* ref_counts_out, const int32_t* ref_counts, int64_
  * ascending order, to the free ones below L in ascending order; counts and lookup
  * entries follow.  remap int32 [pages]: where each page is now (-1: it was free).  An
  * entry that names a free page is unset. */
-size_t uocr_compact_pages_workspace_bytes(int64_t pages);
+size_t uocr_compact_pages_workspace_bytes(int64_t pages, int64_t in_place);
 int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
                        int64_t head_dim, int32_t* ref_counts_out, const int32_t* ref_counts, uint32_t* lookup_out,
                        const uint32_t* lookup, int64_t requests, int64_t lookup_cols, int32_t* remap, void* workspace,

@@ -61,8 +61,8 @@ def test_chunk_attention_refuses_unaligned_and_overlapping_tensors() -> None:
 
 def test_chunk_attention_qkv_refusals() -> None:
     def call(stride=3840, table_rows=16, table_dim=128, heads=10, qkv=None, rest=None, out=None, cos=None, sin=None):
-        return _err("uocr_paged_chunk_attention_qkv", out, qkv, 4, heads, 128, stride, rest, cos or rest, sin or rest, table_rows,
-                    table_dim, rest, 3, 2, 128, 0, rest, 1, 2, rest, rest, 4, 1.0, None, 0, None)
+        return _err("uocr_paged_chunk_attention_qkv", out, qkv, 4, heads, 128, stride, rest, cos or rest, sin or rest,
+                    table_rows, table_dim, rest, 3, 2, 128, 0, rest, 1, 2, rest, rest, 4, 1.0, None, 0, None)
 
     op = "paged_chunk_attention_qkv: "
     assert call(table_dim=64) == op + "the cos/sin tables are 64 wide, not head_dim 128"
@@ -135,11 +135,11 @@ def test_workspace_sizes_of_bad_shapes_are_zero() -> None:
     lib = _lib.load()
     assert lib.uocr_paged_chunk_workspace_bytes(-1, 1, 10, 5) == 0
     assert lib.uocr_paged_chunk_workspace_bytes(4, 1, 10, 0) == 0
-    assert lib.uocr_fork_pages_workspace_bytes(9, 3, 0, 2) == 0
+    assert lib.uocr_fork_pages_workspace_bytes(9, 3, 0, 2, 1) == 0
     assert lib.uocr_resize_pages_workspace_bytes(0) == 0
     assert lib.uocr_resize_pages_workspace_bytes(9) == 0  # in LDS
     assert lib.uocr_resize_pages_workspace_bytes(20000) == 80000
-    assert lib.uocr_compact_pages_workspace_bytes(-1) == 0
+    assert lib.uocr_compact_pages_workspace_bytes(-1, 1) == 0
 
 
 def test_the_wrappers_refuse_cpu_tensors_and_other_types() -> None:

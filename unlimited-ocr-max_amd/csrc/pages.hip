@@ -7,10 +7,12 @@
 //           an entry outside [0, pages - 1) is unset (unset entries are written as pages - 1)
 //   counts  [pages]: the entries that name each page; <= 0: free
 //
-// The table kernels are one workgroup each: a fork, a resize and a compaction are scans
-// over the counts and the table in a fixed order, so that which page an entry gets does
-// not depend on timing.  Each output may be its input.  What they decide to copy goes, as (source, destination, rows)
-// triples, to a second launch over the whole device.
+// A fork, a resize and a compaction are scans over the counts and the table by one
+// workgroup, in a fixed order, so that which page an entry gets does not depend on
+// timing.  Each output may be its input.  What they decide to copy goes, as (source,
+// destination, rows) triples, to a second launch over the whole device; or, where the
+// outputs are other tensors and the tables small, every workgroup makes the same scans
+// and then its share of the copies.
 #include <algorithm>
 
 #include "uocr_device.h"
@@ -28,10 +30,17 @@ constexpr int kTableWaves = kTableThreads / kWave;
 constexpr int kPer = 2;
 constexpr int kRound = kPer * kTableThreads;
 constexpr int kCopyThreads = 256;
-constexpr int kSegment = 4 * kCopyThreads;  // float4s of one plane that a workgroup copies at a time
 
 // Up to these sizes counts, lists and the rest of a table kernel's state are in LDS (145 KB of 160), else in memory.
 constexpr int kLdsPages = 16384, kLdsRows = 4096;
+
+// Where a table kernel works.  kEvery: every workgroup of the grid works the tables out for itself, in LDS, the first
+// writes them, and all make the copies, with no launch between.  The tables' outputs are then other tensors than their
+// inputs (which the others may still read), and the sizes those of one round.
+enum Where { kMemory, kLds, kEvery };
+constexpr int kEveryGroups = 512;  // two to a CU
+template <Where kAt>
+constexpr int kHeld = kAt == kMemory ? 1 : kAt == kLds ? kLdsPages : kRound;
 
 // f(u, e) for this thread's elements e < n of the round that starts at e0.
 template <typename F>
@@ -186,6 +195,40 @@ __global__ void __launch_bounds__(kTableThreads) k_resize(PageTables t, int page
   }
 }
 
+struct Move {
+  int src, dst, rows;
+};
+struct Copies {
+  f32x4* pool;
+  int planes, P, slot4;
+};
+// The copies that a fork or a compaction comes to: (page, plane, segment) triples over the grid.  Destinations are
+// distinct and no page is both a source and a destination.
+template <int kThreads, typename F>
+__device__ __forceinline__ void copy_moves(const Copies& c, int moves, const F& move) {
+  constexpr int kAtOnce = 4, kSegment = kAtOnce * kThreads;  // float4s of one plane that a workgroup copies at a time
+  const int64_t plane4 = (int64_t)c.P * c.slot4;
+  const int segments = (int)((plane4 + kSegment - 1) / kSegment);
+  const int64_t items = (int64_t)moves * c.planes * segments;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const int seg = (int)(i % segments);
+    const int64_t mp = i / segments;
+    const int plane = (int)(mp % c.planes);
+    const Move m = move((int)(mp / c.planes));
+    const int64_t end = (int64_t)m.rows * c.slot4;
+    const f32x4* src = c.pool + ((int64_t)m.src * c.planes + plane) * plane4;
+    f32x4* dst = c.pool + ((int64_t)m.dst * c.planes + plane) * plane4;
+    const int64_t e0 = (int64_t)seg * kSegment + threadIdx.x;
+    f32x4 v[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      if (e0 + u * kThreads < end) v[u] = *(const UOCR_GLOBAL f32x4*)(src + e0 + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      if (e0 + u * kThreads < end) *(UOCR_GLOBAL f32x4*)(dst + e0 + u * kThreads) = v[u];
+  }
+}
+
 struct ForkScratch {
   int32_t* moves;   // [0]: pages to copy
   int32_t* plan;    // [3 * count * cols]: source, destination, rows
@@ -198,21 +241,24 @@ struct ForkScratch {
 // below shared_rows are shared, the others up to the length are copied to pages that were
 // free before the call, in (pair, column) order from the lowest; then the child's old
 // pages are released.  Bound by latency, as k_resize is.
-template <bool kLds>
+template <Where kAt>
 __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages, int P, Divide by_page, Divide by_cols,
                                                         const int32_t* __restrict__ parents,
                                                         const int32_t* __restrict__ children,
                                                         const int32_t* __restrict__ lengths,
                                                         const int32_t* __restrict__ shared_rows, int count,
-                                                        int32_t* missing, ForkScratch w) {
+                                                        int32_t* missing, ForkScratch w, Copies copies) {
+  constexpr bool kLds = kAt != kMemory;
+  const bool writes = kAt != kEvery || blockIdx.x == 0;
   __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
-  __shared__ int32_t lds_counts[kLds ? kLdsPages : 1], lds_list[kLds ? kLdsPages : 1], lds_winner[kLds ? kLdsRows : 1];
+  __shared__ int32_t lds_counts[kHeld<kAt>], lds_list[kHeld<kAt>], lds_winner[kLds ? kLdsRows : 1];
+  __shared__ int32_t lds_from[kAt == kEvery ? kRound : 1], lds_rows[kAt == kEvery ? kRound : 1];
   int32_t* counts = kLds ? lds_counts : t.counts_out;
   int32_t* list = kLds ? lds_list : w.list;
   int32_t* winner = kLds ? lds_winner : w.winner;
   constexpr int kScope = kLds ? __HIP_MEMORY_SCOPE_WORKGROUP : __HIP_MEMORY_SCOPE_AGENT;
   const int null = pages - 1, tid = (int)threadIdx.x;
-  if (t.lookup_out != t.lookup)
+  if (t.lookup_out != t.lookup && writes)
     for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound) {
       uint32_t v[kPer];
       each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { v[u] = ldg(t.lookup + e); });
@@ -258,9 +304,15 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
         page[u] = null;
         if (r < free) {
           page[u] = list[r];
-          w.plan[3 * r] = old;
-          w.plan[3 * r + 1] = page[u];
-          w.plan[3 * r + 2] = min(P, ldg(lengths + c) - (e - c * t.cols) * P);
+          const int rows = min(P, ldg(lengths + c) - (e - c * t.cols) * P);
+          if constexpr (kAt == kEvery) {  // to the free page r
+            lds_from[r] = old;
+            lds_rows[r] = rows;
+          } else {
+            w.plan[3 * r] = old;
+            w.plan[3 * r + 1] = page[u];
+            w.plan[3 * r + 2] = rows;
+          }
           set_count<kLds>(counts + page[u], 1);
         }
       }
@@ -269,6 +321,10 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
     taken += all;
   }
   __syncthreads();  // every new entry is counted, and every row read, before an old one is released
+  if constexpr (kAt == kEvery) {
+    copy_moves<kTableThreads>(copies, min(taken, free), [&](int m) { return Move{lds_from[m], list[m], lds_rows[m]}; });
+    if (!writes) return;
+  }
   for (int64_t e = tid; e < entries; e += kTableThreads) {
     const int c = by_cols((int)e), child = child_of(c);
     const uint32_t old = child < 0 ? null : ldg(t.lookup + (int64_t)child * t.cols + (e - c * t.cols));
@@ -282,7 +338,7 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
       if (child >= 0) t.lookup_out[(int64_t)child * t.cols + (e - c * t.cols)] = (uint32_t)now;
     });
   if (tid == 0) {
-    w.moves[0] = min(taken, free);
+    if constexpr (kAt != kEvery) w.moves[0] = min(taken, free);
     missing[0] = max(0, taken - free);
   }
   if constexpr (kLds) {
@@ -294,11 +350,15 @@ __global__ void __launch_bounds__(kTableThreads) k_fork(PageTables t, int pages,
 // The pages in use move to the front: with L of them, those at or past L go, in ascending
 // order, to the free ones below L in ascending order.  With b(p) the used pages below p,
 // the free page p < L is hole p - b(p), and the used page p >= L goes to hole b(p) - b(L).
-template <bool kLds>
+template <Where kAt>
 __global__ void __launch_bounds__(kTableThreads) k_compact(PageTables t, int pages, int P, int32_t* remap,
-                                                           int32_t* moves, int32_t* plan, int32_t* holes_mem) {
+                                                           int32_t* moves, int32_t* plan, int32_t* holes_mem,
+                                                           Copies copies) {
+  constexpr bool kLds = kAt != kMemory;
+  const bool writes = kAt != kEvery || blockIdx.x == 0;
   __shared__ __attribute__((aligned(16))) int totals[kPer * kTableWaves];
-  __shared__ int32_t lds_remap[kLds ? kLdsPages : 1], lds_holes[kLds ? kLdsPages / 2 : 1];
+  __shared__ int32_t lds_remap[kHeld<kAt>], lds_holes[kLds ? kHeld<kAt> / 2 : 1];
+  __shared__ int32_t lds_from[kAt == kEvery ? kRound / 2 : 1];
   __shared__ int below_live;
   int32_t* holes = kLds ? lds_holes : holes_mem;
   const int null = pages - 1, tid = (int)threadIdx.x;
@@ -336,24 +396,35 @@ __global__ void __launch_bounds__(kTableThreads) k_compact(PageTables t, int pag
       if (in_use && p >= live) {
         const int64_t i = rank[u] - below_live;
         now = holes[i];
-        plan[3 * i] = p;
-        plan[3 * i + 1] = now;
-        plan[3 * i + 2] = P;
-        t.counts_out[now] = v[u];
-        t.counts_out[p] = 0;
-      } else if ((in_use || p >= live) && t.counts_out != t.counts) {
+        if constexpr (kAt == kEvery) {
+          lds_from[i] = p;
+        } else {
+          plan[3 * i] = p;
+          plan[3 * i + 1] = now;
+          plan[3 * i + 2] = P;
+        }
+        if (writes) {
+          t.counts_out[now] = v[u];
+          t.counts_out[p] = 0;
+        }
+      } else if ((in_use || p >= live) && t.counts_out != t.counts && writes) {
         t.counts_out[p] = v[u];
       }
       if constexpr (kLds) lds_remap[p] = now;
-      remap[p] = now;
+      if (writes) remap[p] = now;
     });
   }
-  if (tid == 0) {
+  __syncthreads();
+  const int count = live < null ? live - below_live : 0;
+  if (tid == 0 && writes) {
     remap[null] = null;
     if (t.counts_out != t.counts) t.counts_out[null] = t.counts[null];
-    moves[0] = live < null ? live - below_live : 0;
+    if constexpr (kAt != kEvery) moves[0] = count;
   }
-  __syncthreads();
+  if constexpr (kAt == kEvery) {
+    copy_moves<kTableThreads>(copies, count, [&](int m) { return Move{lds_from[m], holes[m], P}; });
+    if (!writes) return;
+  }
   for (int64_t e0 = 0; e0 < (int64_t)t.requests * t.cols; e0 += kRound) {
     uint32_t page[kPer];
     each(e0, (int64_t)t.requests * t.cols, [&](int u, int e) { page[u] = ldg(t.lookup + e); });
@@ -364,31 +435,13 @@ __global__ void __launch_bounds__(kTableThreads) k_compact(PageTables t, int pag
   }
 }
 
-// The planned copies: (page, plane, segment) triples over the grid.  Destinations are
-// distinct and no page is both a source and a destination.
-__global__ void __launch_bounds__(kCopyThreads) k_copy_plan(f32x4* pool, int planes, int P, int slot4,
-                                                            const int32_t* __restrict__ moves,
+// The planned copies, a launch of their own.
+__global__ void __launch_bounds__(kCopyThreads) k_copy_plan(Copies c, const int32_t* __restrict__ moves,
                                                             const int32_t* __restrict__ plan) {
-  const int64_t plane4 = (int64_t)P * slot4;
-  const int segments = (int)((plane4 + kSegment - 1) / kSegment);
-  const int64_t items = (int64_t)ldc(moves) * planes * segments;
-  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const int seg = (int)(i % segments);
-    const int64_t mp = i / segments;
-    const int plane = (int)(mp % planes);
-    const int32_t* m = plan + 3 * (mp / planes);
-    const int64_t end = (int64_t)ldc(m + 2) * slot4;
-    const f32x4* src = pool + ((int64_t)ldc(m) * planes + plane) * plane4;
-    f32x4* dst = pool + ((int64_t)ldc(m + 1) * planes + plane) * plane4;
-    const int64_t e0 = (int64_t)seg * kSegment + threadIdx.x;
-    f32x4 v[kSegment / kCopyThreads];
-#pragma unroll
-    for (int u = 0; u < kSegment / kCopyThreads; ++u)
-      if (e0 + u * kCopyThreads < end) v[u] = *(const UOCR_GLOBAL f32x4*)(src + e0 + u * kCopyThreads);
-#pragma unroll
-    for (int u = 0; u < kSegment / kCopyThreads; ++u)
-      if (e0 + u * kCopyThreads < end) *(UOCR_GLOBAL f32x4*)(dst + e0 + u * kCopyThreads) = v[u];
-  }
+  copy_moves<kCopyThreads>(c, ldc(moves), [&](int m) {
+    const int32_t* p = plan + 3 * (int64_t)m;
+    return Move{ldc(p), ldc(p + 1), ldc(p + 2)};
+  });
 }
 
 // Copies in the order of the pairs: a thread does its element of every pair, one pair after the other, so a page may be
@@ -412,9 +465,9 @@ __global__ void __launch_bounds__(kCopyThreads) k_copy_pages(f32x4* pool, int pa
   }
 }
 
+Copies copies_of(const PagePool& p) { return {(f32x4*)p.kv_blocks, 2 * p.layers, p.page_size, p.slot / 4}; }
 hipError_t launch_plan(const PagePool& p, const int32_t* moves, const int32_t* plan, hipStream_t s) {
-  UOCR_LAUNCH("copy_plan", k_copy_plan, dim3(2048), dim3(kCopyThreads), 0, s, (f32x4*)p.kv_blocks, 2 * p.layers,
-              p.page_size, p.slot / 4, moves, plan);
+  UOCR_LAUNCH("copy_plan", k_copy_plan, dim3(2048), dim3(kCopyThreads), 0, s, copies_of(p), moves, plan);
   return hipGetLastError();
 }
 
@@ -433,10 +486,18 @@ hipError_t launch_copy_pages(const PagePool& p, const int32_t* src, const int32_
 
 namespace {
 bool in_lds(int64_t pages, int64_t requests) { return pages <= kLdsPages && requests <= kLdsRows; }
+bool in_place(const PageTables& t) { return t.counts == t.counts_out || t.lookup == t.lookup_out; }
+// One launch, against the tables' and then the copies' (us, the host's call included; on the device): a fork of three
+// requests 14.3 for 18.8 (6.8 for 4.5 + 1.8), a compaction of 6 requests 11.8 for 16.1 (10.8 for 3.4 + 6.4), of 24 and
+// 12 layers 247 for 279 (250 for 4.9 + 273).
+bool by_every(int64_t pages, int64_t requests, int64_t entries, bool in_place) {
+  return !in_place && pages <= kRound && requests <= kLdsRows && entries <= kRound;
+}
 }  // namespace
 
-size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count) {
+size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count, bool in_place) {
   const int64_t entries = count * cols;
+  if (by_every(pages, requests, entries, in_place)) return 0;
   return sizeof(int32_t) * (4 + 3 * entries + (entries > kRound ? entries : 0) +
                             (in_lds(pages, requests) ? 0 : requests + pages));
 }
@@ -445,16 +506,20 @@ hipError_t launch_fork_pages(const PagePool& p, const PageTables& t, const int32
                              const int32_t* lengths, const int32_t* shared_rows, int count, int32_t* missing,
                              void* workspace, hipStream_t s) {
   const int64_t entries = (int64_t)count * t.cols;
+  const bool every = by_every(p.pages, t.requests, entries, in_place(t));
   ForkScratch w{};
-  w.moves = (int32_t*)workspace;
-  w.plan = w.moves + 4;
-  w.fresh = w.plan + 3 * entries;
-  w.winner = w.fresh + (entries > kRound ? entries : 0);
-  w.list = w.winner + t.requests;
-  const auto kernel = in_lds(p.pages, t.requests) ? k_fork<true> : k_fork<false>;
-  UOCR_LAUNCH("fork_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size,
-              divide_by(p.page_size), divide_by(t.cols), parents, children, lengths, shared_rows, count, missing, w);
-  if (count == 0) return hipGetLastError();
+  if (!every) {
+    w.moves = (int32_t*)workspace;
+    w.plan = w.moves + 4;
+    w.fresh = w.plan + 3 * entries;
+    w.winner = w.fresh + (entries > kRound ? entries : 0);
+    w.list = w.winner + t.requests;
+  }
+  const auto kernel = every ? k_fork<kEvery> : in_lds(p.pages, t.requests) ? k_fork<kLds> : k_fork<kMemory>;
+  UOCR_LAUNCH("fork_tables", kernel, dim3(every && count > 0 ? kEveryGroups : 1), dim3(kTableThreads), 0, s, t, p.pages,
+              p.page_size, divide_by(p.page_size), divide_by(t.cols), parents, children, lengths, shared_rows, count,
+              missing, w, copies_of(p));
+  if (every || count == 0) return hipGetLastError();
   return launch_plan(p, w.moves, w.plan, s);
 }
 
@@ -469,18 +534,21 @@ hipError_t launch_resize_pages(const PagePool& p, const PageTables& t, const int
 }
 
 // At most half of the pages move.
-size_t compact_workspace_bytes(int64_t pages) {
+size_t compact_workspace_bytes(int64_t pages, bool in_place) {
+  if (by_every(pages, 0, 0, in_place)) return 0;
   return sizeof(int32_t) * (4 + (in_lds(pages, 0) ? 3 : 4) * (pages / 2 + 1));
 }
 
 hipError_t launch_compact_pages(const PagePool& p, const PageTables& t, int32_t* remap, void* workspace,
                                 hipStream_t s) {
+  const bool every = by_every(p.pages, 0, 0, in_place(t));
   int32_t* moves = (int32_t*)workspace;
-  int32_t* plan = moves + 4;
-  const auto kernel = in_lds(p.pages, 0) ? k_compact<true> : k_compact<false>;
-  UOCR_LAUNCH("compact_tables", kernel, dim3(1), dim3(kTableThreads), 0, s, t, p.pages, p.page_size, remap, moves,
-              plan, plan + 3 * ((int64_t)p.pages / 2 + 1));
-  return launch_plan(p, moves, plan, s);
+  int32_t* plan = every ? nullptr : moves + 4;
+  int32_t* holes = every || in_lds(p.pages, 0) ? nullptr : plan + 3 * ((int64_t)p.pages / 2 + 1);
+  const auto kernel = every ? k_compact<kEvery> : in_lds(p.pages, 0) ? k_compact<kLds> : k_compact<kMemory>;
+  UOCR_LAUNCH("compact_tables", kernel, dim3(every ? kEveryGroups : 1), dim3(kTableThreads), 0, s, t, p.pages,
+              p.page_size, remap, moves, plan, holes, copies_of(p));
+  return every ? hipGetLastError() : launch_plan(p, moves, plan, s);
 }
 
 }  // namespace uocr

@@ -972,11 +972,12 @@ int uocr_copy_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t pag
   return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
 }
 
-size_t uocr_fork_pages_workspace_bytes(int64_t pages, int64_t requests, int64_t lookup_cols, int64_t count) {
+size_t uocr_fork_pages_workspace_bytes(int64_t pages, int64_t requests, int64_t lookup_cols, int64_t count,
+                                       int64_t in_place) {
   if (pages < 1 || pages > INT32_MAX || requests < 0 || requests > INT32_MAX || count < 0 || lookup_cols < 1 ||
       lookup_cols > INT32_MAX || count > INT32_MAX / lookup_cols)
     return 0;
-  return fork_workspace_bytes(pages, requests, lookup_cols, count);
+  return fork_workspace_bytes(pages, requests, lookup_cols, count, in_place != 0);
 }
 
 int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
@@ -996,7 +997,8 @@ int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t pag
   if (!kv_blocks || !missing || (count > 0 && (!parents || !children || !lengths || !shared_rows)))
     return fail(err, errlen, "%s: a tensor is missing", op);
   void* ws = nullptr;
-  if (chunk_workspace(op, workspace, workspace_bytes, fork_workspace_bytes(pages, requests, lookup_cols, count),
+  if (chunk_workspace(op, workspace, workspace_bytes, fork_workspace_bytes(pages, requests, lookup_cols, count,
+                                           ref_counts == ref_counts_out || lookup == lookup_out),
                       (hipStream_t)stream, &ws, err, errlen))
     return 1;
   const hipError_t e = launch_fork_pages(p, t, parents, children, lengths, shared_rows, (int)count, missing, ws,
@@ -1030,8 +1032,8 @@ int uocr_resize_pages(int32_t* ref_counts_out, const int32_t* ref_counts, int64_
   return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
 }
 
-size_t uocr_compact_pages_workspace_bytes(int64_t pages) {
-  return pages < 1 || pages > INT32_MAX ? 0 : compact_workspace_bytes(pages);
+size_t uocr_compact_pages_workspace_bytes(int64_t pages, int64_t in_place) {
+  return pages < 1 || pages > INT32_MAX ? 0 : compact_workspace_bytes(pages, in_place != 0);
 }
 
 int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
@@ -1046,7 +1048,8 @@ int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t 
     return 1;
   if (!kv_blocks || !remap) return fail(err, errlen, "%s: a tensor is missing", op);
   void* ws = nullptr;
-  if (chunk_workspace(op, workspace, workspace_bytes, compact_workspace_bytes(pages), (hipStream_t)stream, &ws, err,
+  if (chunk_workspace(op, workspace, workspace_bytes, compact_workspace_bytes(pages, ref_counts == ref_counts_out || lookup == lookup_out),
+                      (hipStream_t)stream, &ws, err,
                       errlen))
     return 1;
   const hipError_t e = launch_compact_pages(p, t, remap, ws, (hipStream_t)stream);

@@ -69,12 +69,12 @@ SIGNATURES: dict[str, list] = {
                                        _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _sz, _vp, _cp,
                                        _sz],
     "uocr_copy_pages": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _cp, _sz],
-    "uocr_fork_pages_workspace_bytes": [_i64, _i64, _i64, _i64],
+    "uocr_fork_pages_workspace_bytes": [_i64, _i64, _i64, _i64, _i64],
     "uocr_fork_pages": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp,
                         _vp, _sz, _vp, _cp, _sz],
     "uocr_resize_pages_workspace_bytes": [_i64],
     "uocr_resize_pages": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp, _cp, _sz],
-    "uocr_compact_pages_workspace_bytes": [_i64],
+    "uocr_compact_pages_workspace_bytes": [_i64, _i64],
     "uocr_compact_pages": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _sz, _vp, _cp,
                            _sz],
     "uocr_moe_workspace_bytes": [ctypes.POINTER(Layer), _i64, _int],

@@ -637,18 +637,23 @@ def fork_pages(kv_blocks, ref_counts, lookup_table, parents, children, lengths, 
     counts, lookup, new_counts, new_lookup = _tables(op, ref_counts, lookup_table, out_ref_counts, out_lookup)
     if counts.shape[0] != pages:
         raise ValueError(f"{op}: ref_counts is for {counts.shape[0]} pages, the pool has {pages}")
-    lists = [_gpu(op, name, t, torch.int32, 1) for name, t in
-             (("parents", parents), ("children", children), ("lengths", lengths), ("shared_rows", shared_rows))]
-    n = lists[0].shape[0]
-    if any(t.shape[0] != n for t in lists):
+    parents = _gpu(op, "parents", parents, torch.int32, 1)
+    children = _gpu(op, "children", children, torch.int32, 1)
+    lengths = _gpu(op, "lengths", lengths, torch.int32, 1)
+    shared_rows = _gpu(op, "shared_rows", shared_rows, torch.int32, 1)
+    n = parents.shape[0]
+    if children.shape[0] != n or lengths.shape[0] != n or shared_rows.shape[0] != n:
         raise ValueError(f"{op}: parents, children, lengths and shared_rows must have one length")
     requests, cols = lookup.shape
-    ws = _workspace(op, workspace, _lib.load().uocr_fork_pages_workspace_bytes(pages, requests, cols, n), blocks)
+    in_place = out_ref_counts is not None or out_lookup is not None
+    need = _lib.load().uocr_fork_pages_workspace_bytes(pages, requests, cols, n, in_place)
+    ws = _workspace(op, workspace, need, blocks)
     missing = counts.new_empty(1)
     _on_device(op, "uocr_fork_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim,
                new_counts.data_ptr(), counts.data_ptr(), new_lookup.data_ptr(), lookup.data_ptr(), requests, cols,
-               *(t.data_ptr() for t in lists), n, missing.data_ptr(), _ptr(ws), _nbytes(ws),
-               tensors=[blocks, counts, lookup, new_counts, new_lookup, *lists, ws])
+               parents.data_ptr(), children.data_ptr(), lengths.data_ptr(), shared_rows.data_ptr(), n,
+               missing.data_ptr(), _ptr(ws), _nbytes(ws),
+               tensors=[blocks, counts, lookup, new_counts, new_lookup, parents, children, lengths, shared_rows, ws])
     return new_lookup, new_counts, missing
 
 
@@ -687,7 +692,8 @@ def compact_pages(kv_blocks, ref_counts, lookup_table, *, out_ref_counts: torch.
     if counts.shape[0] != pages:
         raise ValueError(f"{op}: ref_counts is for {counts.shape[0]} pages, the pool has {pages}")
     requests, cols = lookup.shape
-    ws = _workspace(op, workspace, _lib.load().uocr_compact_pages_workspace_bytes(pages), blocks)
+    in_place = out_ref_counts is not None or out_lookup is not None
+    ws = _workspace(op, workspace, _lib.load().uocr_compact_pages_workspace_bytes(pages, in_place), blocks)
     remap = torch.empty_like(counts)
     _on_device(op, "uocr_compact_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim,
                new_counts.data_ptr(), counts.data_ptr(), new_lookup.data_ptr(), lookup.data_ptr(), requests, cols,
