@@ -206,8 +206,9 @@ int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens,
  *   [c P, c P + P); an entry that is not below pages - 1 is unset, and unset entries are
  *   written as pages - 1.  ref_counts int32 [pages]: how many entries name the page;
  *   a page with a count <= 0 is free.  The table outputs may be their inputs (in
- *   place) and must not overlap them otherwise.  Each result is the same whatever the
- *   timing: pages are taken from the lowest free one up, in (row, column) order.
+ *   place) and must not overlap them, nor a list or another output, otherwise.  Each
+ *   result is the same whatever the timing: pages are taken from the lowest free one
+ *   up, in (row, column) order.
  *   missing int32 [1]: the entries that found no free page (they stay unset).
  *   A workspace is NULL (the library's own) or of the size asked for, 16-byte aligned
  *   (in_place: whether a table output is its input; a call that needs 0 bytes reads none);

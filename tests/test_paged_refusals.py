@@ -125,6 +125,14 @@ def test_table_operators_refuse_bad_tables() -> None:
     assert fork(lists=None) == "fork_pages: a tensor is missing"
     assert fork(count=1 << 30) == "fork_pages: bad number of pairs 1073741824"
     assert "fork_pages: workspace of 0 bytes is smaller than" in fork()
+    apart = "an output must not overlap a list"
+    for lists in (FAKE + 32, 2 * FAKE + 44, 4 * FAKE - 4):
+        assert fork(lists=lists) == "fork_pages: " + apart
+    for lengths in (FAKE + 32, 2 * FAKE + 44, 4 * FAKE - 8):
+        assert resize(lengths=lengths) == op + apart
+    for remap in (FAKE - 32, 2 * FAKE + 44):
+        assert _err("uocr_compact_pages", 5 * FAKE, 9, 2, 128, 10, 128, FAKE, FAKE, 2 * FAKE, 2 * FAKE, 3, 4, remap, None,
+                    0, None) == "compact_pages: remap must not overlap the tables"
     assert _err("uocr_compact_pages", 5 * FAKE, 9, 2, 128, 10, 128, FAKE, FAKE, 2 * FAKE, 2 * FAKE, 3, 4, None, None, 0,
                 None) == "compact_pages: a tensor is missing"
 

@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -959,6 +960,17 @@ static int page_tables(const char* op, PageTables& t, int32_t* counts_out, const
   return 0;
 }
 
+// Refuses outputs that overlap a list: the workgroups that read it need not wait for the one that writes them.
+static int lists_apart(const char* op, const PageTables& t, int64_t pages, const int32_t* other, int64_t others,
+                       std::initializer_list<const int32_t*> lists, int64_t count, char* err, size_t errlen) {
+  for (const int32_t* list : lists)
+    for (const auto& [out, n] : {std::pair<const void*, int64_t>{t.counts_out, pages},
+                                 {t.lookup_out, (int64_t)t.requests * t.cols}, {other, others}})
+      if (overlap(out, (size_t)n * 4, list, (size_t)count * 4))
+        return fail(err, errlen, "%s: an output must not overlap a list", op);
+  return 0;
+}
+
 int uocr_copy_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
                     int64_t head_dim, const int32_t* src, const int32_t* dst, const int32_t* rows, int64_t count,
                     void* stream, char* err, size_t errlen) {
@@ -996,6 +1008,7 @@ int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t pag
     return fail(err, errlen, "%s: bad number of pairs %lld", op, (long long)count);
   if (!kv_blocks || !missing || (count > 0 && (!parents || !children || !lengths || !shared_rows)))
     return fail(err, errlen, "%s: a tensor is missing", op);
+  if (lists_apart(op, t, pages, missing, 1, {parents, children, lengths, shared_rows}, count, err, errlen)) return 1;
   void* ws = nullptr;
   if (chunk_workspace(op, workspace, workspace_bytes, fork_workspace_bytes(pages, requests, lookup_cols, count,
                                            ref_counts == ref_counts_out || lookup == lookup_out),
@@ -1024,6 +1037,7 @@ int uocr_resize_pages(int32_t* ref_counts_out, const int32_t* ref_counts, int64_
   if (page_tables(op, t, ref_counts_out, ref_counts, pages, lookup_out, lookup, requests, lookup_cols, err, errlen))
     return 1;
   if (!missing || (requests > 0 && !lengths)) return fail(err, errlen, "%s: a tensor is missing", op);
+  if (lists_apart(op, t, pages, missing, 1, {lengths}, requests, err, errlen)) return 1;
   void* ws = nullptr;
   if (chunk_workspace(op, workspace, workspace_bytes, resize_workspace_bytes(pages), (hipStream_t)stream, &ws, err,
                       errlen))
@@ -1047,6 +1061,10 @@ int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t 
       page_tables(op, t, ref_counts_out, ref_counts, pages, lookup_out, lookup, requests, lookup_cols, err, errlen))
     return 1;
   if (!kv_blocks || !remap) return fail(err, errlen, "%s: a tensor is missing", op);
+  const size_t cb = (size_t)pages * 4, lb = (size_t)(requests * lookup_cols) * 4;
+  if (overlap(remap, cb, ref_counts, cb) || overlap(remap, cb, ref_counts_out, cb) || overlap(remap, cb, lookup, lb) ||
+      overlap(remap, cb, lookup_out, lb))
+    return fail(err, errlen, "%s: remap must not overlap the tables", op);
   void* ws = nullptr;
   if (chunk_workspace(op, workspace, workspace_bytes, compact_workspace_bytes(pages, ref_counts == ref_counts_out || lookup == lookup_out),
                       (hipStream_t)stream, &ws, err,
