@@ -125,6 +125,12 @@ def test_table_operators_refuse_bad_tables() -> None:
     assert fork(lists=None) == "fork_pages: a tensor is missing"
     assert fork(count=1 << 30) == "fork_pages: bad number of pairs 1073741824"
     assert "fork_pages: workspace of 0 bytes is smaller than" in fork()
+    lib = __import__("uocr_moe")._lib.load()
+    assert lib.uocr_fork_pages_workspace_bytes(9, 3, 4, 2, 0) == 0  # one launch, which keeps its state in LDS
+    assert lib.uocr_fork_pages_workspace_bytes(9, 3, 4, 2, 1) > 0
+    assert lib.uocr_fork_pages_workspace_bytes(2049, 3, 4, 2, 0) > 0
+    assert lib.uocr_compact_pages_workspace_bytes(2048, 0) == 0
+    assert min(lib.uocr_compact_pages_workspace_bytes(2048, 1), lib.uocr_compact_pages_workspace_bytes(2049, 0)) > 0
     apart = "an output must not overlap a list"
     for lists in (FAKE + 32, 2 * FAKE + 44, 4 * FAKE - 4):
         assert fork(lists=lists) == "fork_pages: " + apart

@@ -486,7 +486,6 @@ hipError_t launch_copy_pages(const PagePool& p, const int32_t* src, const int32_
 
 namespace {
 bool in_lds(int64_t pages, int64_t requests) { return pages <= kLdsPages && requests <= kLdsRows; }
-bool in_place(const PageTables& t) { return t.counts == t.counts_out || t.lookup == t.lookup_out; }
 // One launch, against the tables' and then the copies' (us, the host's call included; on the device): a fork of three
 // requests 14.3 for 18.8 (6.8 for 4.5 + 1.8), a compaction of 6 requests 11.8 for 16.1 (10.8 for 3.4 + 6.4), of 24 and
 // 12 layers 247 for 279 (250 for 4.9 + 273).
@@ -494,6 +493,10 @@ bool by_every(int64_t pages, int64_t requests, int64_t entries, bool in_place) {
   return !in_place && pages <= kRound && requests <= kLdsRows && entries <= kRound;
 }
 }  // namespace
+
+bool in_place(const PageTables& t) {
+  return t.counts == t.counts_out || (t.requests > 0 && t.lookup == t.lookup_out);
+}
 
 size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count, bool in_place) {
   const int64_t entries = count * cols;

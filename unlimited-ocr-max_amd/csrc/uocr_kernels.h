@@ -309,6 +309,7 @@ struct PageTables {
 };
 hipError_t launch_copy_pages(const PagePool& p, const int32_t* src, const int32_t* dst, const int32_t* rows,
                              int count, hipStream_t s);
+bool in_place(const PageTables& t);  // whether a table output is its input
 size_t fork_workspace_bytes(int64_t pages, int64_t requests, int64_t cols, int64_t count, bool in_place);
 hipError_t launch_fork_pages(const PagePool& p, const PageTables& t, const int32_t* parents, const int32_t* children,
                              const int32_t* lengths, const int32_t* shared_rows, int count, int32_t* missing,

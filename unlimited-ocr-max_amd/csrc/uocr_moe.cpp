@@ -1010,10 +1010,8 @@ int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t pag
     return fail(err, errlen, "%s: a tensor is missing", op);
   if (lists_apart(op, t, pages, missing, 1, {parents, children, lengths, shared_rows}, count, err, errlen)) return 1;
   void* ws = nullptr;
-  if (chunk_workspace(op, workspace, workspace_bytes, fork_workspace_bytes(pages, requests, lookup_cols, count,
-                                           ref_counts == ref_counts_out || lookup == lookup_out),
-                      (hipStream_t)stream, &ws, err, errlen))
-    return 1;
+  const size_t need = fork_workspace_bytes(pages, requests, lookup_cols, count, in_place(t));
+  if (chunk_workspace(op, workspace, workspace_bytes, need, (hipStream_t)stream, &ws, err, errlen)) return 1;
   const hipError_t e = launch_fork_pages(p, t, parents, children, lengths, shared_rows, (int)count, missing, ws,
                                          (hipStream_t)stream);
   return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
@@ -1066,10 +1064,8 @@ int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t 
       overlap(remap, cb, lookup_out, lb))
     return fail(err, errlen, "%s: remap must not overlap the tables", op);
   void* ws = nullptr;
-  if (chunk_workspace(op, workspace, workspace_bytes, compact_workspace_bytes(pages, ref_counts == ref_counts_out || lookup == lookup_out),
-                      (hipStream_t)stream, &ws, err,
-                      errlen))
-    return 1;
+  const size_t need = compact_workspace_bytes(pages, in_place(t));
+  if (chunk_workspace(op, workspace, workspace_bytes, need, (hipStream_t)stream, &ws, err, errlen)) return 1;
   const hipError_t e = launch_compact_pages(p, t, remap, ws, (hipStream_t)stream);
   return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
 }
