@@ -635,7 +635,7 @@ __device__ __forceinline__ void store_queries(const Queries& w, const ChunkArgs&
 // be, an operand's 64 lanes side by side.
 //
 // Bound by the matrix instruction and the power it draws: 2048 tokens over 14001 rows, 10 heads, are 158 GFLOP, three
-// times that as fp16 products, in 441 us: 1.07 PFLOP/s, where a large fp16 matrix product reaches 1.13 (and an fp32 one
+// times that as fp16 products, in 441 to 452 us: 1.05 PFLOP/s, where a large fp16 matrix product reaches 1.13 (and an fp32 one
 // 0.153, which would be 1031 us).  256 queries, since each row is converted once for all of them; the operands, 144 KB,
 // take a CU's LDS.  Waves that convert for themselves, without the four: 538 us; blocks of 64 rows: 716 (spills);
 // conversions between the matrix instructions: 588; both waves of a SIMD in step: 527; the new rows stored and rotated
