@@ -177,7 +177,7 @@ constexpr int kAbove = 2;     // binades of the walk's scales above its first bl
 constexpr int kBelow = 10;    // and below the scale that a group's largest may be
 constexpr int kFlag = 1 << 16;  // a group that the fp16 pairs cannot hold
 constexpr int kFrag = 64 * 8;   // halves of an operand: 8 of each lane
-constexpr int kMaxSplitRows = 1 << 16;  // rows of one workgroup: a bit each of their blocks in LDS
+constexpr int kMaxSplitRows = 1 << 16;  // rows of one workgroup
 
 // Six instructions with the scaling before it.  (Four, where each half is one product rounded to fp16 in place: 474 us
 // for 450 in k_chunk_tiles at 2048 tokens over 14001 rows, and nothing gained in k_chunk_few.)
@@ -259,7 +259,7 @@ struct Queries {
   int limit;   // rows the query attends
   float m, l;  // running maximum (log2), sum of the weights (times 2^kLift)
   int ev;      // o is in units of 2^(ev - 141)
-  int most;    // the largest exponent of the values so far
+  int most;    // the largest exponent of the values so far, less the binades by which their weights shrank since
   f32x16 o[4];
 };
 
@@ -301,6 +301,14 @@ __device__ __forceinline__ void load_queries(Queries& w, _Float16* qlo, const fl
   start_queries(w, scale, limit);
 }
 
+__device__ __forceinline__ void scale_sums(Queries& w, int by) {  // by 2^by, past fp32's exponents in two steps
+  const int most = min(max(by, -126), 126);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w.o[u] *= pow2_of(most);
+  if (__ballot(by != most) == 0) return;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w.o[u] *= __builtin_ldexpf(1.0f, by - most);
+}
 // Brings a lane's unit to where values of exponent eb can be added: at or above it, and not more
 // than kNear below, as far as the sum of larger ones (2^kRoom at most) stays in range.
 __device__ __forceinline__ void set_unit(Queries& w, int eb, bool attends) {
@@ -308,9 +316,7 @@ __device__ __forceinline__ void set_unit(Queries& w, int eb, bool attends) {
   const int need = max(eb, w.most - kRoom);
   const bool move = attends && (need > w.ev || need < w.ev - kNear);
   if (__ballot(move) == 0) return;
-  const float f = move ? __builtin_ldexpf(1.0f, w.ev - need) : 1.0f;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) w.o[u] *= f;
+  scale_sums(w, move ? w.ev - need : 0);
   w.ev = move ? need : w.ev;
 }
 
@@ -320,6 +326,7 @@ __device__ __forceinline__ float move_max(Queries& w, float mx) {
   const bool up = mx > w.m + kSlack;
   if (__ballot(up) != 0) {
     const float alpha = up ? __builtin_amdgcn_exp2f(w.m - mx) : 1.0f;
+    w.most = up ? max(w.most - (int)fminf(mx - w.m, 256.0f), kMinExp) : w.most;
     w.m = up ? mx : w.m;
     w.l *= alpha;
 #pragma unroll
@@ -328,83 +335,139 @@ __device__ __forceinline__ float move_max(Queries& w, float mx) {
   return w.m == -kInf ? 0.0f : w.m;
 }
 
-// What the slow path reads: a block's rows from the pool, and from old_rows on from the inputs.
+// What the fp32 form reads: a request's rows from the pool, and from old_rows on from the inputs.
 struct SlowRows {
-  const float* k;  // the block's first row
-  const float* q;  // this lane's query
-  int64_t kv_stride, slot_stride, in_stride;
-  const float* k_new;  // as if the block's first row were new
+  const float* pool;  // of the layer, the head and k
+  const uint32_t* lookup;
+  const float* k_new;  // as if row 0 were new
   const float* v_new;
-  int old_rows;  // of the block
-  const Rope* rope;
-  int64_t q_pos, row_pos;  // the query's token, and the block's first row's
-  __device__ __forceinline__ const float* table(const float* t, int64_t token) const {
-    return t + (int64_t)min(max(ldg(rope->positions + token), 0), rope->table_rows - 1) * kD;
-  }
-  __device__ __forceinline__ float q_at(int d) const {
-    if (rope == nullptr || rope->positions == nullptr) return ldg(q + d);
-    return rotated(q, table(rope->cos_t, q_pos), table(rope->sin_t, q_pos), d);
-  }
-  __device__ __forceinline__ float k_at(int key, int d) const {
-    if (key < old_rows) return ldg(k + key * slot_stride + d);
-    const float* x = k_new + key * in_stride;
-    if (rope->positions == nullptr) return ldg(x + d);
-    return rotated(x, table(rope->cos_t, row_pos + key), table(rope->sin_t, row_pos + key), d);
-  }
-  __device__ __forceinline__ const float* v_row(int key) const {
-    return key < old_rows ? k + kv_stride + key * slot_stride : v_new + key * in_stride;
-  }
+  int64_t page_stride, kv_stride, slot_stride, in_stride;
+  int P, last_page, old_rows, end;
+  Rope rope;
+  int64_t token;  // row 0's
 };
-
-// A block that the fp16 pairs cannot hold (a value that is not finite, or rows of unlike sizes beside
-// hidden ones), in fp32 and one key at a time.  stash: 32 floats a lane.
-__device__ __forceinline__ void slow_block(Queries& w, const SlowRows& rows, float scale, int live, float* stash) {
-  const int h = lane_id() >> 5;
-  float y[16], mx = -kInf;
+__device__ __forceinline__ void rotate_at(const Rope& rope, int64_t token, int col, f32x4& lo, f32x4& hi) {
+  const int64_t at = (int64_t)min(max(ldg(rope.positions + token), 0), rope.table_rows - 1) * kD + col;
+  const float *c = rope.cos_t + at, *s = rope.sin_t + at;
+  rotate4(lo, hi, *(const UOCR_GLOBAL f32x4*)c, *(const UOCR_GLOBAL f32x4*)(c + 64), *(const UOCR_GLOBAL f32x4*)s,
+          *(const UOCR_GLOBAL f32x4*)(s + 64));
+}
+// The binades of a weight above 1 (NaN: as the largest).
+__device__ __forceinline__ int weight_exp(float p) {
+  return p == 0.0f ? -kMaxExp : min((int)(__float_as_uint(p) >> 23) - 127, 16) - kLift;
+}
+// A block of rows in fp32, for inputs that the pairs cannot hold: the matrix instruction of that type, whose results have
+// the same layout (step r of the second product is keys 8 (r / 4) + r % 4 of lanes 0 to 31 and 4 on of the others, whose
+// weights the lanes hold).  Each value row is brought to its own largest and its weights take up the binades, and a
+// lane's unit follows what the weighted rows come to: a row without weight costs the others nothing, whatever its size.
+// Values that are not finite reach the queries that attend them only.  q: the lane's query, of token q_token.
+// stash: 32 floats a lane.
+__device__ __forceinline__ void slow_block(Queries& w, const SlowRows& rows, const float* q, int64_t q_token, int key0,
+                                           float scale, float* stash) {
+  const int lane = lane_id(), h = lane >> 5, last = min(rows.end - 1 - key0, kBlock - 1), live = w.limit - key0;
+  const int old_rows = rows.old_rows - key0;  // of the block
+  const uint32_t page = min(ldg(rows.lookup + key0 / rows.P), (uint32_t)rows.last_page);
+  const float* base = rows.pool + (int64_t)page * rows.page_stride + (int64_t)(key0 % rows.P) * rows.slot_stride;
+  f32x16 s = {};
+  {
+    const int key = min(lane & 31, last);
+    const float* k = (key < old_rows ? base + key * rows.slot_stride : rows.k_new + (int64_t)(key0 + key) * rows.in_stride) +
+                     4 * h;
 #pragma unroll 1
-  for (int r = 0; r < 16; ++r) {
-    const int key = 8 * (r / 4) + 4 * h + r % 4;
-    float s = 0.0f;
-    if (key < live) {
-#pragma unroll 1
-      for (int d = 0; d < kD; ++d) s = __builtin_fmaf(rows.q_at(d), rows.k_at(key, d), s);
+    for (int i = 0; i < 8; ++i) {
+      f32x4 kl = *(const UOCR_GLOBAL f32x4*)(k + 8 * i), kh = *(const UOCR_GLOBAL f32x4*)(k + 8 * i + 64);
+      f32x4 ql = *(const UOCR_GLOBAL f32x4*)(q + 8 * i + 4 * h), qh = *(const UOCR_GLOBAL f32x4*)(q + 8 * i + 4 * h + 64);
+      if (rows.rope.positions != nullptr) {
+        rotate_at(rows.rope, q_token, 8 * i + 4 * h, ql, qh);
+        if (key >= old_rows) rotate_at(rows.rope, rows.token + key0 + key, 8 * i + 4 * h, kl, kh);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(kl[e], ql[e], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(kh[e], qh[e], s, 0, 0, 0);
+      }
     }
-    stash[r * kWave] = key < live ? s * scale * 1.44269504f : -kInf;
   }
+  float mx = -kInf;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    y[r] = stash[r * kWave];
-    mx = fmaxf(mx, y[r]);
+    s[r] = 8 * (r / 4) + 4 * h + r % 4 < live ? s[r] * scale * 1.44269504f : -kInf;
+    mx = fmaxf(mx, s[r]);
   }
   const float mu = move_max(w, mx);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const float p = __builtin_amdgcn_exp2f(y[r] - mu + (float)kLift);
+    const float p = __builtin_amdgcn_exp2f(s[r] - mu + (float)kLift);
     w.l += p;
-    const float theirs = other32(p);
-    stash[(8 * (r / 4) + r % 4) * kWave] = h == 0 ? p : theirs;  // by key, for this lane's query
-    stash[(8 * (r / 4) + 4 + r % 4) * kWave] = h == 0 ? theirs : p;
+    stash[r * kWave] = p;
   }
-  uint32_t most = 0;  // of the attended rows' finite values
+  const auto key_of = [](int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; };
+  const auto finite = [](float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; };
+  const auto only_finite = [&](f32x4 x) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = finite(x[u]) ? x[u] : 0.0f;
+    return x;
+  };
+  const auto v_row = [&](int key) {
+    return key < old_rows ? base + rows.kv_stride + key * rows.slot_stride
+                          : rows.v_new + (int64_t)(key0 + key) * rows.in_stride;
+  };
+  const auto value = [&](int r) {  // columns 4 (l % 32) on of the lane's row
+    return *(const UOCR_GLOBAL f32x4*)(v_row(min(key_of(r, h), last)) + 4 * (lane & 31));
+  };
+  int top = 0;  // of the weighted rows, as an exponent of values
 #pragma unroll 1
-  for (int i = 0; i < live * 64; ++i) {
-    const uint32_t x = __float_as_uint(ldg(rows.v_row(i / 64) + 64 * h + i % 64)) & 0x7fffffffu;
-    if (x < 0x7f800000u) most = max(most, x);
+  for (int r = 0; r < 16; ++r) {
+    const f32x4 x = only_finite(value(r));
+    uint32_t bits = __float_as_uint(amax3(amax3(0.0f, x.x, x.y), x.z, x.w));
+    bits = row_max(max(bits, other<16>(bits)));
+    const int e = clamp_exp(bits);
+    stash[(16 + r) * kWave] = __int_as_float(e);
+    if (bits != 0) top = max(top, e + weight_exp(stash[r * kWave]));
   }
-  most = max(most, other<32>(most));
-  set_unit(w, clamp_exp(most), live > 0);
-  const float down = pow2_of(141 - w.ev);
+  top = max(top, (int)other<32>((uint32_t)top));
+  set_unit(w, max(top, kMinExp), live > 0);
+  uint32_t odd = 0;  // rows with values that are not finite
 #pragma unroll 1
-  for (int key = 0; key < live; ++key) {
-    const float p = stash[key * kWave];
-    const float* v = rows.v_row(key) + 16 * h;
+  for (int r = 0; r < 16; ++r) {
+    const int e = __float_as_int(stash[(16 + r) * kWave]);
+    const f32x4 v = value(r), x = only_finite(v) * pow2_of(141 - e);
+    const float p = __builtin_ldexpf(stash[r * kWave], e - w.ev);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w.o[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[u], p, w.o[u], 0, 0, 0);
+    const uint64_t bad = __ballot(!finite(v.x) || !finite(v.y) || !finite(v.z) || !finite(v.w));
+    if ((uint32_t)bad != 0) odd |= 1u << key_of(r, 0);
+    if (bad >> 32 != 0) odd |= 1u << key_of(r, 1);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (; odd != 0; odd &= odd - 1) {
+    const int key = __builtin_ctz(odd);
+    if (key >= live) continue;
+    // the weight is held by the lane of the key's half
+    const float p = stash[(4 * (key / 8) + key % 4) * kWave + (lane & 31) + 8 * (key & 4) - lane];
+    const float* v = v_row(key) + 16 * h;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const f32x4 x = *(const UOCR_GLOBAL f32x4*)(v + 32 * (i / 4) + 4 * (i % 4));
 #pragma unroll
-      for (int u = 0; u < 4; ++u) w.o[u][i] = __builtin_fmaf(p, x[u] * down, w.o[u][i]);
+      for (int u = 0; u < 4; ++u)
+        if (!finite(x[u])) w.o[u][i] = __builtin_fmaf(p, x[u], w.o[u][i]);
     }
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the stash is read before the next block's is written
+}
+// The kernel's arguments read once more, so that a part that hardly ever runs keeps none of them in registers before it.
+template <typename T>
+__device__ __forceinline__ T arguments_again() {
+  uint64_t at = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  static_assert(sizeof(T) % 4 == 0, "whole words");
+  uint32_t words[sizeof(T) / 4];
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) words[i] = ((const UOCR_CONST uint32_t*)at)[i];
+  T args;
+  __builtin_memcpy(&args, words, sizeof(T));
+  return args;
 }
 
 struct Weights {
@@ -609,6 +672,45 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs& a, const Cuts& c, Pi
   return true;
 }
 
+// The arguments of the attending kernels.
+struct Attend {
+  ChunkArgs a;
+  Rope rope;
+  Inputs in;  // where no row is new to the kernel, q alone
+  float scale;
+  float* out;
+  float* part;
+  float* weights;
+  Cuts cuts;
+};
+// What one piece of them is: rows [begin, end) of its request's, of all_rows that the tile attends.
+struct Work : Piece {
+  int begin, end, all_rows;
+};
+__device__ __forceinline__ bool find_work(const Attend& p, Work& w) {
+  if (!find_piece(p.a, p.cuts, w)) return false;
+  w.all_rows = rows_of(p.a, w, w.t_last);
+  w.begin = w.split * p.cuts.split_rows;
+  w.end = min(w.begin + p.cuts.split_rows, w.all_rows);
+  return true;
+}
+// A wave's queries, from the tile's token t0 on, over the blocks from row `first` on, `step` rows apart, in fp32.
+__device__ __forceinline__ void attend_in_fp32(Queries& w, const Attend& p, const Work& work, int t0, int first, int step,
+                                               bool news, float* stash) {
+  const int my_t = min(t0 + (lane_id() & 31), work.t_last);
+  const int64_t head = (int64_t)work.head * kD, token = work.first - work.cached;  // row 0's
+  const SlowRows rows{p.a.pool + p.a.layer_off + head, p.a.lookup + (int64_t)work.n * p.a.lookup_cols,
+                      news ? p.in.k_new + token * p.a.in_stride + head : nullptr,
+                      news ? p.in.v_new + token * p.a.in_stride + head : nullptr, p.a.page_stride, p.a.kv_stride,
+                      p.a.slot_stride, p.a.in_stride, p.a.P, p.a.pages - 1, news ? work.cached : work.end, work.end,
+                      p.rope, token};
+  start_queries(w, p.scale, min(rows_of(p.a, work, my_t), work.end));
+#pragma unroll 1
+  for (int key0 = first; key0 >= work.begin && key0 < work.end; key0 += step)
+    if (__ballot(w.limit > key0) != 0)
+      slow_block(w, rows, p.in.q + (int64_t)my_t * p.a.in_stride + head, my_t, key0, p.scale, stash);
+}
+
 // Results of one wave: into out, or, where the rows of the tile are split, normalised into part with
 // their weight's logarithm, [split][token][head][D] and [split][token][head].
 __device__ __forceinline__ void store_queries(const Queries& w, const ChunkArgs& a, int t, bool live, int head,
@@ -747,21 +849,12 @@ struct Stage {
     *(u32x2*)(at + kStep * j * kFrag) = u32x2{h0, h1};
     *(u32x2*)(at + (kStep * j + 1) * kFrag) = u32x2{l0, l1};
   }
-  __device__ __forceinline__ static void wipe(_Float16* at) {
-    constexpr int kStep = kValues ? 2 : 4;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      *(u32x2*)(at + kStep * j * kFrag) = u32x2{};
-      *(u32x2*)(at + (kStep * j + 1) * kFrag) = u32x2{};
-    }
-  }
 };
 
 // What the waves of a workgroup share besides the operands.
 struct Shared {
   int meta[4][8];  // a block's words: of its key groups, then of its value groups
   int apart[4];    // whether one of them is not 0
-  uint32_t slow[kMaxSplitRows / kBlock / 32];  // blocks left to the slow path
 };
 // The walk's scales, from the largest of each group of its first block.
 __device__ __forceinline__ int walk_scale(const int* e) {
@@ -824,12 +917,8 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     x.choose(unit, flag);
     sh.meta[i & 3][which + group] = x.word;
     if (x.word != 0) atomicOr(&sh.apart[i & 3], 1);
-    if (flag) {  // the block's weights will be zero, and so must be what they multiply
-      x.wipe(at);
-    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x.convert(j, at);
-    }
+    for (int j = 0; j < 4; ++j) x.convert(j, at);
   };
   rows.start(begin);
   load(0, 0);
@@ -893,11 +982,11 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
   }
 }
 
-// An attending wave.  The two of a SIMD (w and w + 4) take turns: between two barriers the first runs the
+// An attending wave; returns whether the pairs held all that it met.  The two of a SIMD (w and w + 4) take turns: between two barriers the first runs the
 // products of block i (the values of i - 1, the scores of i) and then its weights, the second the weights of
 // i - 1 first, so that the matrix pipe has one wave's products while the other's exponentials issue.
-__device__ __forceinline__ void attend_walk(Queries& w, int begin, int end, bool idle, bool second, const _Float16* lds,
-                                            const _Float16* qlo, Shared& sh) {
+__device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool idle, bool second, const _Float16* lds,
+                                            const _Float16* qlo, const Shared& sh) {
   const int blocks = (end - begin + kBlock - 1) / kBlock;
   lds_barrier();
   const int kunit = walk_scale(sh.meta[0]), vunit = walk_scale(sh.meta[0] + 4);
@@ -926,13 +1015,10 @@ __device__ __forceinline__ void attend_walk(Queries& w, int begin, int end, bool
     v_at = i == 0 ? 0 : v_at == 2 ? 0 : v_at + 1;
     if (second) lds_barrier();
     if (have) {
-      int live = w.limit - key0;
+      const int live = w.limit - key0;
       const bool apart = moved || __builtin_amdgcn_readfirstlane(other_scales) != 0;
       if (apart) {
-        if (apart_scores(w, s, sh.meta[i & 3], kunit, vunit, live > 0)) {
-          if (now == 0) atomicOr(&sh.slow[i / 32], 1u << (i % 32));
-          live = 0;
-        }
+        if (apart_scores(w, s, sh.meta[i & 3], kunit, vunit, live > 0)) idle = true;
         moved = __ballot(w.ev != vunit) != 0;
       }
       hide(s, live, now);
@@ -942,48 +1028,41 @@ __device__ __forceinline__ void attend_walk(Queries& w, int begin, int end, bool
     }
     if (!second) lds_barrier();
   }
+  return !idle;
 }
 
-__global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3)
-    k_chunk_tiles(ChunkArgs a, const float* q, int64_t q_stride, float* out, float scale, float* part, float* weights,
-                  Cuts cuts) {
+__global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3) k_chunk_tiles(Attend p) {
   __shared__ __align__(16) _Float16 lds[kLdsHalves];
   __shared__ __align__(16) Shared sh;
+  const ChunkArgs& a = p.a;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-  Piece qt;
-  if (!find_piece(a, cuts, qt)) return;
-  const int head = qt.head, split = qt.split, t_last = qt.t_last, split_rows = cuts.split_rows;
-  const int all_rows = rows_of(a, qt, t_last);
-  const int begin = split * split_rows, end = min(begin + split_rows, all_rows);
-  const int shown = rows_of(a, qt, qt.t0);  // rows past these are hidden from some query
-  RowWalk rows{a.pool + a.layer_off + (int64_t)head * kD, a.lookup + (int64_t)qt.n * a.lookup_cols, a.page_stride,
-               a.slot_stride, a.P, a.pages - 1, end, nullptr, nullptr, 0};
+  Work qt;
+  if (!find_work(p, qt) || qt.begin >= qt.end) return;
   if (wave >= kTileWaves) {
-    if (begin < end) convert_walk(rows, a.kv_stride, begin, shown, wave - kTileWaves, lds, sh);
+    const RowWalk rows{a.pool + a.layer_off + (int64_t)qt.head * kD, a.lookup + (int64_t)qt.n * a.lookup_cols, a.page_stride,
+                       a.slot_stride, a.P, a.pages - 1, qt.end, nullptr, nullptr, 0};
+    const int shown = rows_of(a, qt, qt.t0);  // rows past these are hidden from some query
+    convert_walk(rows, a.kv_stride, qt.begin, shown, wave - kTileWaves, lds, sh);
     return;
   }
-  if (begin >= end) return;
-  for (int i = (int)threadIdx.x; i < kMaxSplitRows / kBlock / 32; i += 64 * kTileWaves) sh.slow[i] = 0;
-  const bool idle = qt.t0 + 32 * wave > t_last;  // a wave without queries
+  const int t0 = qt.t0 + 32 * wave;
+  const bool idle = t0 > qt.t_last;  // a wave without queries
   Queries w;
   _Float16* qlo = lds + 2 * kKHalves + 3 * kVHalves + wave * kQHalves;
-  const auto my_token = [&](int lane) { return min(qt.t0 + 32 * wave + (lane & 31), t_last); };
-  const auto my_query = [&](int t) { return q + (int64_t)t * q_stride + (int64_t)head * kD; };
-  load_queries(w, qlo, my_query(my_token(lane)), scale, min(rows_of(a, qt, my_token(lane)), end));
-  attend_walk(w, begin, end, idle, wave >= kTileWaves / 2, lds, qlo, sh);
+  const int my_t = min(t0 + (lane & 31), qt.t_last);
+  load_queries(w, qlo, p.in.q + (int64_t)my_t * a.in_stride + (int64_t)qt.head * kD, p.scale,
+               min(rows_of(a, qt, my_t), qt.end));
+  const bool held = attend_walk(w, qt.begin, qt.end, idle, wave >= kTileWaves / 2, lds, qlo, sh);
   if (idle) return;
-  const int now = lane_now(), my_t = my_token(now);  // not kept through the walk
-  float* stash = (float*)lds + wave * 32 * kWave + now;
-#pragma unroll 1
-  for (int i = 0; i < (end - begin + kBlock - 1) / kBlock; ++i) {
-    const int k0 = begin + i * kBlock;
-    if ((sh.slow[i / 32] >> (i % 32) & 1) == 0 || __ballot(w.limit > k0) == 0) continue;
-    const SlowRows from{rows.at(k0), my_query(my_t), a.kv_stride, a.slot_stride, 0, nullptr, nullptr, kBlock, nullptr, 0,
-                        0};
-    slow_block(w, from, scale, min(w.limit - k0, kBlock), stash);
+  if (!held) {
+    const Attend again = arguments_again<Attend>();
+    find_work(again, qt);
+    attend_in_fp32(w, again, qt, qt.t0 + 32 * wave, qt.begin, kBlock, false, (float*)lds + wave * 32 * kWave + lane_now());
   }
-  const bool live = qt.t0 + 32 * wave + (now & 31) <= t_last;
-  store_queries(w, a, my_t, live, head, split, all_rows <= split_rows, out, part, weights);
+  const Attend to = arguments_again<Attend>();
+  const int t = qt.t0 + 32 * wave + (lane_now() & 31);  // not kept through the walk
+  store_queries(w, to.a, min(t, qt.t_last), t <= qt.t_last, qt.head, qt.split, qt.all_rows <= to.cuts.split_rows, to.out,
+                to.part, to.weights);
 }
 
 // k_chunk_few: 32 queries a workgroup, whose 4 waves take the rows' blocks in turn, each straight from memory into the
@@ -996,7 +1075,7 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3)
 // other multiplies.
 constexpr int kFewWaves = 4;
 constexpr int kFewLog2 = 5;  // queries of a workgroup
-constexpr int kFewSplitRows = kFewWaves * 64 * kBlock;  // a wave notes its slow blocks in 64 bits
+constexpr int kFewSplitRows = kFewWaves * 64 * kBlock;
 
 // 32 rows of keys or values on their way from memory to the operands of one wave.
 struct FewStage {
@@ -1031,20 +1110,25 @@ __device__ __forceinline__ int few_scale(float m, int& unit, bool& finite, bool&
   return e;
 }
 
-__global__ void __launch_bounds__(64 * kFewWaves, 2)
-    k_chunk_few(ChunkArgs a, Rope rope, Inputs in, float* out, float scale, float* part, float* weights,
-                Cuts cuts) {
-  __shared__ __align__(16) float sums[kFewWaves][32 * kD];  // the waves' sums, before that their slow paths' stash,
+// The last block of a wave, which begins with it.
+__device__ __forceinline__ int few_first(const Work& w, int wave) {
+  return w.begin + ((w.end - w.begin + kBlock - 1) / kBlock - 1 - wave) * kBlock;
+}
+
+__global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
+  const ChunkArgs& a = p.a;
+  const Rope& rope = p.rope;
+  const Inputs& in = p.in;
+  const float scale = p.scale;
+  __shared__ __align__(16) float sums[kFewWaves][32 * kD];  // the waves' sums, before that the fp32 form's stash,
   _Float16* const qs = (_Float16*)sums;             // and first the queries' operands, [part][step][lane][8]
   __shared__ float peak[kFewWaves][32], total[kFewWaves][32];
-  __shared__ int q_exp[32];
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = lane >> 5;
-  Piece qt;
-  if (!find_piece(a, cuts, qt)) return;
-  const int head = qt.head, split = qt.split, t_last = qt.t_last, split_rows = cuts.split_rows;
-  const int all_rows = rows_of(a, qt, t_last);
-  const int begin = split * split_rows, end = min(begin + split_rows, all_rows);
-  if (split == 0)  // new rows that none attends
+  __shared__ int q_exp[32], redo[kFewWaves];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  Work qt;
+  if (!find_work(p, qt)) return;
+  const int head = qt.head, t_last = qt.t_last, begin = qt.begin, end = qt.end;
+  if (qt.split == 0)  // new rows that none attends
     for (int t = qt.t0 + wave; t <= t_last; t += kFewWaves)
       if ((int64_t)qt.cached + (t - qt.first) >= a.attend_max) store_pair(a, rope, in, qt, t, head, lane);
   if (begin >= end) return;
@@ -1122,7 +1206,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
   // The blocks are dealt from the last one, which has the new rows: their latencies begin first.  What does not wait
   // for one another is asked for together: the first block's page, the queries and their positions; then the rows
   // and the tables.
-  const int first = begin + ((end - begin + kBlock - 1) / kBlock - 1 - wave) * kBlock;
+  const int first = few_first(qt, wave);
   {
     constexpr int R = 32 / kFewWaves, kPieces = 16 / kFewWaves, kStep = kD / kPieces;
     const float* base = first >= begin ? row_base(first) : pool;
@@ -1177,12 +1261,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
   const int my_t = min(qt.t0 + (lane & 31), t_last);
   start_queries(w, scale, min(rows_of(a, qt, my_t), end));
   int kunit = 0, vunit = 0;
-  uint64_t slow = 0;
+  bool held = true;  // by the pairs
 #pragma unroll 1
-  for (int key0 = first, i = 0; key0 >= begin; key0 -= kFewWaves * kBlock, ++i) {
+  for (int key0 = first; key0 >= begin; key0 -= kFewWaves * kBlock) {
     const int lane = lane_now(), h = lane >> 5;
     const int last = end - 1 - key0, next = key0 - kFewWaves * kBlock;
-    int live = w.limit - key0;
+    const int live = w.limit - key0;
     bool finite = true, own = false;
     if (key0 + kBlock > old_rows) take_new(key0, lane);
     if (last < kBlock - 1) {  // rows past the last were its copies
@@ -1214,7 +1298,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
       s = mfma(halves(hi), qh, s);
     }
     const float vm = v.largest();
-    int ev = few_scale(vm, vunit, finite, own);
+    const int ev = few_scale(vm, vunit, finite, own);
     if (own && key0 + kBlock > shown) {
       // rows hidden from some query: what they hold must not cost the others their bits
       const auto apart = [](uint32_t least, int e) {
@@ -1235,13 +1319,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
       unlike = unlike || apart(least, min(ev, clamp_exp(wave_largest(vm))));
       finite = finite && !unlike;
     }
-    if (!finite) {  // left to the slow path
-      slow |= 1ull << i;
-      live = 0;
-      ev = __builtin_amdgcn_readfirstlane(w.ev);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v.x[j] = f32x4{};
-    }
+    held = held && finite;
     const float* next_base = next >= begin ? row_base(next) : pool;
     if (next >= begin) load_k(next_base, next, lane);
     const float c = scale_of(w, ek);
@@ -1251,9 +1329,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
     if (__ballot(w.ev != ev) != 0) {
       // every lane to the block's unit, which a sum of larger values may leave no room for
       const int unit = max(ev, w.most - kRoom);
-      const float f = __builtin_ldexpf(1.0f, w.ev - unit);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w.o[u] *= f;
+      scale_sums(w, w.ev - unit);
       w.ev = unit;
     }
     Weights p;
@@ -1276,24 +1352,27 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
       }
     if (next >= begin) load_v(next_base, next, lane);
   }
-  __syncthreads();
-#pragma unroll 1
-  for (int i = 0; slow != 0; ++i, slow >>= 1) {
-    if ((slow & 1) == 0) continue;
-    const int key0 = first - i * kFewWaves * kBlock;
-    const int64_t token = token_of(key0), new0 = token * a.in_stride + (int64_t)head * kD;
-    const SlowRows from{row_base(key0), in.q + (int64_t)my_t * a.in_stride + (int64_t)head * kD, a.kv_stride,
-                        a.slot_stride, a.in_stride, in.k_new + new0, in.v_new + new0, old_rows - key0,
-                        &rope, my_t, token};
-    slow_block(w, from, scale, min(w.limit - key0, kBlock), sums[0] + wave * 32 * kWave + lane);
+  const int h = lane_now() >> 5;  // not kept through the walk
+  const auto publish = [&] {
+    const int lane = lane_now();
+    const float l = w.l + other32(w.l);
+    if (lane < 32) {
+      peak[wave][lane] = w.m;
+      total[wave][lane] = l;
+    }
+    if (lane == 0) redo[wave] = !held;
+    __syncthreads();
+  };
+  publish();
+  if (__builtin_amdgcn_readfirstlane(redo[0] | redo[1] | redo[2] | redo[3]) != 0) {
+    const Attend again = arguments_again<Attend>();
+    find_work(again, qt);
+    __syncthreads();
+    attend_in_fp32(w, again, qt, qt.t0, few_first(qt, wave), -kFewWaves * kBlock, true, sums[wave] + lane_now());
+    publish();
   }
   // the waves' sums at one maximum, in the values' own unit
-  const float l = w.l + other32(w.l);
-  if (h == 0) {
-    peak[wave][lane] = w.m;
-    total[wave][lane] = l;
-  }
-  __syncthreads();
+  const float l = total[wave][lane & 31];
   float m = peak[0][lane & 31];
 #pragma unroll
   for (int j = 1; j < kFewWaves; ++j) m = fmaxf(m, peak[j][lane & 31]);
@@ -1315,21 +1394,22 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2)
 #pragma unroll
   for (int r = 0; r < 16; ++r) *(f32x4*)(sums[wave] + at(r)) = mine(r);
   __syncthreads();
-  const bool whole = all_rows <= split_rows;
-  const int64_t stride = (int64_t)a.tokens * a.heads;
+  const Attend to = arguments_again<Attend>();
+  const bool whole = qt.all_rows <= to.cuts.split_rows;
+  const int64_t stride = (int64_t)to.a.tokens * to.a.heads;
 #pragma unroll
   for (int j = 0; j < 32 * 32 / (64 * kFewWaves); ++j) {
     const int i = j * 64 * kFewWaves + (int)threadIdx.x, query = i / 32, piece = i % 32;
-    if (qt.t0 + query > t_last) continue;
+    if (qt.t0 + query > qt.t_last) continue;
     const int from = query * kD + 4 * ((piece + query) & 31);
     f32x4 y = *(const f32x4*)(sums[0] + from);
 #pragma unroll
     for (int k2 = 1; k2 < kFewWaves; ++k2) y += *(const f32x4*)(sums[k2] + from);
-    const int64_t th = (int64_t)(qt.t0 + query) * a.heads + head;
-    *(UOCR_GLOBAL f32x4*)((whole ? out + th * kD : part + (split * stride + th) * kD) + 4 * piece) = y;
+    const int64_t th = (int64_t)(qt.t0 + query) * to.a.heads + qt.head;
+    *(UOCR_GLOBAL f32x4*)((whole ? to.out + th * kD : to.part + (qt.split * stride + th) * kD) + 4 * piece) = y;
   }
-  if (!whole && wave == 0 && h == 0 && qt.t0 + lane <= t_last)
-    weights[split * stride + ((int64_t)(qt.t0 + lane) * a.heads + head)] =
+  if (!whole && wave == 0 && h == 0 && qt.t0 + lane <= qt.t_last)
+    to.weights[qt.split * stride + ((int64_t)(qt.t0 + lane) * to.a.heads + qt.head)] =
         sum == 0.0f ? -kInf : m + __builtin_amdgcn_logf(sum);
 }
 
@@ -1477,12 +1557,12 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
   if (!c.few) {
     UOCR_LAUNCH("chunk_store", k_chunk_store, by_pair, dim3(256), 0, s, a, rope, in, p.out);
     const bool rotated_q = p.positions != nullptr;  // they wait in out
-    UOCR_LAUNCH("chunk_tiles", k_chunk_tiles, grid, dim3(64 * (kTileWaves + kStageWaves)), 0, s, a,
-                rotated_q ? p.out : p.q, rotated_q ? (int64_t)p.heads * kD : p.in_stride, p.out, p.scale, part, weights,
-                c);
+    if (rotated_q) a.in_stride = (int64_t)p.heads * kD;
+    const Attend tiles{a, Rope{}, Inputs{rotated_q ? p.out : p.q, nullptr, nullptr}, p.scale, p.out, part, weights, c};
+    UOCR_LAUNCH("chunk_tiles", k_chunk_tiles, grid, dim3(64 * (kTileWaves + kStageWaves)), 0, s, tiles);
   } else {
-    UOCR_LAUNCH("chunk_few", k_chunk_few, grid, dim3(64 * kFewWaves), 0, s, a, rope, in, p.out, p.scale, part, weights,
-                c);
+    const Attend few{a, rope, in, p.scale, p.out, part, weights, c};
+    UOCR_LAUNCH("chunk_few", k_chunk_few, grid, dim3(64 * kFewWaves), 0, s, few);
   }
   if (c.splits > 1)
     UOCR_LAUNCH("chunk_join", k_chunk_join, dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, s, a, p.out, part, weights,
