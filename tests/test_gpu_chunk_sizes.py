@@ -47,6 +47,15 @@ def _check(s, upto=None) -> None:
     assert _same_bits(pool.cpu(), s.stored(1, k, v))
 
 
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e30])
+@pytest.mark.parametrize("which", [1, 2])
+def test_large_rows_that_a_token_does_not_attend(scene, size, which) -> None:
+    """Finite ones: the second half of the chunk is large; the first half does not see it."""
+    half = scene.chunks[0] // 2
+    scene.qkv[half:scene.chunks[0], which] *= size
+    _check(scene, half)
+
+
 @pytest.mark.parametrize("odd", [math.nan, math.inf])
 def test_values_far_apart_in_a_block_beside_one_that_is_not_finite(scene, odd) -> None:
     """The first new row is 1e36 and has no weight, the others 1e-30; the tenth, in the same block, is not finite."""

@@ -1319,22 +1319,24 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
       unlike = unlike || apart(least, min(ev, clamp_exp(wave_largest(vm))));
       finite = finite && !unlike;
     }
-    held = held && finite;
+    const bool attends = live > 0;
+    // (a sum of larger values may leave no room for the block's unit)
+    held = held && finite && __ballot(attends && w.most - ev > kRoom) == 0;
     const float* next_base = next >= begin ? row_base(next) : pool;
     if (next >= begin) load_k(next_base, next, lane);
     const float c = scale_of(w, ek);
     hide(s, live, lane);
     const float lift = (float)kLift - move_max(w, largest_of(s) * c);
-    w.most = max(w.most, ev);
-    if (__ballot(w.ev != ev) != 0) {
-      // every lane to the block's unit, which a sum of larger values may leave no room for
-      const int unit = max(ev, w.most - kRoom);
-      scale_sums(w, w.ev - unit);
-      w.ev = unit;
+    // the queries that attend it to the block's unit; to the others nothing is added
+    w.most = attends ? max(w.most, ev) : w.most;
+    const int by = attends ? w.ev - ev : 0;
+    if (__ballot(by != 0) != 0) {
+      scale_sums(w, by);
+      w.ev -= by;
     }
     Weights p;
     w.l += weigh(s, c, lift, p);
-    const float vup = pow2_of(141 - max(ev, w.ev));
+    const float vup = pow2_of(141 - ev);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
