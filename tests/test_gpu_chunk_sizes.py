@@ -47,6 +47,28 @@ def _check(s, upto=None) -> None:
     assert _same_bits(pool.cpu(), s.stored(1, k, v))
 
 
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("rows", [(0,), (77,), (5, 40, 41, 100, 149)])
+def test_a_large_key_without_weight(scene, size, rows) -> None:
+    for r in rows:
+        _slot(scene, r)[0] *= 1e-3 * size
+        _slot(scene, r)[0, :, 0] = -size
+    _check(scene)
+
+
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e30])
+def test_large_elements_that_meet_zeros(scene, size) -> None:
+    """A large element of a key where the queries have a zero, and of a query where the keys have one."""
+    scene.qkv[:, 0, :, 9] = 0.0
+    _slot(scene, 60)[0, :, 9] = size
+    scene.qkv[3, 1, :, 9] = -size
+    _check(scene)
+    scene.qkv[:, 1, :, 17] = 0.0
+    scene.pool[:, 0, 1, :, :, 17] = 0.0
+    scene.qkv[::3, 0, :, 17] = size
+    _check(scene)
+
+
 @pytest.mark.parametrize("size", [1e6, 1e12, 1e30])
 @pytest.mark.parametrize("which", [1, 2])
 def test_large_rows_that_a_token_does_not_attend(scene, size, which) -> None:
@@ -72,3 +94,11 @@ def test_values_far_apart_in_a_block_beside_one_that_is_not_finite(scene, odd) -
     assert not torch.isfinite(got[9:scene.chunks[0], :, 3]).any()
     rest = [d for d in range(128) if d != 3]
     assert _far(got[9:scene.chunks[0], :, rest], want[9:scene.chunks[0], :, rest]) <= BAR
+
+
+def test_tiny_and_huge_queries_side_by_side(scene) -> None:
+    """Each query's own size costs the others nothing."""
+    n = scene.chunks[0]
+    size = 10.0 ** torch.randint(-30, 2, (n,), generator=torch.Generator().manual_seed(7)).float()
+    scene.qkv[:n, 0] *= size[:, None, None]
+    _check(scene)

@@ -172,7 +172,8 @@ constexpr int kLift = 7;      // weights are held as 2^kLift p: they stay above 
 constexpr float kSlack = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled: 2^15 p at most
 constexpr int kNear = 6;      // binades between value groups that the weights take up
 constexpr int kRoom = 60;     // binades that a sum may stand above the values now added to it
-constexpr int kSpread = 12;   // binades between the rows of one group beside hidden rows
+constexpr int kSpread = 12;   // binades between the values of one group beside hidden rows
+constexpr float kSharp = 0x1p-15f;  // the most of a score, in binades, that one step of the operands' products may be
 constexpr int kAbove = 2;     // binades of the walk's scales above its first block's largest,
 constexpr int kBelow = 10;    // and below the scale that a group's largest may be
 constexpr int kFlag = 1 << 16;  // a group that the fp16 pairs cannot hold
@@ -272,6 +273,8 @@ __device__ __forceinline__ void start_queries(Queries& w, float scale, int limit
 #pragma unroll
   for (int u = 0; u < 4; ++u) w.o[u] = f32x16{};
 }
+// The exponent of a query's scale (one that is not finite has no scores, whatever it is scaled by).
+__device__ __forceinline__ int query_exp(uint32_t bits) { return bits < 0x7f800000u ? clamp_exp(bits) : kMinExp; }
 __device__ __forceinline__ void load_queries(Queries& w, _Float16* qlo, const float* row, float scale, int limit) {
   const int h = lane_id() >> 5;
   f32x4 x[16];
@@ -281,7 +284,7 @@ __device__ __forceinline__ void load_queries(Queries& w, _Float16* qlo, const fl
 #pragma unroll
   for (int i = 0; i < 16; ++i) m = amax3(amax3(m, x[i].x, x[i].y), x[i].z, x[i].w);
   const uint32_t bits = max(__float_as_uint(m), other<32>(__float_as_uint(m)));
-  w.exp = clamp_exp(bits);
+  w.exp = query_exp(bits);
   const float up = __builtin_copysignf(pow2_of(141 - w.exp), scale);  // the scale's sign goes into the query
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
@@ -525,7 +528,11 @@ __device__ __forceinline__ void hide(f32x16& s, int live, int lane) {
   for (int r = 0; r < 16; ++r)
     if (8 * (r / 4) + r % 4 >= mine) s[r] = -kInf;
 }
-__device__ __forceinline__ float scale_of(const Queries& w, int ek) {  // > 0: hidden rows stay at -inf
+// What one of the products' sum counts as in a score's binades, where the keys' scale is ek.  (> 0: hidden rows stay at
+// -inf.)  A small element of a key or a query is off by 2^-25 of such a unit, and meets 2^15 at most: with 128 of each, a
+// score is off by a quarter of it.  Up to kSharp that is 2^-17, whatever the rows' sizes; beyond, scores of 2^15 and more
+// are at hand, and the block is not for the pairs.
+__device__ __forceinline__ float scale_of(const Queries& w, int ek) {
   return __builtin_amdgcn_fmed3f(__builtin_ldexpf(w.unit, w.exp + (ek - 282)), 1e-37f, 3.4e38f);
 }
 // The largest score of the lane's query in the block's 16 rows that the lane holds.
@@ -559,8 +566,9 @@ __device__ __forceinline__ float weigh(const f32x16& s, float c, float lift, Wei
 // Where a block's groups are at scales of their own (or an earlier block moved a lane's unit).  Before the
 // weights: the scores at the walk's scale, and the units of the sums.  Returns whether the block is the slow
 // path's.
-__device__ __forceinline__ bool apart_scores(Queries& w, f32x16& s, const int* meta, int kunit, int vunit, bool attends) {
-  int any = 0, most = 0, least = kMaxExp, far = 0;
+__device__ __forceinline__ bool apart_scores(Queries& w, f32x16& s, const int* meta, int kunit, int vunit, float c,
+                                             bool attends) {
+  int any = 0, most = 0, least = kMaxExp, far = -kMaxExp;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int wk = meta[g], wv = meta[4 + g];
@@ -572,7 +580,8 @@ __device__ __forceinline__ bool apart_scores(Queries& w, f32x16& s, const int* m
 #pragma unroll
     for (int r = 4 * g; r < 4 * g + 4; ++r) s[r] = __builtin_ldexpf(s[r], ek - kunit);
   }
-  const bool slow = __ballot(any >= kFlag || most - least > kNear || far > kRoom) != 0;
+  const bool blunt = attends && __builtin_ldexpf(c, far) > kSharp;
+  const bool slow = __ballot(any >= kFlag || most - least > kNear || far > kRoom || blunt) != 0;
   set_unit(w, most, attends && !slow);
   return slow;
 }
@@ -808,25 +817,17 @@ struct Stage {
     const float most = pow2_of(min(unit + 1, kMaxExp) - 127), least = pow2_of(max(unit - kBelow, 1) - 127);
     return __ballot(!(m < most)) == 0 && __ballot(m >= least) != 0;
   }
-  // Whether the rows are of unlike sizes: kSpread binades between the largest and the least.
+  // Whether the rows (of values) are of unlike sizes: kSpread binades between the largest and the least.
   __device__ __forceinline__ bool unlike() {
     uint32_t least = 255;
-    if constexpr (!kValues) {
-      uint32_t r = __float_as_uint(m);  // a row's lanes are 8 apart
-      r = max(r, other<32>(r));
-      r = max(r, other<16>(r));
-      r = max(r, ror<8>(r));
-      if (r != 0) least = r >> 23;
-    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t r = __float_as_uint(amax3(amax3(0.0f, x[j].x, x[j].y), x[j].z, x[j].w));
-        r = max(r, other<16>(r));
-        r = row_max(r);
-        if (r != 0) least = min(least, r >> 23);
-      }
-      least = min(least, other<32>(least));
+    for (int j = 0; j < 4; ++j) {
+      uint32_t r = __float_as_uint(amax3(amax3(0.0f, x[j].x, x[j].y), x[j].z, x[j].w));
+      r = max(r, other<16>(r));
+      r = row_max(r);
+      if (r != 0) least = min(least, r >> 23);
     }
+    least = min(least, other<32>(least));
     return e - __builtin_amdgcn_readfirstlane((int)row_min(least)) > kSpread;
   }
   // Where the group's halves go; fragments j of hi and lo are 4 (keys) or 2 (values) j on, the lo one behind.
@@ -904,14 +905,14 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     k[at].load(rows.base, row_bytes, group, last, lane);
     v[at].load(rows.base + kv_stride, row_bytes, group, last, lane);
   };
-  const auto measure = [&](auto& x, int i) {
+  const auto measure = [&](auto& x, int which, int i) {
     const int key0 = begin + i * kBlock, last = end - 1 - key0;
     if (8 * group + 7 > last) x.clear_past(group, last, lane);
     x.largest();
     x.of_all_lanes_1();
     x.of_all_lanes_2();
     // rows hidden from some query: what they hold must not cost the others their bits
-    return x.bits >= 0x7f800000u || (key0 + 8 * group + 7 >= shown && x.unlike());
+    return x.bits >= 0x7f800000u || (which != 0 && key0 + 8 * group + 7 >= shown && x.unlike());
   };
   const auto convert = [&](auto& x, int which, int i, bool flag, int unit, _Float16* at) {
     x.choose(unit, flag);
@@ -926,7 +927,7 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     rows.step(begin + kBlock);
     load(1, 1);
   }
-  const bool kflag = measure(k[0], 0), vflag = measure(v[0], 0);
+  const bool kflag = measure(k[0], 0, 0), vflag = measure(v[0], 4, 0);
   sh.meta[0][group] = k[0].bits == 0 || kflag ? 0 : k[0].e;
   sh.meta[0][4 + group] = v[0].bits == 0 || vflag ? 0 : v[0].e;
   if (group == 0 && lane < 4) sh.apart[lane] = 0;
@@ -962,9 +963,9 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[at].convert(j, vp);
       } else {
-        const bool kf = measure(k[at], i + 1);
+        const bool kf = measure(k[at], 0, i + 1);
         convert(k[at], 0, i + 1, kf, kunit, kp);
-        const bool vf = measure(v[at], i + 1);
+        const bool vf = measure(v[at], 4, i + 1);
         convert(v[at], 4, i + 1, vf, vunit, vp);
       }
       v_buf = v_buf == 2 ? 0 : v_buf + 1;
@@ -994,7 +995,8 @@ __device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool
   w.ev = w.most = vunit;
   lds_barrier();
   lds_barrier();
-  bool have = false, moved = false;
+  const bool blunt = __ballot(c > kSharp) != 0;  // the walk's scale is not for these queries: each block's is looked at
+  bool have = false, moved = blunt;
   Weights p;
   f32x16 s = {};
   int v_at = 0;  // the buffer of block i - 1's values
@@ -1018,8 +1020,8 @@ __device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool
       const int live = w.limit - key0;
       const bool apart = moved || __builtin_amdgcn_readfirstlane(other_scales) != 0;
       if (apart) {
-        if (apart_scores(w, s, sh.meta[i & 3], kunit, vunit, live > 0)) idle = true;
-        moved = __ballot(w.ev != vunit) != 0;
+        if (apart_scores(w, s, sh.meta[i & 3], kunit, vunit, c, live > 0)) idle = true;
+        moved = blunt || __ballot(w.ev != vunit) != 0;
       }
       hide(s, live, now);
       const float lift = (float)kLift - move_max(w, largest_of(s) * c);
@@ -1241,7 +1243,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
     bits = max(bits, other<32>(bits));
     bits = max(bits, other<16>(bits));
     bits = max(bits, ror<8>(bits));
-    const int e = clamp_exp(bits);
+    const int e = query_exp(bits);
     q_exp[row] = e;
     const float up = __builtin_copysignf(pow2_of(141 - e), scale);  // the scale's sign goes into the query
 #pragma unroll
@@ -1301,30 +1303,25 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
     const int ev = few_scale(vm, vunit, finite, own);
     if (own && key0 + kBlock > shown) {
       // rows hidden from some query: what they hold must not cost the others their bits
-      const auto apart = [](uint32_t least, int e) {
-        least = min(least, other<32>(least));
-        least = min(least, other<16>(least));
-        return e - __builtin_amdgcn_readfirstlane((int)row_min(least)) > kSpread;
-      };
-      uint32_t r = max(__float_as_uint(km), other<32>(__float_as_uint(km)));
-      bool unlike = apart(r != 0 ? r >> 23 : 255, min(ek, clamp_exp(wave_largest(km))));
       uint32_t least = 255;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        r = __float_as_uint(amax3(amax3(0.0f, v.x[j].x, v.x[j].y), v.x[j].z, v.x[j].w));
+        uint32_t r = __float_as_uint(amax3(amax3(0.0f, v.x[j].x, v.x[j].y), v.x[j].z, v.x[j].w));
         r = max(r, other<16>(r));
         r = row_max(r);
         if (r != 0) least = min(least, r >> 23);
       }
-      unlike = unlike || apart(least, min(ev, clamp_exp(wave_largest(vm))));
-      finite = finite && !unlike;
+      least = min(least, other<32>(least));
+      least = min(least, other<16>(least));
+      const int most = min(ev, clamp_exp(wave_largest(vm)));
+      finite = finite && most - __builtin_amdgcn_readfirstlane((int)row_min(least)) <= kSpread;
     }
+    const float c = scale_of(w, ek);
     const bool attends = live > 0;
     // (a sum of larger values may leave no room for the block's unit)
-    held = held && finite && __ballot(attends && w.most - ev > kRoom) == 0;
+    held = held && finite && __ballot(attends && (c > kSharp || w.most - ev > kRoom)) == 0;
     const float* next_base = next >= begin ? row_base(next) : pool;
     if (next >= begin) load_k(next_base, next, lane);
-    const float c = scale_of(w, ek);
     hide(s, live, lane);
     const float lift = (float)kLift - move_max(w, largest_of(s) * c);
     // the queries that attend it to the block's unit; to the others nothing is added
