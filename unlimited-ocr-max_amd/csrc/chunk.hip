@@ -168,11 +168,14 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr int kBlock = 32;    // rows (keys) a wave takes at a time: the rows of one matrix instruction
 constexpr int kMinExp = 15;   // exponents of a group's scale: 2^(141 - e) is a normal fp32
 constexpr int kMaxExp = 254;
-constexpr int kLift = 7;      // weights are held as 2^kLift p: they stay above fp16's smallest
-constexpr float kSlack = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled: 2^15 p at most
-constexpr int kNear = 6;      // binades between value groups that the weights take up
+// Weights are held as 2^kLift p, high above fp16's smallest, and a maximum may lag by 2^kSlack before the sums are rescaled:
+// 2^15.9 is below fp16's largest.  (A lift of 15 and a slack of 0.9 rescale more often: eight chunks of 256 over 1000 rows
+// 73.2 us for 72.1.)
+constexpr int kLift = 13;
+constexpr float kSlack = 2.9f;
+constexpr int kNear = 6;      // binades by which a lane's unit may be above the values now added
+constexpr int kGone = 64;     // binades below a lane's unit from which on values leave nothing in it
 constexpr int kRoom = 60;     // binades that a sum may stand above the values now added to it
-constexpr int kSpread = 12;   // binades between the values of one group beside hidden rows
 constexpr float kSharp = 0x1p-15f;  // the most of a score, in binades, that one step of the operands' products may be
 constexpr int kAbove = 2;     // binades of the walk's scales above its first block's largest,
 constexpr int kBelow = 10;    // and below the scale that a group's largest may be
@@ -229,11 +232,12 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   v = max(v, ror<2>(v));
   return max(v, ror<1>(v));
 }
-__device__ __forceinline__ uint32_t row_min(uint32_t v) {
-  v = min(v, ror<8>(v));
-  v = min(v, ror<4>(v));
-  v = min(v, ror<2>(v));
-  return min(v, ror<1>(v));
+// The largest of 64 lanes, as bits (every lane has it).
+__device__ __forceinline__ uint32_t wave_largest(float m) {
+  uint32_t bits = __float_as_uint(m);
+  bits = max(bits, other<32>(bits));
+  bits = max(bits, other<16>(bits));
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(bits));
 }
 // The lane's number as the compiler cannot know it: what is computed from it inside a loop is computed there,
 // and takes no register around the loop.
@@ -260,7 +264,7 @@ struct Queries {
   int limit;   // rows the query attends
   float m, l;  // running maximum (log2), sum of the weights (times 2^kLift)
   int ev;      // o is in units of 2^(ev - 141)
-  int most;    // the largest exponent of the values so far, less the binades by which their weights shrank since
+  int most;    // the largest unit of the sum so far, less the binades by which its weights shrank since
   f32x16 o[4];
 };
 
@@ -269,7 +273,7 @@ __device__ __forceinline__ void start_queries(Queries& w, float scale, int limit
   w.limit = limit;
   w.m = -kInf;
   w.l = 0.0f;
-  w.ev = w.most = kMinExp;
+  w.ev = w.most = kMinExp;  // (a sum of zeros)
 #pragma unroll
   for (int u = 0; u < 4; ++u) w.o[u] = f32x16{};
 }
@@ -315,12 +319,13 @@ __device__ __forceinline__ void scale_sums(Queries& w, int by) {  // by 2^by, pa
 // Brings a lane's unit to where values of exponent eb can be added: at or above it, and not more
 // than kNear below, as far as the sum of larger ones (2^kRoom at most) stays in range.
 __device__ __forceinline__ void set_unit(Queries& w, int eb, bool attends) {
-  w.most = attends ? max(w.most, eb) : w.most;
   const int need = max(eb, w.most - kRoom);
   const bool move = attends && (need > w.ev || need < w.ev - kNear);
-  if (__ballot(move) == 0) return;
-  scale_sums(w, move ? w.ev - need : 0);
-  w.ev = move ? need : w.ev;
+  if (__ballot(move) != 0) {
+    scale_sums(w, move ? w.ev - need : 0);
+    w.ev = move ? need : w.ev;
+  }
+  w.most = attends ? max(w.most, w.ev) : w.most;
 }
 
 // Moves a lane's running maximum to mx, where that is more by kSlack; returns what to take off its scores.
@@ -336,6 +341,22 @@ __device__ __forceinline__ float move_max(Queries& w, float mx) {
     for (int u = 0; u < 4; ++u) w.o[u] *= alpha;
   }
   return w.m == -kInf ? 0.0f : w.m;
+}
+
+// Whether a lane's sum is too small for what the pairs leave out of it; rows: how many, top: the largest of their values'
+// exponents (0: none but zeros).  In the sum's units a row is off by 2^-25, of its weight, times a value of 2^15 at most,
+// and by its weight times 2^-25, of its value (beside 2^-22 of the product): rows 2^-10 + l 2^-25 in all, of which the sum
+// has to be 2^17 times as much.  Values of like sizes make it so by far; less it is where a row of large values has no
+// weight, or a row of small ones nearly all of it.
+__device__ __forceinline__ bool faint(const Queries& w, int rows, int top) {
+  float m = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) m = amax3(m, w.o[u][r], w.o[u][r + 1]);
+  m = amax3(m, m, other32(m));
+  const float l = w.l + other32(w.l), off = __builtin_ldexpf((float)rows, 7 + min(top - w.most, 0)) + 0x1p-8f * l;
+  return top != 0 && l > 0.0f && m < __builtin_ldexpf(off, w.most - w.ev);
 }
 
 // What the fp32 form reads: a request's rows from the pool, and from old_rows on from the inputs.
@@ -533,7 +554,7 @@ __device__ __forceinline__ void hide(f32x16& s, int live, int lane) {
 // score is off by a quarter of it.  Up to kSharp that is 2^-17, whatever the rows' sizes; beyond, scores of 2^15 and more
 // are at hand, and the block is not for the pairs.
 __device__ __forceinline__ float scale_of(const Queries& w, int ek) {
-  return __builtin_amdgcn_fmed3f(__builtin_ldexpf(w.unit, w.exp + (ek - 282)), 1e-37f, 3.4e38f);
+  return __builtin_amdgcn_fmed3f(__builtin_ldexpf(w.unit, w.exp + (ek - 282)), 1e-35f, 3.4e38f);
 }
 // The largest score of the lane's query in the block's 16 rows that the lane holds.
 __device__ __forceinline__ float largest_of(const f32x16& s) {
@@ -568,20 +589,19 @@ __device__ __forceinline__ float weigh(const f32x16& s, float c, float lift, Wei
 // path's.
 __device__ __forceinline__ bool apart_scores(Queries& w, f32x16& s, const int* meta, int kunit, int vunit, float c,
                                              bool attends) {
-  int any = 0, most = 0, least = kMaxExp, far = -kMaxExp;
+  int any = 0, most = 0, far = -kMaxExp;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int wk = meta[g], wv = meta[4 + g];
     const int ek = wk == 0 ? kunit : wk & (kFlag - 1), ev = wv == 0 ? vunit : wv & (kFlag - 1);
     any |= wk | wv;
     most = max(most, ev);
-    least = min(least, ev);
     far = max(far, ek - kunit);
 #pragma unroll
     for (int r = 4 * g; r < 4 * g + 4; ++r) s[r] = __builtin_ldexpf(s[r], ek - kunit);
   }
   const bool blunt = attends && __builtin_ldexpf(c, far) > kSharp;
-  const bool slow = __ballot(any >= kFlag || most - least > kNear || far > kRoom || blunt) != 0;
+  const bool slow = __ballot(any >= kFlag || far > kRoom || blunt) != 0;
   set_unit(w, most, attends && !slow);
   return slow;
 }
@@ -590,7 +610,7 @@ __device__ __forceinline__ bool apart_scores(Queries& w, f32x16& s, const int* m
 __device__ __forceinline__ void apart_weights(Queries& w, f32x16& s, const int* meta, int vunit, float c, float lift) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int wv = meta[4 + g], by = min((wv == 0 ? vunit : wv & (kFlag - 1)) - w.ev, 0);
+    const int wv = meta[4 + g], by = max(min((wv == 0 ? vunit : wv & (kFlag - 1)) - w.ev, 0), -kGone);
     const float lack = __builtin_ldexpf(1.0f, -by) - 1.0f, move = (float)by / c;
 #pragma unroll
     for (int r = 4 * g; r < 4 * g + 4; ++r) {
@@ -703,7 +723,9 @@ __device__ __forceinline__ bool find_work(const Attend& p, Work& w) {
   w.end = min(w.begin + p.cuts.split_rows, w.all_rows);
   return true;
 }
-// A wave's queries, from the tile's token t0 on, over the blocks from row `first` on, `step` rows apart, in fp32.
+// A wave's queries, from the tile's token t0 on, over the blocks from row `first` on, `step` rows apart, in fp32.  Bound by
+// that matrix instruction, an eighth of the pairs' rate with their three products, and by the loads before it; with the
+// pairs' walk before, 2048 tokens over 14001 rows take 3894 us for 455, 8 requests of 7 over 1150 78 for 23.5.
 __device__ __forceinline__ void attend_in_fp32(Queries& w, const Attend& p, const Work& work, int t0, int first, int step,
                                                bool news, float* stash) {
   const int my_t = min(t0 + (lane_id() & 31), work.t_last);
@@ -817,19 +839,6 @@ struct Stage {
     const float most = pow2_of(min(unit + 1, kMaxExp) - 127), least = pow2_of(max(unit - kBelow, 1) - 127);
     return __ballot(!(m < most)) == 0 && __ballot(m >= least) != 0;
   }
-  // Whether the rows (of values) are of unlike sizes: kSpread binades between the largest and the least.
-  __device__ __forceinline__ bool unlike() {
-    uint32_t least = 255;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t r = __float_as_uint(amax3(amax3(0.0f, x[j].x, x[j].y), x[j].z, x[j].w));
-      r = max(r, other<16>(r));
-      r = row_max(r);
-      if (r != 0) least = min(least, r >> 23);
-    }
-    least = min(least, other<32>(least));
-    return e - __builtin_amdgcn_readfirstlane((int)row_min(least)) > kSpread;
-  }
   // Where the group's halves go; fragments j of hi and lo are 4 (keys) or 2 (values) j on, the lo one behind.
   __device__ __forceinline__ static _Float16* place(_Float16* lds, int i, int group, int lane) {
     if constexpr (kValues) {
@@ -856,6 +865,7 @@ struct Stage {
 struct Shared {
   int meta[4][8];  // a block's words: of its key groups, then of its value groups
   int apart[4];    // whether one of them is not 0
+  int top;         // the largest of the values' exponents (0: none but zeros)
 };
 // The walk's scales, from the largest of each group of its first block.
 __device__ __forceinline__ int walk_scale(const int* e) {
@@ -893,7 +903,7 @@ struct RowWalk {
 };
 
 // A converting wave: 8 key rows and 8 value rows of each block, loaded two blocks ahead.
-__device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, int begin, int shown, int group,
+__device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, int begin, int group,
                                              _Float16* lds, Shared& sh) {
   const int end = rows.end, blocks = (end - begin + kBlock - 1) / kBlock, lane = lane_id();
   __builtin_amdgcn_s_setprio(3);
@@ -905,14 +915,13 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     k[at].load(rows.base, row_bytes, group, last, lane);
     v[at].load(rows.base + kv_stride, row_bytes, group, last, lane);
   };
-  const auto measure = [&](auto& x, int which, int i) {
-    const int key0 = begin + i * kBlock, last = end - 1 - key0;
+  const auto measure = [&](auto& x, int i) {
+    const int last = end - 1 - (begin + i * kBlock);
     if (8 * group + 7 > last) x.clear_past(group, last, lane);
     x.largest();
     x.of_all_lanes_1();
     x.of_all_lanes_2();
-    // rows hidden from some query: what they hold must not cost the others their bits
-    return x.bits >= 0x7f800000u || (which != 0 && key0 + 8 * group + 7 >= shown && x.unlike());
+    return x.bits >= 0x7f800000u;
   };
   const auto convert = [&](auto& x, int which, int i, bool flag, int unit, _Float16* at) {
     x.choose(unit, flag);
@@ -927,10 +936,11 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     rows.step(begin + kBlock);
     load(1, 1);
   }
-  const bool kflag = measure(k[0], 0, 0), vflag = measure(v[0], 4, 0);
+  const bool kflag = measure(k[0], 0), vflag = measure(v[0], 0);
   sh.meta[0][group] = k[0].bits == 0 || kflag ? 0 : k[0].e;
   sh.meta[0][4 + group] = v[0].bits == 0 || vflag ? 0 : v[0].e;
   if (group == 0 && lane < 4) sh.apart[lane] = 0;
+  if (group == 0 && lane == 0) sh.top = 0;
   lds_barrier();
   const int kunit = walk_scale(sh.meta[0]), vunit = walk_scale(sh.meta[0] + 4);
   lds_barrier();
@@ -942,6 +952,12 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
     rows.step(begin + 2 * kBlock);
     load(2, 0);
   }
+  float top = v[0].m;  // of the lane's values
+  const auto give_top = [&] {
+    const uint32_t bits = wave_largest(top);
+    if (lane == 0 && bits != 0) atomicMax(&sh.top, clamp_exp(bits));
+  };
+  if (blocks == 1) give_top();
   lds_barrier();
   const int full = (end - begin) / kBlock;
   int v_buf = 1;
@@ -952,6 +968,8 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
       if (group == 0) sh.apart[(i + 3) & 3] = 0;  // of block i - 1, which all have read, for block i + 3
       k[at].largest();
       v[at].largest();
+      top = fmaxf(top, v[at].m);
+      if (i + 2 == blocks) give_top();
       // (at the walk's scale a hidden row costs the others nothing, whatever its size)
       if (i + 1 < full && k[at].fits(kunit) && v[at].fits(vunit)) {
         k[at].up = pow2_of(141 - kunit);
@@ -963,9 +981,9 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[at].convert(j, vp);
       } else {
-        const bool kf = measure(k[at], 0, i + 1);
+        const bool kf = measure(k[at], i + 1);
         convert(k[at], 0, i + 1, kf, kunit, kp);
-        const bool vf = measure(v[at], 4, i + 1);
+        const bool vf = measure(v[at], i + 1);
         convert(v[at], 4, i + 1, vf, vunit, vp);
       }
       v_buf = v_buf == 2 ? 0 : v_buf + 1;
@@ -992,11 +1010,11 @@ __device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool
   lds_barrier();
   const int kunit = walk_scale(sh.meta[0]), vunit = walk_scale(sh.meta[0] + 4);
   const float c = scale_of(w, kunit);
-  w.ev = w.most = vunit;
+  w.ev = vunit;
   lds_barrier();
   lds_barrier();
   const bool blunt = __ballot(c > kSharp) != 0;  // the walk's scale is not for these queries: each block's is looked at
-  bool have = false, moved = blunt;
+  bool have = false, moved = blunt, ever = false;  // whether a block was apart
   Weights p;
   f32x16 s = {};
   int v_at = 0;  // the buffer of block i - 1's values
@@ -1020,6 +1038,7 @@ __device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool
       const int live = w.limit - key0;
       const bool apart = moved || __builtin_amdgcn_readfirstlane(other_scales) != 0;
       if (apart) {
+        ever = true;
         if (apart_scores(w, s, sh.meta[i & 3], kunit, vunit, c, live > 0)) idle = true;
         moved = blunt || __ballot(w.ev != vunit) != 0;
       }
@@ -1027,10 +1046,13 @@ __device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool
       const float lift = (float)kLift - move_max(w, largest_of(s) * c);
       if (apart) apart_weights(w, s, sh.meta[i & 3], vunit, c, lift);
       w.l += weigh(s, c, lift, p);
+      if (live > 0) w.most = max(w.most, w.ev);
     }
     if (!second) lds_barrier();
   }
-  return !idle;
+  // (weights that took up binades are off by as much beside small values as beside large ones)
+  const int top = sh.top != 0 && ever ? kMaxExp : sh.top;
+  return !idle && __ballot(faint(w, w.limit - begin, top)) == 0;
 }
 
 __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3) k_chunk_tiles(Attend p) {
@@ -1043,8 +1065,7 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3) k_chunk_ti
   if (wave >= kTileWaves) {
     const RowWalk rows{a.pool + a.layer_off + (int64_t)qt.head * kD, a.lookup + (int64_t)qt.n * a.lookup_cols, a.page_stride,
                        a.slot_stride, a.P, a.pages - 1, qt.end, nullptr, nullptr, 0};
-    const int shown = rows_of(a, qt, qt.t0);  // rows past these are hidden from some query
-    convert_walk(rows, a.kv_stride, qt.begin, shown, wave - kTileWaves, lds, sh);
+    convert_walk(rows, a.kv_stride, qt.begin, wave - kTileWaves, lds, sh);
     return;
   }
   const int t0 = qt.t0 + 32 * wave;
@@ -1089,21 +1110,13 @@ struct FewStage {
     return m;
   }
 };
-// The largest of 64 lanes, as bits (every lane has it).
-__device__ __forceinline__ uint32_t wave_largest(float m) {
-  uint32_t bits = __float_as_uint(m);
-  bits = max(bits, other<32>(bits));
-  bits = max(bits, other<16>(bits));
-  return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(bits));
-}
 // The scale of a block whose lanes' largest are m: the walk's if that fits (unit 0: there is none yet, and the
 // block sets it).
-__device__ __forceinline__ int few_scale(float m, int& unit, bool& finite, bool& own) {
+__device__ __forceinline__ int few_scale(float m, int& unit, bool& finite) {
   if (unit != 0) {
     const float most = pow2_of(min(unit + 1, kMaxExp) - 127), least = pow2_of(max(unit - kBelow, 1) - 127);
     if (__ballot(!(m < most)) == 0 && __ballot(m >= least) != 0) return unit;
   }
-  own = true;
   const uint32_t bits = wave_largest(m);
   finite = finite && bits < 0x7f800000u;
   const int e = clamp_exp(bits);
@@ -1134,7 +1147,6 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
     for (int t = qt.t0 + wave; t <= t_last; t += kFewWaves)
       if ((int64_t)qt.cached + (t - qt.first) >= a.attend_max) store_pair(a, rope, in, qt, t, head, lane);
   if (begin >= end) return;
-  const int shown = rows_of(a, qt, qt.t0);
   const float* pool = a.pool + a.layer_off + (int64_t)head * kD;
   const uint32_t* lookup = a.lookup + (int64_t)qt.n * a.lookup_cols;
   const uint32_t row_bytes = (uint32_t)a.slot_stride * 4u;
@@ -1263,13 +1275,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
   const int my_t = min(qt.t0 + (lane & 31), t_last);
   start_queries(w, scale, min(rows_of(a, qt, my_t), end));
   int kunit = 0, vunit = 0;
-  bool held = true;  // by the pairs
+  bool held = true;  // whether the pairs hold all so far
+  float top = 0.0f;  // the largest of the lane's values
 #pragma unroll 1
   for (int key0 = first; key0 >= begin; key0 -= kFewWaves * kBlock) {
     const int lane = lane_now(), h = lane >> 5;
     const int last = end - 1 - key0, next = key0 - kFewWaves * kBlock;
     const int live = w.limit - key0;
-    bool finite = true, own = false;
+    bool finite = true;
     if (key0 + kBlock > old_rows) take_new(key0, lane);
     if (last < kBlock - 1) {  // rows past the last were its copies
 #pragma unroll
@@ -1279,7 +1292,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
       }
     }
     const float km = k.largest();
-    const int ek = few_scale(km, kunit, finite, own);
+    const int ek = few_scale(km, kunit, finite);
     f32x16 s = {};
     const float kup = pow2_of(141 - ek);
 #pragma unroll
@@ -1300,22 +1313,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
       s = mfma(halves(hi), qh, s);
     }
     const float vm = v.largest();
-    const int ev = few_scale(vm, vunit, finite, own);
-    if (own && key0 + kBlock > shown) {
-      // rows hidden from some query: what they hold must not cost the others their bits
-      uint32_t least = 255;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        uint32_t r = __float_as_uint(amax3(amax3(0.0f, v.x[j].x, v.x[j].y), v.x[j].z, v.x[j].w));
-        r = max(r, other<16>(r));
-        r = row_max(r);
-        if (r != 0) least = min(least, r >> 23);
-      }
-      least = min(least, other<32>(least));
-      least = min(least, other<16>(least));
-      const int most = min(ev, clamp_exp(wave_largest(vm)));
-      finite = finite && most - __builtin_amdgcn_readfirstlane((int)row_min(least)) <= kSpread;
-    }
+    const int ev = few_scale(vm, vunit, finite);
+    top = fmaxf(top, vm);
     const float c = scale_of(w, ek);
     const bool attends = live > 0;
     // (a sum of larger values may leave no room for the block's unit)
@@ -1351,6 +1350,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
       }
     if (next >= begin) load_v(next_base, next, lane);
   }
+  const uint32_t bits = wave_largest(top);
+  held = held && __ballot(faint(w, min(w.limit - begin, first - begin + kBlock), bits == 0 ? 0 : clamp_exp(bits))) == 0;
   const int h = lane_now() >> 5;  // not kept through the walk
   const auto publish = [&] {
     const int lane = lane_now();
