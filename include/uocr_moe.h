@@ -172,7 +172,8 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
  * workspace may be NULL (the library's own) or at least
  * uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max) bytes, 16-byte
  * aligned; calls that overlap in time must not share one (nor, with NULL, a stream's
- * own one across captured graphs).  out must not overlap the inputs. */
+ * own one across captured graphs).  out must not overlap the inputs, nor kv_blocks any of
+ * them. */
 size_t uocr_paged_chunk_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max);
 int uocr_paged_chunk_attention(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
                                int64_t heads, int64_t head_dim, int64_t row_stride, float* kv_blocks, int64_t pages,

@@ -842,10 +842,16 @@ static int paged_chunk_call(const char* op, float* out, const float* q, const fl
     return fail(err, errlen, "%s: the cos/sin tables must be 16-byte aligned", op);
   if (in_stride >= (int64_t)1 << 25) return fail(err, errlen, "%s: input rows must be less than 2^25 floats apart", op);
   const size_t row = (size_t)(heads * head_dim) * sizeof(float);
-  const size_t in_bytes = (size_t)(tokens - 1) * in_stride * sizeof(float) + row;
+  const size_t in_bytes = (size_t)(tokens - 1) * in_stride * sizeof(float) + row, out_bytes = (size_t)tokens * row;
   for (const float* in : {q, k_new, v_new})
-    if (overlap(out, (size_t)tokens * row, in, in_bytes))
-      return fail(err, errlen, "%s: out must not overlap the inputs", op);
+    if (overlap(out, out_bytes, in, in_bytes)) return fail(err, errlen, "%s: out must not overlap the inputs", op);
+  // a pool past 2^63 bytes is none
+  const __int128 pool = (__int128)pages * layers * 2 * page_size * (int64_t)row;
+  if (pool > INT64_MAX) return fail(err, errlen, "%s: the pool is too large", op);
+  if (overlap(out, out_bytes, kv_blocks, (size_t)pool)) return fail(err, errlen, "%s: out must not overlap kv_blocks", op);
+  for (const float* in : {q, k_new, v_new})
+    if (overlap(in, in_bytes, kv_blocks, (size_t)pool))
+      return fail(err, errlen, "%s: the inputs must not overlap kv_blocks", op);
   const hipStream_t s = (hipStream_t)stream;
   void* ws = nullptr;
   if (chunk_workspace(op, workspace, workspace_bytes,
