@@ -210,7 +210,8 @@ int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens,
  *   place) and must not overlap them, nor a list or another output, otherwise.  Each
  *   result is the same whatever the timing: pages are taken from the lowest free one
  *   up, in (row, column) order.
- *   missing int32 [1]: the entries that found no free page (they stay unset).
+ *   missing int32 [1], apart from the tables: the entries that found no free page (they
+ *   stay unset).
  *   A workspace is NULL (the library's own) or of the size asked for, 16-byte aligned
  *   (in_place: whether a table output is its input; a call that needs 0 bytes reads none);
  *   calls that overlap in time must not share one.

@@ -1,7 +1,9 @@
-"""Outputs of the chunk attention that overlap what other workgroups of the same call still
+"""Outputs of the chunk attention and of the page operators that overlap what other workgroups of the same call still
 read: refused on the host before anything is enqueued (no GPU)."""
 
 from __future__ import annotations
+
+import pytest
 
 from test_paged_refusals import _err
 
@@ -43,3 +45,17 @@ def test_a_pool_past_the_address_space_is_refused() -> None:
     assert _err("uocr_paged_chunk_attention", MB, 2 * MB, 3 * MB, 4 * MB, 4, 2, 128, 256, 16 * MB, (1 << 31) - 1,
                 (1 << 31) - 1, 128, 0, 32 * MB, 1, 2, 32 * MB, 32 * MB, 4, 1.0, 8, 0, None) == \
         "paged_chunk_attention: the pool is too large"
+
+
+# counts of nine pages at 1 and 2 MB, tables of three rows of four at 3 and 4 MB
+INPUTS, OUTPUTS = [MB, MB + 32, 3 * MB, 3 * MB + 44], [2 * MB, 2 * MB + 32, 4 * MB, 4 * MB + 44]
+
+
+@pytest.mark.parametrize(("in_place", "missing"),
+                         [(True, x) for x in INPUTS] + [(False, x) for x in INPUTS + OUTPUTS])
+def test_missing_apart_from_the_tables(in_place, missing) -> None:
+    args = (MB, MB, 3 * MB, 3 * MB, 3, 4) if in_place else (2 * MB, MB, 4 * MB, 3 * MB, 3, 4)
+    assert _err("uocr_fork_pages", 16 * MB, 9, 2, 128, 2, 128, *args, *[8 * MB] * 4, 2, missing, 6 * MB, MB, None) == \
+        "fork_pages: missing must not overlap the tables"
+    assert _err("uocr_resize_pages", args[0], MB, 9, 128, args[2], 3 * MB, 3, 4, 8 * MB, missing, None, 0, None) == \
+        "resize_pages: missing must not overlap the tables"

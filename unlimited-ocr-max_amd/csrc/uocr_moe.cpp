@@ -977,6 +977,16 @@ static int lists_apart(const char* op, const PageTables& t, int64_t pages, const
   return 0;
 }
 
+// Refuses a word of the result that is one of the tables', for the same reason.
+static int missing_apart(const char* op, const PageTables& t, int64_t pages, const int32_t* missing, char* err,
+                         size_t errlen) {
+  const size_t cb = (size_t)pages * 4, lb = (size_t)t.requests * t.cols * 4;
+  if (overlap(missing, 4, t.counts, cb) || overlap(missing, 4, t.counts_out, cb) || overlap(missing, 4, t.lookup, lb) ||
+      overlap(missing, 4, t.lookup_out, lb))
+    return fail(err, errlen, "%s: missing must not overlap the tables", op);
+  return 0;
+}
+
 int uocr_copy_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t heads,
                     int64_t head_dim, const int32_t* src, const int32_t* dst, const int32_t* rows, int64_t count,
                     void* stream, char* err, size_t errlen) {
@@ -1018,6 +1028,7 @@ int uocr_fork_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t pag
   void* ws = nullptr;
   const size_t need = fork_workspace_bytes(pages, requests, lookup_cols, count, in_place(t));
   if (chunk_workspace(op, workspace, workspace_bytes, need, (hipStream_t)stream, &ws, err, errlen)) return 1;
+  if (missing_apart(op, t, pages, missing, err, errlen)) return 1;
   const hipError_t e = launch_fork_pages(p, t, parents, children, lengths, shared_rows, (int)count, missing, ws,
                                          (hipStream_t)stream);
   return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
@@ -1046,6 +1057,7 @@ int uocr_resize_pages(int32_t* ref_counts_out, const int32_t* ref_counts, int64_
   if (chunk_workspace(op, workspace, workspace_bytes, resize_workspace_bytes(pages), (hipStream_t)stream, &ws, err,
                       errlen))
     return 1;
+  if (missing_apart(op, t, pages, missing, err, errlen)) return 1;
   const hipError_t e = launch_resize_pages(p, t, lengths, missing, ws, (hipStream_t)stream);
   return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
 }
