@@ -505,8 +505,10 @@ def _chunk_call(op: str, name: str, inputs: tuple, tokens: int, heads: int, head
     if tuple(out.shape) != (tokens, heads, head_dim):
         raise ValueError(f"{op}: out must be {(tokens, heads, head_dim)}, got {tuple(out.shape)}")
     attend_max = int(kv.attend_max)
-    ws = _workspace(op, workspace, _lib.load().uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max),
-                    like)
+    # nothing is allocated for more rows than the table addresses: the entry refuses them
+    need = _lib.load().uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max) \
+        if attend_max <= lookup.shape[1] * page_size else 0
+    ws = _workspace(op, workspace, need, like)
     _on_device(op, name, out.data_ptr(), *inputs, blocks.data_ptr(), pages, layers, page_size, int(layer_idx),
                lookup.data_ptr(), requests, lookup.shape[1], cached.data_ptr(), offsets.data_ptr(), attend_max,
                float(scale), _ptr(ws), _nbytes(ws), tensors=[*tensors, out, blocks, lookup, cached, offsets, ws])
