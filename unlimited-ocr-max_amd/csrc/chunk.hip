@@ -1550,7 +1550,8 @@ hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s) {
   const int64_t pairs = p.tokens * p.heads, items = (int64_t)c.slots * p.heads * c.splits;
   const int64_t joins = p.tokens * ((p.heads + kJoinHeads - 1) / kJoinHeads);
   const dim3 by_pair((unsigned)((pairs + 3) / 4)), grid((unsigned)((items + 7) / 8 * 8));
-  if (items > INT32_MAX - 8) return hipErrorInvalidValue;
+  // (where a wave counts the pieces, offsets that do not ascend may give each request all of them)
+  if (items > (p.requests <= 64 ? INT32_MAX / p.requests : INT32_MAX) - 8) return hipErrorInvalidValue;
   const Inputs in{p.q, p.k_new, p.v_new};
   float* part = (float*)p.workspace;
   float* weights = part + (int64_t)c.splits * pairs * kD;
