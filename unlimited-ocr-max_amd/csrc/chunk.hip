@@ -14,7 +14,9 @@
 // the workgroup whose queries its token is among; nothing else in the launch reads that pool row.
 //
 // k_chunk_tiles (256 queries a workgroup) and k_chunk_few (32) run the two products on the fp16 matrix instruction,
-// each operand as a pair of halves, and keep a running maximum and sum of every query (below).
+// each operand as a pair of halves, and keep a running maximum and sum of every query (below).  A piece that the pairs
+// cannot hold (values that are not finite, keys whose scores would lose bits beside larger ones, sums that came out too
+// small for what the pairs leave out) is done again in fp32 by the same workgroup.
 #include <algorithm>
 
 #include "uocr_device.h"
@@ -158,6 +160,7 @@ __global__ void __launch_bounds__(256) k_chunk_store(ChunkArgs a, Rope rope, Inp
 // An operand x (times a power of two that brings its group's largest to [2^14, 2^15)) is held
 // as hi = fp16(x), lo = fp16(x - hi): 22 bits, or 2^-39 of the group's largest where
 // that is more.  hi hi + hi lo + lo hi leaves out lo lo, 2^-22 of the product at most.
+// Where 2^-39 of the largest could count, kSharp (scores) and faint (sums) find it out.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -585,8 +588,8 @@ __device__ __forceinline__ float weigh(const f32x16& s, float c, float lift, Wei
 }
 
 // Where a block's groups are at scales of their own (or an earlier block moved a lane's unit).  Before the
-// weights: the scores at the walk's scale, and the units of the sums.  Returns whether the block is the slow
-// path's.
+// weights: the scores at the walk's scale, and the units of the sums.  Returns whether the block is not for
+// the pairs.
 __device__ __forceinline__ bool apart_scores(Queries& w, f32x16& s, const int* meta, int kunit, int vunit, float c,
                                              bool attends) {
   int any = 0, most = 0, far = -kMaxExp;
@@ -712,15 +715,15 @@ struct Attend {
   float* weights;
   Cuts cuts;
 };
-// What one piece of them is: rows [begin, end) of its request's, of all_rows that the tile attends.
+// What one piece of them is: rows [begin, stop) of its request's, of all_rows that the tile attends.
 struct Work : Piece {
-  int begin, end, all_rows;
+  int begin, stop, all_rows;
 };
 __device__ __forceinline__ bool find_work(const Attend& p, Work& w) {
   if (!find_piece(p.a, p.cuts, w)) return false;
   w.all_rows = rows_of(p.a, w, w.t_last);
   w.begin = w.split * p.cuts.split_rows;
-  w.end = min(w.begin + p.cuts.split_rows, w.all_rows);
+  w.stop = min(w.begin + p.cuts.split_rows, w.all_rows);
   return true;
 }
 // A wave's queries, from the tile's token t0 on, over the blocks from row `first` on, `step` rows apart, in fp32.  Bound by
@@ -733,15 +736,17 @@ __device__ __forceinline__ void attend_in_fp32(Queries& w, const Attend& p, cons
   const SlowRows rows{p.a.pool + p.a.layer_off + head, p.a.lookup + (int64_t)work.n * p.a.lookup_cols,
                       news ? p.in.k_new + token * p.a.in_stride + head : nullptr,
                       news ? p.in.v_new + token * p.a.in_stride + head : nullptr, p.a.page_stride, p.a.kv_stride,
-                      p.a.slot_stride, p.a.in_stride, p.a.P, p.a.pages - 1, news ? work.cached : work.end, work.end,
+                      p.a.slot_stride, p.a.in_stride, p.a.P, p.a.pages - 1, news ? work.cached : work.stop, work.stop,
                       p.rope, token};
-  start_queries(w, p.scale, min(rows_of(p.a, work, my_t), work.end));
+  start_queries(w, p.scale, min(rows_of(p.a, work, my_t), work.stop));
 #pragma unroll 1
-  for (int key0 = first; key0 >= work.begin && key0 < work.end; key0 += step)
+  for (int key0 = first; key0 >= work.begin && key0 < work.stop; key0 += step)
     if (__ballot(w.limit > key0) != 0)
       slow_block(w, rows, p.in.q + (int64_t)my_t * p.a.in_stride + head, my_t, key0, p.scale, stash);
 }
 
+// The logarithm of a sum of weights, of which the lift would leave fewer bits.
+__device__ __forceinline__ float log2_weight(float l) { return __builtin_amdgcn_logf(l * pow2_of(-kLift)); }
 // Results of one wave: into out, or, where the rows of the tile are split, normalised into part with
 // their weight's logarithm, [split][token][head][D] and [split][token][head].
 __device__ __forceinline__ void store_queries(const Queries& w, const ChunkArgs& a, int t, bool live, int head,
@@ -760,7 +765,7 @@ __device__ __forceinline__ void store_queries(const Queries& w, const ChunkArgs&
     *(UOCR_GLOBAL f32x4*)(dst + 32 * (r / 4) + 4 * (r % 4)) = v;
   }
   if (!whole && h == 0)  // no row attended: no weight
-    weights[(int64_t)split * a.tokens * a.heads + th] = l == 0.0f ? -kInf : w.m + __builtin_amdgcn_logf(l);
+    weights[(int64_t)split * a.tokens * a.heads + th] = l == 0.0f ? -kInf : w.m + log2_weight(l);
 }
 
 // k_chunk_tiles: 8 waves of 32 queries each walk the rows together, a block of 32 at a time.  4 more bring the
@@ -768,11 +773,11 @@ __device__ __forceinline__ void store_queries(const Queries& w, const ChunkArgs&
 // be, an operand's 64 lanes side by side.
 //
 // Bound by the matrix instruction and the power it draws: 2048 tokens over 14001 rows, 10 heads, are 158 GFLOP, three
-// times that as fp16 products, in 441 to 452 us: 1.05 PFLOP/s, where a large fp16 matrix product reaches 1.13 (and an fp32 one
-// 0.153, which would be 1031 us).  256 queries, since each row is converted once for all of them; the operands, 144 KB,
-// take a CU's LDS.  Waves that convert for themselves, without the four: 538 us; blocks of 64 rows: 716 (spills);
-// conversions between the matrix instructions: 588; both waves of a SIMD in step: 527; the new rows stored and rotated
-// here and not by k_chunk_store: 551, and 8 prompts 83 us for 68.
+// times that as fp16 products, in 433 to 469 us (cards differ): 1.01 to 1.09 PFLOP/s, where a large fp16 matrix product
+// reaches 1.13 (and an fp32 one 0.153, which would be 1031 us).  256 queries, since each row is converted once for all of
+// them; the operands, 144 KB, take a CU's LDS.  Waves that convert for themselves, without the four: 538 us; blocks of 64
+// rows: 716 (spills); conversions between the matrix instructions: 588; both waves of a SIMD in step: 527; the new rows
+// stored and rotated here and not by k_chunk_store: 551, and 8 prompts 83 us for 68.
 constexpr int kTileWaves = 8;   // that attend
 constexpr int kStageWaves = 4;  // that convert: one a SIMD, beside two that attend
 constexpr int kTileLog2 = 8;    // queries of a workgroup
@@ -970,7 +975,6 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
       v[at].largest();
       top = fmaxf(top, v[at].m);
       if (i + 2 == blocks) give_top();
-      // (at the walk's scale a hidden row costs the others nothing, whatever its size)
       if (i + 1 < full && k[at].fits(kunit) && v[at].fits(vunit)) {
         k[at].up = pow2_of(141 - kunit);
         v[at].up = pow2_of(141 - vunit);
@@ -1001,9 +1005,10 @@ __device__ __forceinline__ void convert_walk(RowWalk rows, int64_t kv_stride, in
   }
 }
 
-// An attending wave; returns whether the pairs held all that it met.  The two of a SIMD (w and w + 4) take turns: between two barriers the first runs the
-// products of block i (the values of i - 1, the scores of i) and then its weights, the second the weights of
-// i - 1 first, so that the matrix pipe has one wave's products while the other's exponentials issue.
+// An attending wave; returns whether the pairs held all that it met.  The two of a SIMD (w and w + 4) take turns: between
+// two barriers the first runs the products of block i (the values of i - 1, the scores of i) and then its weights, the
+// second the weights of i - 1 first, so that the matrix pipe has one wave's products while the other's exponentials
+// issue.
 __device__ __forceinline__ bool attend_walk(Queries& w, int begin, int end, bool idle, bool second, const _Float16* lds,
                                             const _Float16* qlo, const Shared& sh) {
   const int blocks = (end - begin + kBlock - 1) / kBlock;
@@ -1061,10 +1066,10 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3) k_chunk_ti
   const ChunkArgs& a = p.a;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   Work qt;
-  if (!find_work(p, qt) || qt.begin >= qt.end) return;
+  if (!find_work(p, qt) || qt.begin >= qt.stop) return;
   if (wave >= kTileWaves) {
     const RowWalk rows{a.pool + a.layer_off + (int64_t)qt.head * kD, a.lookup + (int64_t)qt.n * a.lookup_cols, a.page_stride,
-                       a.slot_stride, a.P, a.pages - 1, qt.end, nullptr, nullptr, 0};
+                       a.slot_stride, a.P, a.pages - 1, qt.stop, nullptr, nullptr, 0};
     convert_walk(rows, a.kv_stride, qt.begin, wave - kTileWaves, lds, sh);
     return;
   }
@@ -1074,8 +1079,8 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3) k_chunk_ti
   _Float16* qlo = lds + 2 * kKHalves + 3 * kVHalves + wave * kQHalves;
   const int my_t = min(t0 + (lane & 31), qt.t_last);
   load_queries(w, qlo, p.in.q + (int64_t)my_t * a.in_stride + (int64_t)qt.head * kD, p.scale,
-               min(rows_of(a, qt, my_t), qt.end));
-  const bool held = attend_walk(w, qt.begin, qt.end, idle, wave >= kTileWaves / 2, lds, qlo, sh);
+               min(rows_of(a, qt, my_t), qt.stop));
+  const bool held = attend_walk(w, qt.begin, qt.stop, idle, wave >= kTileWaves / 2, lds, qlo, sh);
   if (idle) return;
   if (!held) {
     const Attend again = arguments_again<Attend>();
@@ -1094,8 +1099,8 @@ __global__ void __launch_bounds__(64 * (kTileWaves + kStageWaves), 3) k_chunk_ti
 //
 // Bound by the trips to memory where there are few rows (metadata; queries, page and positions; rows and tables: 11 us
 // for 4 tokens over 300 rows) and by the rows' bytes where there are many: 8 requests of 7 over 1150 rows, 68 MB, in
-// 19 us, 3.6 TB/s.  No row goes by way of LDS, so two workgroups share a CU, and one's loads are under way while the
-// other multiplies.
+// 21 us, 3.2 TB/s.  (The form in fp32 behind it costs 0.8 of them by being there, whichever way it is called.)  No row goes
+// by way of LDS, so two workgroups share a CU, and one's loads are under way while the other multiplies.
 constexpr int kFewWaves = 4;
 constexpr int kFewLog2 = 5;  // queries of a workgroup
 constexpr int kFewSplitRows = kFewWaves * 64 * kBlock;
@@ -1127,7 +1132,7 @@ __device__ __forceinline__ int few_scale(float m, int& unit, bool& finite) {
 
 // The last block of a wave, which begins with it.
 __device__ __forceinline__ int few_first(const Work& w, int wave) {
-  return w.begin + ((w.end - w.begin + kBlock - 1) / kBlock - 1 - wave) * kBlock;
+  return w.begin + ((w.stop - w.begin + kBlock - 1) / kBlock - 1 - wave) * kBlock;
 }
 
 __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
@@ -1142,7 +1147,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   Work qt;
   if (!find_work(p, qt)) return;
-  const int head = qt.head, t_last = qt.t_last, begin = qt.begin, end = qt.end;
+  const int head = qt.head, t_last = qt.t_last, begin = qt.begin, end = qt.stop;
   if (qt.split == 0)  // new rows that none attends
     for (int t = qt.t0 + wave; t <= t_last; t += kFewWaves)
       if ((int64_t)qt.cached + (t - qt.first) >= a.attend_max) store_pair(a, rope, in, qt, t, head, lane);
@@ -1410,7 +1415,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) k_chunk_few(Attend p) {
   }
   if (!whole && wave == 0 && h == 0 && qt.t0 + lane <= qt.t_last)
     to.weights[qt.split * stride + ((int64_t)(qt.t0 + lane) * to.a.heads + qt.head)] =
-        sum == 0.0f ? -kInf : m + __builtin_amdgcn_logf(sum);
+        sum == 0.0f ? -kInf : m + log2_weight(sum);
 }
 
 // Joins the splits of a token's rows: a wave takes four heads of a token, four columns a lane, half a wave a head.  The
@@ -1482,14 +1487,17 @@ __global__ void __launch_bounds__(256) k_chunk_join(ChunkArgs a, float* out, con
 // How a call's rows are cut: tiles of 256 or of 32 queries, and splits of their rows where the tiles alone do not fill
 // the device.  A tile of 256 has a CU to itself and converts each row once for all its queries, but a short chunk
 // leaves most of it empty, and it has more to set up; tiles of 32 convert and read each row eight times as often.
-// Measured, 10 heads, tiles of 256 / tiles of 32, in us: one request of 256 tokens 33 / 24, of 512 41 / 30, of 1024
-// 50 / 69; of 256 tokens over 2000 cached rows 45 / 41, of 512 51 / 68, of 32 over 14000 48 / 42, of 64 52 / 55, of 128
-// 59 / 80, of 512 206 / 240; four of 128 tokens 24 / 19, of 512 57 / 69; eight of 32 over 1000 rows 35 / 28, of 64
-// 39 / 43, of 128 49 / 68; 64 of 33 over 300 81 / 72, of 64 107 / 90; 100 of 7 over 500 124 / 94.
+// Measured, 10 heads, tiles of 256 / tiles of 32, in us: one request of 256 tokens 32 / 18, of 512 39 / 23, of 1024
+// 46 / 58; of 256 tokens over 2000 cached rows 43 / 38, of 512 49 / 72, of 32 over 14000 50 / 46, of 64 53 / 58, of 128
+// 59 / 95, of 512 202 / 348; four of 128 tokens 22 / 18, of 512 50 / 43; eight of 32 over 1000 rows 34 / 25, of 64
+// 37 / 42, of 128 45 / 61; 64 of 33 over 300 73 / 57, of 64 95 / 73; 100 of 7 over 500 118 / 87.  The rule goes by two
+// numbers and takes the slower near its border: one of 64 over 14000, eight of 64 over 1000, four of 512, by up to a
+// sixth.  It was measured at 10 heads, and takes every request for an average one: a chunk of 2048 over 14001 rows, 456
+// us alone, takes 1081 beside 31 of one token, and 4 tokens over 14001 rows 44 us alone and 110 beside seven empty chunks.
 //
 // More splits than fill the device once make some CUs take two pieces while others wait: two requests of 1024 in
-// splits of 256 rows 60 us, of 1024 rows 86.  Tiles of 32 go two to a CU, and share it: 256, 384 and 512 pieces, eight
-// requests of 7 over 1150 rows 27 / 25 / 28 us, of 32 over 1000 33 / 28 / 28, one of 8 over 14000 37 / 39 / 40.
+// splits of 256 rows 55 us, of 1024 rows 86.  Tiles of 32 go two to a CU, and share it: 256, 384 and 512 pieces, eight
+// requests of 7 over 1150 rows 27 / 24 / 27 us, of 32 over 1000 32 / 25 / 25, one of 8 over 14000 39 / 44 / 44.
 namespace {
 constexpr int kCus = 256;
 struct Cut : Cuts {

@@ -132,9 +132,10 @@ __device__ __forceinline__ int pages_for(int32_t rows, const Divide& by_page, in
 // then missing ones are taken, in (request, column) order, from the free pages in
 // ascending order (the released ones among them).
 //
-// One scan over the counts and one over the entries, of 16384 elements each at a time; what bounds it is latency: a
-// trip to memory for the counts, lengths and entries together, and one for the results.  256 requests of 32 pages in a
-// pool of 6001: 11.2 us on the device, of 8 requests in 81 pages 3.6.
+// One scan over the counts and one over the entries, in rounds of 2048 elements; what bounds it is latency: where each
+// is one round, a trip to memory for the counts, lengths and entries together and one for the results (8 requests in 81
+// pages: 3.5 us on the device), else a trip for each round (256 requests of 32 pages in a pool of 6001, three rounds of
+// counts and four of entries: 11.1).
 template <bool kLds>
 __global__ void __launch_bounds__(kTableThreads) k_resize(PageTables t, int pages, Divide by_page, Divide by_cols,
                                                           const int32_t* __restrict__ lengths, int32_t* missing,
