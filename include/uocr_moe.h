@@ -166,9 +166,14 @@ int uocr_paged_decode_attention_qkv(float* out, const float* qkv, int64_t rows, 
  * Rows of out that no chunk holds are left as they were, as is every row of the
  * pool that is no new token's.  Device metadata is clamped as there: a row past what
  * the lookup row addresses is neither stored nor attended, nor is one past attend_max
- * attended.  Two requests may share pages that no chunk writes.  fp32 in and out;
- * the products are of operands held to 22 bits (pairs of fp16) and summed in fp32, as
- * are the softmax's maxima and sums.
+ * attended.  Two requests may share pages that no chunk writes.  A chunk is appended:
+ * rows that are written again, as a ring's are by paged_decode_attention's write_index,
+ * have no form here, so a draft ends where its ring wraps.
+ *   fp32 in and out; the products are of operands held to 22 bits (pairs of fp16) and
+ * summed in fp32, as are the softmax's maxima and sums.  Where rows or elements of
+ * unlike sizes, or small weights, would lose more than that of a score or a sum, and
+ * where a value is not finite, the products are fp32's; such calls take up to nine
+ * times as long.
  * workspace may be NULL (the library's own) or at least
  * uocr_paged_chunk_workspace_bytes(tokens, requests, heads, attend_max) bytes, 16-byte
  * aligned; calls that overlap in time must not share one (nor, with NULL, a stream's

@@ -436,6 +436,9 @@ class PagedChunk:
     uint32), each request's rows in the cache before its chunk; ``chunk_offsets`` int32 ``[N + 1]``, ascending:
     request ``n``'s chunk is token rows ``chunk_offsets[n]`` up to ``chunk_offsets[n + 1]`` (none: an empty
     chunk); ``attend_max`` the largest sum of the two, a host int.
+
+    Chunks are appended.  A ring's rows, which :class:`PagedKv` writes again by its ``write_index``, have no form here:
+    a draft ends where its ring wraps.
     """
 
     kv_blocks: torch.Tensor
