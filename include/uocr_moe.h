@@ -265,6 +265,116 @@ int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t 
                        const uint32_t* lookup, int64_t requests, int64_t lookup_cols, int32_t* remap, void* workspace,
                        size_t workspace_bytes, void* stream, char* err, size_t errlen);
 
+/* ---------------------------------------------------------------------------
+ * An int8 pool (quantised as it is written), and trees of drafted tokens.  The
+ * reference's pool is fp32 and its decode step one token a request; these are the
+ * forms of paged_decode_attention and paged_chunk_attention (decoder.py:425-437) next
+ * to them.
+ *   int8 pool: int8 [pages, 2 (k, v), layers, page_size, slot_bytes].  A row's slot holds
+ *   its heads' 128 values each, then an fp32 scale of each head; slot_bytes is at least
+ *   132 * heads and a multiple of 16 (of 128: a head's row is then one line).  A value q of
+ *   a head stands for q * scale.  A row x is written as scale = max|x| * (1 / 127 as fp32), 1
+ *   where that is 0, q = rint(x / scale), each step rounded to fp32 (the weights' form per 128
+ *   values, tools/quantize_int8.py:54-70); a row with a value that is not
+ *   finite gets the scale NaN, and what attends it is NaN.
+ *   q, k_new, v_new: fp32 [tokens, heads, 128] whose rows are row_stride floats apart;
+ *   with `positions` (int32 [tokens], else NULL) q and k_new come before RoPE and are
+ *   rotated as uocr_rope does (tables fp32 [table_rows, 128], 16-byte aligned).
+ *   New rows are stored first; what is attended is what the pool then holds.
+ *   Lookup, lengths, offsets and attend_max as for the fp32 entries; tokens * heads at most
+ *   2^25.  workspace: uocr_paged_pool_workspace_bytes(tokens, requests, heads, attend_max)
+ *   bytes, 16-byte aligned, or NULL (the library's own).
+ * ------------------------------------------------------------------------- */
+size_t uocr_paged_pool_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max);
+
+/* paged_decode_attention over an int8 pool: row b's new row at write_index[b], rows
+ * [0, attend_lengths[b] + 1) attended. */
+int uocr_paged_decode_attention_int8(float* out, const float* q, const float* k_new, const float* v_new, int64_t rows,
+                                     int64_t heads, int64_t head_dim, int64_t row_stride, const int32_t* positions,
+                                     const float* cos_table, const float* sin_table, int64_t table_rows, int8_t* kv_blocks,
+                                     int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes, int64_t layer,
+                                     const uint32_t* lookup, int64_t lookup_cols, const uint32_t* attend_lengths,
+                                     int64_t attend_max, const uint32_t* write_index, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream, char* err, size_t errlen);
+
+/* paged_chunk_attention over an int8 pool.  visible NULL: token i of a chunk attends its
+ * request's rows [0, cached + i].  visible int64 [tokens]: it attends the rows [0, cached)
+ * and, of its own chunk, row cached + j for every set bit j of its word (the first 64
+ * tokens of a chunk can be attended; itself is one of the bits).  A token that attends
+ * nothing gets 0. */
+int uocr_paged_chunk_attention_int8(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
+                                    int64_t heads, int64_t head_dim, int64_t row_stride, const int32_t* positions,
+                                    const float* cos_table, const float* sin_table, int64_t table_rows, int8_t* kv_blocks,
+                                    int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes, int64_t layer,
+                                    const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                                    const uint32_t* cache_lengths, const int32_t* chunk_offsets, int64_t attend_max,
+                                    const int64_t* visible, float scale, void* workspace, size_t workspace_bytes,
+                                    void* stream, char* err, size_t errlen);
+
+/* The same with `visible` over the fp32 pool [pages, 2, layers, page_size, heads, 128].  A
+ * token that attends a row with a value that is not finite gets NaN. */
+int uocr_paged_tree_attention(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
+                              int64_t heads, int64_t head_dim, int64_t row_stride, const int32_t* positions,
+                              const float* cos_table, const float* sin_table, int64_t table_rows, float* kv_blocks,
+                              int64_t pages, int64_t layers, int64_t page_size, int64_t layer, const uint32_t* lookup,
+                              int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
+                              const int32_t* chunk_offsets, int64_t attend_max, const int64_t* visible, float scale,
+                              void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
+
+/* quantize_pages / dequantize_pages -- page dst[i] of the one pool = page src[i] of the
+ * other, k and v of all layers, as if one pair after the other; with rows (int32 [count],
+ * may be NULL) the first rows[i] rows of each layer only.  Pairs with an id outside its
+ * pool are skipped.  Lists on the device. */
+int uocr_quantize_pages(const float* kv_blocks, int64_t fp32_pages, int8_t* kv_int8, int64_t int8_pages, int64_t layers,
+                        int64_t page_size, int64_t heads, int64_t slot_bytes, const int32_t* src, const int32_t* dst,
+                        const int32_t* rows, int64_t count, void* stream, char* err, size_t errlen);
+int uocr_dequantize_pages(const int8_t* kv_int8, int64_t int8_pages, float* kv_blocks, int64_t fp32_pages, int64_t layers,
+                          int64_t page_size, int64_t heads, int64_t slot_bytes, const int32_t* src, const int32_t* dst,
+                          const int32_t* rows, int64_t count, void* stream, char* err, size_t errlen);
+
+/* draft_masks -- the words `visible` of trees.  A request's chunk is its tree: token 0 the
+ * root, parents int32 [tokens] the place in the chunk of each one's parent, which comes
+ * before it (any other value: it has none).  masks int64 [tokens]: bits of a token's
+ * ancestors and its own. */
+int uocr_draft_masks(int64_t* masks, const int32_t* parents, int64_t tokens, const int32_t* chunk_offsets, int64_t requests,
+                     void* stream, char* err, size_t errlen);
+
+/* accept_drafts -- what of the trees the model's answers confirm.  drafted int32 [tokens] the
+ * trees' tokens, answers int32 [tokens] what the model says after each.  The path starts at
+ * token 0 and goes on to the first child whose token is its parent's answer; the first 64
+ * tokens of a chunk count.  counts int32 [requests] its length (0: an empty chunk), path
+ * int32 [tokens] its tokens' places in the chunk, at the front of the chunk's words, -1
+ * behind them; next_tokens int32 [requests] the answer to the last (-1: an empty chunk);
+ * cache_lengths_out uint32 [requests] = cache_lengths + counts.  The path's rows, k and v of all
+ * layers, move to rows cached, cached + 1, ... of the request.  kv_blocks: a pool of either
+ * kind, slot_bytes a multiple of 16 (fp32: heads * 512).  Outputs overlap nothing. */
+int uocr_accept_drafts(void* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes,
+                       const uint32_t* lookup, int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
+                       const int32_t* chunk_offsets, const int32_t* parents, const int32_t* drafted, const int32_t* answers,
+                       int64_t tokens, int32_t* counts, int32_t* path, int32_t* next_tokens, uint32_t* cache_lengths_out,
+                       void* stream, char* err, size_t errlen);
+
+/* beam_select -- a step of beam search: of each request's `beams` rows (1 to 32) and their next
+ * tokens the best `beams`, in order.  logits fp32 [rows, vocab]; scores fp32 [rows], each
+ * beam's sum of log probabilities (-inf: none yet, as all but the first beam of a new request).
+ *   key = scores[b] + (logits[b, v] - log sum exp logits[b]); a beam with ended[b] (int32
+ *   [rows], may be NULL) not 0 has one candidate, eos with key = scores[b].
+ *   rank = key, or, given lengths (int32 [rows]), key / length^alpha, the length being
+ *   lengths[b] + 1, of an ended beam lengths[b].
+ * Keys and ranks are in 64 bits, ties go to the lower (row, token).  Candidates without a finite rank come
+ * last and get the score -inf.  Outputs, row by row: the token, the parent row, the key as fp32, whether it has
+ * ended (its parent had, or the token is eos), the length, and the history (int32 [rows,
+ * width]): the parent's, of a live one without its first id and with the token at the end.
+ * lengths and history have an output each, or both are NULL.  workspace:
+ * uocr_beam_select_workspace_bytes, 16-byte aligned, or NULL (the library's own).  Outputs
+ * overlap nothing.  No counterpart in the reference, which decodes one beam. */
+size_t uocr_beam_select_workspace_bytes(int64_t rows, int64_t vocab, int64_t beams);
+int uocr_beam_select(int32_t* tokens, int32_t* parents, float* scores_out, int32_t* ended_out, int32_t* lengths_out,
+                     int32_t* history_out, const float* logits, int64_t rows, int64_t vocab, int64_t beams,
+                     const float* scores, int64_t eos, const int32_t* ended, const int32_t* lengths, double alpha,
+                     const int32_t* history, int64_t width, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                     size_t errlen);
+
 /* rms_norm -- replaces RmsNorm.__call__ (unlimited_ocr_max/decoder.py:252-261,
  * ops.rms_norm with gamma cast to fp32) and, given `residual`, the residual add
  * before it (DecoderLayer.decode, decoder.py:702-709).

@@ -19,14 +19,12 @@
 // small for what the pairs leave out) is done again in fp32 by the same workgroup.
 #include <algorithm>
 
-#include "uocr_device.h"
+#include "chunk_device.h"
 #include "uocr_kernels.h"
 
 namespace uocr {
 
 namespace {
-
-constexpr int kD = 128;
 
 struct ChunkArgs {
   float* pool;
@@ -48,68 +46,10 @@ struct ChunkArgs {
   int64_t in_stride;  // floats between rows of q / k_new / v_new
 };
 
-// A request's chunk: its token rows [first, end) and its cached rows.
-struct Chunk {
-  int n, first, end, cached;
-};
-// The last request n with floor(off[n] / 2^log2) + (n if `numbered`) <= key, found by the whole wave: 64 probes at a
-// time, whose last round brings the request's metadata along.  Offsets are device data: whatever they hold, the
-// request is one of them.
-__device__ __forceinline__ Chunk find_chunk(const ChunkArgs& a, int log2, bool numbered, int64_t key) {
-  const int lane = lane_id();
-  const auto below = [&](int off, int i) { return (int64_t)(off >> log2) + (numbered ? i : 0) <= key; };
-  int lo = 0, hi = a.requests;
-  while (hi - lo > 64) {
-    const int step = (hi - lo + 63) / 64, i = lo + lane * step;
-    const bool b = i < hi && below(ldg(a.offsets + min(i, hi - 1)), i);
-    lo = min(lo + (max(1, __popcll(__ballot(b))) - 1) * step, hi - 1);
-    hi = min(hi, lo + step);
-  }
-  const int i = min(lo + lane, hi - 1);
-  const int off = ldg(a.offsets + i), next = ldg(a.offsets + i + 1);
-  const uint32_t cached = min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
-  const int at = __builtin_amdgcn_readfirstlane(max(1, __popcll(__ballot(lo + lane < hi && below(off, i)))) - 1);
-  Chunk c;
-  c.n = __builtin_amdgcn_readfirstlane(lo) + at;
-  c.first = __builtin_amdgcn_readlane(off, at);
-  c.end = min(__builtin_amdgcn_readlane(next, at), a.tokens);
-  c.cached = __builtin_amdgcn_readlane((int)cached, at);
-  return c;
-}
-// The chunk that holds token t (wave-uniform); false where none does.
-__device__ __forceinline__ bool chunk_of(const ChunkArgs& a, int t, Chunk& c) {
-  c = find_chunk(a, 0, false, t);
-  return c.first >= 0 && c.first <= t && t < c.end;
-}
-
 __device__ __forceinline__ float* row_ptr(const ChunkArgs& a, int n, int h, int r, int kv) {
   const uint32_t page = min(ldg(a.lookup + (int64_t)n * a.lookup_cols + r / a.P), (uint32_t)(a.pages - 1));
   return a.pool + (int64_t)page * a.page_stride + kv * a.kv_stride + a.layer_off +
          (int64_t)(r % a.P) * a.slot_stride + (int64_t)h * kD;
-}
-
-// RoPE's tables (positions null: q and k come rotated).
-struct Rope {
-  const int32_t* positions;
-  const float* cos_t;
-  const float* sin_t;
-  int table_rows;
-};
-
-// Element d of the rotated row x, and four pairs of such: k_rope's arithmetic.
-__device__ __forceinline__ float rotated(const float* x, const float* c, const float* s, int d) {
-#pragma clang fp contract(off)
-  return d < 64 ? ldg(x + d) * ldg(c + d) + (-ldg(x + d + 64)) * ldg(s + d)
-                : ldg(x + d) * ldg(c + d) + ldg(x + d - 64) * ldg(s + d);
-}
-__device__ __forceinline__ void rotate4(f32x4& lo, f32x4& hi, f32x4 cl, f32x4 ch, f32x4 sl, f32x4 sh) {
-#pragma clang fp contract(off)
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float l = lo[e], u = hi[e];
-    lo[e] = l * cl[e] + (-u) * sl[e];
-    hi[e] = u * ch[e] + l * sh[e];
-  }
 }
 
 // The tensors whose rows are in_stride floats apart.
@@ -213,18 +153,6 @@ __device__ __forceinline__ float amax3(float m, float a, float b) {
   asm("v_maximum3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(m), "v"(a), "v"(b));
   return r;
 }
-// Reductions in which every lane gets the result: over lanes 16 or 32 apart, and over 16 lanes in a row.
-template <int OFF>
-__device__ __forceinline__ uint32_t other(uint32_t v) {  // of the lane whose number differs in bit OFF, or this one's
-  if constexpr (OFF == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return lane_id() < 32 ? r[1] : r[0];
-  } else {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return (lane_id() & 16) == 0 ? r[1] : r[0];
-  }
-}
-__device__ __forceinline__ float other32(float v) { return __uint_as_float(other<32>(__float_as_uint(v))); }
 template <int ROR>
 __device__ __forceinline__ uint32_t ror(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + ROR, 0xf, 0xf, false);
@@ -241,13 +169,6 @@ __device__ __forceinline__ uint32_t wave_largest(float m) {
   bits = max(bits, other<32>(bits));
   bits = max(bits, other<16>(bits));
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(bits));
-}
-// The lane's number as the compiler cannot know it: what is computed from it inside a loop is computed there,
-// and takes no register around the loop.
-__device__ __forceinline__ int lane_now() {
-  int l = lane_id();
-  asm volatile("" : "+v"(l));
-  return l;
 }
 __device__ __forceinline__ float pow2_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ int clamp_exp(uint32_t bits) {

@@ -1,0 +1,758 @@
+// Attention over a KV page pool that holds int8, and of trees of drafted tokens over either pool: the decode op and its
+// form for a chunk (unlimited_ocr_max/decoder.py:425-437, store_k/v_cache_ragged then flash_attention_ragged; the
+// pages and their rows of unlimited_ocr_max/kv_cache.py:1-36).
+//
+//   fp32 pool  [pages][2 (k, v)][layers][P][heads][D] floats, D = 128
+//   int8 pool  [pages][2 (k, v)][layers][P][slot] bytes; a slot is a row: its heads' 128 values each, then a float
+//              scale of each head, padded to a multiple of 128 bytes.  A value stands for itself times the scale.
+//
+// Token t of request n has a new row (its k and v), which is stored first, and attends a set of its request's rows:
+//   out = sum_r softmax_r(scale * q.k_r) v_r, 0 where the set is empty;
+//   decode  rows [0, attend_length + 1), the new row at write_index (a ring's may be anywhere),
+//   chunk   rows [0, cached + i], i the token's place in its chunk, the new row the last of them,
+//   tree    rows [0, cached) and row cached + j for every bit j < 64 of the token's mask.
+// What is attended is what the pool holds: an int8 pool's new rows count as they were rounded, so that a prompt's
+// results do not depend on how it was cut.
+//
+// Products: the matrix instruction of bf16, fp32 sums.  An fp32 operand is held as three bf16 numbers whose sum it is
+// (24 bits, of its own exponent: no scale is shared, and nothing is out of range); an int8 one is a bf16 number.  So a
+// product with an int8 operand is exact in three, and one of two fp32 operands leaves out 2^-24 of itself in six.
+// The scores are S^T = K Q^T and the results O^T = V^T P^T: a lane owns a query, and its 16 scores of a block of 32 rows
+// come in the order in which the second product wants the weights.
+#include <algorithm>
+
+#include "chunk_device.h"
+#include "int8_rows.h"
+#include "uocr_kernels.h"
+
+namespace uocr {
+
+namespace {
+
+constexpr int kBlock = 32;     // rows a wave takes at a time: the rows of one matrix instruction
+constexpr int kQueries = 32;   // of a workgroup
+constexpr int kQueriesLog2 = 5;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr float kInf = __builtin_huge_valf();
+// A maximum may lag by so many binades before the sums are rescaled (the weights are floats: nothing is lost).
+constexpr float kSlack = 8.0f;
+
+enum Mode { kOne, kCausal, kTree };
+
+struct PoolArgs {
+  char* pool;
+  int64_t page_bytes, kv_bytes, layer_bytes;  // of a page, of its k half, from its start to the layer
+  int slot_bytes;
+  int P, heads, pages;
+  int max_rows;  // lookup_cols * P: rows a lookup row can address
+  const uint32_t* lookup;
+  int lookup_cols;
+  int requests, tokens;
+  const uint32_t* cache_lengths;  // decode: attend lengths
+  const int32_t* offsets;         // [requests + 1]; decode: none, request i is token i
+  const uint32_t* write_index;    // decode
+  const int64_t* visible;         // tree
+  int attend_max;
+  int64_t in_stride;  // floats between rows of q / k_new / v_new
+  const float* q;
+  const float* k_new;
+  const float* v_new;
+  float* out;
+  float scale;
+  Rope rope;
+};
+
+// Where row r of request n is, and head h's values in it.
+__device__ __forceinline__ char* slot_of(const PoolArgs& a, int n, int r) {
+  const uint32_t page = min(ldg(a.lookup + (int64_t)n * a.lookup_cols + r / a.P), (uint32_t)(a.pages - 1));
+  return a.pool + (int64_t)page * a.page_bytes + a.layer_bytes + (int64_t)(r % a.P) * a.slot_bytes;
+}
+
+// One wave per (token, head): lane d has the pair (d, d + 64) of k and of v.  Queries that come before RoPE are rotated
+// where they are read.
+template <bool kInt8, Mode kMode>
+__global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
+  const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  if (th >= (int64_t)a.tokens * a.heads) return;
+  const int t = (int)(th / a.heads), h = (int)(th % a.heads), d = lane_id();
+  int n = t;
+  int64_t row;
+  if constexpr (kMode == kOne) {
+    row = ldg(a.write_index + t);
+  } else {
+    Chunk c;
+    if (!chunk_of(a, t, c)) return;
+    n = c.n;
+    row = (int64_t)c.cached + (t - c.first);
+  }
+  if (row >= a.max_rows) return;  // past what the lookup row addresses: not stored
+  const int64_t src = (int64_t)t * a.in_stride + (int64_t)h * kD;
+  const float *k = a.k_new + src, *v = a.v_new + src;
+  float x[4] = {ldg(k + d), ldg(k + d + 64), ldg(v + d), ldg(v + d + 64)};
+  if (a.rope.positions != nullptr) {
+    const int64_t at = (int64_t)min(max(ldg(a.rope.positions + t), 0), a.rope.table_rows - 1) * kD;
+    x[0] = rotated(k, a.rope.cos_t + at, a.rope.sin_t + at, d);
+    x[1] = rotated(k, a.rope.cos_t + at, a.rope.sin_t + at, d + 64);
+  }
+  char* slot = slot_of(a, n, (int)row);
+  if constexpr (kInt8) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      char* to = slot + j * a.kv_bytes;
+      const float scale = row_scale(tree_umax(max(abs_bits(x[2 * j]), abs_bits(x[2 * j + 1]))));
+      stg((uint8_t*)to + h * kD + d, (uint8_t)to_int8(x[2 * j], scale));
+      stg((uint8_t*)to + h * kD + d + 64, (uint8_t)to_int8(x[2 * j + 1], scale));
+      if (d == 0) stg((float*)(to + a.heads * kD) + h, scale);
+    }
+  } else {
+    float* to = (float*)slot + h * kD + d;
+    stg(to, x[0]);
+    stg(to + 64, x[1]);
+    to = (float*)(slot + a.kv_bytes) + h * kD + d;
+    stg(to, x[2]);
+    stg(to + 64, x[3]);
+  }
+}
+
+// ------------------------------------------------------------------ which piece of the work a workgroup takes
+
+// A call's rows are cut into splits where the tiles of queries alone do not fill the device.
+struct PoolCuts {
+  int split_rows, splits, slots;  // slots: tiles of queries at most
+  Divide by_split, by_heads;
+};
+// A tile of a request's tokens [t0, t_last], a head, and rows [begin, stop) of the all_rows that the tile attends.
+struct Piece : Chunk {
+  int t0, t_last, head, split, begin, stop, all_rows;
+};
+// Rows that a tile attends whose last token is t_last.
+template <Mode kMode>
+__device__ __forceinline__ int tile_rows(const PoolArgs& a, int cached, int length, int last) {
+  const int64_t rows = kMode == kOne ? (int64_t)cached + 1
+                       : kMode == kCausal ? (int64_t)cached + last + 1
+                                         : (int64_t)cached + min(length, 64);
+  return (int)min(rows, (int64_t)a.attend_max);
+}
+template <Mode kMode>
+__device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
+  Chunk c;
+  c.n = i;
+  c.first = kMode == kOne ? i : ldg(a.offsets + i);
+  c.end = kMode == kOne ? i + 1 : min(ldg(a.offsets + i + 1), a.tokens);
+  c.cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)(kMode == kOne ? a.max_rows - 1 : a.max_rows));
+  return c;
+}
+// Items go to the XCDs in stretches, an item's heads side by side: the heads of a row are neighbours in memory (an int8
+// pool's share the line of their scales), and their XCD reads it once.  Up to 64 requests every wave counts the pieces
+// that there are; of more, an item is a slot, whose tile and split may not exist.
+template <Mode kMode>
+__device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c, Piece& p) {
+  const int turn = (int)(blockIdx.x / 8), xcd = (int)(blockIdx.x % 8);
+  int j;  // the tile
+  if (a.requests <= 64) {
+    const Chunk mine = request_at<kMode>(a, min(lane_id(), a.requests - 1));
+    const bool some = lane_id() < a.requests && mine.first >= 0 && mine.first < mine.end;
+    const int length = some ? mine.end - mine.first : 0;
+    const int tiles = (length + kQueries - 1) >> kQueriesLog2;
+    const auto cuts = [&](int cached, int length, int j) {
+      return c.by_split(tile_rows<kMode>(a, cached, length, min((j + 1) << kQueriesLog2, length) - 1) - 1) + 1;
+    };
+    int pieces = tiles;
+    if (c.splits > 1) {
+      if constexpr (kMode == kCausal) {
+        pieces = 0;
+        for (int k = 0; __ballot(k < tiles) != 0; ++k)
+          if (k < tiles) pieces += cuts(mine.cached, length, k);
+      } else {
+        pieces = tiles == 0 ? 0 : tiles * cuts(mine.cached, length, 0);
+      }
+    }
+    const int upto = wave_scan_i(pieces), total = __builtin_amdgcn_readlane(upto, 63);
+    const int per = (total * a.heads + 7) / 8, item = xcd * per + turn;
+    if (turn >= per || item >= total * a.heads) return false;
+    int left = c.by_heads(item);
+    p.head = item - left * a.heads;
+    const int at = __popcll(__ballot(upto <= left));  // the request whose pieces reach past it
+    left -= __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(pieces, at);
+    p.n = at;
+    p.first = __builtin_amdgcn_readlane(mine.first, at);
+    p.end = __builtin_amdgcn_readlane(mine.end, at);
+    p.cached = __builtin_amdgcn_readlane(mine.cached, at);
+    j = __builtin_amdgcn_readlane(tiles, at) - 1;
+    if (c.splits > 1) {
+      for (; j > 0; --j) {
+        const int here = cuts(p.cached, p.end - p.first, j);
+        if (left < here) break;
+        left -= here;
+      }
+      p.split = left;
+    } else {
+      p.split = 0;
+      j -= left;
+    }
+  } else {
+    const int item = xcd * (int)(gridDim.x / 8) + turn;
+    const int cell = c.by_heads(item), slot = cell / c.splits;  // the splits of a tile one after the other
+    if (slot >= c.slots) return false;
+    p.head = item - cell * a.heads;
+    p.split = cell - slot * c.splits;
+    if constexpr (kMode == kOne) {
+      if (slot >= a.requests) return false;
+      (Chunk&)p = request_at<kMode>(a, slot);
+      j = 0;
+    } else {
+      (Chunk&)p = find_chunk(a, kQueriesLog2, true, slot);
+      j = slot - ((p.first >> kQueriesLog2) + p.n);
+      if (p.first < 0 || j < 0 || (int64_t)j << kQueriesLog2 >= p.end - p.first) return false;
+    }
+  }
+  p.t0 = p.first + (j << kQueriesLog2);
+  p.t_last = min(p.t0 + kQueries, p.end) - 1;
+  p.all_rows = tile_rows<kMode>(a, p.cached, p.end - p.first, p.t_last - p.first);
+  p.begin = p.split * c.split_rows;
+  p.stop = min(p.begin + c.split_rows, p.all_rows);
+  return p.begin < p.stop;
+}
+
+// ------------------------------------------------------------------ operands
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ bf16x8 bf(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// The upper halves of a and b, a's in the lower half.
+__device__ __forceinline__ uint32_t uppers(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float upper(float a) { return __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+// a and b as sums of three bf16 numbers each, the bits of a float from the first on: exact.
+__device__ __forceinline__ uint32_t split3(float a, float b, uint32_t& mid, uint32_t& lo) {
+  const float ra = a - upper(a), rb = b - upper(b);
+  mid = uppers(ra, rb);
+  lo = uppers(ra - upper(ra), rb - upper(rb));
+  return uppers(a, b);
+}
+// Signed bytes B and C of v as a bf16 pair.
+template <int B, int C>
+__device__ __forceinline__ uint32_t bytes_bf16(uint32_t v, uint32_t w) {
+  return uppers(i8_to_f32<B>((int)v), i8_to_f32<C>((int)w));
+}
+
+constexpr int kFrag = 64 * 8;                 // numbers of an operand: 8 of each lane
+constexpr int kQTerm = 8 * kFrag;             // of a term of the queries, [step][lane][8]
+
+// 32 rows of keys or of values on their way from memory to the operands of one wave.
+template <bool kInt8>
+struct Stage;
+template <>
+struct Stage<false> {
+  f32x4 x[16];
+};
+template <>
+struct Stage<true> {
+  uint32_t x[16];
+  float scale;  // of row l % 32
+};
+
+// Slot (lane half h, j) of step t of the first product is column 32 (t / 2) + 16 h + 8 (t % 2) + j;
+// slot (h, j) of step t of the second one is row 16 t + 8 (j / 4) + 4 h + j % 4 of the block.
+__device__ __forceinline__ int value_row(int j, int h) { return 16 * (j / 8) + 8 * (j / 4 % 2) + 4 * h + j % 4; }
+
+// `from`: the block's first slot; last: its last row that is read.
+template <bool kInt8>
+__device__ __forceinline__ void load_keys(Stage<kInt8>& k, const PoolArgs& a, const char* from, int head, int last, int lane) {
+  const int h = lane >> 5;
+  const uint32_t row = (uint32_t)(min(lane & 31, last) * a.slot_bytes), at = (uint32_t)head * kD;
+  if constexpr (kInt8) {
+    k.scale = *(const UOCR_GLOBAL float*)(from + (row + (uint32_t)(a.heads * kD + 4 * head)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 v = *(const UOCR_GLOBAL u32x4*)(from + (row + at + 16u * h) + 32 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k.x[4 * i + e] = v[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      k.x[i] = *(const UOCR_GLOBAL f32x4*)(from + (row + 4 * at + 64u * h) + 128 * (i / 4) + 16 * (i % 4));
+  }
+}
+template <bool kInt8>
+__device__ __forceinline__ void load_values(Stage<kInt8>& v, const PoolArgs& a, const char* from, int head, int last,
+                                            int lane) {
+  from += a.kv_bytes;
+  const int h = lane >> 5, c = lane & 31;
+  if constexpr (kInt8)
+    v.scale = *(const UOCR_GLOBAL float*)(from + (uint32_t)(min(c, last) * a.slot_bytes + a.heads * kD + 4 * head));
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint32_t row = (uint32_t)(min(value_row(j, h), last) * a.slot_bytes + head * (kInt8 ? kD : 4 * kD));
+    if constexpr (kInt8)
+      v.x[j] = *(const UOCR_GLOBAL uint32_t*)(from + (row + 4u * c));
+    else
+      v.x[j] = *(const UOCR_GLOBAL f32x4*)(from + (row + 16u * c));
+  }
+}
+
+// S^T of a block: 32 rows by 32 queries.  q: the queries' terms in LDS.
+template <bool kInt8>
+__device__ __forceinline__ f32x16 scores(const Stage<kInt8>& k, const uint16_t* q, int lane) {
+  f32x16 s = {};
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const bf16x8 qh = *(const bf16x8*)(q + t * kFrag + lane * 8);
+    const bf16x8 qm = *(const bf16x8*)(q + kQTerm + t * kFrag + lane * 8);
+    const bf16x8 ql = *(const bf16x8*)(q + 2 * kQTerm + t * kFrag + lane * 8);
+    if constexpr (kInt8) {
+      u32x4 kk;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t x = k.x[4 * (t / 2) + 2 * (t % 2) + e];
+        kk[2 * e] = bytes_bf16<0, 1>(x, x);
+        kk[2 * e + 1] = bytes_bf16<2, 3>(x, x);
+      }
+      s = mfma(bf(kk), ql, s);
+      s = mfma(bf(kk), qm, s);
+      s = mfma(bf(kk), qh, s);
+    } else {
+      u32x4 hi, mid, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 x = k.x[2 * t + e / 2];
+        uint32_t m, l;
+        hi[e] = split3(x[2 * (e % 2)], x[2 * (e % 2) + 1], m, l);
+        mid[e] = m;
+        lo[e] = l;
+      }
+      s = mfma(bf(lo), qh, s);
+      s = mfma(bf(hi), ql, s);
+      s = mfma(bf(mid), qm, s);
+      s = mfma(bf(mid), qh, s);
+      s = mfma(bf(hi), qm, s);
+      s = mfma(bf(hi), qh, s);
+      __builtin_amdgcn_sched_barrier(0);  // no steps' terms ahead: they would take the registers of the rows under way
+    }
+  }
+  return s;
+}
+
+
+struct Attend {
+  PoolArgs a;
+  PoolCuts cuts;
+  float* part;  // [split][token][head][D], where a tile has several splits
+  float* tops;  // [split][token][head][2]: the maximum (log2) and the sum of the weights
+};
+
+// A lane's query: running maximum (log2), the sum of the weights of the lane's rows, the weighted values.
+struct Running {
+  float m, l;
+  f32x16 o[4];  // register r of o[u]: column 4 (8 (r / 4) + 4 h + r % 4) + u
+};
+
+// Which of a block's rows a lane's query attends: those below `live`, or, for a tree, the bits of a word.
+__device__ __forceinline__ uint32_t tree_rows(uint64_t visible, int off, int live) {
+  uint32_t set;
+  if (off >= 0)
+    set = off < 64 ? (uint32_t)(visible >> off) : 0u;
+  else
+    set = off > -32 ? (uint32_t)(visible << -off) | ((1u << -off) - 1u) : ~0u;
+  return live >= 32 ? set : set & ((1u << max(live, 0)) - 1u);
+}
+
+// Scores (times log2 e) to weights: the maximum moves where it lags by more than kSlack, and what was summed follows.
+__device__ __forceinline__ void weigh(Running& w, f32x16& s) {
+  float mx = s[0];
+#pragma unroll
+  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+  mx = fmaxf(mx, other32(mx));
+  const bool up = mx > w.m + kSlack;
+  if (__ballot(up) != 0) {
+    const float alpha = up ? __builtin_amdgcn_exp2f(w.m - mx) : 1.0f;
+    w.m = up ? mx : w.m;
+    w.l *= alpha;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w.o[u] *= alpha;
+  }
+  const float off = w.m == -kInf ? 0.0f : w.m;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(s[r] - off);
+    w.l += s[r];
+  }
+}
+
+// Step t of the second product: the weights of 8 rows as three terms, and the values' columns in turn.
+template <int T>
+__device__ __forceinline__ void split_weights(const f32x16& p, u32x4& hi, u32x4& mid, u32x4& lo) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t m, l;
+    hi[e] = split3(p[8 * T + 2 * e], p[8 * T + 2 * e + 1], m, l);
+    mid[e] = m;
+    lo[e] = l;
+  }
+}
+template <int T, int U>
+__device__ __forceinline__ void add_column(Running& w, const Stage<true>& v, u32x4 ph, u32x4 pm, u32x4 pl) {
+  u32x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = bytes_bf16<U, U>(v.x[8 * T + 2 * e], v.x[8 * T + 2 * e + 1]);
+  w.o[U] = mfma(bf(x), bf(pl), w.o[U]);
+  w.o[U] = mfma(bf(x), bf(pm), w.o[U]);
+  w.o[U] = mfma(bf(x), bf(ph), w.o[U]);
+}
+template <int T, int U>
+__device__ __forceinline__ void add_column(Running& w, const Stage<false>& v, u32x4 ph, u32x4 pm, u32x4 pl) {
+  u32x4 hi, mid, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t m, l;
+    hi[e] = split3(v.x[8 * T + 2 * e][U], v.x[8 * T + 2 * e + 1][U], m, l);
+    mid[e] = m;
+    lo[e] = l;
+  }
+  w.o[U] = mfma(bf(lo), bf(ph), w.o[U]);
+  w.o[U] = mfma(bf(hi), bf(pl), w.o[U]);
+  w.o[U] = mfma(bf(mid), bf(pm), w.o[U]);
+  w.o[U] = mfma(bf(mid), bf(ph), w.o[U]);
+  w.o[U] = mfma(bf(hi), bf(pm), w.o[U]);
+  w.o[U] = mfma(bf(hi), bf(ph), w.o[U]);
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int T, bool kInt8>
+__device__ __forceinline__ void add_values(Running& w, const Stage<kInt8>& v, const f32x16& p) {
+  u32x4 hi, mid, lo;
+  split_weights<T>(p, hi, mid, lo);
+  add_column<T, 0>(w, v, hi, mid, lo);
+  add_column<T, 1>(w, v, hi, mid, lo);
+  add_column<T, 2>(w, v, hi, mid, lo);
+  add_column<T, 3>(w, v, hi, mid, lo);
+}
+
+// The rows (bits of the block's) with a value that is not finite, whose values become 0: a row that a query does not
+// attend must leave nothing in its sum, and one that it attends makes it NaN.
+__device__ __forceinline__ uint32_t take_infinite(Stage<false>& v) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, abs_bits(v.x[j][e]));
+  if (__ballot(top >= 0x7f800000u) == 0) return 0;
+  uint32_t bad = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most = max(most, abs_bits(v.x[j][e]));
+    const uint64_t who = __ballot(most >= 0x7f800000u);
+    if ((uint32_t)who != 0) bad |= 1u << value_row(j, 0);
+    if ((who >> 32) != 0) bad |= 1u << value_row(j, 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t none = abs_bits(v.x[j][e]) >= 0x7f800000u ? 0u : ~0u;
+      v.x[j][e] = __uint_as_float(__float_as_uint(v.x[j][e]) & none);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return bad;
+}
+
+// 32 queries of a head, whose rows' blocks the workgroup's waves take in turn and whose sums they join in LDS.
+template <bool kInt8, Mode kMode>
+__global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
+  const PoolArgs& a = p.a;
+  __shared__ __align__(16) float sums[kWaves][kQueries * kD];  // first the queries' terms, [term][step][lane][8]
+  uint16_t* const qs = (uint16_t*)sums;
+  __shared__ __align__(16) float row_scales[kWaves][2][kBlock];  // of a block's keys and values
+  __shared__ float peak[kWaves][kQueries], total[kWaves][kQueries];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = lane >> 5;
+  Piece w;
+  if (!find_piece<kMode>(a, p.cuts, w)) return;
+  const int stop = w.stop, head = w.head;
+  const uint32_t* lookup = a.lookup + (int64_t)w.n * a.lookup_cols;
+  const auto block_at = [&](int row) {
+    return a.pool + (int64_t)min(ldc(lookup + row / a.P), (uint32_t)(a.pages - 1)) * a.page_bytes + a.layer_bytes +
+           (int64_t)(row % a.P) * a.slot_bytes;
+  };
+  const int first = w.begin + kBlock * wave;
+  Stage<kInt8> k, v;
+  {
+    // the queries' terms: thread (query tid / 8, octets tid % 8 and 8 on)
+    const int query = (int)threadIdx.x / 8, d = 8 * ((int)threadIdx.x % 8), t = min(w.t0 + query, w.t_last);
+    const float* src = a.q + (int64_t)t * a.in_stride + (int64_t)head * kD + d;
+    f32x4 x[4] = {*(const UOCR_GLOBAL f32x4*)src, *(const UOCR_GLOBAL f32x4*)(src + 4),
+                  *(const UOCR_GLOBAL f32x4*)(src + 64), *(const UOCR_GLOBAL f32x4*)(src + 68)};
+    int pos = 0;
+    if (a.rope.positions != nullptr) pos = min(max(ldg(a.rope.positions + t), 0), a.rope.table_rows - 1);
+    if (first < stop) {
+      const char* from = block_at(first);
+      load_keys(k, a, from, head, stop - 1 - first, lane);
+      load_values(v, a, from, head, stop - 1 - first, lane);
+    }
+    if (a.rope.positions != nullptr) {
+      const float *ct = a.rope.cos_t + (int64_t)pos * kD + d, *st = a.rope.sin_t + (int64_t)pos * kD + d;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        rotate4(x[i], x[i + 2], *(const UOCR_GLOBAL f32x4*)(ct + 4 * i), *(const UOCR_GLOBAL f32x4*)(ct + 4 * i + 64),
+                *(const UOCR_GLOBAL f32x4*)(st + 4 * i), *(const UOCR_GLOBAL f32x4*)(st + 4 * i + 64));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = d + 64 * i, step = 2 * (col / 32) + col / 8 % 2, half = col / 16 % 2;
+      u32x4 hi, mid, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t m, l;
+        hi[e] = split3(x[2 * i + e / 2][2 * (e % 2)], x[2 * i + e / 2][2 * (e % 2) + 1], m, l);
+        mid[e] = m;
+        lo[e] = l;
+      }
+      uint16_t* at = qs + step * kFrag + (half * 32 + query) * 8;
+      *(u32x4*)at = hi;
+      *(u32x4*)(at + kQTerm) = mid;
+      *(u32x4*)(at + 2 * kQTerm) = lo;
+    }
+  }
+  const float c = a.scale * 1.44269504f;
+  const int my_t = min(w.t0 + (lane & 31), w.t_last);
+  // rows below `all` are attended by every query of the tile
+  const int all = min(stop, kMode == kOne ? stop : kMode == kCausal ? w.cached + (w.t0 - w.first) + 1 : w.cached);
+  const int limit = kMode == kCausal ? min(w.cached + (my_t - w.first) + 1, stop) : stop;
+  uint64_t visible = 0;
+  if constexpr (kMode == kTree) visible = (uint64_t)ldg(a.visible + my_t);
+  Running run;
+  run.m = -kInf;
+  run.l = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) run.o[u] = f32x16{};
+  __syncthreads();
+#pragma unroll 1
+  for (int key0 = first; key0 < stop; key0 += kWaves * kBlock) {
+    const int next = key0 + kWaves * kBlock;
+    const char* next_base = next < stop ? block_at(next) : a.pool;
+    f32x16 s = scores(k, qs, lane);
+    f32x4 vs[4];
+    if constexpr (kInt8) {
+      row_scales[wave][h][lane & 31] = h == 0 ? k.scale * c : v.scale;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ks = *(const f32x4*)&row_scales[wave][0][8 * g + 4 * h];
+        vs[g] = *(const f32x4*)&row_scales[wave][1][8 * g + 4 * h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * g + e] *= ks[e];
+      }
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      s *= c;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < stop) load_keys(k, a, next_base, head, stop - 1 - next, lane);
+    const bool masked = key0 + kBlock > all;
+    if (masked) {
+      uint32_t set = 0;
+      if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
+      const int live = limit - key0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 8 * (r / 4) + 4 * h + r % 4;
+        const bool seen = kMode == kTree ? (set >> row & 1u) != 0 : row < live;
+        s[r] = seen ? s[r] : -kInf;
+      }
+    }
+    if constexpr (!kInt8) {
+      const uint32_t bad = take_infinite(v);
+      if (bad != 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (bad >> (8 * (r / 4) + 4 * h + r % 4) & 1u && s[r] != -kInf) run.l = __uint_as_float(0x7fc00000u);
+      }
+    }
+    weigh(run, s);
+    if constexpr (kInt8) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= vs[r / 4][r % 4];
+      if (masked) {  // the scales of rows that are not attended may be anything
+        uint32_t set = 0;
+        if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
+        const int live = limit - key0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = 8 * (r / 4) + 4 * h + r % 4;
+          const bool seen = kMode == kTree ? (set >> row & 1u) != 0 : row < live;
+          s[r] = seen ? s[r] : 0.0f;
+        }
+      }
+    }
+    add_values<0>(run, v, s);
+    add_values<1>(run, v, s);
+    if (next < stop) load_values(v, a, next_base, head, stop - 1 - next, lane);
+  }
+  const float mine = run.l + other32(run.l);
+  if (h == 0) {
+    peak[wave][lane] = run.m;
+    total[wave][lane] = mine;
+  }
+  __syncthreads();
+  // the waves' sums at one maximum (a wave without rows has a sum of 0; NaN stays NaN)
+  float m = peak[0][lane & 31];
+#pragma unroll
+  for (int j = 1; j < kWaves; ++j) m = fmaxf(m, peak[j][lane & 31]);
+  const auto weight = [&](float mj) { return mj == -kInf ? (m == -kInf ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(mj - m); };
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kWaves; ++j) {
+    const float lj = total[j][lane & 31];
+    sum += lj == 0.0f || lj != lj ? lj : lj * weight(peak[j][lane & 31]);
+  }
+  const bool whole = w.all_rows <= p.cuts.split_rows;
+  float f = weight(run.m);
+  if (whole) f = sum == 0.0f ? 0.0f : sum != sum ? sum : f / sum;
+  // query l % 32, a row of 128 floats whose 16-byte pieces are rotated by the query
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    f32x4 y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y[u] = run.o[u][r] * f;
+    *(f32x4*)(sums[wave] + (lane & 31) * kD + 4 * ((8 * (r / 4) + 4 * h + r % 4 + lane) & 31)) = y;
+  }
+  const int64_t stride = (int64_t)a.tokens * a.heads;
+  if (!whole && wave == 0 && h == 0 && w.t0 + lane <= w.t_last) {
+    float* to = p.tops + 2 * (w.split * stride + (int64_t)(w.t0 + lane) * a.heads + head);
+    stg(to, m);
+    stg(to + 1, sum);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kQueries * 32 / kThreads; ++j) {
+    const int i = j * kThreads + (int)threadIdx.x, query = i / 32, piece = i % 32;
+    if (w.t0 + query > w.t_last) continue;
+    const int at = query * kD + 4 * ((piece + query) & 31);
+    f32x4 y = *(const f32x4*)(sums[0] + at);
+#pragma unroll
+    for (int u = 1; u < kWaves; ++u) y += *(const f32x4*)(sums[u] + at);
+    const int64_t th = (int64_t)(w.t0 + query) * a.heads + head;
+    *(UOCR_GLOBAL f32x4*)((whole ? a.out + th * kD : p.part + (w.split * stride + th) * kD) + 4 * piece) = y;
+  }
+}
+
+// Joins the splits of a token's rows: half a wave a (token, head), four columns a lane.
+template <Mode kMode>
+__global__ void __launch_bounds__(256) k_pool_join(Attend p) {
+  const PoolArgs& a = p.a;
+  const int groups = (a.heads + 1) / 2;
+  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int64_t t = item / groups;
+  if (t >= a.tokens) return;
+  Chunk c;
+  if constexpr (kMode == kOne)
+    c = request_at<kMode>(a, (int)t);
+  else if (!chunk_of(a, (int)t, c))
+    return;
+  const int i = (int)t - c.first, length = c.end - c.first;
+  const int t_last = min(((i >> kQueriesLog2) + 1) << kQueriesLog2, length) - 1;  // of its tile
+  const int splits = p.cuts.by_split(tile_rows<kMode>(a, c.cached, length, t_last) - 1) + 1;
+  if (splits == 1) return;  // written by its tile
+  const int lane = lane_id(), head = (int)(item - t * groups) * 2 + lane / 32;
+  if (head >= a.heads) return;
+  const int64_t stride = (int64_t)a.tokens * a.heads, th = t * a.heads + head;
+  float m = -kInf;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, ldg(p.tops + 2 * (s * stride + th)));
+  float l = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float ms = ldg(p.tops + 2 * (s * stride + th)), ls = ldg(p.tops + 2 * (s * stride + th) + 1);
+    const f32x4 y = *(const UOCR_GLOBAL f32x4*)(p.part + (s * stride + th) * kD + 4 * (lane & 31));
+    const float f = ls == 0.0f ? 0.0f : ms == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
+    l = __builtin_fmaf(f, ls, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, y[e], o[e]);
+  }
+  *(UOCR_GLOBAL f32x4*)(a.out + th * kD + 4 * (lane & 31)) = l == 0.0f ? f32x4{} : o / l;
+}
+
+}  // namespace
+
+// How a call's rows are cut: splits of at least a round of the waves, as many as fill the device once with two
+// workgroups a CU.
+namespace {
+constexpr int kCus = 256;
+PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max) {
+  PoolCuts c{};
+  const int64_t tiles = requests > 64 ? tokens / kQueries + requests
+                        : tokens < requests ? tokens : (tokens - requests) / kQueries + requests;
+  c.slots = (int)tiles;
+  const int64_t splits = std::max<int64_t>(1, 2 * kCus / std::max<int64_t>(1, tiles * heads));
+  const int round = kWaves * kBlock;
+  c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
+  c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
+  c.by_split = divide_by(c.split_rows);
+  c.by_heads = divide_by(heads);
+  return c;
+}
+
+template <bool kInt8, Mode kMode>
+hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
+  const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max);
+  const int64_t pairs = p.tokens * p.heads, items = (int64_t)c.slots * p.heads * c.splits;
+  const int64_t joins = p.tokens * ((p.heads + 1) / 2);
+  // (where a wave counts the pieces, offsets that do not ascend may give each request all of them)
+  if (items > (p.requests <= 64 ? INT32_MAX / p.requests : INT32_MAX) - 8) return hipErrorInvalidValue;
+  const Attend at{a, c, (float*)p.workspace, (float*)p.workspace + (int64_t)c.splits * pairs * kD};
+  auto store = k_pool_store<kInt8, kMode>;
+  UOCR_LAUNCH("pool_store", store, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, s, a);
+  auto attend = k_pool_attend<kInt8, kMode>;
+  UOCR_LAUNCH("pool_attend", attend, dim3((unsigned)((items + 7) / 8 * 8)), dim3(kThreads), 0, s, at);
+  if (c.splits > 1) {
+    auto join = k_pool_join<kMode>;
+    UOCR_LAUNCH("pool_join", join, dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, s, at);
+  }
+  return hipGetLastError();
+}
+}  // namespace
+
+size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max) {
+  const PoolCuts c = cuts_of(tokens, requests, heads, attend_max);
+  return c.splits > 1 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s) {
+  if (p.tokens == 0 || p.requests == 0) return hipSuccess;
+  PoolArgs a{};
+  a.pool = (char*)p.kv_blocks;
+  a.slot_bytes = p.slot_bytes;
+  a.kv_bytes = (int64_t)p.layers * p.page_size * p.slot_bytes;
+  a.page_bytes = 2 * a.kv_bytes;
+  a.layer_bytes = (int64_t)p.layer * p.page_size * p.slot_bytes;
+  a.P = p.page_size;
+  a.heads = p.heads;
+  a.pages = p.pages;
+  a.max_rows = p.lookup_cols * p.page_size;
+  a.lookup = p.lookup;
+  a.lookup_cols = p.lookup_cols;
+  a.requests = (int)p.requests;
+  a.tokens = (int)p.tokens;
+  a.cache_lengths = p.cache_lengths;
+  a.offsets = p.chunk_offsets;
+  a.write_index = p.write_index;
+  a.visible = p.visible;
+  a.attend_max = p.attend_max;
+  a.in_stride = p.in_stride;
+  a.q = p.q;
+  a.k_new = p.k_new;
+  a.v_new = p.v_new;
+  a.out = p.out;
+  a.scale = p.scale;
+  a.rope = Rope{p.positions, p.cos_table, p.sin_table, p.table_rows};
+  if (p.write_index != nullptr) return launch<true, kOne>(p, a, s);
+  if (p.visible == nullptr) return launch<true, kCausal>(p, a, s);
+  return p.int8 ? launch<true, kTree>(p, a, s) : launch<false, kTree>(p, a, s);
+}
+
+}  // namespace uocr

@@ -293,6 +293,99 @@ struct ChunkAttention {
 size_t chunk_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max);
 hipError_t launch_chunk_attention(const ChunkAttention& p, hipStream_t s);
 
+// ---- attention over an int8 page pool, and of drafted trees over either pool (pool_attention.hip) ----
+
+struct PoolAttention {
+  float* out;            // [tokens, heads, D]
+  const float* q;        // rows in_stride floats apart
+  const float* k_new;
+  const float* v_new;
+  void* kv_blocks;       // int8 [pages, 2, layers, page_size, slot_bytes] or fp32 [pages, 2, layers, page_size, heads, D]
+  int pages, layers, page_size, heads, layer;
+  int slot_bytes;        // of a row of either
+  bool int8;
+  const uint32_t* lookup;         // [requests, lookup_cols]
+  int lookup_cols;
+  const uint32_t* cache_lengths;  // [requests]: rows before the chunk; decode: the rows attended, less one
+  const int32_t* chunk_offsets;   // [requests + 1]; decode: null, request i is token i
+  const uint32_t* write_index;    // decode: [requests]; else null
+  const int64_t* visible;         // a tree's masks, [tokens]; else null
+  int64_t tokens, requests;
+  int attend_max;                 // the most rows a token attends (host)
+  float scale;
+  void* workspace;                // pool_workspace_bytes(tokens, requests, heads, attend_max)
+  int64_t in_stride;
+  const int32_t* positions;       // null: q, k_new come rotated; else rotated here at these positions
+  const float* cos_table;         // [table_rows, head_dim]
+  const float* sin_table;
+  int table_rows;
+};
+size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max);
+hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s);
+
+// ---- pages between the fp32 pool and the int8 one (int8_pages.hip) ----
+
+struct ConvertPages {
+  float* fp32;  // [fp32_pages, 2, layers, page_size, heads, 128]
+  char* int8;   // [int8_pages, 2, layers, page_size, slot_bytes]
+  int fp32_pages, int8_pages, layers, page_size, heads, slot_bytes;
+  const int32_t* src;   // [count] pages of the one
+  const int32_t* dst;   // [count] pages of the other
+  const int32_t* rows;  // [count] rows converted, or null: all
+  int count;
+};
+hipError_t launch_convert_pages(const ConvertPages& p, bool quantize, hipStream_t s);
+
+// ---- trees of drafted tokens (drafts.hip) ----
+
+hipError_t launch_draft_masks(int64_t* masks, const int32_t* parents, const int32_t* offsets, int requests, int tokens,
+                              hipStream_t s);
+struct AcceptDrafts {
+  char* pool;  // of either kind: [pages, 2, layers, page_size, slot_bytes]
+  int pages, layers, page_size, slot_bytes;
+  const uint32_t* lookup;
+  int lookup_cols, max_rows;
+  const uint32_t* cache_lengths;
+  const int32_t* offsets;
+  int tokens;
+  const int32_t* parents;
+  const int32_t* drafted;
+  const int32_t* answers;
+  int32_t* counts;
+  int32_t* path;
+  int32_t* next;
+  uint32_t* lengths_out;
+};
+hipError_t launch_accept_drafts(const AcceptDrafts& p, int requests, hipStream_t s);
+
+// ---- a step of beam search (beam.hip) ----
+
+constexpr int kBeamsMost = 32;
+struct BeamSelect {
+  const float* logits;  // [rows, vocab]
+  const float* scores;  // [rows]
+  const int32_t* ended;    // [rows] or null
+  const int32_t* lengths;  // [rows] or null
+  const int32_t* history;  // [rows, width] or null
+  int vocab, beams, eos;
+  int64_t width;
+  double alpha;
+  int32_t* tokens_out;
+  int32_t* parents_out;
+  float* scores_out;
+  int32_t* ended_out;
+  int32_t* lengths_out;
+  int32_t* history_out;
+};
+struct BeamWork {  // of each row's pieces: the largest logit and the sum, the best tokens
+  int pieces;
+  float* tops;
+  float* values;
+  int* ids;
+};
+size_t beam_workspace_bytes(int64_t rows, int beams, int vocab);
+hipError_t launch_beam_select(const BeamSelect& p, int64_t rows, void* workspace, hipStream_t s);
+
 // ---- the pages of the pool (pages.hip) ----
 
 struct PagePool {

@@ -926,6 +926,350 @@ int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens,
                           errlen);
 }
 
+// ------------------------------------------------------------------ an int8 pool, and trees of drafted tokens
+
+size_t uocr_paged_pool_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max) {
+  if (tokens < 0 || tokens > INT32_MAX || requests < 0 || requests > INT32_MAX || heads < 1 || heads > 65535 ||
+      attend_max < 1 || attend_max > INT32_MAX)
+    return 0;
+  return pool_workspace_bytes(tokens, requests, (int)heads, (int)attend_max);
+}
+
+// The bytes of a pool; 0: its sizes are none that a pool has (refused, the message in err).
+static size_t pool_bytes(const char* op, const void* kv_blocks, int64_t pages, int64_t layers, int64_t page_size,
+                         int64_t heads, int64_t slot_bytes, bool int8, char* err, size_t errlen) {
+  if (heads < 1 || heads > 65535) return fail(err, errlen, "%s: heads must be in [1, 65535]", op), 0;
+  if (pages < 1 || pages > INT32_MAX || layers < 1 || layers > 32767 || page_size < 1 || page_size > INT32_MAX)
+    return fail(err, errlen, "%s: bad pool of %lld pages, %lld layers, %lld rows a page", op, (long long)pages,
+                (long long)layers, (long long)page_size), 0;
+  if (int8 && (slot_bytes < heads * 132 || slot_bytes % 16 || slot_bytes > (int64_t)1 << 26))
+    return fail(err, errlen, "%s: a slot of %lld bytes does not hold %lld heads of 128 values and a scale in pieces of 16", op,
+                (long long)slot_bytes, (long long)heads), 0;
+  const __int128 bytes = (__int128)pages * 2 * layers * page_size * slot_bytes;
+  if (bytes > INT64_MAX / 2) return fail(err, errlen, "%s: the pool is too large", op), 0;
+  if (!aligned16(kv_blocks)) return fail(err, errlen, "%s: the pool must be 16-byte aligned", op), 0;
+  return (size_t)bytes;
+}
+
+// The checks and launch of the attention entries; p has the tensors, the sizes are still as they came.
+static int pool_attention_call(const char* op, PoolAttention p, int64_t heads, int64_t head_dim, int64_t row_stride,
+                               int64_t table_rows, int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes,
+                               int64_t layer, int64_t lookup_cols, int64_t attend_max, bool decode, void* workspace,
+                               size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  const int64_t tokens = p.tokens, requests = p.requests;
+  if (head_dim != 128) return fail(err, errlen, "%s: head_dim must be 128, got %lld", op, (long long)head_dim);
+  const size_t pool = pool_bytes(op, p.kv_blocks, pages, layers, page_size, heads, slot_bytes, p.int8, err, errlen);
+  if (pool == 0) return 1;
+  if (page_size % kAttnSplitRows)
+    return fail(err, errlen, "%s: page_size must be a positive multiple of %d", op, kAttnSplitRows);
+  if (layer < 0 || layer >= layers)
+    return fail(err, errlen, "%s: layer %lld is not in the pool's %lld layers", op, (long long)layer, (long long)layers);
+  if (tokens < 0 || requests < 0 || requests > 65535 || tokens > (1 << 25) / heads)
+    return fail(err, errlen, "%s: requests must be in [0, 65535] and tokens * heads in [0, 2^25]", op);
+  if (lookup_cols < 1 || lookup_cols > INT32_MAX / page_size)
+    return fail(err, errlen, "%s: bad lookup table width %lld", op, (long long)lookup_cols);
+  if (attend_max < 1 || attend_max > lookup_cols * page_size)
+    return fail(err, errlen, "%s: attend_max %lld is not in [1, %lld], the rows the lookup table addresses", op,
+                (long long)attend_max, (long long)(lookup_cols * page_size));
+  if (!(p.scale - p.scale == 0.0f)) return fail(err, errlen, "%s: scale must be finite", op);
+  if (row_stride < heads * head_dim || row_stride >= (int64_t)1 << 25 || row_stride % 4)
+    return fail(err, errlen, "%s: input rows must be a multiple of 4 floats apart, at least %lld and less than 2^25, got %lld", op,
+                (long long)(heads * head_dim), (long long)row_stride);
+  if (p.positions != nullptr && (table_rows < 1 || table_rows > INT32_MAX || !p.cos_table || !p.sin_table))
+    return fail(err, errlen, "%s: bad cos/sin table", op);
+  if (tokens == 0 || requests == 0) return 0;
+  if (!p.out || !p.q || !p.k_new || !p.v_new || !p.kv_blocks || !p.lookup || !p.cache_lengths ||
+      (decode ? !p.write_index : !p.chunk_offsets) || (!p.int8 && !p.visible))
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  if (!aligned16(p.out) || !aligned16(p.q) || !aligned16(p.k_new) || !aligned16(p.v_new))
+    return fail(err, errlen, "%s: q, k_new, v_new and out must be 16-byte aligned", op);
+  if (!aligned16(p.cos_table) || !aligned16(p.sin_table))
+    return fail(err, errlen, "%s: the cos/sin tables must be 16-byte aligned", op);
+  const size_t row = (size_t)(heads * head_dim) * sizeof(float);
+  const size_t in_bytes = (size_t)(tokens - 1) * row_stride * sizeof(float) + row, out_bytes = (size_t)tokens * row;
+  if (overlap(p.out, out_bytes, p.kv_blocks, pool)) return fail(err, errlen, "%s: out must not overlap the pool", op);
+  for (const float* in : {p.q, p.k_new, p.v_new}) {
+    if (overlap(p.out, out_bytes, in, in_bytes)) return fail(err, errlen, "%s: out must not overlap the inputs", op);
+    if (overlap(in, in_bytes, p.kv_blocks, pool)) return fail(err, errlen, "%s: the inputs must not overlap the pool", op);
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  void* ws = nullptr;
+  const size_t need = pool_workspace_bytes(tokens, requests, (int)heads, (int)attend_max);
+  if (chunk_workspace(op, workspace, workspace_bytes, need, s, &ws, err, errlen)) return 1;
+  p.pages = (int)pages;
+  p.layers = (int)layers;
+  p.page_size = (int)page_size;
+  p.heads = (int)heads;
+  p.layer = (int)layer;
+  p.slot_bytes = (int)slot_bytes;
+  p.lookup_cols = (int)lookup_cols;
+  p.attend_max = (int)attend_max;
+  p.workspace = ws;
+  p.in_stride = row_stride;
+  p.table_rows = (int)table_rows;
+  const hipError_t e = launch_pool_attention(p, s);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+static PoolAttention pool_tensors(float* out, const float* q, const float* k_new, const float* v_new, const int32_t* positions,
+                                  const float* cos_table, const float* sin_table, const uint32_t* lookup, float scale) {
+  PoolAttention p{};
+  p.out = out;
+  p.q = q;
+  p.k_new = k_new;
+  p.v_new = v_new;
+  p.positions = positions;
+  p.cos_table = cos_table;
+  p.sin_table = sin_table;
+  p.lookup = lookup;
+  p.scale = scale;
+  return p;
+}
+
+int uocr_paged_decode_attention_int8(float* out, const float* q, const float* k_new, const float* v_new, int64_t rows,
+                                     int64_t heads, int64_t head_dim, int64_t row_stride, const int32_t* positions,
+                                     const float* cos_table, const float* sin_table, int64_t table_rows, int8_t* kv_blocks,
+                                     int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes, int64_t layer,
+                                     const uint32_t* lookup, int64_t lookup_cols, const uint32_t* attend_lengths,
+                                     int64_t attend_max, const uint32_t* write_index, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  PoolAttention p = pool_tensors(out, q, k_new, v_new, positions, cos_table, sin_table, lookup, scale);
+  p.kv_blocks = kv_blocks;
+  p.int8 = true;
+  p.tokens = p.requests = rows;
+  p.cache_lengths = attend_lengths;
+  p.write_index = write_index;
+  return pool_attention_call("paged_decode_attention_int8", p, heads, head_dim, row_stride, table_rows, pages, layers,
+                             page_size, slot_bytes, layer, lookup_cols, attend_max, true, workspace, workspace_bytes, stream,
+                             err, errlen);
+}
+
+int uocr_paged_chunk_attention_int8(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
+                                    int64_t heads, int64_t head_dim, int64_t row_stride, const int32_t* positions,
+                                    const float* cos_table, const float* sin_table, int64_t table_rows, int8_t* kv_blocks,
+                                    int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes, int64_t layer,
+                                    const uint32_t* lookup, int64_t requests, int64_t lookup_cols,
+                                    const uint32_t* cache_lengths, const int32_t* chunk_offsets, int64_t attend_max,
+                                    const int64_t* visible, float scale, void* workspace, size_t workspace_bytes,
+                                    void* stream, char* err, size_t errlen) {
+  PoolAttention p = pool_tensors(out, q, k_new, v_new, positions, cos_table, sin_table, lookup, scale);
+  p.kv_blocks = kv_blocks;
+  p.int8 = true;
+  p.tokens = tokens;
+  p.requests = requests;
+  p.cache_lengths = cache_lengths;
+  p.chunk_offsets = chunk_offsets;
+  p.visible = visible;
+  return pool_attention_call("paged_chunk_attention_int8", p, heads, head_dim, row_stride, table_rows, pages, layers,
+                             page_size, slot_bytes, layer, lookup_cols, attend_max, false, workspace, workspace_bytes,
+                             stream, err, errlen);
+}
+
+int uocr_paged_tree_attention(float* out, const float* q, const float* k_new, const float* v_new, int64_t tokens,
+                              int64_t heads, int64_t head_dim, int64_t row_stride, const int32_t* positions,
+                              const float* cos_table, const float* sin_table, int64_t table_rows, float* kv_blocks,
+                              int64_t pages, int64_t layers, int64_t page_size, int64_t layer, const uint32_t* lookup,
+                              int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
+                              const int32_t* chunk_offsets, int64_t attend_max, const int64_t* visible, float scale,
+                              void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  PoolAttention p = pool_tensors(out, q, k_new, v_new, positions, cos_table, sin_table, lookup, scale);
+  p.kv_blocks = kv_blocks;
+  p.tokens = tokens;
+  p.requests = requests;
+  p.cache_lengths = cache_lengths;
+  p.chunk_offsets = chunk_offsets;
+  p.visible = visible;
+  return pool_attention_call("paged_tree_attention", p, heads, head_dim, row_stride, table_rows, pages, layers, page_size,
+                             heads > 0 && heads <= 65535 ? heads * 512 : 0, layer, lookup_cols, attend_max, false, workspace,
+                             workspace_bytes, stream, err, errlen);
+}
+
+static int convert_pages(const char* op, bool quantize, float* kv_blocks, int64_t fp32_pages, int8_t* kv_int8,
+                         int64_t int8_pages, int64_t layers, int64_t page_size, int64_t heads, int64_t slot_bytes,
+                         const int32_t* src, const int32_t* dst, const int32_t* rows, int64_t count, void* stream, char* err,
+                         size_t errlen) {
+  const size_t wide = pool_bytes(op, kv_blocks, fp32_pages, layers, page_size, heads, heads * 512, false, err, errlen);
+  if (wide == 0) return 1;
+  const size_t narrow = pool_bytes(op, kv_int8, int8_pages, layers, page_size, heads, slot_bytes, true, err, errlen);
+  if (narrow == 0) return 1;
+  if (count < 0 || count > INT32_MAX) return fail(err, errlen, "%s: bad number of pairs %lld", op, (long long)count);
+  if (page_size > 1 << 20) return fail(err, errlen, "%s: more than 2^20 rows a page", op);
+  if (count == 0) return 0;
+  if (!kv_blocks || !kv_int8 || !src || !dst) return fail(err, errlen, "%s: a tensor is missing", op);
+  if (overlap(kv_blocks, wide, kv_int8, narrow)) return fail(err, errlen, "%s: the pools must not overlap", op);
+  for (const int32_t* list : {src, dst, rows})
+    if (list && (overlap(list, (size_t)count * 4, kv_blocks, wide) || overlap(list, (size_t)count * 4, kv_int8, narrow)))
+      return fail(err, errlen, "%s: a list must not overlap a pool", op);
+  ConvertPages p{};
+  p.fp32 = kv_blocks;
+  p.int8 = (char*)kv_int8;
+  p.fp32_pages = (int)fp32_pages;
+  p.int8_pages = (int)int8_pages;
+  p.layers = (int)layers;
+  p.page_size = (int)page_size;
+  p.heads = (int)heads;
+  p.slot_bytes = (int)slot_bytes;
+  p.src = src;
+  p.dst = dst;
+  p.rows = rows;
+  p.count = (int)count;
+  const hipError_t e = launch_convert_pages(p, quantize, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+int uocr_quantize_pages(const float* kv_blocks, int64_t fp32_pages, int8_t* kv_int8, int64_t int8_pages, int64_t layers,
+                        int64_t page_size, int64_t heads, int64_t slot_bytes, const int32_t* src, const int32_t* dst,
+                        const int32_t* rows, int64_t count, void* stream, char* err, size_t errlen) {
+  return convert_pages("quantize_pages", true, const_cast<float*>(kv_blocks), fp32_pages, kv_int8, int8_pages, layers,
+                       page_size, heads, slot_bytes, src, dst, rows, count, stream, err, errlen);
+}
+
+int uocr_dequantize_pages(const int8_t* kv_int8, int64_t int8_pages, float* kv_blocks, int64_t fp32_pages, int64_t layers,
+                          int64_t page_size, int64_t heads, int64_t slot_bytes, const int32_t* src, const int32_t* dst,
+                          const int32_t* rows, int64_t count, void* stream, char* err, size_t errlen) {
+  return convert_pages("dequantize_pages", false, kv_blocks, fp32_pages, const_cast<int8_t*>(kv_int8), int8_pages, layers,
+                       page_size, heads, slot_bytes, src, dst, rows, count, stream, err, errlen);
+}
+
+int uocr_draft_masks(int64_t* masks, const int32_t* parents, int64_t tokens, const int32_t* chunk_offsets, int64_t requests,
+                     void* stream, char* err, size_t errlen) {
+  const char* op = "draft_masks";
+  if (tokens < 0 || tokens > 1 << 25 || requests < 0 || requests > 65535)
+    return fail(err, errlen, "%s: requests must be in [0, 65535] and tokens in [0, 2^25]", op);
+  if (tokens == 0 || requests == 0) return 0;
+  if (!masks || !parents || !chunk_offsets) return fail(err, errlen, "%s: a tensor is missing", op);
+  if (overlap(masks, (size_t)tokens * 8, parents, (size_t)tokens * 4) ||
+      overlap(masks, (size_t)tokens * 8, chunk_offsets, (size_t)(requests + 1) * 4))
+    return fail(err, errlen, "%s: the masks must not overlap the inputs", op);
+  const hipError_t e = launch_draft_masks(masks, parents, chunk_offsets, (int)requests, (int)tokens, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+int uocr_accept_drafts(void* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes,
+                       const uint32_t* lookup, int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
+                       const int32_t* chunk_offsets, const int32_t* parents, const int32_t* drafted, const int32_t* answers,
+                       int64_t tokens, int32_t* counts, int32_t* path, int32_t* next_tokens, uint32_t* cache_lengths_out,
+                       void* stream, char* err, size_t errlen) {
+  const char* op = "accept_drafts";
+  const size_t pool = pool_bytes(op, kv_blocks, pages, layers, page_size, 1, slot_bytes, true, err, errlen);
+  if (pool == 0) return 1;
+  if (tokens < 0 || tokens > 1 << 25 || requests < 0 || requests > 65535)
+    return fail(err, errlen, "%s: requests must be in [0, 65535] and tokens in [0, 2^25]", op);
+  if (lookup_cols < 1 || lookup_cols > INT32_MAX / page_size)
+    return fail(err, errlen, "%s: bad lookup table width %lld", op, (long long)lookup_cols);
+  if (requests == 0) return 0;
+  if (!kv_blocks || !lookup || !cache_lengths || !chunk_offsets || !counts || !next_tokens || !cache_lengths_out ||
+      (tokens > 0 && (!parents || !drafted || !answers || !path)))
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  // every workgroup of a request reads its inputs: none may be an output, and outputs are apart from one another
+  const std::pair<const void*, size_t> outs[] = {{counts, (size_t)requests * 4}, {path, (size_t)tokens * 4},
+                                                 {next_tokens, (size_t)requests * 4},
+                                                 {cache_lengths_out, (size_t)requests * 4}, {kv_blocks, pool}};
+  const std::pair<const void*, size_t> ins[] = {{lookup, (size_t)(requests * lookup_cols) * 4},
+                                                {cache_lengths, (size_t)requests * 4},
+                                                {chunk_offsets, (size_t)(requests + 1) * 4}, {parents, (size_t)tokens * 4},
+                                                {drafted, (size_t)tokens * 4}, {answers, (size_t)tokens * 4}};
+  for (const auto& out : outs) {
+    for (const auto& in : ins)
+      if (overlap(out.first, out.second, in.first, in.second))
+        return fail(err, errlen, "%s: an output must not overlap an input", op);
+    for (const auto& o : outs)
+      if (&o != &out && overlap(out.first, out.second, o.first, o.second))
+        return fail(err, errlen, "%s: the outputs must not overlap one another", op);
+  }
+  AcceptDrafts p{};
+  p.pool = (char*)kv_blocks;
+  p.pages = (int)pages;
+  p.layers = (int)layers;
+  p.page_size = (int)page_size;
+  p.slot_bytes = (int)slot_bytes;
+  p.lookup = lookup;
+  p.lookup_cols = (int)lookup_cols;
+  p.max_rows = (int)(lookup_cols * page_size);
+  p.cache_lengths = cache_lengths;
+  p.offsets = chunk_offsets;
+  p.tokens = (int)tokens;
+  p.parents = parents;
+  p.drafted = drafted;
+  p.answers = answers;
+  p.counts = counts;
+  p.path = path;
+  p.next = next_tokens;
+  p.lengths_out = cache_lengths_out;
+  const hipError_t e = launch_accept_drafts(p, (int)requests, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
+// ------------------------------------------------------------------ beams
+
+static bool beam_sizes(int64_t rows, int64_t vocab, int64_t beams) {
+  return beams >= 1 && beams <= kBeamsMost && vocab >= beams && vocab <= INT32_MAX - (1 << 20) && rows >= 0 && rows <= 65535 &&
+         rows % beams == 0;
+}
+
+size_t uocr_beam_select_workspace_bytes(int64_t rows, int64_t vocab, int64_t beams) {
+  return beam_sizes(rows, vocab, beams) ? beam_workspace_bytes(rows, (int)beams, (int)vocab) : 0;
+}
+
+int uocr_beam_select(int32_t* tokens, int32_t* parents, float* scores_out, int32_t* ended_out, int32_t* lengths_out,
+                     int32_t* history_out, const float* logits, int64_t rows, int64_t vocab, int64_t beams,
+                     const float* scores, int64_t eos, const int32_t* ended, const int32_t* lengths, double alpha,
+                     const int32_t* history, int64_t width, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                     size_t errlen) {
+  const char* op = "beam_select";
+  if (!beam_sizes(rows, vocab, beams))
+    return fail(err, errlen,
+                "%s: %lld rows of %lld logits are not at most 65535 beams in groups of %lld (1 to %d, at most the vocabulary)", op,
+                (long long)rows, (long long)vocab, (long long)beams, kBeamsMost);
+  if (eos < 0 || eos >= vocab) return fail(err, errlen, "%s: eos %lld is not in the vocabulary", op, (long long)eos);
+  if (!(alpha - alpha == 0.0)) return fail(err, errlen, "%s: alpha must be finite", op);
+  if (width < 0 || width > INT32_MAX || (history == nullptr) != (history_out == nullptr) ||
+      (lengths == nullptr) != (lengths_out == nullptr))
+    return fail(err, errlen, "%s: lengths and history need an output each, and only then", op);
+  if (rows == 0) return 0;
+  if (!tokens || !parents || !scores_out || !ended_out || !logits || !scores)
+    return fail(err, errlen, "%s: a tensor is missing", op);
+  const size_t words = (size_t)rows * 4, kept = (size_t)(rows * width) * 4;
+  const std::pair<const void*, size_t> outs[] = {{tokens, words}, {parents, words}, {scores_out, words}, {ended_out, words},
+                                                 {lengths_out, lengths_out ? words : 0},
+                                                 {history_out, history_out ? kept : 0}};
+  const std::pair<const void*, size_t> ins[] = {{logits, (size_t)(rows * vocab) * 4}, {scores, words},
+                                                {ended, ended ? words : 0}, {lengths, lengths ? words : 0},
+                                                {history, history ? kept : 0}};
+  for (const auto& out : outs) {
+    if (out.second == 0) continue;
+    for (const auto& in : ins)
+      if (in.second != 0 && overlap(out.first, out.second, in.first, in.second))
+        return fail(err, errlen, "%s: an output must not overlap an input", op);
+    for (const auto& o : outs)
+      if (&o != &out && o.second != 0 && overlap(out.first, out.second, o.first, o.second))
+        return fail(err, errlen, "%s: the outputs must not overlap one another", op);
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  void* ws = nullptr;
+  if (chunk_workspace(op, workspace, workspace_bytes, beam_workspace_bytes(rows, (int)beams, (int)vocab), s, &ws, err, errlen))
+    return 1;
+  BeamSelect p{};
+  p.logits = logits;
+  p.scores = scores;
+  p.ended = ended;
+  p.lengths = lengths;
+  p.history = history;
+  p.vocab = (int)vocab;
+  p.beams = (int)beams;
+  p.eos = (int)eos;
+  p.width = width;
+  p.alpha = alpha;
+  p.tokens_out = tokens;
+  p.parents_out = parents;
+  p.scores_out = scores_out;
+  p.ended_out = ended_out;
+  p.lengths_out = lengths_out;
+  p.history_out = history_out;
+  const hipError_t e = launch_beam_select(p, rows, ws, s);
+  return e == hipSuccess ? 0 : hip_fail(err, errlen, op, e);
+}
+
 // ------------------------------------------------------------------ the pages of the pool
 
 static int page_pool(const char* op, PagePool& p, float* kv_blocks, int64_t pages, int64_t layers, int64_t page_size,

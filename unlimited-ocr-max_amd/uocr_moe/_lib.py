@@ -68,6 +68,23 @@ SIGNATURES: dict[str, list] = {
     "uocr_paged_chunk_attention_qkv": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
                                        _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _sz, _vp, _cp,
                                        _sz],
+    "uocr_paged_pool_workspace_bytes": [_i64, _i64, _i64, _i64],
+    "uocr_paged_decode_attention_int8": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
+                                         _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _sz, _vp, _cp,
+                                         _sz],
+    "uocr_paged_chunk_attention_int8": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
+                                        _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _sz,
+                                        _vp, _cp, _sz],
+    "uocr_paged_tree_attention": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
+                                  _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _sz, _vp, _cp, _sz],
+    "uocr_quantize_pages": [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _cp, _sz],
+    "uocr_dequantize_pages": [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _cp, _sz],
+    "uocr_draft_masks": [_vp, _vp, _i64, _vp, _i64, _vp, _cp, _sz],
+    "uocr_accept_drafts": [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp,
+                           _vp, _cp, _sz],
+    "uocr_beam_select_workspace_bytes": [_i64, _i64, _i64],
+    "uocr_beam_select": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, ctypes.c_double, _vp,
+                         _i64, _vp, _sz, _vp, _cp, _sz],
     "uocr_copy_pages": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _cp, _sz],
     "uocr_fork_pages_workspace_bytes": [_i64, _i64, _i64, _i64, _i64],
     "uocr_fork_pages": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp,
@@ -91,7 +108,8 @@ SIGNATURES: dict[str, list] = {
     "uocr_moe_timing_end": [_int, _vp, _vp, _sz, ctypes.POINTER(_int), _cp, _sz],
 }
 _RESTYPES = {"uocr_moe_workspace_bytes": _sz, "uocr_paged_attention_workspace_bytes": _sz, "uocr_moe_release": None,
-             "uocr_paged_chunk_workspace_bytes": _sz, "uocr_fork_pages_workspace_bytes": _sz,
+             "uocr_paged_chunk_workspace_bytes": _sz, "uocr_paged_pool_workspace_bytes": _sz,
+             "uocr_beam_select_workspace_bytes": _sz, "uocr_fork_pages_workspace_bytes": _sz,
              "uocr_resize_pages_workspace_bytes": _sz, "uocr_compact_pages_workspace_bytes": _sz}
 
 _LIB: ctypes.CDLL | None = None

@@ -18,8 +18,12 @@ ngram_block            logits f32 [B,V], history i32 [B,W], ngram i32 [1]   f32 
 
 :func:`paged_decode_attention` (decoder.py:425-437) takes its page pool and
 step metadata as a :class:`PagedKv`, :func:`paged_chunk_attention` (several new
-tokens a request) as a :class:`PagedChunk`; :func:`copy_pages`, :func:`fork_pages`,
-:func:`resize_pages` and :func:`compact_pages` move the pool's pages.
+tokens a request, or a tree of drafted ones) as a :class:`PagedChunk`; the pool is
+float32 or int8 (:func:`int8_kv_blocks`).  :func:`copy_pages`, :func:`fork_pages`,
+:func:`resize_pages` and :func:`compact_pages` move the pool's pages,
+:func:`quantize_pages` and :func:`dequantize_pages` convert them,
+:func:`accept_drafts` keeps what a draft got right, :func:`beam_select` chooses
+the next beams.
 
 :func:`custom` dispatches by symbol like ``ops.custom(symbol, values=...)``.
 Inputs must be GPU tensors; non-contiguous views are packed first (the
@@ -32,6 +36,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -319,7 +324,8 @@ class PagedKv:
     ``PagedKv`` / ``PagedStep`` hold them (unlimited_ocr_max/decoder.py:407-422,
     unlimited_ocr_max/kv_cache.py:169-207).
 
-    ``kv_blocks`` f32 ``[pages, 2, layers, page_size, heads, head_dim]`` (its last page the null page);
+    ``kv_blocks`` f32 ``[pages, 2, layers, page_size, heads, head_dim]`` (its last page the null page), or an int8
+    pool (:func:`int8_kv_blocks`);
     ``lookup_table`` ``[B, cols]``, ``attend_lengths`` ``[B]`` (``attend_len - 1``, the attention's cache
     lengths) and ``write_index`` ``[B]`` (the store's), int32 or uint32 on the GPU; ``attend_max`` the
     largest ``attend_len``, a host int.
@@ -346,9 +352,13 @@ def paged_decode_attention(q, k_new, v_new, *, kv: PagedKv, layer_idx: int, scal
     ``q`` / ``k_new`` / ``v_new`` are post-RoPE f32 ``[B, heads, head_dim]``, row ``b`` for request ``b``;
     returns ``[B, heads, head_dim]``, row ``b`` attended over its logical rows ``[0, attend_lengths[b] + 1)``
     of layer ``layer_idx``, logical row ``r`` being slot ``r % page_size`` of page
-    ``lookup_table[b, r // page_size]``.  ``kv.kv_blocks`` is written in place (it must be contiguous).
+    ``lookup_table[b, r // page_size]``.  ``kv.kv_blocks`` is written in place (it must be contiguous); over an int8
+    pool the new row is attended as it was rounded.
     """
     op = "paged_decode_attention"
+    if isinstance(kv.kv_blocks, torch.Tensor) and kv.kv_blocks.dtype is torch.int8:
+        q, views, stride = _rows_apart(op, q, (("k_new", k_new), ("v_new", v_new)))
+        return _decode_int8(op, (q, *views), stride, q.shape[1], q.shape[2], kv, layer_idx, scale, out, workspace)
     q = _gpu(op, "q", q, torch.float32, 3)
     k_new = _gpu(op, "k_new", k_new, torch.float32, 3)
     v_new = _gpu(op, "v_new", v_new, torch.float32, 3)
@@ -390,6 +400,11 @@ def paged_decode_attention_qkv(qkv, positions, cos_table, sin_table, *, heads: i
     bits: ``qkv [B, 3 * heads * head_dim]`` (q, k, v side by side, q and k before RoPE; rows may be
     strided) is one fused projection's output (unlimited_ocr_max/decoder.py:487-492 with :425-437)."""
     op = "paged_decode_attention_qkv"
+    if isinstance(kv.kv_blocks, torch.Tensor) and kv.kv_blocks.dtype is torch.int8:
+        rows = _fused_rows(op, qkv, heads)
+        rope_at = _rope_at(op, positions, cos_table, sin_table, rows)
+        return _decode_int8(op, (rows,), rows.stride(0), heads, rows.shape[1] // (3 * heads), kv, layer_idx, scale, out,
+                            workspace, rope_at)
     if not isinstance(qkv, torch.Tensor) or qkv.dtype != torch.float32 or qkv.dim() != 2 or not qkv.is_cuda:
         raise ValueError(f"{op}: qkv must be an fp32 [rows, 3 * heads * head_dim] GPU tensor")
     if qkv.stride(1) != 1:
@@ -428,6 +443,62 @@ def paged_decode_attention_qkv(qkv, positions, cos_table, sin_table, *, heads: i
     return out
 
 
+def _decode_int8(op: str, inputs: tuple, stride: int, heads: int, head_dim: int, kv: PagedKv, layer_idx: int,
+                 scale: float, out, workspace, rope_at: tuple = ()) -> torch.Tensor:
+    """The decode attention over an int8 pool: ``inputs`` q, k_new and v_new, or one tensor with all three side by side,
+    rows ``stride`` floats apart; ``rope_at`` positions and tables, where q and k come before RoPE."""
+    rows = inputs[0].shape[0]
+    lookup = _ids(op, "lookup_table", kv.lookup_table, 2)
+    attend = _ids(op, "attend_lengths", kv.attend_lengths, 1)
+    write = _ids(op, "write_index", kv.write_index, 1)
+    if lookup.shape[0] != rows or attend.shape[0] != rows or write.shape[0] != rows:
+        raise ValueError(f"{op}: the step metadata is not for {rows} rows")
+    return _pool_call(op, "uocr_paged_decode_attention_int8", inputs, stride, heads, head_dim, kv.kv_blocks, layer_idx,
+                      lookup, (), int(kv.attend_max), (attend, write), scale, out, workspace, rope_at)
+
+
+def _pool_call(op: str, name: str, inputs: tuple, stride: int, heads: int, head_dim: int, blocks, layer_idx: int, lookup,
+               requests: tuple, attend_max: int, metadata: tuple, scale: float, out, workspace,
+               rope_at: tuple) -> torch.Tensor:
+    """An attention entry over an int8 pool, or of trees: ``metadata`` is (lengths, write_index) of the decode entry,
+    (lengths, offsets, visible or None) of the others."""
+    like = inputs[0]
+    tokens = like.shape[0]
+    if blocks.dtype is torch.int8:
+        pages, _, layers, page_size, slot = _int8_pool(op, blocks).shape
+        slots = (slot,)
+        if slot < 132 * heads:
+            raise ValueError(f"{op}: kv_blocks has slots of {slot} bytes, too few for {heads} heads")
+    else:
+        pages, _, layers, page_size, bh, bd = _pool(op, blocks).shape
+        slots = ()
+        if (bh, bd) != (heads, head_dim):
+            raise ValueError(f"{op}: kv_blocks {tuple(blocks.shape)} does not hold {heads} heads of {head_dim}")
+    if out is None:
+        out = like.new_empty((tokens, heads, head_dim))
+    elif tuple(_out(op, "out", out, torch.float32, 3).shape) != (tokens, heads, head_dim):
+        raise ValueError(f"{op}: out must be {(tokens, heads, head_dim)}, got {tuple(out.shape)}")
+    need = 0
+    # nothing is allocated for more rows than the table addresses: the entry refuses them
+    if workspace is not None or attend_max <= lookup.shape[1] * page_size:
+        need = _lib.load().uocr_paged_pool_workspace_bytes(tokens, lookup.shape[0], heads, attend_max)
+    ws = _workspace(op, workspace, need, like)
+    if len(inputs) == 1:
+        q = like.data_ptr()
+        pointers = (q, q + 4 * heads * head_dim, q + 8 * heads * head_dim)
+    else:
+        pointers = tuple(t.data_ptr() for t in inputs)
+    positions = (rope_at[0].data_ptr(), rope_at[1].data_ptr(), rope_at[2].data_ptr(), rope_at[1].shape[0]) if rope_at else \
+        (None, None, None, 0)
+    lengths, other, *visible = metadata
+    tail = (other.data_ptr(), attend_max, _ptr(visible[0])) if visible else (attend_max, other.data_ptr())
+    _on_device(op, name, out.data_ptr(), *pointers, tokens, heads, head_dim, stride, *positions, blocks.data_ptr(), pages,
+               layers, page_size, *slots, int(layer_idx), lookup.data_ptr(), *requests, lookup.shape[1],
+               lengths.data_ptr(), *tail, float(scale), _ptr(ws), _nbytes(ws),
+               tensors=(*inputs, out, blocks, lookup, *metadata, ws, *rope_at))
+    return out
+
+
 @dataclass(frozen=True)
 class PagedChunk:
     """The page pool and the metadata of a call that appends a chunk of new tokens to each of ``N`` requests.
@@ -436,6 +507,10 @@ class PagedChunk:
     uint32), each request's rows in the cache before its chunk; ``chunk_offsets`` int32 ``[N + 1]``, ascending:
     request ``n``'s chunk is token rows ``chunk_offsets[n]`` up to ``chunk_offsets[n + 1]`` (none: an empty
     chunk); ``attend_max`` the largest sum of the two, a host int.
+
+    ``visible`` int64 ``[tokens]``: which tokens of its own chunk each one attends, bit ``j`` the chunk's token ``j``
+    (of the first 64; itself is one of the bits), beside all of its request's cached rows: a tree's words are
+    :func:`draft_masks`'.  None: the ones up to itself.
 
     Chunks are appended.  A ring's rows, which :class:`PagedKv` writes again by its ``write_index``, have no form here:
     a draft ends where its ring wraps.
@@ -446,10 +521,33 @@ class PagedChunk:
     cache_lengths: torch.Tensor
     chunk_offsets: torch.Tensor
     attend_max: int
+    visible: torch.Tensor | None = None
+
+
+def int8_kv_blocks(pages: int, layers: int, page_size: int, heads: int, *, device="cuda") -> torch.Tensor:
+    """An int8 page pool of zeros, ``[pages, 2, layers, page_size, slot]``, for heads of 128 values.
+
+    A row's slot holds its heads' 128 values each, then a float32 scale of each head (``value * scale`` is what is
+    meant), padded to a multiple of 128 bytes: 27 % of the float32 pool's for ten heads.  Rows are quantised as they
+    are written: ``scale = max|x| * float32(1 / 127)`` (1 where that is 0), ``rint(x / scale)``, in float32; a row with
+    a value that is not finite is kept as NaN.  The attention entries, the page
+    operators and :func:`accept_drafts` take it where they take a float32 pool."""
+    return torch.zeros((pages, 2, layers, page_size, -(-132 * heads // 128) * 128), dtype=torch.int8, device=device)
+
+
+def _int8_pool(op: str, blocks) -> torch.Tensor:
+    """An int8 page pool: written in place, so it must be contiguous."""
+    if not isinstance(blocks, torch.Tensor) or blocks.dtype != torch.int8 or blocks.dim() != 5 or \
+            not blocks.is_cuda or not blocks.is_contiguous() or blocks.shape[1] != 2 or blocks.shape[4] % 16:
+        raise ValueError(f"{op}: an int8 pool must be a contiguous [pages, 2, layers, page_size, slot] GPU tensor with "
+                         "slots of whole 16 bytes (int8_kv_blocks)")
+    return blocks
 
 
 def _pool(op: str, blocks) -> torch.Tensor:
-    """A page pool: written in place, so it must be contiguous."""
+    """A page pool: written in place, so it must be contiguous.  Of an int8 one the same bytes, a slot as one head."""
+    if isinstance(blocks, torch.Tensor) and blocks.dtype == torch.int8:
+        return _int8_pool(op, blocks).view(torch.float32).unsqueeze(4)
     if not isinstance(blocks, torch.Tensor) or blocks.dtype != torch.float32 or blocks.dim() != 6 or \
             not blocks.is_cuda or not blocks.is_contiguous() or blocks.shape[1] != 2:
         raise ValueError(f"{op}: kv_blocks must be a contiguous f32 [pages, 2, layers, page_size, heads, head_dim] "
@@ -530,22 +628,52 @@ def paged_chunk_attention(q, k_new, v_new, *, kv: PagedChunk, layer_idx: int, sc
     written in place.
     """
     op = "paged_chunk_attention"
-    q = _rows_view(op, "q", q)
-    # rows of one stride: views of unlike ones are packed
-    views = [_rows_view(op, name, t) for name, t in (("k_new", k_new), ("v_new", v_new))]
-    if any(t.shape != q.shape for t in views):
-        raise ValueError(f"{op}: q, k_new and v_new disagree on shape: {tuple(q.shape)}, {tuple(views[0].shape)}, "
-                         f"{tuple(views[1].shape)}")
+    q, (k, v), stride = _rows_apart(op, q, (("k_new", k_new), ("v_new", v_new)))
     tokens, heads, head_dim = q.shape
-    stride = q.stride(0)
-    if any(t.stride(0) != stride or t.data_ptr() % 16 for t in (q, *views)) or stride % 4 or \
-            not heads * head_dim <= stride < _CHUNK_STRIDE:
-        q, views = _packed(q), [_packed(t) for t in views]
-        stride = heads * head_dim
-    k, v = views
+    if _with_masks_or_int8(kv):
+        return _chunk_masked(op, (q, k, v), stride, heads, head_dim, kv, layer_idx, scale, out, workspace)
     return _chunk_call(op, "uocr_paged_chunk_attention", (q.data_ptr(), k.data_ptr(), v.data_ptr(), tokens, heads,
                                                           head_dim, stride),
                        tokens, heads, head_dim, kv, layer_idx, scale, out, workspace, q, [q, k, v])
+
+
+def _rows_apart(op: str, q, others: tuple) -> tuple:
+    """q and the others as ``[tokens, heads, D]`` views whose rows are one stride apart (views of unlike ones are packed)."""
+    q = _rows_view(op, "q", q)
+    views = [_rows_view(op, name, t) for name, t in others]
+    if any(t.shape != q.shape for t in views):
+        raise ValueError(f"{op}: q, k_new and v_new disagree on shape: {tuple(q.shape)}, {tuple(views[0].shape)}, "
+                         f"{tuple(views[1].shape)}")
+    stride = q.stride(0)
+    if any(t.stride(0) != stride or t.data_ptr() % 16 for t in (q, *views)) or stride % 4 or \
+            not q.shape[1] * q.shape[2] <= stride < _CHUNK_STRIDE:
+        q, views = _packed(q), [_packed(t) for t in views]
+        stride = q.shape[1] * q.shape[2]
+    return q, views, stride
+
+
+def _with_masks_or_int8(kv: PagedChunk) -> bool:
+    return kv.visible is not None or (isinstance(kv.kv_blocks, torch.Tensor) and kv.kv_blocks.dtype is torch.int8)
+
+
+def _chunk_masked(op: str, inputs: tuple, stride: int, heads: int, head_dim: int, kv: PagedChunk, layer_idx: int,
+                  scale: float, out, workspace, rope_at: tuple = ()) -> torch.Tensor:
+    """The chunk attention over an int8 pool, or of tokens that see chosen ones of their chunk."""
+    lookup = _ids(op, "lookup_table", kv.lookup_table, 2)
+    cached = _ids(op, "cache_lengths", kv.cache_lengths, 1)
+    offsets = _gpu(op, "chunk_offsets", kv.chunk_offsets, torch.int32, 1)
+    requests = lookup.shape[0]
+    if cached.shape[0] != requests or offsets.shape[0] != requests + 1:
+        raise ValueError(f"{op}: the chunks' metadata is not for {requests} requests")
+    visible = kv.visible
+    if visible is not None:
+        visible = _gpu(op, "visible", visible, torch.int64, 1)
+        if visible.shape[0] != inputs[0].shape[0]:
+            raise ValueError(f"{op}: {visible.shape[0]} masks for {inputs[0].shape[0]} tokens")
+    int8 = isinstance(kv.kv_blocks, torch.Tensor) and kv.kv_blocks.dtype is torch.int8
+    return _pool_call(op, "uocr_paged_chunk_attention_int8" if int8 else "uocr_paged_tree_attention", inputs, stride, heads,
+                      head_dim, kv.kv_blocks, layer_idx, lookup, (requests,), int(kv.attend_max),
+                      (cached, offsets, visible), scale, out, workspace, rope_at)
 
 
 #: Input rows must be fewer floats apart than this (rows further apart are packed).
@@ -565,25 +693,40 @@ def paged_chunk_attention_qkv(qkv, positions, cos_table, sin_table, *, heads: in
     ``positions`` int32 ``[tokens]`` (unlimited_ocr_max/decoder.py:459-462 with :425-437).  The stored k rows
     have the bits of :func:`rope`."""
     op = "paged_chunk_attention_qkv"
-    if not isinstance(qkv, torch.Tensor) or qkv.dtype != torch.float32 or qkv.dim() != 2 or not qkv.is_cuda:
-        raise ValueError(f"{op}: qkv must be an fp32 [tokens, 3 * heads * head_dim] GPU tensor")
+    qkv = _fused_rows(op, qkv, heads)
     tokens, width = qkv.shape
-    if heads < 1 or width % (3 * heads):
-        raise ValueError(f"{op}: qkv width {width} is not 3 x {heads} heads")
-    if qkv.stride(1) != 1 or not width <= qkv.stride(0) < _CHUNK_STRIDE or qkv.stride(0) % 4 or qkv.data_ptr() % 16:
-        qkv = _packed(qkv)
     head_dim = width // (3 * heads)
-    positions = _gpu(op, "positions", positions, torch.int32, 1)
-    cos_table = _gpu(op, "cos_table", cos_table, torch.float32, 2)
-    sin_table = _gpu(op, "sin_table", sin_table, torch.float32, 2)
-    cos_table, sin_table = _packed(cos_table), _packed(sin_table)
-    if positions.shape[0] != tokens or cos_table.shape != sin_table.shape:
-        raise ValueError(f"{op}: positions or the cos/sin tables do not fit {tokens} tokens")
+    positions, cos_table, sin_table = rope_at = _rope_at(op, positions, cos_table, sin_table, qkv)
+    if _with_masks_or_int8(kv):
+        return _chunk_masked(op, (qkv,), max(qkv.stride(0), width), heads, head_dim, kv, layer_idx, scale, out, workspace,
+                             rope_at)
     return _chunk_call(op, "uocr_paged_chunk_attention_qkv",
                        (qkv.data_ptr(), tokens, heads, head_dim, max(qkv.stride(0), width), positions.data_ptr(),
                         cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0], cos_table.shape[1]),
                        tokens, heads, head_dim, kv, layer_idx, scale, out, workspace, qkv,
                        [qkv, positions, cos_table, sin_table])
+
+
+def _fused_rows(op: str, qkv, heads: int) -> torch.Tensor:
+    """One projection's q, k and v side by side, rows at 16-byte boundaries."""
+    if not isinstance(qkv, torch.Tensor) or qkv.dtype != torch.float32 or qkv.dim() != 2 or not qkv.is_cuda:
+        raise ValueError(f"{op}: qkv must be an fp32 [tokens, 3 * heads * head_dim] GPU tensor")
+    width = qkv.shape[1]
+    if heads < 1 or width % (3 * heads):
+        raise ValueError(f"{op}: qkv width {width} is not 3 x {heads} heads")
+    if qkv.stride(1) != 1 or not width <= qkv.stride(0) < _CHUNK_STRIDE or qkv.stride(0) % 4 or qkv.data_ptr() % 16:
+        qkv = _packed(qkv)
+    return qkv
+
+
+def _rope_at(op: str, positions, cos_table, sin_table, rows: torch.Tensor) -> tuple:
+    """The rows' positions and RoPE's tables, checked."""
+    positions = _gpu(op, "positions", positions, torch.int32, 1)
+    cos_table = _packed(_gpu(op, "cos_table", cos_table, torch.float32, 2))
+    sin_table = _packed(_gpu(op, "sin_table", sin_table, torch.float32, 2))
+    if positions.shape[0] != rows.shape[0] or cos_table.shape != sin_table.shape:
+        raise ValueError(f"{op}: positions or the cos/sin tables do not fit {rows.shape[0]} tokens")
+    return positions, cos_table, sin_table
 
 
 def copy_pages(kv_blocks, src, dst, *, rows=None) -> torch.Tensor:
@@ -601,7 +744,154 @@ def copy_pages(kv_blocks, src, dst, *, rows=None) -> torch.Tensor:
     pages, _, layers, page_size, heads, head_dim = blocks.shape
     _on_device(op, "uocr_copy_pages", blocks.data_ptr(), pages, layers, page_size, heads, head_dim, src.data_ptr(),
                dst.data_ptr(), _ptr(rows), src.shape[0], tensors=[blocks, src, dst, rows])
-    return blocks
+    return kv_blocks
+
+
+def _convert_pages(op: str, name: str, kv_blocks, kv_int8, first: tuple, src, dst, rows) -> None:
+    wide, narrow = _pool(op, kv_blocks), _int8_pool(op, kv_int8)
+    if wide.dim() != 6 or kv_blocks.dtype is torch.int8:
+        raise ValueError(f"{op}: kv_blocks must be the float32 pool")
+    pages, _, layers, page_size, heads, head_dim = wide.shape
+    if head_dim != 128 or narrow.shape[2:4] != wide.shape[2:4] or narrow.shape[4] < 132 * heads:
+        raise ValueError(f"{op}: pools of {tuple(wide.shape)} and {tuple(narrow.shape)} do not hold the same rows of heads of "
+                         "128")
+    src = _gpu(op, "src", src, torch.int32, 1)
+    dst = _gpu(op, "dst", dst, torch.int32, 1)
+    rows = None if rows is None else _gpu(op, "rows", rows, torch.int32, 1)
+    if dst.shape != src.shape or (rows is not None and rows.shape != src.shape):
+        raise ValueError(f"{op}: src, dst and rows must have one length")
+    sides = {"wide": (wide.data_ptr(), pages), "narrow": (narrow.data_ptr(), narrow.shape[0])}
+    _on_device(op, name, *sides[first[0]], *sides[first[1]], layers, page_size, heads, narrow.shape[4], src.data_ptr(),
+               dst.data_ptr(), _ptr(rows), src.shape[0], tensors=(wide, narrow, src, dst, rows))
+
+
+def quantize_pages(kv_blocks, src, kv_int8, dst, *, rows=None) -> torch.Tensor:
+    """Page ``dst[i]`` of the int8 pool = page ``src[i]`` of the float32 one, k and v of all layers, quantised as the
+    attention entries quantise new rows (:func:`int8_kv_blocks`), as if one pair after the other.  ``src``, ``dst``
+    int32 ``[n]`` on the GPU; with ``rows`` (int32 ``[n]``) only each layer's first ``rows[i]`` rows.  Pairs with an id
+    outside its pool are skipped.  Returns ``kv_int8``, written in place."""
+    _convert_pages("quantize_pages", "uocr_quantize_pages", kv_blocks, kv_int8, ("wide", "narrow"), src, dst, rows)
+    return kv_int8
+
+
+def dequantize_pages(kv_int8, src, kv_blocks, dst, *, rows=None) -> torch.Tensor:
+    """:func:`quantize_pages` the other way: page ``dst[i]`` of the float32 pool = the values that page ``src[i]`` of the
+    int8 one stands for.  Returns ``kv_blocks``, written in place."""
+    _convert_pages("dequantize_pages", "uocr_dequantize_pages", kv_blocks, kv_int8, ("narrow", "wide"), src, dst, rows)
+    return kv_blocks
+
+
+def draft_masks(parents, chunk_offsets, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The words :attr:`PagedChunk.visible` of trees of drafted tokens: int64 ``[tokens]``, the bits of each token's
+    ancestors and its own.  A request's chunk is its tree, token 0 the root; ``parents`` int32 ``[tokens]`` is the place
+    in the chunk of each one's parent, which comes before it (any other value: it has none)."""
+    op = "draft_masks"
+    parents = _gpu(op, "parents", parents, torch.int32, 1)
+    offsets = _gpu(op, "chunk_offsets", chunk_offsets, torch.int32, 1)
+    if offsets.shape[0] < 1:
+        raise ValueError(f"{op}: chunk_offsets must have a word more than there are requests")
+    if out is None:
+        out = parents.new_empty(parents.shape[0], dtype=torch.int64)
+    elif _out(op, "out", out, torch.int64, 1).shape != parents.shape:
+        raise ValueError(f"{op}: out must have {parents.shape[0]} words")
+    _on_device(op, "uocr_draft_masks", out.data_ptr(), parents.data_ptr(), parents.shape[0], offsets.data_ptr(),
+               offsets.shape[0] - 1, tensors=(parents, offsets, out))
+    return out
+
+
+def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What the model's answers confirm of trees that :func:`paged_chunk_attention` attended: from token 0 of a
+    request's chunk to the first child whose token is its parent's answer, and so on.
+
+    ``parents`` as for :func:`draft_masks`, ``tokens`` int32 ``[tokens]`` the trees' tokens, ``answers`` int32
+    ``[tokens]`` what the model says after each.  The path's rows, k and v of every layer of ``kv.kv_blocks`` (a pool of
+    either kind, written in place), move together behind the cached ones.  Returns ``(counts, path, next_tokens,
+    cache_lengths)``: int32 ``[N]`` the paths' lengths (0: an empty chunk); int32 ``[tokens]`` their tokens' places in the
+    chunk, at the front of its words, -1 behind; int32 ``[N]`` the answer to the last (-1: an empty chunk); the cached rows
+    now, as ``kv.cache_lengths``.  Of a chunk the first 64 tokens count."""
+    op = "accept_drafts"
+    blocks = _pool(op, kv.kv_blocks)
+    pages, _, layers, page_size, heads, head_dim = blocks.shape
+    lookup = _ids(op, "lookup_table", kv.lookup_table, 2)
+    cached = _ids(op, "cache_lengths", kv.cache_lengths, 1)
+    offsets = _gpu(op, "chunk_offsets", kv.chunk_offsets, torch.int32, 1)
+    parents = _gpu(op, "parents", parents, torch.int32, 1)
+    tokens = _gpu(op, "tokens", tokens, torch.int32, 1)
+    answers = _gpu(op, "answers", answers, torch.int32, 1)
+    n, total = lookup.shape[0], parents.shape[0]
+    if cached.shape[0] != n or offsets.shape[0] != n + 1:
+        raise ValueError(f"{op}: the chunks' metadata is not for {n} requests")
+    if tokens.shape[0] != total or answers.shape[0] != total:
+        raise ValueError(f"{op}: parents, tokens and answers must have one length")
+    counts, path, following = parents.new_empty(n), parents.new_empty(total), parents.new_empty(n)
+    lengths = torch.empty_like(cached)
+    _on_device(op, "uocr_accept_drafts", blocks.data_ptr(), pages, layers, page_size, 4 * heads * head_dim,
+               lookup.data_ptr(), n, lookup.shape[1], cached.data_ptr(), offsets.data_ptr(), parents.data_ptr(),
+               tokens.data_ptr(), answers.data_ptr(), total, counts.data_ptr(), path.data_ptr(), following.data_ptr(),
+               lengths.data_ptr(), tensors=(blocks, lookup, cached, offsets, parents, tokens, answers))
+    return counts, path, following, lengths
+
+
+class Beams(NamedTuple):
+    """The beams that :func:`beam_select` chose, a request's rows in their order (``lengths`` and ``history`` where they
+    were given)."""
+
+    tokens: torch.Tensor
+    parents: torch.Tensor
+    scores: torch.Tensor
+    ended: torch.Tensor
+    lengths: torch.Tensor | None
+    history: torch.Tensor | None
+
+
+#: The most beams of a request.
+BEAMS_MOST = 32
+
+
+def beam_select(logits, scores, *, beams: int, eos: int, ended=None, lengths=None, alpha: float = 0.0, history=None,
+                workspace: torch.Tensor | None = None) -> Beams:
+    """A step of beam search: of each request's ``beams`` rows and their next tokens the best ``beams``.
+
+    ``logits`` f32 ``[rows, vocab]`` (after :func:`ngram_block`), request ``r``'s beams rows ``r * beams`` on; ``scores``
+    f32 ``[rows]`` the beams' sums of log probabilities (``-inf``: none yet, as all but the first beam of a new request).
+    A candidate's key is ``scores[b] + logits[b, v] - logsumexp(logits[b])``; a beam whose ``ended`` (int32 ``[rows]``)
+    is set has one candidate, ``eos`` at its score.  They rank by key, or, given ``lengths`` (int32 ``[rows]``, the
+    tokens of each beam), by ``key / length ** alpha`` with the new token counted.  Keys and ranks are in 64 bits; ties go to
+    the lower (row, token); candidates without a finite rank come last, with score ``-inf``.
+
+    ``history`` int32 ``[rows, width]`` (:func:`ngram_block`'s) follows its beam: without its first id, and with the token
+    at the end (an ended beam's as it is).  ``parents`` are rows of ``logits``, for :func:`fork_pages` with the rows
+    themselves as children.  Results are new tensors."""
+    op = "beam_select"
+    logits = _gpu(op, "logits", logits, torch.float32, 2)
+    scores = _gpu(op, "scores", scores, torch.float32, 1)
+    rows, vocab = logits.shape
+    given = [scores]
+    if ended is not None:
+        ended = _gpu(op, "ended", ended, torch.int32, 1)
+        given.append(ended)
+    if lengths is not None:
+        lengths = _gpu(op, "lengths", lengths, torch.int32, 1)
+        given.append(lengths)
+    width = 0
+    if history is not None:
+        history = _gpu(op, "history", history, torch.int32, 2)
+        width = history.shape[1]
+        given.append(history)
+    if any(t.shape[0] != rows for t in given):
+        raise ValueError(f"{op}: scores, ended, lengths and history must have {rows} rows")
+    need = _lib.load().uocr_beam_select_workspace_bytes(rows, vocab, beams)
+    ws = _workspace(op, workspace, need, logits)
+    out_scores = torch.empty_like(scores)
+    tokens = scores.new_empty(rows, dtype=torch.int32)
+    parents, now_ended = torch.empty_like(tokens), torch.empty_like(tokens)
+    now_lengths = None if lengths is None else torch.empty_like(tokens)
+    now_history = None if history is None else torch.empty_like(history)
+    _on_device(op, "uocr_beam_select", tokens.data_ptr(), parents.data_ptr(), out_scores.data_ptr(), now_ended.data_ptr(),
+               _ptr(now_lengths), _ptr(now_history), logits.data_ptr(), rows, vocab, int(beams), scores.data_ptr(), int(eos),
+               _ptr(ended), _ptr(lengths), float(alpha), _ptr(history), width, _ptr(ws), _nbytes(ws),
+               tensors=(logits, *given, ws))
+    return Beams(tokens, parents, out_scores, now_ended, now_lengths, now_history)
 
 
 def _tables(op: str, ref_counts, lookup_table, out_ref_counts, out_lookup) -> tuple:
