@@ -20,6 +20,7 @@
 // The scores are S^T = K Q^T and the results O^T = V^T P^T: a lane owns a query, and its 16 scores of a block of 32 rows
 // come in the order in which the second product wants the weights.
 #include <algorithm>
+#include <type_traits>
 
 #include "chunk_device.h"
 #include "int8_rows.h"
@@ -37,6 +38,15 @@ constexpr int kThreads = kWaves * kWave;
 constexpr float kInf = __builtin_huge_valf();
 // A maximum may lag by so many binades before the sums are rescaled (the weights are floats: nothing is lost).
 constexpr float kSlack = 8.0f;
+#ifndef UOCR_ONE_FILL
+#define UOCR_ONE_FILL 1
+#endif
+#ifndef UOCR_ONE_FEW
+#define UOCR_ONE_FEW 4
+#endif
+#ifndef UOCR_ONE_ROUND
+#define UOCR_ONE_ROUND 4
+#endif
 
 enum Mode { kOne, kCausal, kTree };
 
@@ -71,21 +81,14 @@ __device__ __forceinline__ char* slot_of(const PoolArgs& a, int n, int r) {
 
 // One wave per (token, head): lane d has the pair (d, d + 64) of k and of v.  Queries that come before RoPE are rotated
 // where they are read.
-template <bool kInt8, Mode kMode>
+template <bool kInt8>
 __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
   const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   if (th >= (int64_t)a.tokens * a.heads) return;
   const int t = (int)(th / a.heads), h = (int)(th % a.heads), d = lane_id();
-  int n = t;
-  int64_t row;
-  if constexpr (kMode == kOne) {
-    row = ldg(a.write_index + t);
-  } else {
-    Chunk c;
-    if (!chunk_of(a, t, c)) return;
-    n = c.n;
-    row = (int64_t)c.cached + (t - c.first);
-  }
+  Chunk c;
+  if (!chunk_of(a, t, c)) return;
+  const int64_t row = (int64_t)c.cached + (t - c.first);
   if (row >= a.max_rows) return;  // past what the lookup row addresses: not stored
   const int64_t src = (int64_t)t * a.in_stride + (int64_t)h * kD;
   const float *k = a.k_new + src, *v = a.v_new + src;
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
     x[0] = rotated(k, a.rope.cos_t + at, a.rope.sin_t + at, d);
     x[1] = rotated(k, a.rope.cos_t + at, a.rope.sin_t + at, d + 64);
   }
-  char* slot = slot_of(a, n, (int)row);
+  char* slot = slot_of(a, c.n, (int)row);
   if constexpr (kInt8) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -120,6 +123,8 @@ __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
 // A call's rows are cut into splits where the tiles of queries alone do not fill the device.
 struct PoolCuts {
   int split_rows, splits, slots;  // slots: tiles of queries at most
+  int groups;                     // a request's pieces side by side: its heads, or pairs of them
+  bool few;                       // decode: fewer (request, head) pairs than half the CUs
   Divide by_split, by_heads;
 };
 // A tile of a request's tokens [t0, t_last], a head, and rows [begin, stop) of the all_rows that the tile attends.
@@ -143,9 +148,10 @@ __device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
   c.cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)(kMode == kOne ? a.max_rows - 1 : a.max_rows));
   return c;
 }
-// Items go to the XCDs in stretches, an item's heads side by side: the heads of a row are neighbours in memory (an int8
-// pool's share the line of their scales), and their XCD reads it once.  Up to 64 requests every wave counts the pieces
-// that there are; of more, an item is a slot, whose tile and split may not exist.
+// Items go to the XCDs in stretches, a piece's heads side by side: the heads of a row are neighbours in memory (an int8
+// pool's share the line of their scales), as the tiles of a request read the same rows, and their XCD reads them once.
+// (Pieces that go round the XCDs: eight trees of 61 over 4000 rows 130 us for 110.)  Up to 64 requests every wave counts
+// the pieces that there are; of more, a piece is a slot, whose tile and split may not exist.
 template <Mode kMode>
 __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c, Piece& p) {
   const int turn = (int)(blockIdx.x / 8), xcd = (int)(blockIdx.x % 8);
@@ -354,6 +360,13 @@ struct Running {
   f32x16 o[4];  // register r of o[u]: column 4 (8 (r / 4) + 4 h + r % 4) + u
 };
 
+__device__ __forceinline__ void start(Running& w) {
+  w.m = -kInf;
+  w.l = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w.o[u] = f32x16{};
+}
+
 // Which of a block's rows a lane's query attends: those below `live`, or, for a tree, the bits of a word.
 __device__ __forceinline__ uint32_t tree_rows(uint64_t visible, int off, int live) {
   uint32_t set;
@@ -436,6 +449,7 @@ __device__ __forceinline__ void add_values(Running& w, const Stage<kInt8>& v, co
 
 // The rows (bits of the block's) with a value that is not finite, whose values become 0: a row that a query does not
 // attend must leave nothing in its sum, and one that it attends makes it NaN.
+__device__ __forceinline__ uint32_t take_infinite(Stage<true>&) { return 0; }  // int8 is finite
 __device__ __forceinline__ uint32_t take_infinite(Stage<false>& v) {
   uint32_t top = 0;
 #pragma unroll
@@ -526,58 +540,33 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   uint64_t visible = 0;
   if constexpr (kMode == kTree) visible = (uint64_t)ldg(a.visible + my_t);
   Running run;
-  run.m = -kInf;
-  run.l = 0.0f;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) run.o[u] = f32x16{};
+  start(run);
   __syncthreads();
+  const auto walk = [&](auto careful) {
 #pragma unroll 1
-  for (int key0 = first; key0 < stop; key0 += kWaves * kBlock) {
-    const int next = key0 + kWaves * kBlock;
-    const char* next_base = next < stop ? block_at(next) : a.pool;
-    f32x16 s = scores(k, qs, lane);
-    f32x4 vs[4];
-    if constexpr (kInt8) {
-      row_scales[wave][h][lane & 31] = h == 0 ? k.scale * c : v.scale;
-      __builtin_amdgcn_wave_barrier();
+    for (int key0 = first; key0 < stop; key0 += kWaves * kBlock) {
+      const int next = key0 + kWaves * kBlock;
+      const char* next_base = next < stop ? block_at(next) : a.pool;
+      f32x16 s = scores(k, qs, lane);
+      f32x4 vs[4];
+      if constexpr (kInt8) {
+        row_scales[wave][h][lane & 31] = h == 0 ? k.scale * c : v.scale;
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 ks = *(const f32x4*)&row_scales[wave][0][8 * g + 4 * h];
-        vs[g] = *(const f32x4*)&row_scales[wave][1][8 * g + 4 * h];
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 ks = *(const f32x4*)&row_scales[wave][0][8 * g + 4 * h];
+          vs[g] = *(const f32x4*)&row_scales[wave][1][8 * g + 4 * h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * g + e] *= ks[e];
+          for (int e = 0; e < 4; ++e) s[4 * g + e] *= ks[e];
+        }
+        __builtin_amdgcn_wave_barrier();
+      } else {
+        s *= c;
       }
-      __builtin_amdgcn_wave_barrier();
-    } else {
-      s *= c;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (next < stop) load_keys(k, a, next_base, head, stop - 1 - next, lane);
-    const bool masked = key0 + kBlock > all;
-    if (masked) {
-      uint32_t set = 0;
-      if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
-      const int live = limit - key0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 8 * (r / 4) + 4 * h + r % 4;
-        const bool seen = kMode == kTree ? (set >> row & 1u) != 0 : row < live;
-        s[r] = seen ? s[r] : -kInf;
-      }
-    }
-    if constexpr (!kInt8) {
-      const uint32_t bad = take_infinite(v);
-      if (bad != 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (bad >> (8 * (r / 4) + 4 * h + r % 4) & 1u && s[r] != -kInf) run.l = __uint_as_float(0x7fc00000u);
-      }
-    }
-    weigh(run, s);
-    if constexpr (kInt8) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= vs[r / 4][r % 4];
-      if (masked) {  // the scales of rows that are not attended may be anything
+      __builtin_amdgcn_sched_barrier(0);
+      if (next < stop) load_keys(k, a, next_base, head, stop - 1 - next, lane);
+      const bool masked = key0 + kBlock > all;
+      if (masked) {
         uint32_t set = 0;
         if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
         const int live = limit - key0;
@@ -585,13 +574,55 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
         for (int r = 0; r < 16; ++r) {
           const int row = 8 * (r / 4) + 4 * h + r % 4;
           const bool seen = kMode == kTree ? (set >> row & 1u) != 0 : row < live;
-          s[r] = seen ? s[r] : 0.0f;
+          s[r] = seen ? s[r] : -kInf;
         }
       }
+      if constexpr (decltype(careful)::value) {
+        const uint32_t bad = take_infinite(v);
+        if (bad != 0) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (bad >> (8 * (r / 4) + 4 * h + r % 4) & 1u && s[r] != -kInf) run.l = __uint_as_float(0x7fc00000u);
+        }
+      }
+      weigh(run, s);
+      if constexpr (kInt8) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= vs[r / 4][r % 4];
+        if (masked) {  // the scales of rows that are not attended may be anything
+          uint32_t set = 0;
+          if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
+          const int live = limit - key0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int row = 8 * (r / 4) + 4 * h + r % 4;
+            const bool seen = kMode == kTree ? (set >> row & 1u) != 0 : row < live;
+            s[r] = seen ? s[r] : 0.0f;
+          }
+        }
+      }
+      add_values<0>(run, v, s);
+      add_values<1>(run, v, s);
+      if (next < stop) load_values(v, a, next_base, head, stop - 1 - next, lane);
     }
-    add_values<0>(run, v, s);
-    add_values<1>(run, v, s);
-    if (next < stop) load_values(v, a, next_base, head, stop - 1 - next, lane);
+  };
+  walk(std::false_type{});
+  if constexpr (!kInt8) {
+    // A value that is not finite leaves NaN in every sum, of queries that do not attend its row too: then once more, such
+    // values apart.  (Looked for in every block, they would take the registers of the rows under way.)
+    float none = 0.0f * run.l;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) none = __builtin_fmaf(run.o[u][r], 0.0f, none);
+    if (__ballot(none != none) != 0) {
+      start(run);
+      if (first < stop) {
+        load_keys(k, a, block_at(first), head, stop - 1 - first, lane);
+        load_values(v, a, block_at(first), head, stop - 1 - first, lane);
+      }
+      walk(std::true_type{});
+    }
   }
   const float mine = run.l + other32(run.l);
   if (h == 0) {
@@ -641,6 +672,290 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   }
 }
 
+// ------------------------------------------------------------------ one token a request, over an int8 pool
+//
+// A single query leaves 31 of 32 columns of the matrix instruction empty, and one head's rows are its alone: the products
+// are fp32 multiply-adds on converted bytes, two instructions a byte, which at 64 lanes a clock is 32 bytes a clock of a
+// CU, three times what memory brings.  8 lanes have a row, 16 columns each, of the keys as of the values, so a row's weight
+// is where its values are: every group of 8 lanes has a softmax of its own, and nothing crosses lanes in the loop but a
+// score's three sums.
+constexpr int kOneWaves = 12;  // as many as have their registers on a CU
+constexpr int kOneParts = 16;  // columns of a lane
+
+// The sum over the 8 lanes of a group; the largest.
+template <typename F>
+__device__ __forceinline__ uint32_t of_group(uint32_t v, F f) {
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));   // lane ^ 1
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));   // lane ^ 2
+  return f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // 7 - lane
+}
+__device__ __forceinline__ float group_sum(float v) {
+  return __uint_as_float(of_group(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  return of_group(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+// Over the groups of a head, 8, 16 and, where the wave has one head, 32 lanes apart.
+template <int kHeads, typename F>
+__device__ __forceinline__ float of_head(float v, F f) {
+  v = f(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x128, 0xf, 0xf, false)));
+  v = f(v, __uint_as_float(other<16>(__float_as_uint(v))));
+  return kHeads == 1 ? f(v, other32(v)) : v;
+}
+
+// What a lane reads of a wave's heads: 64 / kHeads lanes have a head, whose group g has rows (8 / kHeads) i + g of a block,
+// columns 16 part on.
+template <int kHeads>
+struct OneLane {
+  static constexpr int kRows = 32 / kHeads;  // of a block
+  int part, group, sub, head;
+  __device__ __forceinline__ int row(int i) const { return 8 / kHeads * i + group; }
+};
+template <int kHeads>
+struct OneRows {
+  u32x4 k[4], v[4];
+  float ks, vs;  // of row sub % kRows
+};
+template <int kHeads>
+__device__ __forceinline__ void one_load(u32x4 (&x)[4], float& scale, const PoolArgs& a, const char* from,
+                                         const OneLane<kHeads>& l) {
+  const uint32_t at = (uint32_t)(l.group * a.slot_bytes + l.head * kD + 16 * l.part);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = *(const UOCR_GLOBAL u32x4*)(from + 8 / kHeads * i * a.slot_bytes + at);
+  scale = *(const UOCR_GLOBAL float*)(from + (uint32_t)(l.sub % OneLane<kHeads>::kRows * a.slot_bytes + a.heads * kD + 4 * l.head));
+}
+
+// A lane's 16 columns of a row, rotated where `ct` is not null (its tables' row): the pair of column d is d +- 64.
+__device__ __forceinline__ void load_columns(float (&x)[kOneParts], const float* row, const float* ct, const float* st, int part) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < kOneParts / 4; ++i) {
+    const f32x4 y = *(const UOCR_GLOBAL f32x4*)(row + 16 * part + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
+  }
+  if (ct == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < kOneParts / 4; ++i) {
+    const f32x4 y = *(const UOCR_GLOBAL f32x4*)(row + 16 * (part ^ 4) + 4 * i);
+    const f32x4 c = *(const UOCR_GLOBAL f32x4*)(ct + 16 * part + 4 * i), s = *(const UOCR_GLOBAL f32x4*)(st + 16 * part + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = x[4 * i + e] * c[e] + (part < 4 ? -y[e] : y[e]) * s[e];
+  }
+}
+// A group's row as its lanes' bytes, and its scale.
+__device__ __forceinline__ u32x4 quantize_columns(const float (&x)[kOneParts], float& scale) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < kOneParts; ++e) most = max(most, abs_bits(x[e]));
+  scale = row_scale(group_max(most));
+  u32x4 q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q[i] = to_int8(x[4 * i], scale) | to_int8(x[4 * i + 1], scale) << 8 | to_int8(x[4 * i + 2], scale) << 16 |
+           to_int8(x[4 * i + 3], scale) << 24;
+  return q;
+}
+
+// What is computed from x after this is computed after this: conversions ahead of their use would take the registers of the
+// rows under way.
+__device__ __forceinline__ uint32_t held_back(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+// A group's score: the lane's 16 products in four sums, then the lanes'.
+__device__ __forceinline__ float dot16(const float (&q)[kOneParts], u32x4 x) {
+  float s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s[i] = q[4 * i] * i8_to_f32<0>((int)x[i]);
+    s[i] = __builtin_fmaf(q[4 * i + 1], i8_to_f32<1>((int)x[i]), s[i]);
+    s[i] = __builtin_fmaf(q[4 * i + 2], i8_to_f32<2>((int)x[i]), s[i]);
+    s[i] = __builtin_fmaf(q[4 * i + 3], i8_to_f32<3>((int)x[i]), s[i]);
+  }
+  return group_sum((s[0] + s[1]) + (s[2] + s[3]));
+}
+__device__ __forceinline__ void add16(float (&o)[kOneParts], float w, u32x4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int y = (int)held_back(x[i]);
+    o[4 * i] = __builtin_fmaf(w, i8_to_f32<0>(y), o[4 * i]);
+    o[4 * i + 1] = __builtin_fmaf(w, i8_to_f32<1>(y), o[4 * i + 1]);
+    o[4 * i + 2] = __builtin_fmaf(w, i8_to_f32<2>(y), o[4 * i + 2]);
+    o[4 * i + 3] = __builtin_fmaf(w, i8_to_f32<3>(y), o[4 * i + 3]);
+  }
+}
+// The weight of a sum at maximum mj beside one at m; of sums without rows (0) and NaN.
+__device__ __forceinline__ float weight_at(float mj, float l, float m) {
+  if (l == 0.0f || l != l) return l;
+  return mj == -kInf ? (m == -kInf ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(mj - m);
+}
+
+template <int kHeads>
+__global__ void __launch_bounds__(kOneWaves * kWave) k_pool_one(Attend p) {
+  const PoolArgs& a = p.a;
+  __shared__ __align__(16) float sums[kOneWaves][kHeads][kD];
+  __shared__ float peak[kOneWaves][kHeads], total[kOneWaves][kHeads];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  // Every request has a piece for each split and its heads, whose place follows from the workgroup's number: what does not
+  // depend on one another is asked for together.
+  const int turn = (int)(blockIdx.x / 8), round = p.cuts.by_heads(turn), cell = 8 * round + (int)(blockIdx.x % 8);
+  const int head0 = kHeads * (turn - round * ((a.heads + kHeads - 1) / kHeads));
+  const int n = cell / p.cuts.splits, split = cell - n * p.cuts.splits;
+  if (n >= a.requests) return;
+  OneLane<kHeads> me;
+  me.sub = lane_id() % (kWave / kHeads);
+  me.part = me.sub % 8;
+  me.group = me.sub / 8;
+  const int side = lane_id() / (kWave / kHeads);
+  me.head = min(head0 + side, a.heads - 1);
+  constexpr int kRows = OneLane<kHeads>::kRows, kStep = (kOneWaves - 1) * kRows;  // the last wave has the new row
+  const int begin = split * p.cuts.split_rows, first = begin + kRows * wave;
+  const uint32_t* lookup = a.lookup + (int64_t)n * a.lookup_cols;
+  const auto block_at = [&](int row) {  // (rows past the table's are asked for nowhere)
+    const int at = min(row, a.max_rows - kRows);
+    return a.pool + (int64_t)min(ldc(lookup + at / a.P), (uint32_t)(a.pages - 1)) * a.page_bytes + a.layer_bytes +
+           (int64_t)(at % a.P) * a.slot_bytes;
+  };
+  const char* first_at = block_at(first);
+  const int all_rows = (int)min((int64_t)min(ldc(a.cache_lengths + n), (uint32_t)(a.max_rows - 1)) + 1, (int64_t)a.attend_max);
+  const uint32_t write = ldc(a.write_index + n);
+  const int64_t src = (int64_t)n * a.in_stride + (int64_t)me.head * kD;
+  const float *ct = nullptr, *st = nullptr;
+  if (a.rope.positions != nullptr) {
+    const int64_t pos = (int64_t)min(max(ldc(a.rope.positions + n), 0), a.rope.table_rows - 1) * kD;
+    ct = a.rope.cos_t + pos;
+    st = a.rope.sin_t + pos;
+  }
+  const int stop = min(begin + p.cuts.split_rows, all_rows);
+  if (begin >= stop) return;
+  const float c = a.scale * 1.44269504f;
+  const int new_row = write < (uint32_t)all_rows ? (int)write : -1;
+  float q[kOneParts], m = -kInf, l = 0.0f, o[kOneParts] = {};
+  if (wave < kOneWaves - 1) {
+    // A block's rows lie in one page, so that all of them can be read, whether attended or not.
+    OneRows<kHeads> r;
+    if (first < stop) {
+      one_load(r.k, r.ks, a, first_at, me);
+      one_load(r.v, r.vs, a, first_at + a.kv_bytes, me);
+    }
+    load_columns(q, a.q + src, ct, st, me.part);
+    // the next rows are asked for as these are used up
+#pragma unroll 1
+    for (int key0 = first; key0 < stop; key0 += kStep) {
+      const int next = key0 + kStep;
+      const float ks = r.ks * c;
+      float s[4], vs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int from = side * (kWave / kHeads) + me.row(i);
+        s[i] = dot16(q, r.k[i]) * __shfl(ks, from, kWave);
+        vs[i] = __shfl(r.vs, from, kWave);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const char* next_at = next < stop ? block_at(next) : nullptr;
+      __builtin_amdgcn_sched_barrier(0);
+      if (next < stop) one_load(r.k, r.ks, a, next_at, me);
+      __builtin_amdgcn_sched_barrier(0);
+      if (key0 + kRows > stop || (uint32_t)(new_row - key0) < (uint32_t)kRows)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = key0 + me.row(i);
+          if (row >= stop || row == new_row) {  // what is there may be anything
+            s[i] = -kInf;
+            vs[i] = 0.0f;
+          }
+        }
+      const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      const bool up = mx > m + kSlack;
+      if (__ballot(up) != 0) {
+        const float alpha = up ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+        m = up ? mx : m;
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < kOneParts; ++e) o[e] *= alpha;
+      }
+      const float off = m == -kInf ? 0.0f : m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[i] - off);
+        l += e;
+        add16(o, e * vs[i], r.v[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (next < stop) one_load(r.v, r.vs, a, next_at + a.kv_bytes, me);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else if (write < (uint32_t)a.max_rows && (new_row < 0 ? split == 0 : new_row >= begin && new_row < stop)) {
+    // The new row, while the others wait for memory: stored, and attended as it was rounded.  Every group of a head has all
+    // of it; the first's weight counts.
+    float x[kOneParts], ks, vs;
+    load_columns(x, a.k_new + src, ct, st, me.part);
+    const u32x4 k = quantize_columns(x, ks);
+    load_columns(x, a.v_new + src, nullptr, nullptr, me.part);
+    const u32x4 v = quantize_columns(x, vs);
+    if (head0 + side < a.heads) {
+      char* slot = slot_of(a, n, (int)write);
+      if (me.group == 0) *(UOCR_GLOBAL u32x4*)(slot + me.head * kD + 16 * me.part) = k;
+      if (me.group == 1) *(UOCR_GLOBAL u32x4*)(slot + a.kv_bytes + me.head * kD + 16 * me.part) = v;
+      if (me.sub == 0) {
+        stg((float*)(slot + a.heads * kD) + me.head, ks);
+        stg((float*)(slot + a.kv_bytes + a.heads * kD) + me.head, vs);
+      }
+    }
+    if (new_row >= 0 && me.group == 0) {
+      load_columns(q, a.q + src, ct, st, me.part);
+      const float s = dot16(q, k) * (ks * c);
+      m = s == s ? s : -kInf;
+      l = s == s ? 1.0f : s;
+      add16(o, l * vs, v);
+    }
+  }
+  // the groups' sums at one maximum, then the waves'
+  const auto most = [](float x, float y) { return fmaxf(x, y); };
+  const auto plus = [](float x, float y) { return x + y; };
+  const float top = of_head<kHeads>(m, most), f = weight_at(m, l, top);
+  l = of_head<kHeads>(l * f, plus);
+#pragma unroll
+  for (int e = 0; e < kOneParts; ++e) o[e] = of_head<kHeads>(o[e] * f, plus);
+  if (me.group == 0) {
+#pragma unroll
+    for (int e = 0; e < kOneParts; e += 4)
+      *(f32x4*)&sums[wave][side][16 * me.part + e] = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+  }
+  if (me.sub == 0) {
+    peak[wave][side] = top;
+    total[wave][side] = l;
+  }
+  __syncthreads();
+  const int at = (int)threadIdx.x / kD, d = (int)threadIdx.x % kD;
+  if (at >= kHeads || head0 + at >= a.heads) return;
+  float all = -kInf;
+#pragma unroll
+  for (int j = 0; j < kOneWaves; ++j) all = fmaxf(all, peak[j][at]);
+  float sum = 0.0f, y = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kOneWaves; ++j) {
+    const float fj = weight_at(peak[j][at], total[j][at], all);
+    sum = __builtin_fmaf(total[j][at], fj, sum);
+    y = __builtin_fmaf(sums[j][at][d], fj, y);
+  }
+  const int64_t th = (int64_t)n * a.heads + head0 + at;
+  if (all_rows <= p.cuts.split_rows) {
+    stg(a.out + th * kD + d, y / sum);
+  } else {
+    const int64_t stride = (int64_t)a.tokens * a.heads;
+    stg(p.part + (split * stride + th) * kD + d, y);
+    if (d == 0) {
+      stg(p.tops + 2 * (split * stride + th), all);
+      stg(p.tops + 2 * (split * stride + th) + 1, sum);
+    }
+  }
+}
+
 // Joins the splits of a token's rows: half a wave a (token, head), four columns a lane.
 template <Mode kMode>
 __global__ void __launch_bounds__(256) k_pool_join(Attend p) {
@@ -683,32 +998,43 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p) {
 // workgroups a CU.
 namespace {
 constexpr int kCus = 256;
-PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max) {
+PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, bool one) {
   PoolCuts c{};
-  const int64_t tiles = requests > 64 ? tokens / kQueries + requests
-                        : tokens < requests ? tokens : (tokens - requests) / kQueries + requests;
+  const int64_t tiles = one || requests <= 64 ? (tokens < requests ? tokens : (tokens - requests) / kQueries + requests)
+                                              : tokens / kQueries + requests;
   c.slots = (int)tiles;
-  const int64_t splits = std::max<int64_t>(1, 2 * kCus / std::max<int64_t>(1, tiles * heads));
-  const int round = kWaves * kBlock;
+  c.few = one && requests * heads <= kCus / 2;
+  c.groups = one && !c.few ? (heads + 1) / 2 : heads;
+  const int64_t fill = !one ? 2 * kCus : c.few ? kCus : UOCR_ONE_FILL * kCus;
+  const int64_t splits = std::max<int64_t>(1, fill / std::max<int64_t>(1, tiles * c.groups));
+  const int round = !one ? kWaves * kBlock : c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16;
   c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
   c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
   c.by_split = divide_by(c.split_rows);
-  c.by_heads = divide_by(heads);
+  c.by_heads = divide_by(c.groups);
   return c;
 }
 
 template <bool kInt8, Mode kMode>
 hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
-  const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max);
-  const int64_t pairs = p.tokens * p.heads, items = (int64_t)c.slots * p.heads * c.splits;
+  const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max, kMode == kOne);
+  const int64_t pairs = p.tokens * p.heads, items = ((int64_t)c.slots * c.splits + 7) / 8 * 8 * c.groups;
   const int64_t joins = p.tokens * ((p.heads + 1) / 2);
   // (where a wave counts the pieces, offsets that do not ascend may give each request all of them)
   if (items > (p.requests <= 64 ? INT32_MAX / p.requests : INT32_MAX) - 8) return hipErrorInvalidValue;
   const Attend at{a, c, (float*)p.workspace, (float*)p.workspace + (int64_t)c.splits * pairs * kD};
-  auto store = k_pool_store<kInt8, kMode>;
-  UOCR_LAUNCH("pool_store", store, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, s, a);
-  auto attend = k_pool_attend<kInt8, kMode>;
-  UOCR_LAUNCH("pool_attend", attend, dim3((unsigned)((items + 7) / 8 * 8)), dim3(kThreads), 0, s, at);
+  const dim3 grid((unsigned)items);
+  if constexpr (kMode == kOne) {
+    if (c.few)
+      UOCR_LAUNCH("pool_one", k_pool_one<1>, grid, dim3(kOneWaves * kWave), 0, s, at);
+    else
+      UOCR_LAUNCH("pool_one", k_pool_one<2>, grid, dim3(kOneWaves * kWave), 0, s, at);
+  } else {
+    auto store = k_pool_store<kInt8>;
+    UOCR_LAUNCH("pool_store", store, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, s, a);
+    auto attend = k_pool_attend<kInt8, kMode>;
+    UOCR_LAUNCH("pool_attend", attend, grid, dim3(kThreads), 0, s, at);
+  }
   if (c.splits > 1) {
     auto join = k_pool_join<kMode>;
     UOCR_LAUNCH("pool_join", join, dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, s, at);
@@ -717,8 +1043,8 @@ hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
 }
 }  // namespace
 
-size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max) {
-  const PoolCuts c = cuts_of(tokens, requests, heads, attend_max);
+size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, bool one) {
+  const PoolCuts c = cuts_of(tokens, requests, heads, attend_max, one);
   return c.splits > 1 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) : 0;
 }
 

@@ -68,7 +68,7 @@ SIGNATURES: dict[str, list] = {
     "uocr_paged_chunk_attention_qkv": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
                                        _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _sz, _vp, _cp,
                                        _sz],
-    "uocr_paged_pool_workspace_bytes": [_i64, _i64, _i64, _i64],
+    "uocr_paged_pool_workspace_bytes": [_i64, _i64, _i64, _i64, _i64],
     "uocr_paged_decode_attention_int8": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
                                          _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _sz, _vp, _cp,
                                          _sz],

@@ -481,7 +481,7 @@ def _pool_call(op: str, name: str, inputs: tuple, stride: int, heads: int, head_
     need = 0
     # nothing is allocated for more rows than the table addresses: the entry refuses them
     if workspace is not None or attend_max <= lookup.shape[1] * page_size:
-        need = _lib.load().uocr_paged_pool_workspace_bytes(tokens, lookup.shape[0], heads, attend_max)
+        need = _lib.load().uocr_paged_pool_workspace_bytes(tokens, lookup.shape[0], heads, attend_max, not requests)
     ws = _workspace(op, workspace, need, like)
     if len(inputs) == 1:
         q = like.data_ptr()
