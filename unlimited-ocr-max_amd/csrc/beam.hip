@@ -19,43 +19,56 @@ namespace {
 
 typedef float f32x4_at_float __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kThreads = 256;
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kList = 1024;  // candidates that are ranked against one another in LDS
 
-// Of the candidates that the threads of a workgroup hold, the first `most` by value (descending) and id (ascending).
-// each(f) calls f(value, id) for a thread's candidates, put(rank, value, id) takes a chosen one; returns their number.
+// A float's bits in the order of the floats.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return (int)b < 0 ? ~b : b | 0x80000000u;
+}
+// A border that at least `most` lanes of a wave reach with `mine`, and few more: the most-th largest, its last 12 bits cut.
+__device__ __forceinline__ uint32_t border_of(uint32_t mine, int most) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 12; --bit) {
+    const uint32_t up = t | 1u << bit;
+    if (__popcll(__ballot(mine >= up)) >= most) t = up;
+  }
+  return t;
+}
+
+// Of the candidates that the threads of a workgroup hold, the first `most` (at most 32) by value (descending) and id
+// (ascending).  each(f) calls f(value, id) for a thread's candidates, put(rank, value, id) takes a chosen one; returns
+// their number.
 //
-// At least `most` candidates are no smaller than the most-th largest of the threads' largest ones, and few are as large:
-// those are listed, and ranked by counting.  Where equal values fill the list, each next one is looked for among all.
-template <typename V, typename Id>
+// At least `most` candidates are no smaller than the most-th largest of a wave's lanes' largest ones (as floats, whose
+// rounding keeps the order), and few are as large: those of the highest such border are listed, and ranked by counting.
+// Where equal values fill the list, each next one is looked for among all.
+template <typename V, typename Id, int kThreads>
 struct Best {
-  V largest[kThreads];
   V value[kList];
   Id id[kList];
-  V border;
+  uint32_t border[kThreads / kWave];
   int listed;
 };
-template <typename V, typename Id, typename Each, typename Put>
-__device__ __forceinline__ int choose(Best<V, Id>& b, int most, Each each, Put put) {
+template <typename V, typename Id, int kThreads, typename Each, typename Put>
+__device__ __forceinline__ int choose(Best<V, Id, kThreads>& b, int most, Each each, Put put) {
   const int tid = (int)threadIdx.x;
+  static_assert(kThreads <= kList, "a thread has a place in the list");
   const V none = -(V)__builtin_huge_val();
   V mine = none;
   each([&](V v, Id) { mine = v > mine ? v : mine; });
-  b.largest[tid] = mine;
+  const uint32_t own_border = border_of(ordered((float)mine), most);
+  if (lane_id() == 0) b.border[tid / kWave] = own_border;
   if (tid == 0) b.listed = 0;
   __syncthreads();
-  int before = 0;
-  for (int i = 0; i < kThreads; ++i) {
-    const V o = b.largest[i];
-    before += o > mine || (o == mine && i < tid);
-  }
-  if (before == most - 1) b.border = mine;
-  __syncthreads();
-  const V border = b.border;
-  if (mine >= border)
+  uint32_t border = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / kWave; ++i) border = max(border, b.border[i]);
+  if (ordered((float)mine) >= border)
     each([&](V v, Id id) {
-      if (v >= border) {
+      if (ordered((float)v) >= border) {
         const int at = atomicAdd(&b.listed, 1);
         if (at < kList) {
           b.value[at] = v;
@@ -70,6 +83,7 @@ __device__ __forceinline__ int choose(Best<V, Id>& b, int most, Each each, Put p
       const V v = b.value[i];
       const Id id = b.id[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += b.value[j] > v || (b.value[j] == v && b.id[j] < id);
       if (rank < most) put(rank, v, id);
     }
@@ -107,18 +121,28 @@ __device__ __forceinline__ int choose(Best<V, Id>& b, int most, Each each, Put p
   return most;
 }
 
+constexpr int kRowThreads = 256, kJoinThreads = 512;
+
+struct BeamWork {  // of each row's pieces: the largest logit and the sum, the best tokens
+  int pieces;
+  Divide by_beam;  // candidates of a beam
+  float* tops;
+  float* values;
+  int* ids;
+};
+
 // A workgroup has a piece of a row: its largest logit, its sum of exponentials, and its best K tokens.  Rows begin at any
 // float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.
 template <int kPer>
-__global__ void __launch_bounds__(kThreads) k_beam_rows(BeamSelect p, BeamWork w) {
-  __shared__ Best<float, int> best;
-  __shared__ float parts[kThreads / kWave];
+__global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWork w) {
+  __shared__ Best<float, int, kRowThreads> best;
+  __shared__ float parts[kRowThreads / kWave];
   const int row = (int)blockIdx.y, piece = (int)blockIdx.x, tid = (int)threadIdx.x;
   if (p.ended != nullptr && ldg(p.ended + row) != 0) return;
-  const int begin = piece * kThreads * kPer;
+  const int begin = piece * kRowThreads * kPer;
   const float* x = p.logits + (int64_t)row * p.vocab;
   float v[kPer];
-  const auto token = [&](int i) { return begin + (i / 4 * kThreads + tid) * 4 + i % 4; };
+  const auto token = [&](int i) { return begin + (i / 4 * kRowThreads + tid) * 4 + i % 4; };
 #pragma unroll
   for (int i = 0; i < kPer; i += 4) {
     const int at = token(i);
@@ -167,64 +191,78 @@ __global__ void __launch_bounds__(kThreads) k_beam_rows(BeamSelect p, BeamWork w
                              values[rank] = value;
                              ids[rank] = id;
                            });
-  for (int i = found + tid; i < p.beams; i += kThreads) ids[i] = -1;
+  for (int i = found + tid; i < p.beams; i += kRowThreads) ids[i] = -1;
 }
 
+__device__ __attribute__((noinline)) double full_exp(double x) { return exp(x); }
+
 // A workgroup has a request: its beams' sums, their candidates, and the states of the chosen ones.
-__global__ void __launch_bounds__(kThreads) k_beam_join(BeamSelect p, BeamWork w) {
-  __shared__ Best<double, int64_t> best;
+__global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWork w) {
+  __shared__ Best<double, int64_t, kJoinThreads> best;
   __shared__ double sums[kBeamsMost], scores[kBeamsMost], by[kBeamsMost];
   __shared__ int lengths[kBeamsMost], state[kBeamsMost];  // 0: live, 1: ended, 2: no finite sum
   __shared__ int tokens[kBeamsMost], parents[kBeamsMost];
   const int K = p.beams, tid = (int)threadIdx.x, wave = tid / kWave, lane = lane_id();
   const int64_t row0 = (int64_t)blockIdx.x * K;
-  for (int b = wave; b < K; b += kThreads / kWave) {
+  // The first candidates are asked for before the sums, which they wait for: of a request they lie one after another.
+  constexpr int kHeld = 4;
+  const int per = w.pieces * K, candidates = K * per;
+  const int64_t first = row0 * per;
+  int held_id[kHeld];
+  float held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    const int i = tid + u * kJoinThreads;
+    held_id[u] = i < candidates ? ldg(w.ids + first + i) : -1;
+    held[u] = i < candidates ? ldg(w.values + first + i) : 0.0f;
+  }
+  for (int b = wave; b < K; b += kJoinThreads / kWave) {
     const int64_t row = row0 + b;
+    const float* tops = w.tops + 2 * row * w.pieces;  // (an ended beam's are nobody's)
     const bool ended = p.ended != nullptr && ldg(p.ended + row) != 0;
     const double score = ldg(p.scores + row);
-    double lse = 0.0;
-    if (!ended) {
-      const float* tops = w.tops + 2 * row * w.pieces;
-      float m = -kInf;
-      for (int i = lane; i < w.pieces; i += kWave) m = fmaxf(m, ldg(tops + 2 * i));
-      m = tree_max(m);
-      double l = 0.0;
-      for (int i = lane; i < w.pieces; i += kWave) {
-        const float mi = ldg(tops + 2 * i);
-        const double li = ldg(tops + 2 * i + 1);
-        l += li == 0.0 ? 0.0 : li * exp((double)mi - (double)m);
-      }
-      for (int off = 32; off >= 1; off /= 2) l += __shfl_xor(l, off, kWave);
-      lse = (double)m + log(l);
-    }
+    const int length = p.lengths != nullptr ? ldg(p.lengths + row) + (ended ? 0 : 1) : 0;
+    const bool some = lane < w.pieces;
+    const float m0 = some ? ldg(tops + 2 * lane) : -kInf, l0 = some ? ldg(tops + 2 * lane + 1) : 0.0f;
+    float m = m0;
+    for (int i = lane + kWave; i < w.pieces; i += kWave) m = fmaxf(m, ldg(tops + 2 * i));
+    m = tree_max(m);
+    const auto at_most = [&](float mi, float li) { return li == 0.0f ? 0.0 : (double)li * full_exp((double)mi - (double)m); };
+    double l = at_most(m0, l0);
+    for (int i = lane + kWave; i < w.pieces; i += kWave) l += at_most(ldg(tops + 2 * i), ldg(tops + 2 * i + 1));
+    for (int off = 32; off >= 1; off /= 2) l += __shfl_xor(l, off, kWave);
+    // (pow's code alone takes as long to fetch as all else here: length^-alpha by the logarithm, in the lane next to the sum's)
+    const double logs = log(lane == 1 ? (double)length : l);
+    const double lse = (double)m + __shfl(logs, 0, kWave);
+    const double factor = p.lengths != nullptr && p.alpha != 0.0 ? full_exp(-p.alpha * __shfl(logs, 1, kWave)) : 1.0;
     if (lane == 0) {
-      const int length = p.lengths != nullptr ? ldg(p.lengths + row) + (ended ? 0 : 1) : 0;
-      const bool finite = score - score == 0.0 && lse - lse == 0.0;
       sums[b] = lse;
       scores[b] = score;
-      by[b] = p.lengths != nullptr ? pow((double)length, p.alpha) : 1.0;
+      by[b] = factor;
       lengths[b] = length;
-      state[b] = ended ? 1 : finite ? 0 : 2;
+      state[b] = ended ? 1 : score - score == 0.0 && lse - lse == 0.0 ? 0 : 2;
     }
   }
   __syncthreads();
-  const int per = w.pieces * K;
   const auto key_of = [&](int b, float logit) { return state[b] == 1 ? scores[b] : scores[b] + ((double)logit - sums[b]); };
   const auto offer = [&](auto f, int b, double key, int token) {
-    const double rank = key / by[b];
+    const double rank = key * by[b];
     if (rank - rank == 0.0) f(rank, (int64_t)b * p.vocab + token);
   };
-  const auto each = [&](auto f) {
-    for (int i = tid; i < K * per; i += kThreads) {
-      const int b = i / per, j = i - b * per;
-      if (state[b] == 0) {
-        const int64_t at = (row0 + b) * per + j;
-        const int id = ldg(w.ids + at);
-        if (id >= 0) offer(f, b, key_of(b, ldg(w.values + at)), id);
-      } else if (state[b] == 1 && j == 0) {
-        offer(f, b, scores[b], p.eos);
-      }
+  const auto one = [&](auto f, int i, float logit, int id) {
+    const int b = w.by_beam(i);
+    if (state[b] == 0) {
+      if (id >= 0) offer(f, b, key_of(b, logit), id);
+    } else if (state[b] == 1 && i == b * per) {
+      offer(f, b, scores[b], p.eos);
     }
+  };
+  const auto each = [&](auto f) {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (tid + u * kJoinThreads < candidates) one(f, tid + u * kJoinThreads, held[u], held_id[u]);
+    for (int i = tid + kHeld * kJoinThreads; i < candidates; i += kJoinThreads)
+      one(f, i, ldg(w.values + first + i), ldg(w.ids + first + i));
   };
   const int found = choose(best, K, each, [&](int rank, double, int64_t id) {
     const int b = (int)(id / p.vocab);
@@ -261,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) k_beam_join(BeamSelect p, BeamWork w
     if (p.lengths != nullptr) stg(p.lengths_out + row, lengths[b]);
   }
   if (p.history == nullptr) return;
-  for (int k = wave; k < K; k += kThreads / kWave) {
+  for (int k = wave; k < K; k += kJoinThreads / kWave) {
     const int64_t from = (row0 + parents[k]) * p.width, to = (row0 + k) * p.width;
     const int shift = p.ended != nullptr && ldg(p.ended + row0 + parents[k]) != 0 ? 0 : 1;
     for (int64_t i = lane; i < p.width; i += kWave)
@@ -270,9 +308,9 @@ __global__ void __launch_bounds__(kThreads) k_beam_join(BeamSelect p, BeamWork w
 }
 
 // Tokens of a thread: 8 where the rows are few, so that their pieces fill the device, else 32.
-int per_thread(int64_t rows, int vocab) { return rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) < 512 ? 8 : 32; }
+int per_thread(int64_t rows, int vocab) { return rows * ((vocab + 32 * kRowThreads - 1) / (32 * kRowThreads)) < 512 ? 8 : 32; }
 int pieces_of(int64_t rows, int vocab) {
-  const int size = per_thread(rows, vocab) * kThreads;
+  const int size = per_thread(rows, vocab) * kRowThreads;
   return (int)(((int64_t)vocab + size - 1) / size);
 }
 
@@ -286,14 +324,15 @@ hipError_t launch_beam_select(const BeamSelect& p, int64_t rows, void* workspace
   if (rows == 0) return hipSuccess;
   BeamWork w{};
   w.pieces = pieces_of(rows, p.vocab);
+  w.by_beam = divide_by(w.pieces * p.beams);
   const int64_t n = rows * w.pieces;
   w.tops = (float*)workspace;
   w.values = w.tops + 2 * n;
   w.ids = (int*)(w.values + n * p.beams);
-  const dim3 grid((unsigned)w.pieces, (unsigned)rows), block(kThreads);
+  const dim3 grid((unsigned)w.pieces, (unsigned)rows), block(kRowThreads);
   const auto kernel = per_thread(rows, p.vocab) == 8 ? k_beam_rows<8> : k_beam_rows<32>;
   UOCR_LAUNCH("beam_rows", kernel, grid, block, 0, s, p, w);
-  UOCR_LAUNCH("beam_join", k_beam_join, dim3((unsigned)(rows / p.beams)), block, 0, s, p, w);
+  UOCR_LAUNCH("beam_join", k_beam_join, dim3((unsigned)(rows / p.beams)), dim3(kJoinThreads), 0, s, p, w);
   return hipGetLastError();
 }
 

@@ -378,12 +378,6 @@ struct BeamSelect {
   int32_t* lengths_out;
   int32_t* history_out;
 };
-struct BeamWork {  // of each row's pieces: the largest logit and the sum, the best tokens
-  int pieces;
-  float* tops;
-  float* values;
-  int* ids;
-};
 size_t beam_workspace_bytes(int64_t rows, int beams, int vocab);
 hipError_t launch_beam_select(const BeamSelect& p, int64_t rows, void* workspace, hipStream_t s);
 
