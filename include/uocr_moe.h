@@ -283,10 +283,10 @@ int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t 
  *   New rows are stored first; what is attended is what the pool then holds.
  *   Lookup, lengths, offsets and attend_max as for the fp32 entries; tokens * heads at most
  *   2^25.  workspace: uocr_paged_pool_workspace_bytes(tokens, requests, heads, attend_max,
- *   decode: whether the call is uocr_paged_decode_attention_int8) bytes, 16-byte aligned, or NULL
- *   (the library's own).
+ *   form) bytes, 16-byte aligned, or NULL (the library's own); form 0: the decode entry, 1: chunks,
+ *   2: with `visible`.
  * ------------------------------------------------------------------------- */
-size_t uocr_paged_pool_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max, int64_t decode);
+size_t uocr_paged_pool_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max, int64_t form);
 
 /* paged_decode_attention over an int8 pool: row b's new row at write_index[b], rows
  * [0, attend_lengths[b] + 1) attended. */

@@ -237,7 +237,7 @@ def test_strided_rows_other_outputs_and_workspaces() -> None:
     wide = torch.zeros(s.tokens, 3, 5, D, device=DEV)
     wide[:, :, 1:4] = s.qkv.to(DEV)
     again = s.pool.to(DEV)
-    need = u._lib.load().uocr_paged_pool_workspace_bytes(s.tokens, 2, 3, s.attend_max, 0)
+    need = u._lib.load().uocr_paged_pool_workspace_bytes(s.tokens, 2, 3, s.attend_max, 1)
     ws = torch.full((need + 64,), 0xFF, dtype=torch.uint8, device=DEV)
     out = u.paged_chunk_attention(*(wide[:, j, 1:4] for j in range(3)), kv=_chunk(s, again), layer_idx=1, scale=SCALE,
                                   workspace=ws)

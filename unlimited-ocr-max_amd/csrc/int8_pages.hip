@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads) k_convert_pages(ConvertPages p) {
           uint32_t most = max(max(abs_bits(x[i].x), abs_bits(x[i].y)), max(abs_bits(x[i].z), abs_bits(x[i].w)));
           for (int off = 16; off >= 1; off /= 2) most = max(most, (uint32_t)__shfl_xor((int)most, off, kWave));
           const float s = row_scale(most);
-          const uint32_t q = to_int8(x[i].x, s) | to_int8(x[i].y, s) << 8 | to_int8(x[i].z, s) << 16 | to_int8(x[i].w, s) << 24;
+          const uint32_t q = to_int8x4(x[i].x, x[i].y, x[i].z, x[i].w, s);
           if (h0 + 2 * i < p.heads) {
             stg((uint32_t*)(slot + (h0 + 2 * i) * kD) + c, q);
             if (c == 0) stg(scales + h0 + 2 * i, s);

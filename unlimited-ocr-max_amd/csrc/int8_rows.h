@@ -22,6 +22,22 @@ __device__ __forceinline__ uint32_t to_int8(float x, float scale) {
   const float q = fminf(fmaxf(__builtin_rintf(x / scale), -127.0f), 127.0f);
   return scale != scale ? 0u : (uint32_t)(int)q & 0xffu;
 }
+// Four of them.  Divisions take a dozen instructions each: the products with the reciprocal, off by 127 2^-22 at most, round
+// to the same numbers but where they are that near to a tie (or none: a reciprocal that overflows), and then the wave divides.
+__device__ __forceinline__ uint32_t to_int8x4(float x, float y, float z, float w, float scale) {
+  const float r = __builtin_amdgcn_rcpf(scale);
+  const float v[4] = {x * r, y * r, z * r, w * r};
+  uint32_t q = 0;
+  bool far = true;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float n = __builtin_rintf(v[e]);
+    far = far && __builtin_fabsf(v[e] - n) < 0.4999f;
+    q |= ((uint32_t)(int)n & 0xffu) << (8 * e);
+  }
+  if (__ballot(!far) == 0) return q;
+  return to_int8(x, scale) | to_int8(y, scale) << 8 | to_int8(z, scale) << 16 | to_int8(w, scale) << 24;
+}
 
 }  // namespace
 

@@ -49,6 +49,7 @@ constexpr float kSlack = 8.0f;
 #endif
 
 enum Mode { kOne, kCausal, kTree };
+constexpr PoolForm form_of(Mode m) { return m == kOne ? kPoolDecode : m == kCausal ? kPoolChunk : kPoolTree; }
 
 struct PoolArgs {
   char* pool;
@@ -71,6 +72,7 @@ struct PoolArgs {
   float* out;
   float scale;
   Rope rope;
+  bool stores;  // whether the attending kernel stores the new rows, else k_pool_store has
 };
 
 // Where row r of request n is, and head h's values in it.
@@ -79,43 +81,64 @@ __device__ __forceinline__ char* slot_of(const PoolArgs& a, int n, int r) {
   return a.pool + (int64_t)page * a.page_bytes + a.layer_bytes + (int64_t)(r % a.P) * a.slot_bytes;
 }
 
-// One wave per (token, head): lane d has the pair (d, d + 64) of k and of v.  Queries that come before RoPE are rotated
-// where they are read.
+// Stores token t's k and v of the kHeads heads from h0 on as row `row` of request n: half of the wave has the key, half the
+// value, a lane 4 columns.
+template <bool kInt8, int kHeads>
+__device__ __forceinline__ void store_row(const PoolArgs& a, int n, int row, int t, int h0) {
+#pragma clang fp contract(off)
+  const int lane = lane_id(), c = lane & 31;
+  const bool key = lane < 32, turn = a.rope.positions != nullptr;
+  const float* x = (key ? a.k_new : a.v_new) + (int64_t)t * a.in_stride + 4 * c;
+  f32x4 y[kHeads], pair[kHeads];  // the pair of column d is d +- 64
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int64_t at = (int64_t)min(h0 + i, a.heads - 1) * kD;
+    y[i] = *(const UOCR_GLOBAL f32x4*)(x + at);
+    if (turn) pair[i] = *(const UOCR_GLOBAL f32x4*)(x + at + (c < 16 ? 64 : -64));
+  }
+  char* slot = slot_of(a, n, row) + (key ? 0 : a.kv_bytes);
+  if (turn) {
+    const int64_t at = (int64_t)min(max(ldg(a.rope.positions + t), 0), a.rope.table_rows - 1) * kD + 4 * c;
+    const f32x4 cs = *(const UOCR_GLOBAL f32x4*)(a.rope.cos_t + at), sn = *(const UOCR_GLOBAL f32x4*)(a.rope.sin_t + at);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float turned = y[i][e] * cs[e] + (c < 16 ? -pair[i][e] : pair[i][e]) * sn[e];
+        y[i][e] = key ? turned : y[i][e];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = h0 + i;
+    if (h >= a.heads) break;
+    if constexpr (kInt8) {
+      uint32_t most = max(max(abs_bits(y[i].x), abs_bits(y[i].y)), max(abs_bits(y[i].z), abs_bits(y[i].w)));
+#pragma unroll
+      for (int off = 1; off <= 8; off *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, off, kWave));
+      const float scale = row_scale(max(most, other<16>(most)));
+      const uint32_t q = to_int8x4(y[i].x, y[i].y, y[i].z, y[i].w, scale);
+      stg((uint32_t*)(slot + h * kD) + c, q);
+      if (c == 0) stg((float*)(slot + a.heads * kD) + h, scale);
+    } else {
+      *(UOCR_GLOBAL f32x4*)((float*)slot + h * kD + 4 * c) = y[i];
+    }
+  }
+}
+
+// One wave per (token, 4 heads), which waits for the request's words once.  Queries that come before RoPE are rotated where
+// they are read.
+constexpr int kStoreHeads = 4;
 template <bool kInt8>
 __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
-  const int64_t th = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-  if (th >= (int64_t)a.tokens * a.heads) return;
-  const int t = (int)(th / a.heads), h = (int)(th % a.heads), d = lane_id();
+  const int groups = (a.heads + kStoreHeads - 1) / kStoreHeads;
+  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  if (item >= (int64_t)a.tokens * groups) return;
+  const int t = (int)(item / groups), h0 = (int)(item % groups) * kStoreHeads;
   Chunk c;
   if (!chunk_of(a, t, c)) return;
   const int64_t row = (int64_t)c.cached + (t - c.first);
-  if (row >= a.max_rows) return;  // past what the lookup row addresses: not stored
-  const int64_t src = (int64_t)t * a.in_stride + (int64_t)h * kD;
-  const float *k = a.k_new + src, *v = a.v_new + src;
-  float x[4] = {ldg(k + d), ldg(k + d + 64), ldg(v + d), ldg(v + d + 64)};
-  if (a.rope.positions != nullptr) {
-    const int64_t at = (int64_t)min(max(ldg(a.rope.positions + t), 0), a.rope.table_rows - 1) * kD;
-    x[0] = rotated(k, a.rope.cos_t + at, a.rope.sin_t + at, d);
-    x[1] = rotated(k, a.rope.cos_t + at, a.rope.sin_t + at, d + 64);
-  }
-  char* slot = slot_of(a, c.n, (int)row);
-  if constexpr (kInt8) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      char* to = slot + j * a.kv_bytes;
-      const float scale = row_scale(tree_umax(max(abs_bits(x[2 * j]), abs_bits(x[2 * j + 1]))));
-      stg((uint8_t*)to + h * kD + d, (uint8_t)to_int8(x[2 * j], scale));
-      stg((uint8_t*)to + h * kD + d + 64, (uint8_t)to_int8(x[2 * j + 1], scale));
-      if (d == 0) stg((float*)(to + a.heads * kD) + h, scale);
-    }
-  } else {
-    float* to = (float*)slot + h * kD + d;
-    stg(to, x[0]);
-    stg(to + 64, x[1]);
-    to = (float*)(slot + a.kv_bytes) + h * kD + d;
-    stg(to, x[2]);
-    stg(to + 64, x[3]);
-  }
+  if (row < a.max_rows) store_row<kInt8, kStoreHeads>(a, c.n, (int)row, t, h0);  // else past what the lookup row addresses
 }
 
 // ------------------------------------------------------------------ which piece of the work a workgroup takes
@@ -125,6 +148,7 @@ struct PoolCuts {
   int split_rows, splits, slots;  // slots: tiles of queries at most
   int groups;                     // a request's pieces side by side: its heads, or pairs of them
   bool few;                       // decode: fewer (request, head) pairs than half the CUs
+  bool tiles;                     // k_pool_tiles takes the queries
   Divide by_split, by_heads;
 };
 // A tile of a request's tokens [t0, t_last], a head, and rows [begin, stop) of the all_rows that the tile attends.
@@ -152,8 +176,9 @@ __device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
 // pool's share the line of their scales), as the tiles of a request read the same rows, and their XCD reads them once.
 // (Pieces that go round the XCDs: eight trees of 61 over 4000 rows 130 us for 110.)  Up to 64 requests every wave counts
 // the pieces that there are; of more, a piece is a slot, whose tile and split may not exist.
-template <Mode kMode>
+template <Mode kMode, int kLog2>
 __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c, Piece& p) {
+  constexpr int kQueries = 1 << kLog2, kQueriesLog2 = kLog2;  // of a tile
   const int turn = (int)(blockIdx.x / 8), xcd = (int)(blockIdx.x % 8);
   int j;  // the tile
   if (a.requests <= 64) {
@@ -486,8 +511,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   __shared__ float peak[kWaves][kQueries], total[kWaves][kQueries];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = lane >> 5;
   Piece w;
-  if (!find_piece<kMode>(a, p.cuts, w)) return;
+  if (!find_piece<kMode, kQueriesLog2>(a, p.cuts, w)) return;
   const int stop = w.stop, head = w.head;
+  // the first row of the request that no token attends
+  const int unread = tile_rows<kMode>(a, w.cached, w.end - w.first, w.end - w.first - 1);
   const uint32_t* lookup = a.lookup + (int64_t)w.n * a.lookup_cols;
   const auto block_at = [&](int row) {
     return a.pool + (int64_t)min(ldc(lookup + row / a.P), (uint32_t)(a.pages - 1)) * a.page_bytes + a.layer_bytes +
@@ -503,10 +530,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
                   *(const UOCR_GLOBAL f32x4*)(src + 64), *(const UOCR_GLOBAL f32x4*)(src + 68)};
     int pos = 0;
     if (a.rope.positions != nullptr) pos = min(max(ldg(a.rope.positions + t), 0), a.rope.table_rows - 1);
-    if (first < stop) {
-      const char* from = block_at(first);
+    const char* from = block_at(first);
+    const bool early = !a.stores || first + kBlock <= w.cached;  // no row among them that this workgroup has yet to store
+    if (first < stop && early) {
       load_keys(k, a, from, head, stop - 1 - first, lane);
       load_values(v, a, from, head, stop - 1 - first, lane);
+    }
+    if (a.stores) {
+      // The new rows that this workgroup reads, and of its tile's tokens those that none does.  (Workgroups that read the
+      // same rows store the same bits.)
+      for (int r = max(w.begin, w.cached) + wave; r < stop; r += kWaves) store_row<kInt8, 1>(a, w.n, r, w.first + (r - w.cached), head);
+      if (w.split == 0)
+        for (int t = w.t0 + wave; t <= w.t_last; t += kWaves) {
+          const int64_t r = (int64_t)w.cached + (t - w.first);
+          if (r >= unread && r < a.max_rows) store_row<kInt8, 1>(a, w.n, (int)r, t, head);
+        }
+      __syncthreads();
+      if (first < stop && !early) {
+        load_keys(k, a, from, head, stop - 1 - first, lane);
+        load_values(v, a, from, head, stop - 1 - first, lane);
+      }
     }
     if (a.rope.positions != nullptr) {
       const float *ct = a.rope.cos_t + (int64_t)pos * kD + d, *st = a.rope.sin_t + (int64_t)pos * kD + d;
@@ -672,6 +715,209 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   }
 }
 
+// ------------------------------------------------------------------ many tokens a request, over an int8 pool
+//
+// 256 queries of a head, 32 a wave.  Bound by the matrix instruction: a block of 32 rows is 48 of them a wave, beside some
+// 200 other instructions for the scores, and with one row's conversion shared by 8 waves those fit under them (two waves a
+// SIMD, the one's products under the other's exponentials).  64 rows are in LDS as operands, the next 64 on their way:
+//   keys    [block 2][step 8][slot 64][8], slot (32 half + row) ^ step: the columns 16 step + 8 half on.  (The exchange
+//           spreads a row's steps, which 8 lanes write at once, over the banks.)
+//   values  [block 2][step 2][u 4][lane 64][8]: as value_row has them, column 4 (lane % 32) + u.
+#ifndef UOCR_TILE_WAVES
+#define UOCR_TILE_WAVES 4
+#endif
+constexpr int kTileWaves = UOCR_TILE_WAVES, kTileThreads = kTileWaves * kWave, kTileLog2 = kTileWaves == 8 ? 8 : 7;
+constexpr int kTileRows = 8 * kTileWaves;
+constexpr int kTileBlocks = kTileRows / kBlock;
+constexpr int kTileHalves = kTileRows * kD;  // numbers of a tile's keys, or values
+
+struct TileRaw {  // a thread's part of 64 rows: 16 bytes of a key, 4 of 4 values, and a scale
+  u32x4 k;
+  uint32_t v[4];
+  float scale;
+};
+
+__global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
+  const PoolArgs& a = p.a;
+  __shared__ __align__(16) uint16_t keys[2][kTileHalves], values[2][kTileHalves];
+  __shared__ __align__(16) uint16_t q_lo[kTileWaves][kQTerm];
+  __shared__ __align__(16) float scales[2][2][kTileRows];
+  const int tid = (int)threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), h = lane >> 5;
+  Piece w;
+  if (!find_piece<kCausal, kTileLog2>(a, p.cuts, w)) return;
+  const int stop = w.stop, head = w.head;
+  const uint32_t* lookup = a.lookup + (int64_t)w.n * a.lookup_cols;
+  const auto slots_at = [&](int row) {  // of 32 rows, which lie in one page
+    return a.pool + (int64_t)min(ldc(lookup + row / a.P), (uint32_t)(a.pages - 1)) * a.page_bytes + a.layer_bytes +
+           (int64_t)(row % a.P) * a.slot_bytes;
+  };
+  // ---- a tile's rows: memory to registers, registers to LDS
+  const int key = tid / 8, chunk = tid % 8;                                // the thread's key and columns 16 chunk on
+  const int v_block = wave / 4, v_first = 16 * (wave / 2 % 2) + 4 * (wave % 2) + 8 * h;  // its values' rows, v_first on
+  const auto load = [&](TileRaw& r, int row0) {
+    const int last = a.max_rows - kBlock;  // (rows past the table's are asked for nowhere)
+    const char* lower = slots_at(min(row0, last));
+    const char* upper = kTileBlocks > 1 ? slots_at(min(row0 + kBlock, last)) : lower;
+    const char* mine = key < kBlock ? lower : upper;
+    r.k = *(const UOCR_GLOBAL u32x4*)(mine + (uint32_t)((key % kBlock) * a.slot_bytes + head * kD + 16 * chunk));
+    const char* from = (v_block == 0 ? lower : upper) + a.kv_bytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.v[i] = *(const UOCR_GLOBAL uint32_t*)(from + (uint32_t)((v_first + i) * a.slot_bytes + head * kD + 4 * (lane & 31)));
+    if (wave < 2) {  // the first wave the keys' scales, the second the values'
+      const char* at = (lane < kBlock ? lower : upper) + (wave == 0 ? 0 : a.kv_bytes);
+      r.scale = *(const UOCR_GLOBAL float*)(at + (uint32_t)((lane & 31) * a.slot_bytes + a.heads * kD + 4 * head));
+    }
+  };
+  const float c = a.scale * 1.44269504f;
+  const auto convert = [&](const TileRaw& r, int buf) {
+    u32x4 lo, hi;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      lo[2 * e] = bytes_bf16<0, 1>(r.k[e], r.k[e]);
+      lo[2 * e + 1] = bytes_bf16<2, 3>(r.k[e], r.k[e]);
+      hi[2 * e] = bytes_bf16<0, 1>(r.k[2 + e], r.k[2 + e]);
+      hi[2 * e + 1] = bytes_bf16<2, 3>(r.k[2 + e], r.k[2 + e]);
+    }
+    uint16_t* kt = keys[buf] + ((key / kBlock) * 8 + chunk) * kFrag;
+    *(u32x4*)(kt + ((key % kBlock) ^ chunk) * 8) = lo;
+    *(u32x4*)(kt + ((32 + key % kBlock) ^ chunk) * 8) = hi;
+    uint16_t* vt = values[buf] + wave / 2 * 4 * kFrag + (32 * (wave % 2) + (lane & 31)) * 8 + 4 * h;
+    const auto column = [&](auto u) {
+      constexpr int U = decltype(u)::value;
+      *(u32x2*)(vt + U * kFrag) = u32x2{bytes_bf16<U, U>(r.v[0], r.v[1]), bytes_bf16<U, U>(r.v[2], r.v[3])};
+    };
+    column(std::integral_constant<int, 0>{});
+    column(std::integral_constant<int, 1>{});
+    column(std::integral_constant<int, 2>{});
+    column(std::integral_constant<int, 3>{});
+    if (wave < 2) scales[buf][wave][lane % kTileRows] = wave == 0 ? r.scale * c : r.scale;
+  };
+  TileRaw raw;
+  load(raw, w.begin);
+  // ---- the wave's queries: columns 16 t + 8 h on of step t; the last terms in LDS
+  const int t0 = w.t0 + 32 * wave, my_t = min(t0 + (lane & 31), w.t_last);
+  const bool idle = t0 > w.t_last;  // a wave without queries converts
+  u32x4 q_hi[8], q_mid[8];
+  {
+    const float* row = a.q + (int64_t)my_t * a.in_stride + (int64_t)head * kD + 8 * h;
+    const float *ct = nullptr, *st = nullptr;
+    if (a.rope.positions != nullptr) {
+      const int64_t at = (int64_t)min(max(ldg(a.rope.positions + my_t), 0), a.rope.table_rows - 1) * kD + 8 * h;
+      ct = a.rope.cos_t + at;
+      st = a.rope.sin_t + at;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {  // with step t + 4, 64 columns on
+      f32x4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = *(const UOCR_GLOBAL f32x4*)(row + 16 * t + 4 * (i % 2) + 64 * (i / 2));
+      if (ct != nullptr)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int at = 16 * t + 4 * i;
+          rotate4(x[i], x[i + 2], *(const UOCR_GLOBAL f32x4*)(ct + at), *(const UOCR_GLOBAL f32x4*)(ct + at + 64),
+                  *(const UOCR_GLOBAL f32x4*)(st + at), *(const UOCR_GLOBAL f32x4*)(st + at + 64));
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        u32x4 lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t mid, last;
+          q_hi[t + 4 * i][e] = split3(x[2 * i + e / 2][2 * (e % 2)], x[2 * i + e / 2][2 * (e % 2) + 1], mid, last);
+          q_mid[t + 4 * i][e] = mid;
+          lo[e] = last;
+        }
+        *(u32x4*)(q_lo[wave] + (t + 4 * i) * kFrag + lane * 8) = lo;
+      }
+    }
+  }
+  const int most = idle ? 0 : min(w.cached + (min(t0 + 31, w.t_last) - w.first) + 1, stop);  // rows that the wave attends
+  const int all = min(w.cached + (t0 - w.first) + 1, stop);                                 // that all of its queries do
+  const int limit = min(w.cached + (my_t - w.first) + 1, stop);
+  Running run;
+  start(run);
+  convert(raw, 0);
+  if (w.begin + kTileRows < stop) load(raw, w.begin + kTileRows);
+  lds_barrier();
+  const auto attend = [&](int key0, int buf, int block) {
+    const uint16_t* kt = keys[buf] + block * 8 * kFrag;
+    f32x16 s = {};
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const bf16x8 k = *(const bf16x8*)(kt + t * kFrag + (lane ^ t) * 8);
+      s = mfma(k, *(const bf16x8*)(q_lo[wave] + t * kFrag + lane * 8), s);
+      s = mfma(k, bf(q_mid[t]), s);
+      s = mfma(k, bf(q_hi[t]), s);
+    }
+    f32x4 vs[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 ks = *(const f32x4*)&scales[buf][0][32 * block + 8 * g + 4 * h];
+      vs[g] = *(const f32x4*)&scales[buf][1][32 * block + 8 * g + 4 * h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[4 * g + e] *= ks[e];
+    }
+    const bool masked = key0 + kBlock > all;
+    if (masked)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + 4 * h + r % 4 < limit - key0 ? s[r] : -kInf;
+    weigh(run, s);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= vs[r / 4][r % 4];
+    if (masked)  // the scales of rows that are not attended may be anything
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + 4 * h + r % 4 < limit - key0 ? s[r] : 0.0f;
+    const uint16_t* vt = values[buf] + block * 8 * kFrag + lane * 8;
+    const auto step = [&](auto t) {
+      constexpr int T = decltype(t)::value;
+      u32x4 hi, mid, lo;
+      split_weights<T>(s, hi, mid, lo);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bf16x8 v = *(const bf16x8*)(vt + (4 * T + u) * kFrag);
+        run.o[u] = mfma(v, bf(lo), run.o[u]);
+        run.o[u] = mfma(v, bf(mid), run.o[u]);
+        run.o[u] = mfma(v, bf(hi), run.o[u]);
+      }
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+  };
+#ifdef UOCR_PRIO
+  if (wave < kTileWaves / 2) __builtin_amdgcn_s_setprio(UOCR_PRIO);
+#endif
+  int buf = 0;
+#pragma unroll 1
+  for (int key0 = w.begin; key0 < stop; key0 += kTileRows, buf ^= 1) {
+    if (kTileBlocks > 1 && key0 < most) attend(key0, buf, 0);
+    if (key0 + kTileRows < stop) {
+      convert(raw, buf ^ 1);
+      if (key0 + 2 * kTileRows < stop) load(raw, key0 + 2 * kTileRows);
+    }
+    if (key0 + kTileRows - kBlock < most) attend(key0 + kTileRows - kBlock, buf, kTileBlocks - 1);
+    lds_barrier();
+  }
+  if (idle || t0 + (lane & 31) > w.t_last) return;
+  const float sum = run.l + other32(run.l);
+  const bool whole = w.all_rows <= p.cuts.split_rows;
+  const float f = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t th = (int64_t)my_t * a.heads + head, part = w.split * (int64_t)a.tokens * a.heads + th;
+  float* to = (whole ? a.out + th * kD : p.part + part * kD) + 16 * h;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    f32x4 y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y[u] = run.o[u][r] * f;
+    *(UOCR_GLOBAL f32x4*)(to + 32 * (r / 4) + 4 * (r % 4)) = y;
+  }
+  if (!whole && h == 0) {
+    stg(p.tops + 2 * part, run.m);
+    stg(p.tops + 2 * part + 1, sum);
+  }
+}
+
 // ------------------------------------------------------------------ one token a request, over an int8 pool
 //
 // A single query leaves 31 of 32 columns of the matrix instruction empty, and one head's rows are its alone: the products
@@ -754,8 +1000,7 @@ __device__ __forceinline__ u32x4 quantize_columns(const float (&x)[kOneParts], f
   u32x4 q;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    q[i] = to_int8(x[4 * i], scale) | to_int8(x[4 * i + 1], scale) << 8 | to_int8(x[4 * i + 2], scale) << 16 |
-           to_int8(x[4 * i + 3], scale) << 24;
+    q[i] = to_int8x4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], scale);
   return q;
 }
 
@@ -957,7 +1202,7 @@ __global__ void __launch_bounds__(kOneWaves * kWave) k_pool_one(Attend p) {
 }
 
 // Joins the splits of a token's rows: half a wave a (token, head), four columns a lane.
-template <Mode kMode>
+template <Mode kMode, int kQueriesLog2>
 __global__ void __launch_bounds__(256) k_pool_join(Attend p) {
   const PoolArgs& a = p.a;
   const int groups = (a.heads + 1) / 2;
@@ -997,18 +1242,26 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p) {
 // How a call's rows are cut: splits of at least a round of the waves, as many as fill the device once with two
 // workgroups a CU.
 namespace {
-constexpr int kCus = 256;
-PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, bool one) {
+constexpr int kCus = 256, kStoredByReaders = 64;
+#ifndef UOCR_TILES
+#define UOCR_TILES (tokens / requests > 64 && tokens * attend_max >= 1 << 19)
+#endif
+PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
   PoolCuts c{};
-  const int64_t tiles = one || requests <= 64 ? (tokens < requests ? tokens : (tokens - requests) / kQueries + requests)
-                                              : tokens / kQueries + requests;
+  const bool one = form == kPoolDecode;
+  c.tiles = form == kPoolChunk && requests > 0 && UOCR_TILES;
+  const int queries = c.tiles ? 1 << kTileLog2 : kQueries;
+  const int64_t tiles = one || requests <= 64 ? (tokens < requests ? tokens : (tokens - requests) / queries + requests)
+                                              : tokens / queries + requests;
   c.slots = (int)tiles;
   c.few = one && requests * heads <= kCus / 2;
   c.groups = one && !c.few ? (heads + 1) / 2 : heads;
-  const int64_t fill = !one ? 2 * kCus : c.few ? kCus : UOCR_ONE_FILL * kCus;
+  const int64_t fill = one ? (c.few ? kCus : UOCR_ONE_FILL * kCus) : c.tiles && kTileWaves == 8 ? kCus : 2 * kCus;
   const int64_t splits = std::max<int64_t>(1, fill / std::max<int64_t>(1, tiles * c.groups));
-  const int round = !one ? kWaves * kBlock : c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16;
+  const int round = one ? (c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16) : c.tiles ? 256 : 2 * kWaves * kBlock;
   c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
+  // two splits of 256 rows and their join take the time of one of 512, and a launch more
+  if (!one && !c.tiles && attend_max <= 512) c.split_rows = 512;
   c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
   c.by_split = divide_by(c.split_rows);
   c.by_heads = divide_by(c.groups);
@@ -1017,7 +1270,7 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, bo
 
 template <bool kInt8, Mode kMode>
 hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
-  const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max, kMode == kOne);
+  const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max, form_of(kMode));
   const int64_t pairs = p.tokens * p.heads, items = ((int64_t)c.slots * c.splits + 7) / 8 * 8 * c.groups;
   const int64_t joins = p.tokens * ((p.heads + 1) / 2);
   // (where a wave counts the pieces, offsets that do not ascend may give each request all of them)
@@ -1030,21 +1283,30 @@ hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
     else
       UOCR_LAUNCH("pool_one", k_pool_one<2>, grid, dim3(kOneWaves * kWave), 0, s, at);
   } else {
-    auto store = k_pool_store<kInt8>;
-    UOCR_LAUNCH("pool_store", store, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, s, a);
-    auto attend = k_pool_attend<kInt8, kMode>;
-    UOCR_LAUNCH("pool_attend", attend, grid, dim3(kThreads), 0, s, at);
+    if (!a.stores) {
+      auto store = k_pool_store<kInt8>;
+      const int64_t stores = p.tokens * ((p.heads + kStoreHeads - 1) / kStoreHeads);
+      UOCR_LAUNCH("pool_store", store, dim3((unsigned)((stores + 3) / 4)), dim3(256), 0, s, a);
+    }
+    if (kMode == kCausal && c.tiles) {
+      UOCR_LAUNCH("pool_tiles", k_pool_tiles, grid, dim3(kTileThreads), 0, s, at);
+    } else {
+      auto attend = k_pool_attend<kInt8, kMode>;
+      UOCR_LAUNCH("pool_attend", attend, grid, dim3(kThreads), 0, s, at);
+    }
   }
   if (c.splits > 1) {
-    auto join = k_pool_join<kMode>;
+    auto join = k_pool_join<kMode, kQueriesLog2>;
+    if constexpr (kMode == kCausal)
+      if (c.tiles) join = k_pool_join<kMode, kTileLog2>;
     UOCR_LAUNCH("pool_join", join, dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, s, at);
   }
   return hipGetLastError();
 }
 }  // namespace
 
-size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, bool one) {
-  const PoolCuts c = cuts_of(tokens, requests, heads, attend_max, one);
+size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
+  const PoolCuts c = cuts_of(tokens, requests, heads, attend_max, form);
   return c.splits > 1 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) : 0;
 }
 
@@ -1076,6 +1338,8 @@ hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s) {
   a.out = p.out;
   a.scale = p.scale;
   a.rope = Rope{p.positions, p.cos_table, p.sin_table, p.table_rows};
+  // Few new rows are stored by those that read them, which saves a launch; many would be stored again and again.
+  a.stores = p.tokens <= kStoredByReaders;  // (tiles have more tokens)
   if (p.write_index != nullptr) return launch<true, kOne>(p, a, s);
   if (p.visible == nullptr) return launch<true, kCausal>(p, a, s);
   return p.int8 ? launch<true, kTree>(p, a, s) : launch<false, kTree>(p, a, s);

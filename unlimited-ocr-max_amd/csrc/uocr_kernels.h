@@ -313,15 +313,16 @@ struct PoolAttention {
   int64_t tokens, requests;
   int attend_max;                 // the most rows a token attends (host)
   float scale;
-  void* workspace;                // pool_workspace_bytes(tokens, requests, heads, attend_max, write_index != null)
+  void* workspace;                // pool_workspace_bytes(tokens, requests, heads, attend_max, its form)
   int64_t in_stride;
   const int32_t* positions;       // null: q, k_new come rotated; else rotated here at these positions
   const float* cos_table;         // [table_rows, head_dim]
   const float* sin_table;
   int table_rows;
 };
-// one: the decode form, a token a request.
-size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, bool one);
+// kPoolDecode: a token a request (write_index); kPoolTree: with masks.
+enum PoolForm { kPoolDecode, kPoolChunk, kPoolTree };
+size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form);
 hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s);
 
 // ---- pages between the fp32 pool and the int8 one (int8_pages.hip) ----

@@ -928,11 +928,11 @@ int uocr_paged_chunk_attention_qkv(float* out, const float* qkv, int64_t tokens,
 
 // ------------------------------------------------------------------ an int8 pool, and trees of drafted tokens
 
-size_t uocr_paged_pool_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max, int64_t decode) {
+size_t uocr_paged_pool_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t attend_max, int64_t form) {
   if (tokens < 0 || tokens > INT32_MAX || requests < 0 || requests > INT32_MAX || heads < 1 || heads > 65535 ||
-      attend_max < 1 || attend_max > INT32_MAX)
+      attend_max < 1 || attend_max > INT32_MAX || form < kPoolDecode || form > kPoolTree)
     return 0;
-  return pool_workspace_bytes(tokens, requests, (int)heads, (int)attend_max, decode != 0);
+  return pool_workspace_bytes(tokens, requests, (int)heads, (int)attend_max, (PoolForm)form);
 }
 
 // The bytes of a pool; 0: its sizes are none that a pool has (refused, the message in err).
@@ -994,7 +994,8 @@ static int pool_attention_call(const char* op, PoolAttention p, int64_t heads, i
   }
   const hipStream_t s = (hipStream_t)stream;
   void* ws = nullptr;
-  const size_t need = pool_workspace_bytes(tokens, requests, (int)heads, (int)attend_max, decode);
+  const PoolForm form = decode ? kPoolDecode : p.visible == nullptr ? kPoolChunk : kPoolTree;
+  const size_t need = pool_workspace_bytes(tokens, requests, (int)heads, (int)attend_max, form);
   if (chunk_workspace(op, workspace, workspace_bytes, need, s, &ws, err, errlen)) return 1;
   p.pages = (int)pages;
   p.layers = (int)layers;

@@ -479,9 +479,10 @@ def _pool_call(op: str, name: str, inputs: tuple, stride: int, heads: int, head_
     elif tuple(_out(op, "out", out, torch.float32, 3).shape) != (tokens, heads, head_dim):
         raise ValueError(f"{op}: out must be {(tokens, heads, head_dim)}, got {tuple(out.shape)}")
     need = 0
+    form = 0 if not requests else 1 if metadata[2] is None else 2  # decode, chunks, with masks
     # nothing is allocated for more rows than the table addresses: the entry refuses them
     if workspace is not None or attend_max <= lookup.shape[1] * page_size:
-        need = _lib.load().uocr_paged_pool_workspace_bytes(tokens, lookup.shape[0], heads, attend_max, not requests)
+        need = _lib.load().uocr_paged_pool_workspace_bytes(tokens, lookup.shape[0], heads, attend_max, form)
     ws = _workspace(op, workspace, need, like)
     if len(inputs) == 1:
         q = like.data_ptr()
@@ -574,13 +575,25 @@ def _nbytes(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
+_DEVICES: int | None = None
+
+
+def _several_devices() -> bool:
+    """Whether GPU tensors can be on different devices (counted once: the process's devices do not change)."""
+    global _DEVICES
+    if _DEVICES is None:
+        _DEVICES = torch.cuda.device_count()
+    return _DEVICES != 1
+
+
 def _on_device(op: str, name: str, *args, tensors) -> None:
     """Calls entry ``name`` with ``args`` and the current stream of the tensors' device, made current for the
     launch; tensors of several devices are refused."""
     dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{op}: the tensors are on different devices")
+    if _several_devices():
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                raise ValueError(f"{op}: the tensors are on different devices")
     if dev == torch._C._cuda_getDevice():
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
@@ -823,8 +836,9 @@ def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tenso
         raise ValueError(f"{op}: the chunks' metadata is not for {n} requests")
     if tokens.shape[0] != total or answers.shape[0] != total:
         raise ValueError(f"{op}: parents, tokens and answers must have one length")
-    counts, path, following = parents.new_empty(n), parents.new_empty(total), parents.new_empty(n)
-    lengths = torch.empty_like(cached)
+    counts, following, lengths, path = parents.new_empty(3 * n + total).split([n, n, n, total])
+    if cached.dtype is torch.uint32:
+        lengths = lengths.view(torch.uint32)
     _on_device(op, "uocr_accept_drafts", blocks.data_ptr(), pages, layers, page_size, 4 * heads * head_dim,
                lookup.data_ptr(), n, lookup.shape[1], cached.data_ptr(), offsets.data_ptr(), parents.data_ptr(),
                tokens.data_ptr(), answers.data_ptr(), total, counts.data_ptr(), path.data_ptr(), following.data_ptr(),
@@ -883,9 +897,9 @@ def beam_select(logits, scores, *, beams: int, eos: int, ended=None, lengths=Non
     need = _lib.load().uocr_beam_select_workspace_bytes(rows, vocab, beams)
     ws = _workspace(op, workspace, need, logits)
     out_scores = torch.empty_like(scores)
-    tokens = scores.new_empty(rows, dtype=torch.int32)
-    parents, now_ended = torch.empty_like(tokens), torch.empty_like(tokens)
-    now_lengths = None if lengths is None else torch.empty_like(tokens)
+    tokens, parents, now_ended, *now_lengths = scores.new_empty((3 if lengths is None else 4, rows),
+                                                                dtype=torch.int32).unbind()
+    now_lengths = now_lengths[0] if now_lengths else None
     now_history = None if history is None else torch.empty_like(history)
     _on_device(op, "uocr_beam_select", tokens.data_ptr(), parents.data_ptr(), out_scores.data_ptr(), now_ended.data_ptr(),
                _ptr(now_lengths), _ptr(now_history), logits.data_ptr(), rows, vocab, int(beams), scores.data_ptr(), int(eos),
