@@ -610,6 +610,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
       if (next < stop) load_keys(k, a, next_base, head, stop - 1 - next, lane);
       const bool masked = key0 + kBlock > all;
       if (masked) {
+        asm volatile("");  // a branch: as selects the masks would be a sixth of a block's instructions
         uint32_t set = 0;
         if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
         const int live = limit - key0;
@@ -633,6 +634,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= vs[r / 4][r % 4];
         if (masked) {  // the scales of rows that are not attended may be anything
+          asm volatile("");
           uint32_t set = 0;
           if constexpr (kMode == kTree) set = tree_rows(visible, key0 - w.cached, stop - key0);
           const int live = limit - key0;
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
 //           spreads a row's steps, which 8 lanes write at once, over the banks.)
 //   values  [block 2][step 2][u 4][lane 64][8]: as value_row has them, column 4 (lane % 32) + u.
 #ifndef UOCR_TILE_WAVES
-#define UOCR_TILE_WAVES 4
+#define UOCR_TILE_WAVES 8
 #endif
 constexpr int kTileWaves = UOCR_TILE_WAVES, kTileThreads = kTileWaves * kWave, kTileLog2 = kTileWaves == 8 ? 8 : 7;
 constexpr int kTileRows = 8 * kTileWaves;
@@ -860,15 +862,19 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
       for (int e = 0; e < 4; ++e) s[4 * g + e] *= ks[e];
     }
     const bool masked = key0 + kBlock > all;
-    if (masked)
+    if (masked) {
+      asm volatile("");  // a branch: as selects the masks would be a quarter of a block's instructions
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + 4 * h + r % 4 < limit - key0 ? s[r] : -kInf;
+    }
     weigh(run, s);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] *= vs[r / 4][r % 4];
-    if (masked)  // the scales of rows that are not attended may be anything
+    if (masked) {  // the scales of rows that are not attended may be anything
+      asm volatile("");
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + 4 * h + r % 4 < limit - key0 ? s[r] : 0.0f;
+    }
     const uint16_t* vt = values[buf] + block * 8 * kFrag + lane * 8;
     const auto step = [&](auto t) {
       constexpr int T = decltype(t)::value;
@@ -885,9 +891,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
   };
-#ifdef UOCR_PRIO
-  if (wave < kTileWaves / 2) __builtin_amdgcn_s_setprio(UOCR_PRIO);
+#ifndef UOCR_PRIO
+#define UOCR_PRIO 1
 #endif
+  if (wave < kTileWaves / 2) __builtin_amdgcn_s_setprio(UOCR_PRIO);
   int buf = 0;
 #pragma unroll 1
   for (int key0 = w.begin; key0 < stop; key0 += kTileRows, buf ^= 1) {
@@ -1244,7 +1251,7 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p) {
 namespace {
 constexpr int kCus = 256, kStoredByReaders = 64;
 #ifndef UOCR_TILES
-#define UOCR_TILES (tokens / requests > 64 && tokens * attend_max >= 1 << 19)
+#define UOCR_TILES (tokens / requests >= 256 && tokens * attend_max >= 3 << 20)
 #endif
 PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
   PoolCuts c{};
@@ -1257,7 +1264,9 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
   c.few = one && requests * heads <= kCus / 2;
   c.groups = one && !c.few ? (heads + 1) / 2 : heads;
   const int64_t fill = one ? (c.few ? kCus : UOCR_ONE_FILL * kCus) : c.tiles && kTileWaves == 8 ? kCus : 2 * kCus;
-  const int64_t splits = std::max<int64_t>(1, fill / std::max<int64_t>(1, tiles * c.groups));
+  // (of `tiles` at most, about so many are there: half of a request's last one is queries)
+  const int64_t likely = one ? requests : std::max(requests, (tokens + queries - 1) / queries + (requests - 1) / 2);
+  const int64_t splits = std::max<int64_t>(1, fill / std::max<int64_t>(1, std::min(tiles, likely) * c.groups));
   const int round = one ? (c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16) : c.tiles ? 256 : 2 * kWaves * kBlock;
   c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
   // two splits of 256 rows and their join take the time of one of 512, and a launch more
