@@ -33,7 +33,7 @@ namespace {
 constexpr int kBlock = 32;     // rows a wave takes at a time: the rows of one matrix instruction
 constexpr int kQueries = 32;   // of a workgroup
 constexpr int kQueriesLog2 = 5;
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kRound = kWaves * kBlock;
 constexpr int kThreads = kWaves * kWave;
 constexpr float kInf = __builtin_huge_valf();
 // A maximum may lag by so many binades before the sums are rescaled (the weights are floats: nothing is lost).
@@ -145,15 +145,17 @@ __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
 
 // A call's rows are cut into splits where the tiles of queries alone do not fill the device.
 struct PoolCuts {
-  int split_rows, splits, slots;  // slots: tiles of queries at most
+  int split_rows, splits, slots;  // rows of a split at least; splits of a tile and tiles of queries at most
+  int fill;                       // up to 64 requests: pieces of a head that fill the device (0: splits have split_rows)
   int groups;                     // a request's pieces side by side: its heads, or pairs of them
   bool few;                       // decode: fewer (request, head) pairs than half the CUs
   bool tiles;                     // k_pool_tiles takes the queries
   Divide by_split, by_heads;
 };
-// A tile of a request's tokens [t0, t_last], a head, and rows [begin, stop) of the all_rows that the tile attends.
+// A tile of a request's tokens [t0, t_last], a head, and rows [begin, stop) of those that the tile attends.
 struct Piece : Chunk {
-  int t0, t_last, head, split, begin, stop, all_rows;
+  int t0, t_last, head, split, begin, stop;
+  bool whole;  // no other piece of the tile
 };
 // Rows that a tile attends whose last token is t_last.
 template <Mode kMode>
@@ -162,6 +164,12 @@ __device__ __forceinline__ int tile_rows(const PoolArgs& a, int cached, int leng
                        : kMode == kCausal ? (int64_t)cached + last + 1
                                          : (int64_t)cached + min(length, 64);
   return (int)min(rows, (int64_t)a.attend_max);
+}
+// Rows of each of a request's splits, where one has at most `most`: of a size, to a round of the waves.  (None is empty: with
+// n splits of at most `most` rows there are more than (n - 1) * most.)
+__device__ __forceinline__ int rows_of_split(int rows, int most) {
+  const int n = (rows - 1) / most + 1;
+  return n == 1 ? rows : ((rows - 1) / n / kRound + 1) * kRound;
 }
 template <Mode kMode>
 __device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
@@ -172,34 +180,42 @@ __device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
   c.cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)(kMode == kOne ? a.max_rows - 1 : a.max_rows));
   return c;
 }
-// Items go to the XCDs in stretches, a piece's heads side by side: the heads of a row are neighbours in memory (an int8
-// pool's share the line of their scales), as the tiles of a request read the same rows, and their XCD reads them once.
-// (Pieces that go round the XCDs: eight trees of 61 over 4000 rows 130 us for 110.)  Up to 64 requests every wave counts
-// the pieces that there are; of more, a piece is a slot, whose tile and split may not exist.
+// Items go to the XCDs in stretches, a piece's heads side by side and the tiles that read the same rows next: the heads of a
+// row are neighbours in memory (an int8 pool's share the line of their scales), and their XCD reads the rows once.  (Pieces
+// that go round the XCDs: eight trees of 61 over 4000 rows 130 us for 110.)  Up to 64 requests every wave counts the pieces
+// that there are, and cuts them so that the device is filled by them once: the host does not know the lengths (with splits
+// from the longest, eight trees over 1667 to 4000 rows 92 us for 81).  Of more requests, a piece is a slot, whose tile and
+// split may not exist.  most_rows: where the join finds the rows of a split.
 template <Mode kMode, int kLog2>
-__device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c, Piece& p) {
-  constexpr int kQueries = 1 << kLog2, kQueriesLog2 = kLog2;  // of a tile
+__device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c, int* most_rows, Piece& p) {
   const int turn = (int)(blockIdx.x / 8), xcd = (int)(blockIdx.x % 8);
-  int j;  // the tile
+  uint32_t most = (uint32_t)c.split_rows;
+  int j, rows;  // the tile; rows of a split
   if (a.requests <= 64) {
     const Chunk mine = request_at<kMode>(a, min(lane_id(), a.requests - 1));
     const bool some = lane_id() < a.requests && mine.first >= 0 && mine.first < mine.end;
     const int length = some ? mine.end - mine.first : 0;
-    const int tiles = (length + kQueries - 1) >> kQueriesLog2;
-    const auto cuts = [&](int cached, int length, int j) {
-      return c.by_split(tile_rows<kMode>(a, cached, length, min((j + 1) << kQueriesLog2, length) - 1) - 1) + 1;
-    };
-    int pieces = tiles;
-    if (c.splits > 1) {
-      if constexpr (kMode == kCausal) {
-        pieces = 0;
-        for (int k = 0; __ballot(k < tiles) != 0; ++k)
-          if (k < tiles) pieces += cuts(mine.cached, length, k);
-      } else {
-        pieces = tiles == 0 ? 0 : tiles * cuts(mine.cached, length, 0);
-      }
+    const int tiles = (length + (1 << kLog2) - 1) >> kLog2;
+    const int all = some ? tile_rows<kMode>(a, mine.cached, length, length - 1) : 1;
+    if (c.fill > 0) {
+      // (a tile's last split leaves half of one empty)
+      float sum = (float)tiles * (float)all;
+      sum += from_up<32>(sum), sum += from_up<16>(sum), sum += from_up<8>(sum);
+      sum += from_up<4>(sum), sum += from_up<2>(sum), sum += from_up<1>(sum);
+      sum = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sum)));
+      const float guess = sum / (float)max(1, c.fill - wave_sum_i(tiles) / 2);
+      most = max(most, ((uint32_t)fminf(guess, (float)a.attend_max) / kRound + 1) * kRound);
+      while (most < (uint32_t)a.attend_max && wave_sum_i(tiles * (int)((uint32_t)(all - 1) / most + 1)) > c.fill)
+        most += max(most / 8 / kRound, 1u) * kRound;
     }
+    const int my_rows = rows_of_split(all, (int)most);
+    // tiles whose last query comes before the row
+    const auto before = [&](uint32_t row, int cached) { return kMode == kCausal && (int)row > cached ? ((int)row - cached) >> kLog2 : 0; };
+    int pieces = tiles;
+    for (uint32_t row = my_rows; __ballot(row < (uint32_t)all) != 0;)
+      if (row < (uint32_t)all) pieces += tiles - before(row, mine.cached), row += my_rows;
     const int upto = wave_scan_i(pieces), total = __builtin_amdgcn_readlane(upto, 63);
+    if (c.splits > 1 && blockIdx.x == 0) stg(most_rows, (int)most);
     const int per = (total * a.heads + 7) / 8, item = xcd * per + turn;
     if (turn >= per || item >= total * a.heads) return false;
     int left = c.by_heads(item);
@@ -210,40 +226,35 @@ __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c,
     p.first = __builtin_amdgcn_readlane(mine.first, at);
     p.end = __builtin_amdgcn_readlane(mine.end, at);
     p.cached = __builtin_amdgcn_readlane(mine.cached, at);
+    rows = __builtin_amdgcn_readlane(my_rows, at);
     j = __builtin_amdgcn_readlane(tiles, at) - 1;
-    if (c.splits > 1) {
-      for (; j > 0; --j) {
-        const int here = cuts(p.cached, p.end - p.first, j);
-        if (left < here) break;
-        left -= here;
-      }
-      p.split = left;
-    } else {
-      p.split = 0;
-      j -= left;
+    p.split = 0;
+    for (uint32_t row = 0;; row += rows, ++p.split) {
+      const int here = j + 1 - before(row, p.cached);
+      if (left < here) break;
+      left -= here;
     }
+    j -= left;
   } else {
     const int item = xcd * (int)(gridDim.x / 8) + turn;
     const int cell = c.by_heads(item), slot = cell / c.splits;  // the splits of a tile one after the other
+    if (c.splits > 1 && blockIdx.x == 0) stg(most_rows, (int)most);
     if (slot >= c.slots) return false;
     p.head = item - cell * a.heads;
     p.split = cell - slot * c.splits;
-    if constexpr (kMode == kOne) {
-      if (slot >= a.requests) return false;
-      (Chunk&)p = request_at<kMode>(a, slot);
-      j = 0;
-    } else {
-      (Chunk&)p = find_chunk(a, kQueriesLog2, true, slot);
-      j = slot - ((p.first >> kQueriesLog2) + p.n);
-      if (p.first < 0 || j < 0 || (int64_t)j << kQueriesLog2 >= p.end - p.first) return false;
-    }
+    (Chunk&)p = find_chunk(a, kLog2, true, slot);
+    j = slot - ((p.first >> kLog2) + p.n);
+    if (p.first < 0 || j < 0 || (int64_t)j << kLog2 >= p.end - p.first) return false;
+    rows = rows_of_split(tile_rows<kMode>(a, p.cached, p.end - p.first, p.end - p.first - 1), c.split_rows);
   }
-  p.t0 = p.first + (j << kQueriesLog2);
-  p.t_last = min(p.t0 + kQueries, p.end) - 1;
-  p.all_rows = tile_rows<kMode>(a, p.cached, p.end - p.first, p.t_last - p.first);
-  p.begin = p.split * c.split_rows;
-  p.stop = min(p.begin + c.split_rows, p.all_rows);
-  return p.begin < p.stop;
+  p.t0 = p.first + (j << kLog2);
+  p.t_last = min(p.t0 + (1 << kLog2), p.end) - 1;
+  const int all = tile_rows<kMode>(a, p.cached, p.end - p.first, p.t_last - p.first);
+  p.whole = all <= rows;
+  if ((int64_t)p.split * rows >= all) return false;
+  p.begin = p.split * rows;
+  p.stop = p.begin + min(rows, all - p.begin);
+  return true;
 }
 
 // ------------------------------------------------------------------ operands
@@ -377,6 +388,7 @@ struct Attend {
   PoolCuts cuts;
   float* part;  // [split][token][head][D], where a tile has several splits
   float* tops;  // [split][token][head][2]: the maximum (log2) and the sum of the weights
+  int* most_rows;  // [1]: rows of a split at most
 };
 
 // A lane's query: running maximum (log2), the sum of the weights of the lane's rows, the weighted values.
@@ -511,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   __shared__ float peak[kWaves][kQueries], total[kWaves][kQueries];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = lane >> 5;
   Piece w;
-  if (!find_piece<kMode, kQueriesLog2>(a, p.cuts, w)) return;
+  if (!find_piece<kMode, kQueriesLog2>(a, p.cuts, p.most_rows, w)) return;
   const int stop = w.stop, head = w.head;
   // the first row of the request that no token attends
   const int unread = tile_rows<kMode>(a, w.cached, w.end - w.first, w.end - w.first - 1);
@@ -686,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
     const float lj = total[j][lane & 31];
     sum += lj == 0.0f || lj != lj ? lj : lj * weight(peak[j][lane & 31]);
   }
-  const bool whole = w.all_rows <= p.cuts.split_rows;
+  const bool whole = w.whole;
   float f = weight(run.m);
   if (whole) f = sum == 0.0f ? 0.0f : sum != sum ? sum : f / sum;
   // query l % 32, a row of 128 floats whose 16-byte pieces are rotated by the query
@@ -746,7 +758,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
   __shared__ __align__(16) float scales[2][2][kTileRows];
   const int tid = (int)threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave), h = lane >> 5;
   Piece w;
-  if (!find_piece<kCausal, kTileLog2>(a, p.cuts, w)) return;
+  if (!find_piece<kCausal, kTileLog2>(a, p.cuts, p.most_rows, w)) return;
   const int stop = w.stop, head = w.head;
   const uint32_t* lookup = a.lookup + (int64_t)w.n * a.lookup_cols;
   const auto slots_at = [&](int row) {  // of 32 rows, which lie in one page
@@ -908,7 +920,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
   }
   if (idle || t0 + (lane & 31) > w.t_last) return;
   const float sum = run.l + other32(run.l);
-  const bool whole = w.all_rows <= p.cuts.split_rows;
+  const bool whole = w.whole;
   const float f = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
   const int64_t th = (int64_t)my_t * a.heads + head, part = w.split * (int64_t)a.tokens * a.heads + th;
   float* to = (whole ? a.out + th * kD : p.part + part * kD) + 16 * h;
@@ -1208,12 +1220,15 @@ __global__ void __launch_bounds__(kOneWaves * kWave) k_pool_one(Attend p) {
   }
 }
 
-// Joins the splits of a token's rows: half a wave a (token, head), four columns a lane.
+// Joins the splits of a token's rows: half a wave a (token, head), four columns a lane.  Of many splits (`ways`) the four waves
+// of a workgroup take every fourth: one wave would wait for the memory every few of them.
+constexpr int kJoinAtOnce = 4;
 template <Mode kMode, int kQueriesLog2>
-__global__ void __launch_bounds__(256) k_pool_join(Attend p) {
+__global__ void __launch_bounds__(256) k_pool_join(Attend p, bool ways) {
+  __shared__ __align__(16) float sums[4][4 * kWave];
   const PoolArgs& a = p.a;
-  const int groups = (a.heads + 1) / 2;
-  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int groups = (a.heads + 1) / 2, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int64_t item = ways ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int64_t t = item / groups;
   if (t >= a.tokens) return;
   Chunk c;
@@ -1223,31 +1238,59 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p) {
     return;
   const int i = (int)t - c.first, length = c.end - c.first;
   const int t_last = min(((i >> kQueriesLog2) + 1) << kQueriesLog2, length) - 1;  // of its tile
-  const int splits = p.cuts.by_split(tile_rows<kMode>(a, c.cached, length, t_last) - 1) + 1;
-  if (splits == 1) return;  // written by its tile
-  const int lane = lane_id(), head = (int)(item - t * groups) * 2 + lane / 32;
-  if (head >= a.heads) return;
-  const int64_t stride = (int64_t)a.tokens * a.heads, th = t * a.heads + head;
-  float m = -kInf;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, ldg(p.tops + 2 * (s * stride + th)));
-  float l = 0.0f;
-  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float ms = ldg(p.tops + 2 * (s * stride + th)), ls = ldg(p.tops + 2 * (s * stride + th) + 1);
-    const f32x4 y = *(const UOCR_GLOBAL f32x4*)(p.part + (s * stride + th) * kD + 4 * (lane & 31));
-    const float f = ls == 0.0f ? 0.0f : ms == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
-    l = __builtin_fmaf(f, ls, l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, y[e], o[e]);
+  int splits = 1;  // of its tile
+  if constexpr (kMode == kOne) {
+    splits = p.cuts.by_split(tile_rows<kMode>(a, c.cached, length, t_last) - 1) + 1;
+  } else {
+    const int rows = rows_of_split(tile_rows<kMode>(a, c.cached, length, length - 1), ldg(p.most_rows));
+    splits = (tile_rows<kMode>(a, c.cached, length, t_last) - 1) / rows + 1;
   }
-  *(UOCR_GLOBAL f32x4*)(a.out + th * kD + 4 * (lane & 31)) = l == 0.0f ? f32x4{} : o / l;
+  if (splits == 1) return;  // written by its tile
+  const int lane = lane_id(), piece = lane & 31, head = (int)(item - t * groups) * 2 + lane / 32;
+  const int64_t stride = (int64_t)a.tokens * a.heads, th = t * a.heads + min(head, a.heads - 1);
+  float m = -kInf, l = 0.0f;
+  for (int s = piece; s < splits; s += 32) m = fmaxf(m, ldg(p.tops + 2 * (s * stride + th)));
+#pragma unroll
+  for (int off = 1; off < 32; off *= 2) m = fmaxf(m, __shfl_xor(m, off, kWave));
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int base = 0; base < splits; base += 32) {
+    float f = 0.0f;  // of split base + piece
+    if (base + piece < splits) {
+      const float* top = p.tops + 2 * ((base + piece) * stride + th);
+      const float ms = ldg(top), ls = ldg(top + 1);
+      f = ls == 0.0f ? 0.0f : ms == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
+      l = __builtin_fmaf(f, ls, l);
+    }
+    const int upto = min(32, splits - base), step = ways ? 4 : 1;
+    for (int s0 = ways ? wave : 0; s0 < upto; s0 += kJoinAtOnce * step) {
+      f32x4 y[kJoinAtOnce];
+#pragma unroll
+      for (int i = 0; i < kJoinAtOnce; ++i)
+        y[i] = *(const UOCR_GLOBAL f32x4*)(p.part + ((base + min(s0 + i * step, upto - 1)) * stride + th) * kD + 4 * piece);
+#pragma unroll
+      for (int i = 0; i < kJoinAtOnce; ++i) {
+        if (s0 + i * step >= upto) break;
+        const float fs = __shfl(f, s0 + i * step + (lane & 32), kWave);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(fs, y[i][e], o[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 32; off *= 2) l += __shfl_xor(l, off, kWave);
+  if (ways) {
+    *(f32x4*)&sums[wave][4 * lane] = o;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) o += *(const f32x4*)&sums[w][4 * lane];
+  }
+  if (head < a.heads) *(UOCR_GLOBAL f32x4*)(a.out + th * kD + 4 * piece) = l == 0.0f ? f32x4{} : o / l;
 }
 
 }  // namespace
 
-// How a call's rows are cut: splits of at least a round of the waves, as many as fill the device once with two
-// workgroups a CU.
+// How a call's rows are cut.
 namespace {
 constexpr int kCus = 256, kStoredByReaders = 64;
 #ifndef UOCR_TILES
@@ -1263,14 +1306,29 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
   c.slots = (int)tiles;
   c.few = one && requests * heads <= kCus / 2;
   c.groups = one && !c.few ? (heads + 1) / 2 : heads;
-  const int64_t fill = one ? (c.few ? kCus : UOCR_ONE_FILL * kCus) : c.tiles && kTileWaves == 8 ? kCus : 2 * kCus;
-  // (of `tiles` at most, about so many are there: half of a request's last one is queries)
-  const int64_t likely = one ? requests : std::max(requests, (tokens + queries - 1) / queries + (requests - 1) / 2);
-  const int64_t splits = std::max<int64_t>(1, fill / std::max<int64_t>(1, std::min(tiles, likely) * c.groups));
-  const int round = one ? (c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16) : c.tiles ? 256 : 2 * kWaves * kBlock;
-  c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
-  // two splits of 256 rows and their join take the time of one of 512, and a launch more
-  if (!one && !c.tiles && attend_max <= 512) c.split_rows = 512;
+  c.split_rows = attend_max;
+  if (one) {
+    // as many splits as fill the device once, of a few rounds of the waves
+    const int64_t splits = std::max<int64_t>(1, kCus / std::max<int64_t>(1, requests * c.groups));
+    const int round = c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16;
+    c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
+  } else if (attend_max <= 512) {
+    // two splits of 256 rows and their join take the time of one of 512, and a launch more
+    c.split_rows = 512;
+  } else {
+    // With up to half as many workgroups as the device holds (two on a CU, one of tiles' 8 waves) the rows are cut for it to
+    // be full once, with up to as many twice; of more, the next takes the place of one that ends.  As to the lengths, none may
+    // be shorter than the others: splits for all of them to be half as long are what the workspace has to hold.
+    const int64_t mean = requests == 0 ? 1 : (tokens / requests + queries - 1) / queries * requests;
+    const int64_t work = std::max<int64_t>(1, std::min(tiles, mean)) * heads, fits = c.tiles ? kCus : 2 * kCus;
+    const int64_t full = work <= fits / 2 ? fits : work <= fits ? 2 * fits : 0;
+    if (full > 0) {
+      const int64_t longest = (attend_max + full / work - 1) / (full / work);
+      const bool counts = requests > 1 && requests <= 64;
+      c.fill = requests <= 64 ? (int)(full / heads) : 0;
+      c.split_rows = (int)std::max<int64_t>(2 * kRound, ((counts ? longest / 2 : longest) + kRound - 1) / kRound * kRound);
+    }
+  }
   c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
   c.by_split = divide_by(c.split_rows);
   c.by_heads = divide_by(c.groups);
@@ -1280,11 +1338,14 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
 template <bool kInt8, Mode kMode>
 hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
   const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max, form_of(kMode));
-  const int64_t pairs = p.tokens * p.heads, items = ((int64_t)c.slots * c.splits + 7) / 8 * 8 * c.groups;
+  const int64_t pairs = p.tokens * p.heads;
+  const int64_t pieces = c.fill > 0 ? std::max(c.fill, c.slots) : (int64_t)c.slots * c.splits, items = (pieces + 7) / 8 * 8 * c.groups;
   const int64_t joins = p.tokens * ((p.heads + 1) / 2);
   // (where a wave counts the pieces, offsets that do not ascend may give each request all of them)
-  if (items > (p.requests <= 64 ? INT32_MAX / p.requests : INT32_MAX) - 8) return hipErrorInvalidValue;
-  const Attend at{a, c, (float*)p.workspace, (float*)p.workspace + (int64_t)c.splits * pairs * kD};
+  if (pieces > INT32_MAX / c.groups - 8 || (int64_t)c.slots * c.splits * c.groups > INT32_MAX / std::min<int64_t>(p.requests, 64) - 8)
+    return hipErrorInvalidValue;
+  const Attend at{a, c, (float*)p.workspace, (float*)p.workspace + (int64_t)c.splits * pairs * kD,
+                  (int*)((float*)p.workspace + (int64_t)c.splits * pairs * (kD + 2))};
   const dim3 grid((unsigned)items);
   if constexpr (kMode == kOne) {
     if (c.few)
@@ -1308,7 +1369,8 @@ hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
     auto join = k_pool_join<kMode, kQueriesLog2>;
     if constexpr (kMode == kCausal)
       if (c.tiles) join = k_pool_join<kMode, kTileLog2>;
-    UOCR_LAUNCH("pool_join", join, dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, s, at);
+    const bool ways = c.splits > 8;
+    UOCR_LAUNCH("pool_join", join, dim3((unsigned)(ways ? joins : (joins + 3) / 4)), dim3(256), 0, s, at, ways);
   }
   return hipGetLastError();
 }
@@ -1316,7 +1378,7 @@ hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
 
 size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
   const PoolCuts c = cuts_of(tokens, requests, heads, attend_max, form);
-  return c.splits > 1 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) : 0;
+  return c.splits > 1 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) + sizeof(int) : 0;
 }
 
 hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s) {
