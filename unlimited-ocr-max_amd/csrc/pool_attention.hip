@@ -38,15 +38,6 @@ constexpr int kThreads = kWaves * kWave;
 constexpr float kInf = __builtin_huge_valf();
 // A maximum may lag by so many binades before the sums are rescaled (the weights are floats: nothing is lost).
 constexpr float kSlack = 8.0f;
-#ifndef UOCR_ONE_FILL
-#define UOCR_ONE_FILL 1
-#endif
-#ifndef UOCR_ONE_FEW
-#define UOCR_ONE_FEW 4
-#endif
-#ifndef UOCR_ONE_ROUND
-#define UOCR_ONE_ROUND 4
-#endif
 
 enum Mode { kOne, kCausal, kTree };
 constexpr PoolForm form_of(Mode m) { return m == kOne ? kPoolDecode : m == kCausal ? kPoolChunk : kPoolTree; }
@@ -150,6 +141,7 @@ struct PoolCuts {
   int groups;                     // a request's pieces side by side: its heads, or pairs of them
   bool few;                       // decode: fewer (request, head) pairs than half the CUs
   bool tiles;                     // k_pool_tiles takes the queries
+  bool round;                     // pieces go round the XCDs
   Divide by_split, by_heads;
 };
 // A tile of a request's tokens [t0, t_last], a head, and rows [begin, stop) of those that the tile attends.
@@ -160,9 +152,7 @@ struct Piece : Chunk {
 // Rows that a tile attends whose last token is t_last.
 template <Mode kMode>
 __device__ __forceinline__ int tile_rows(const PoolArgs& a, int cached, int length, int last) {
-  const int64_t rows = kMode == kOne ? (int64_t)cached + 1
-                       : kMode == kCausal ? (int64_t)cached + last + 1
-                                         : (int64_t)cached + min(length, 64);
+  const int64_t rows = (int64_t)cached + (kMode == kCausal ? last + 1 : min(length, 64));
   return (int)min(rows, (int64_t)a.attend_max);
 }
 // Rows of each of a request's splits, where one has at most `most`: of a size, to a round of the waves.  (None is empty: with
@@ -171,13 +161,12 @@ __device__ __forceinline__ int rows_of_split(int rows, int most) {
   const int n = (rows - 1) / most + 1;
   return n == 1 ? rows : ((rows - 1) / n / kRound + 1) * kRound;
 }
-template <Mode kMode>
 __device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
   Chunk c;
   c.n = i;
-  c.first = kMode == kOne ? i : ldg(a.offsets + i);
-  c.end = kMode == kOne ? i + 1 : min(ldg(a.offsets + i + 1), a.tokens);
-  c.cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)(kMode == kOne ? a.max_rows - 1 : a.max_rows));
+  c.first = ldg(a.offsets + i);
+  c.end = min(ldg(a.offsets + i + 1), a.tokens);
+  c.cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
   return c;
 }
 // Items go to the XCDs in stretches, a piece's heads side by side and the tiles that read the same rows next: the heads of a
@@ -192,7 +181,7 @@ __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c,
   uint32_t most = (uint32_t)c.split_rows;
   int j, rows;  // the tile; rows of a split
   if (a.requests <= 64) {
-    const Chunk mine = request_at<kMode>(a, min(lane_id(), a.requests - 1));
+    const Chunk mine = request_at(a, min(lane_id(), a.requests - 1));
     const bool some = lane_id() < a.requests && mine.first >= 0 && mine.first < mine.end;
     const int length = some ? mine.end - mine.first : 0;
     const int tiles = (length + (1 << kLog2) - 1) >> kLog2;
@@ -216,10 +205,11 @@ __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c,
       if (row < (uint32_t)all) pieces += tiles - before(row, mine.cached), row += my_rows;
     const int upto = wave_scan_i(pieces), total = __builtin_amdgcn_readlane(upto, 63);
     if (c.splits > 1 && blockIdx.x == 0) stg(most_rows, (int)most);
-    const int per = (total * a.heads + 7) / 8, item = xcd * per + turn;
-    if (turn >= per || item >= total * a.heads) return false;
+    const int per = (total * a.heads + 7) / 8, item = c.round ? turn : xcd * per + turn;
     int left = c.by_heads(item);
     p.head = item - left * a.heads;
+    if (c.round) left = left * 8 + xcd;
+    if (left >= total || (!c.round && turn >= per)) return false;
     const int at = __popcll(__ballot(upto <= left));  // the request whose pieces reach past it
     left -= __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(pieces, at);
     p.n = at;
@@ -590,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   const float c = a.scale * 1.44269504f;
   const int my_t = min(w.t0 + (lane & 31), w.t_last);
   // rows below `all` are attended by every query of the tile
-  const int all = min(stop, kMode == kOne ? stop : kMode == kCausal ? w.cached + (w.t0 - w.first) + 1 : w.cached);
+  const int all = min(stop, kMode == kCausal ? w.cached + (w.t0 - w.first) + 1 : w.cached);
   const int limit = kMode == kCausal ? min(w.cached + (my_t - w.first) + 1, stop) : stop;
   uint64_t visible = 0;
   if constexpr (kMode == kTree) visible = (uint64_t)ldg(a.visible + my_t);
@@ -737,12 +727,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
 //   keys    [block 2][step 8][slot 64][8], slot (32 half + row) ^ step: the columns 16 step + 8 half on.  (The exchange
 //           spreads a row's steps, which 8 lanes write at once, over the banks.)
 //   values  [block 2][step 2][u 4][lane 64][8]: as value_row has them, column 4 (lane % 32) + u.
-#ifndef UOCR_TILE_WAVES
-#define UOCR_TILE_WAVES 8
-#endif
-constexpr int kTileWaves = UOCR_TILE_WAVES, kTileThreads = kTileWaves * kWave, kTileLog2 = kTileWaves == 8 ? 8 : 7;
-constexpr int kTileRows = 8 * kTileWaves;
-constexpr int kTileBlocks = kTileRows / kBlock;
+constexpr int kTileWaves = 8, kTileThreads = kTileWaves * kWave, kTileLog2 = 8;
+constexpr int kTileRows = 2 * kBlock;
 constexpr int kTileHalves = kTileRows * kD;  // numbers of a tile's keys, or values
 
 struct TileRaw {  // a thread's part of 64 rows: 16 bytes of a key, 4 of 4 values, and a scale
@@ -771,7 +757,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
   const auto load = [&](TileRaw& r, int row0) {
     const int last = a.max_rows - kBlock;  // (rows past the table's are asked for nowhere)
     const char* lower = slots_at(min(row0, last));
-    const char* upper = kTileBlocks > 1 ? slots_at(min(row0 + kBlock, last)) : lower;
+    const char* upper = slots_at(min(row0 + kBlock, last));
     const char* mine = key < kBlock ? lower : upper;
     r.k = *(const UOCR_GLOBAL u32x4*)(mine + (uint32_t)((key % kBlock) * a.slot_bytes + head * kD + 16 * chunk));
     const char* from = (v_block == 0 ? lower : upper) + a.kv_bytes;
@@ -805,7 +791,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
     column(std::integral_constant<int, 1>{});
     column(std::integral_constant<int, 2>{});
     column(std::integral_constant<int, 3>{});
-    if (wave < 2) scales[buf][wave][lane % kTileRows] = wave == 0 ? r.scale * c : r.scale;
+    if (wave < 2) scales[buf][wave][lane] = wave == 0 ? r.scale * c : r.scale;
   };
   TileRaw raw;
   load(raw, w.begin);
@@ -903,19 +889,15 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
   };
-#ifndef UOCR_PRIO
-#define UOCR_PRIO 1
-#endif
-  if (wave < kTileWaves / 2) __builtin_amdgcn_s_setprio(UOCR_PRIO);
   int buf = 0;
 #pragma unroll 1
   for (int key0 = w.begin; key0 < stop; key0 += kTileRows, buf ^= 1) {
-    if (kTileBlocks > 1 && key0 < most) attend(key0, buf, 0);
+    if (key0 < most) attend(key0, buf, 0);
     if (key0 + kTileRows < stop) {
       convert(raw, buf ^ 1);
       if (key0 + 2 * kTileRows < stop) load(raw, key0 + 2 * kTileRows);
     }
-    if (key0 + kTileRows - kBlock < most) attend(key0 + kTileRows - kBlock, buf, kTileBlocks - 1);
+    if (key0 + kBlock < most) attend(key0 + kBlock, buf, 1);
     lds_barrier();
   }
   if (idle || t0 + (lane & 31) > w.t_last) return;
@@ -946,6 +928,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
 // score's three sums.
 constexpr int kOneWaves = 12;  // as many as have their registers on a CU
 constexpr int kOneParts = 16;  // columns of a lane
+
+// Rows that request n's token attends.
+__device__ __forceinline__ int one_rows(const PoolArgs& a, int n) {
+  return (int)min((int64_t)min(ldc(a.cache_lengths + n), (uint32_t)(a.max_rows - 1)) + 1, (int64_t)a.attend_max);
+}
 
 // The sum over the 8 lanes of a group; the largest.
 template <typename F>
@@ -1084,7 +1071,7 @@ __global__ void __launch_bounds__(kOneWaves * kWave) k_pool_one(Attend p) {
            (int64_t)(at % a.P) * a.slot_bytes;
   };
   const char* first_at = block_at(first);
-  const int all_rows = (int)min((int64_t)min(ldc(a.cache_lengths + n), (uint32_t)(a.max_rows - 1)) + 1, (int64_t)a.attend_max);
+  const int all_rows = one_rows(a, n);
   const uint32_t write = ldc(a.write_index + n);
   const int64_t src = (int64_t)n * a.in_stride + (int64_t)me.head * kD;
   const float *ct = nullptr, *st = nullptr;
@@ -1231,17 +1218,14 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p, bool ways) {
   const int64_t item = ways ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int64_t t = item / groups;
   if (t >= a.tokens) return;
-  Chunk c;
-  if constexpr (kMode == kOne)
-    c = request_at<kMode>(a, (int)t);
-  else if (!chunk_of(a, (int)t, c))
-    return;
-  const int i = (int)t - c.first, length = c.end - c.first;
-  const int t_last = min(((i >> kQueriesLog2) + 1) << kQueriesLog2, length) - 1;  // of its tile
-  int splits = 1;  // of its tile
+  int splits;  // of its tile
   if constexpr (kMode == kOne) {
-    splits = p.cuts.by_split(tile_rows<kMode>(a, c.cached, length, t_last) - 1) + 1;
+    splits = p.cuts.by_split(one_rows(a, (int)t) - 1) + 1;
   } else {
+    Chunk c;
+    if (!chunk_of(a, (int)t, c)) return;
+    const int i = (int)t - c.first, length = c.end - c.first;
+    const int t_last = min(((i >> kQueriesLog2) + 1) << kQueriesLog2, length) - 1;
     const int rows = rows_of_split(tile_rows<kMode>(a, c.cached, length, length - 1), ldg(p.most_rows));
     splits = (tile_rows<kMode>(a, c.cached, length, t_last) - 1) / rows + 1;
   }
@@ -1293,13 +1277,16 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p, bool ways) {
 // How a call's rows are cut.
 namespace {
 constexpr int kCus = 256, kStoredByReaders = 64;
-#ifndef UOCR_TILES
-#define UOCR_TILES (tokens / requests >= 256 && tokens * attend_max >= 3 << 20)
-#endif
+// Rows of a decode's split at least: two rounds of a wave's 32 rows, four of 16 (one request over 4000 rows 14.5 us in splits
+// of 704, 18.4 of 1408, 26 of 2816, on the device with the join; 24 over 1000 19 and, whole, 16).
+constexpr int kOneLeast = 704;
 PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
   PoolCuts c{};
   const bool one = form == kPoolDecode;
-  c.tiles = form == kPoolChunk && requests > 0 && UOCR_TILES;
+  // Tiles of 256 queries share a row's conversion, and fill the device where there are many of them or their rows are many
+  // (one chunk of 2048 over no rows 76 us against 87, over 14001 450 against 604; 512 over 14000 123 and 138; but 256 over
+  // 14000 82 and 79, eight of 512 over none 46 and 37).
+  c.tiles = form == kPoolChunk && requests > 0 && tokens / requests >= 256 && tokens * attend_max >= 3 << 20;
   const int queries = c.tiles ? 1 << kTileLog2 : kQueries;
   const int64_t tiles = one || requests <= 64 ? (tokens < requests ? tokens : (tokens - requests) / queries + requests)
                                               : tokens / queries + requests;
@@ -1308,10 +1295,9 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
   c.groups = one && !c.few ? (heads + 1) / 2 : heads;
   c.split_rows = attend_max;
   if (one) {
-    // as many splits as fill the device once, of a few rounds of the waves
+    // as many splits as fill the device once, one workgroup a CU
     const int64_t splits = std::max<int64_t>(1, kCus / std::max<int64_t>(1, requests * c.groups));
-    const int round = c.few ? UOCR_ONE_FEW * 11 * 32 : UOCR_ONE_ROUND * 11 * 16;
-    c.split_rows = (int)std::max<int64_t>(round, ((attend_max + splits - 1) / splits + round - 1) / round * round);
+    c.split_rows = (int)std::max<int64_t>(kOneLeast, ((attend_max + splits - 1) / splits + kOneLeast - 1) / kOneLeast * kOneLeast);
   } else if (attend_max <= 512) {
     // two splits of 256 rows and their join take the time of one of 512, and a launch more
     c.split_rows = 512;
@@ -1329,6 +1315,9 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
       c.split_rows = (int)std::max<int64_t>(2 * kRound, ((counts ? longest / 2 : longest) + kRound - 1) / kRound * kRound);
     }
   }
+  // Pieces that are not cut are as long as their requests: stretches of them would leave XCDs without work (64 chunks of 64
+  // over 333 to 1000 rows 90 us, 71 round the XCDs; 32 over 1333 to 4000 168 and 120).
+  c.round = form == kPoolChunk && requests <= 64 && c.fill == 0;
   c.splits = (int)(((int64_t)attend_max + c.split_rows - 1) / c.split_rows);
   c.by_split = divide_by(c.split_rows);
   c.by_heads = divide_by(c.groups);
