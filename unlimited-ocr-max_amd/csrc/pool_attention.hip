@@ -1367,7 +1367,7 @@ hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
 
 size_t pool_workspace_bytes(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
   const PoolCuts c = cuts_of(tokens, requests, heads, attend_max, form);
-  return c.splits > 1 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) + sizeof(int) : 0;
+  return c.splits > 1 && tokens > 0 ? (size_t)c.splits * tokens * heads * (kD + 2) * sizeof(float) + sizeof(int) : 0;
 }
 
 hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s) {
