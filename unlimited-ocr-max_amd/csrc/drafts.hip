@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kWave) k_draft_masks(int64_t* masks, const int
 // itself (a step is a broadcast and a ballot).  Each row moves towards the front and the path ascends, so a thread
 // reads every row before it is overwritten.
 constexpr int kAtOnce = 8;  // rows whose loads are under way together
-__global__ void __launch_bounds__(kThreads) k_accept_drafts(AcceptDrafts p) {
+__global__ void __launch_bounds__(kThreads) k_accept_drafts(AcceptDrafts p, Divide by_page) {
   const int n = (int)blockIdx.x, lane = lane_id();
   const Request q = request_of(p.offsets, n, p.tokens);
   const int length = q.first < 0 ? 0 : max(q.end - q.first, 0);
@@ -90,31 +90,24 @@ __global__ void __launch_bounds__(kThreads) k_accept_drafts(AcceptDrafts p) {
   const int64_t plane = (int64_t)blockIdx.y * p.page_size * p.slot_bytes + 16 * (int64_t)piece;
   const int64_t page_bytes = 2 * (int64_t)p.layers * p.page_size * p.slot_bytes;
   const auto row = [&](int r) {
-    const uint32_t page = min(ldc(p.lookup + (int64_t)n * p.lookup_cols + r / p.page_size), (uint32_t)(p.pages - 1));
-    return p.pool + (int64_t)page * page_bytes + plane + (int64_t)(r % p.page_size) * p.slot_bytes;
+    const int col = by_page(r);
+    const uint32_t page = min(ldc(p.lookup + (int64_t)n * p.lookup_cols + col), (uint32_t)(p.pages - 1));
+    return p.pool + (int64_t)page * page_bytes + plane + (int64_t)(r - col * p.page_size) * p.slot_bytes;
   };
-  // nodes that are where they belong already come first; rows that the table does not address last
+  // nodes that are where they belong already come first; rows that the table does not address stay
   int i = path == ~0ull ? kNodes : __builtin_ctzll(~path);
   uint64_t left = i == kNodes ? 0 : path >> i << i;
-  while (left != 0) {
+  if (p.max_rows - cached < kNodes) left &= (1ull << (p.max_rows - cached)) - 1;
+  for (int rows = __popcll(left); rows > 0; rows -= kAtOnce, i += kAtOnce) {
     f32x4 v[kAtOnce];
-    char* to[kAtOnce];
-    int some = 0;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {  // (behind the last row, the last again)
+      v[u] = *(const UOCR_GLOBAL f32x4*)row(cached + __builtin_ctzll(left));
+      left = (left & (left - 1)) != 0 ? left & (left - 1) : left;
+    }
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
-      if (left != 0) {
-        const int from = cached + __builtin_ctzll(left);
-        left &= left - 1;
-        if (from < p.max_rows) {
-          v[u] = *(const UOCR_GLOBAL f32x4*)row(from);
-          to[u] = row(cached + i + u);
-          some = u + 1;
-        }
-      }
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u)
-      if (u < some) *(UOCR_GLOBAL f32x4*)to[u] = v[u];
-    i += kAtOnce;
+      if (u < rows) *(UOCR_GLOBAL f32x4*)row(cached + i + u) = v[u];
   }
 }
 
@@ -130,7 +123,7 @@ hipError_t launch_draft_masks(int64_t* masks, const int32_t* parents, const int3
 hipError_t launch_accept_drafts(const AcceptDrafts& p, int requests, hipStream_t s) {
   if (requests == 0) return hipSuccess;
   const dim3 grid((unsigned)requests, (unsigned)(2 * p.layers), (unsigned)((p.slot_bytes / 16 + kThreads - 1) / kThreads));
-  UOCR_LAUNCH("accept_drafts", k_accept_drafts, grid, dim3(kThreads), 0, s, p);
+  UOCR_LAUNCH("accept_drafts", k_accept_drafts, grid, dim3(kThreads), 0, s, p, divide_by(p.page_size));
   return hipGetLastError();
 }
 

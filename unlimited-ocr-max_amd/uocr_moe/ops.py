@@ -823,8 +823,13 @@ def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tenso
     chunk, at the front of its words, -1 behind; int32 ``[N]`` the answer to the last (-1: an empty chunk); the cached rows
     now, as ``kv.cache_lengths``.  Of a chunk the first 64 tokens count."""
     op = "accept_drafts"
-    blocks = _pool(op, kv.kv_blocks)
-    pages, _, layers, page_size, heads, head_dim = blocks.shape
+    if isinstance(kv.kv_blocks, torch.Tensor) and kv.kv_blocks.dtype is torch.int8:
+        blocks = _int8_pool(op, kv.kv_blocks)
+        pages, _, layers, page_size, slot = blocks.shape
+    else:
+        blocks = _pool(op, kv.kv_blocks)
+        pages, _, layers, page_size, heads, head_dim = blocks.shape
+        slot = 4 * heads * head_dim
     lookup = _ids(op, "lookup_table", kv.lookup_table, 2)
     cached = _ids(op, "cache_lengths", kv.cache_lengths, 1)
     offsets = _gpu(op, "chunk_offsets", kv.chunk_offsets, torch.int32, 1)
@@ -839,7 +844,7 @@ def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tenso
     counts, following, lengths, path = parents.new_empty(3 * n + total).split([n, n, n, total])
     if cached.dtype is torch.uint32:
         lengths = lengths.view(torch.uint32)
-    _on_device(op, "uocr_accept_drafts", blocks.data_ptr(), pages, layers, page_size, 4 * heads * head_dim,
+    _on_device(op, "uocr_accept_drafts", blocks.data_ptr(), pages, layers, page_size, slot,
                lookup.data_ptr(), n, lookup.shape[1], cached.data_ptr(), offsets.data_ptr(), parents.data_ptr(),
                tokens.data_ptr(), answers.data_ptr(), total, counts.data_ptr(), path.data_ptr(), following.data_ptr(),
                lengths.data_ptr(), tensors=(blocks, lookup, cached, offsets, parents, tokens, answers))
