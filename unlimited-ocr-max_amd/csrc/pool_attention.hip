@@ -1278,7 +1278,9 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p, bool ways) {
 namespace {
 constexpr int kCus = 256, kStoredByReaders = 64;
 // Rows of a decode's split at least: two rounds of a wave's 32 rows, four of 16 (one request over 4000 rows 14.5 us in splits
-// of 704, 18.4 of 1408, 26 of 2816, on the device with the join; 24 over 1000 19 and, whole, 16).
+// of 704, 18.4 of 1408, 26 of 2816, on the device with the join; but 24 over 1000 19 in two and 16 whole).  Equal shares of
+// all requests' rows instead, whose workgroups go from one request to the next: no faster (24 over 1447 to 4000 46 us both
+// ways), as the rows are bound by their loads and not by the longest request.
 constexpr int kOneLeast = 704;
 PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
   PoolCuts c{};
@@ -1295,8 +1297,8 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
   c.groups = one && !c.few ? (heads + 1) / 2 : heads;
   c.split_rows = attend_max;
   if (one) {
-    // as many splits as fill the device once, one workgroup a CU
-    const int64_t splits = std::max<int64_t>(1, kCus / std::max<int64_t>(1, requests * c.groups));
+    // As many splits as fill the device once, one workgroup a CU; with two heads a wave a few more rounds take less than a join.
+    const int64_t splits = !c.few && attend_max <= 2 * kOneLeast ? 1 : std::max<int64_t>(1, kCus / std::max<int64_t>(1, requests * c.groups));
     c.split_rows = (int)std::max<int64_t>(kOneLeast, ((attend_max + splits - 1) / splits + kOneLeast - 1) / kOneLeast * kOneLeast);
   } else if (attend_max <= 512) {
     // two splits of 256 rows and their join take the time of one of 512, and a launch more
