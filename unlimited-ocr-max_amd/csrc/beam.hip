@@ -132,7 +132,9 @@ struct BeamWork {  // of each row's pieces: the largest logit and the sum, the b
 };
 
 // A workgroup has a piece of a row: its largest logit, its sum of exponentials, and its best K tokens.  Rows begin at any
-// float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.
+// float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.  Bound by memory where
+// rows are many (512 of 129280: 45 us, 5.9 TB/s), else by its trip there and the two passes over a thread's tokens (4 rows:
+// 5.6 us).
 template <int kPer>
 __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWork w) {
   __shared__ Best<float, int, kRowThreads> best;
@@ -196,7 +198,8 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWor
 
 __device__ __attribute__((noinline)) double full_exp(double x) { return exp(x); }
 
-// A workgroup has a request: its beams' sums, their candidates, and the states of the chosen ones.
+// A workgroup has a request: its beams' sums, their candidates, and the states of the chosen ones.  Bound by its dependent steps
+// (sums, candidates, chosen, states): 6.7 us for one request of 4 beams, 11 for 64 of 8.
 __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWork w) {
   __shared__ Best<double, int64_t, kJoinThreads> best;
   __shared__ double sums[kBeamsMost], scores[kBeamsMost], by[kBeamsMost];

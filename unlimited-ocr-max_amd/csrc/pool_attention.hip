@@ -117,7 +117,7 @@ __device__ __forceinline__ void store_row(const PoolArgs& a, int n, int row, int
   }
 }
 
-// One wave per (token, 4 heads), which waits for the request's words once.  Queries that come before RoPE are rotated where
+// One wave per (token, 4 heads), which waits for the request's words once.  Bound by memory: 2900 tokens of ten heads in 10 us, 3.6 TB/s.  Queries that come before RoPE are rotated where
 // they are read.
 constexpr int kStoreHeads = 4;
 template <bool kInt8>
@@ -503,7 +503,11 @@ __device__ __forceinline__ uint32_t take_infinite(Stage<false>& v) {
   return bad;
 }
 
-// 32 queries of a head, whose rows' blocks the workgroup's waves take in turn and whose sums they join in LDS.
+// 32 queries of a head, whose rows' blocks the workgroup's waves take in turn and whose sums they join in LDS.  Every wave
+// converts its own rows, from registers to registers: what it waits for is the next block's loads, and two workgroups on a CU
+// wait in turn.  Of few rows bound by the trips to memory before the first block (15 tokens over 300 int8 rows 15 us); of
+// many by the conversions and products, which take about as long as one another (eight trees of 26 to 61 over 1667 to 4000
+// rows: int8 35 us, 1.7 TB/s; fp32, with twice the products and three times the conversions, 80 us, 2.9 TB/s).
 template <bool kInt8, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
   const PoolArgs& a = p.a;
@@ -723,7 +727,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
 //
 // 256 queries of a head, 32 a wave.  Bound by the matrix instruction: a block of 32 rows is 48 of them a wave, beside some
 // 200 other instructions for the scores, and with one row's conversion shared by 8 waves those fit under them (two waves a
-// SIMD, the one's products under the other's exponentials).  64 rows are in LDS as operands, the next 64 on their way:
+// SIMD, the one's products under the other's exponentials): 2048 queries over 14001 rows 430 to 470 us as the card's clock
+// goes, 1.0 to 1.1 PFLOP/s of bf16 products beside 1.24 of a large matrix product.  64 rows are in LDS as operands, the next 64 on their way:
 //   keys    [block 2][step 8][slot 64][8], slot (32 half + row) ^ step: the columns 16 step + 8 half on.  (The exchange
 //           spreads a row's steps, which 8 lanes write at once, over the banks.)
 //   values  [block 2][step 2][u 4][lane 64][8]: as value_row has them, column 4 (lane % 32) + u.
@@ -925,7 +930,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
 // are fp32 multiply-adds on converted bytes, two instructions a byte, which at 64 lanes a clock is 32 bytes a clock of a
 // CU, three times what memory brings.  8 lanes have a row, 16 columns each, of the keys as of the values, so a row's weight
 // is where its values are: every group of 8 lanes has a softmax of its own, and nothing crosses lanes in the loop but a
-// score's three sums.
+// score's three sums.  Bound by the trips to memory where rows are few (one request of 640 rows: 11 us), and by how many
+// loads a CU has under way where they are many (24 of 1445 to 4000: 46 us, 3.8 TB/s).  A row's scale is 4 bytes of a line of
+// its own: with one head a wave the lines cost a fifth of the time, so two heads share them where workgroups are many.
 constexpr int kOneWaves = 12;  // as many as have their registers on a CU
 constexpr int kOneParts = 16;  // columns of a lane
 
@@ -1208,7 +1215,8 @@ __global__ void __launch_bounds__(kOneWaves * kWave) k_pool_one(Attend p) {
 }
 
 // Joins the splits of a token's rows: half a wave a (token, head), four columns a lane.  Of many splits (`ways`) the four waves
-// of a workgroup take every fourth: one wave would wait for the memory every few of them.
+// of a workgroup take every fourth: one wave would wait for the memory every few of them (8 tokens over 14000 rows, 37 splits:
+// 21 us, 7 by four waves).
 constexpr int kJoinAtOnce = 4;
 template <Mode kMode, int kQueriesLog2>
 __global__ void __launch_bounds__(256) k_pool_join(Attend p, bool ways) {
@@ -1279,7 +1287,7 @@ namespace {
 constexpr int kCus = 256, kStoredByReaders = 64;
 // Rows of a decode's split at least: two rounds of a wave's 32 rows, four of 16 (one request over 4000 rows 14.5 us in splits
 // of 704, 18.4 of 1408, 26 of 2816, on the device with the join; but 24 over 1000 19 in two and 16 whole).  Equal shares of
-// all requests' rows instead, whose workgroups go from one request to the next: no faster (24 over 1447 to 4000 46 us both
+// all requests' rows instead, whose workgroups go from one request to the next: no faster (24 over 1445 to 4000 46 us both
 // ways), as the rows are bound by their loads and not by the longest request.
 constexpr int kOneLeast = 704;
 PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, PoolForm form) {
