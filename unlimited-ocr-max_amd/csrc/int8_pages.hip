@@ -11,9 +11,9 @@ constexpr int kD = 128;
 constexpr int kRows = 16;    // rows of a workgroup: four of each wave
 constexpr int kAtOnce = 5;   // pairs of heads whose loads are under way together
 
-// Bound by memory: 24 pages over 12 layers in 106 us, 4.5 TB/s read and written; back, 5 pages in 10 us.  Half a wave has a head's row, four values a lane: 512 contiguous bytes of the fp32 pool and 128 of
-// the int8 one a head.  Pairs count as if one were converted after the other: rows of a page that a later pair writes
-// too are left to it.
+// Bound by memory: 24 pages over 12 layers in 106 us, 4.5 TB/s read and written; back, 5 half pages in 10 us.  Half a wave has
+// a head's row, four values a lane: 512 contiguous bytes of the fp32 pool and 128 of the int8 one a head.  Pairs count as if
+// one were converted after the other: rows of a page that a later pair writes too are left to it.
 template <bool kQuantize>
 __global__ void __launch_bounds__(kThreads) k_convert_pages(ConvertPages p) {
   __shared__ int later;

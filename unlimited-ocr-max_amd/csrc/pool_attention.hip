@@ -117,8 +117,8 @@ __device__ __forceinline__ void store_row(const PoolArgs& a, int n, int row, int
   }
 }
 
-// One wave per (token, 4 heads), which waits for the request's words once.  Bound by memory: 2900 tokens of ten heads in 10 us, 3.6 TB/s.  Queries that come before RoPE are rotated where
-// they are read.
+// One wave per (token, 4 heads), which waits for the request's words once.  Bound by memory: 2900 tokens of ten heads in 10 us,
+// 3.6 TB/s.  Queries that come before RoPE are rotated where they are read.
 constexpr int kStoreHeads = 4;
 template <bool kInt8>
 __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
@@ -199,7 +199,9 @@ __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c,
     }
     const int my_rows = rows_of_split(all, (int)most);
     // tiles whose last query comes before the row
-    const auto before = [&](uint32_t row, int cached) { return kMode == kCausal && (int)row > cached ? ((int)row - cached) >> kLog2 : 0; };
+    const auto before = [&](uint32_t row, int cached) {
+      return kMode == kCausal && (int)row > cached ? ((int)row - cached) >> kLog2 : 0;
+    };
     int pieces = tiles;
     for (uint32_t row = my_rows; __ballot(row < (uint32_t)all) != 0;)
       if (row < (uint32_t)all) pieces += tiles - before(row, mine.cached), row += my_rows;
@@ -545,7 +547,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
     if (a.stores) {
       // The new rows that this workgroup reads, and of its tile's tokens those that none does.  (Workgroups that read the
       // same rows store the same bits.)
-      for (int r = max(w.begin, w.cached) + wave; r < stop; r += kWaves) store_row<kInt8, 1>(a, w.n, r, w.first + (r - w.cached), head);
+      for (int r = max(w.begin, w.cached) + wave; r < stop; r += kWaves)
+        store_row<kInt8, 1>(a, w.n, r, w.first + (r - w.cached), head);
       if (w.split == 0)
         for (int t = w.t0 + wave; t <= w.t_last; t += kWaves) {
           const int64_t r = (int64_t)w.cached + (t - w.first);
@@ -728,7 +731,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
 // 256 queries of a head, 32 a wave.  Bound by the matrix instruction: a block of 32 rows is 48 of them a wave, beside some
 // 200 other instructions for the scores, and with one row's conversion shared by 8 waves those fit under them (two waves a
 // SIMD, the one's products under the other's exponentials): 2048 queries over 14001 rows 430 to 470 us as the card's clock
-// goes, 1.0 to 1.1 PFLOP/s of bf16 products beside 1.24 of a large matrix product.  64 rows are in LDS as operands, the next 64 on their way:
+// goes, 1.0 to 1.1 PFLOP/s of bf16 products beside 1.24 of a large matrix product.  64 rows are in LDS as operands, the next
+// 64 on their way:
 //   keys    [block 2][step 8][slot 64][8], slot (32 half + row) ^ step: the columns 16 step + 8 half on.  (The exchange
 //           spreads a row's steps, which 8 lanes write at once, over the banks.)
 //   values  [block 2][step 2][u 4][lane 64][8]: as value_row has them, column 4 (lane % 32) + u.
@@ -1306,7 +1310,8 @@ PoolCuts cuts_of(int64_t tokens, int64_t requests, int heads, int attend_max, Po
   c.split_rows = attend_max;
   if (one) {
     // As many splits as fill the device once, one workgroup a CU; with two heads a wave a few more rounds take less than a join.
-    const int64_t splits = !c.few && attend_max <= 2 * kOneLeast ? 1 : std::max<int64_t>(1, kCus / std::max<int64_t>(1, requests * c.groups));
+    const int64_t fill = kCus / std::max<int64_t>(1, requests * c.groups);
+    const int64_t splits = !c.few && attend_max <= 2 * kOneLeast ? 1 : std::max<int64_t>(1, fill);
     c.split_rows = (int)std::max<int64_t>(kOneLeast, ((attend_max + splits - 1) / splits + kOneLeast - 1) / kOneLeast * kOneLeast);
   } else if (attend_max <= 512) {
     // two splits of 256 rows and their join take the time of one of 512, and a launch more
@@ -1338,11 +1343,12 @@ template <bool kInt8, Mode kMode>
 hipError_t launch(const PoolAttention& p, const PoolArgs& a, hipStream_t s) {
   const PoolCuts c = cuts_of(p.tokens, p.requests, p.heads, p.attend_max, form_of(kMode));
   const int64_t pairs = p.tokens * p.heads;
-  const int64_t pieces = c.fill > 0 ? std::max(c.fill, c.slots) : (int64_t)c.slots * c.splits, items = (pieces + 7) / 8 * 8 * c.groups;
+  const int64_t pieces = c.fill > 0 ? std::max(c.fill, c.slots) : (int64_t)c.slots * c.splits;
+  const int64_t items = (pieces + 7) / 8 * 8 * c.groups;
   const int64_t joins = p.tokens * ((p.heads + 1) / 2);
   // (where a wave counts the pieces, offsets that do not ascend may give each request all of them)
-  if (pieces > INT32_MAX / c.groups - 8 || (int64_t)c.slots * c.splits * c.groups > INT32_MAX / std::min<int64_t>(p.requests, 64) - 8)
-    return hipErrorInvalidValue;
+  const int64_t most = (int64_t)c.slots * c.splits * c.groups;
+  if (pieces > INT32_MAX / c.groups - 8 || most > INT32_MAX / std::min<int64_t>(p.requests, 64) - 8) return hipErrorInvalidValue;
   const Attend at{a, c, (float*)p.workspace, (float*)p.workspace + (int64_t)c.splits * pairs * kD,
                   (int*)((float*)p.workspace + (int64_t)c.splits * pairs * (kD + 2))};
   const dim3 grid((unsigned)items);
