@@ -227,3 +227,42 @@ def test_two_calls_at_once() -> None:
         stored = s.stored(1, k, v)
         assert torch.equal(pool.cpu(), stored)
         assert far(out.cpu(), _want(s, stored, q)) <= BAR
+
+
+@pytest.mark.parametrize("int8", [True, False], ids=["int8", "fp32"])
+@pytest.mark.parametrize("chunks", [[16] * 8, [17] + [16] * 7, [32] * 4, [33] * 3, [128] + [0] * 3, [97] + [1] * 31, [1] * 128],
+                         ids=lambda v: f"{sum(v)}-{len(v)}")
+def test_either_side_of_rows_stored_by_their_readers(chunks, int8) -> None:
+    """Up to 128 tokens, 32 a request on average; one request may have most of them."""
+    u = _uocr()
+    s = Served(len(chunks), chunks, [(37 * i) % 150 for i in range(len(chunks))], heads=3, int8=int8, lead=1, tail=2)
+    q, k, v = s.qkv.unbind(1)
+    stored = s.stored(1, k, v)
+    bits = [signed((b & (1 << 64) - 1)) for c in chunks for b in masks_of([j - 1 for j in range(c)])]
+    visible = _on([0] + bits + [0, 0], torch.int64)
+    pool, out = s.pool.to(DEV), torch.full((s.tokens, 3, D), 7.0, device=DEV)
+    u.paged_chunk_attention(q.to(DEV), k.to(DEV), v.to(DEV), kv=_chunk(s, pool, None if int8 else visible), layer_idx=1,
+                            scale=SCALE, out=out)
+    assert torch.equal(pool.cpu(), stored)
+    assert bool((out[:1] == 7).all()) and bool((out[-2:] == 7).all())
+    want = _want(s, stored, q)
+    if not int8:  # a tree's tokens past the first 64 see the first 64 alone
+        seen = [min(j, 63) for c in chunks for j in range(c)]
+        keep = torch.tensor([True] + [x == j for x, j in zip(seen, (j for c in chunks for j in range(c)))] + [True] * 2)
+        want, out = want[keep], out[keep.to(DEV)]
+    assert far(out[1:-2].cpu(), want[1:-2]) <= BAR
+
+
+@pytest.mark.parametrize("chunk", [7, 40, 130])
+def test_rows_past_what_is_attended_are_stored(chunk) -> None:
+    """An attend_max below the last rows: all new rows are stored, those below it are attended."""
+    u = _uocr()
+    s = Served(chunk, [chunk], [300], heads=3)
+    q, k, v = s.qkv.unbind(1)
+    stored = s.stored(1, k, v)
+    for most in (302, 300, 128):
+        pool = s.pool.to(DEV)
+        got = u.paged_chunk_attention(q.to(DEV), k.to(DEV), v.to(DEV), kv=_chunk(s, pool, attend_max=most), layer_idx=1, scale=SCALE)
+        assert torch.equal(pool.cpu(), stored)
+        want = s.want(stored, 1, q, seen=lambda i, j: list(range(min(300 + j + 1, most))))
+        assert far(got.cpu(), want) <= BAR

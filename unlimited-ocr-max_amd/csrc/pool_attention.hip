@@ -72,47 +72,63 @@ __device__ __forceinline__ char* slot_of(const PoolArgs& a, int n, int r) {
   return a.pool + (int64_t)page * a.page_bytes + a.layer_bytes + (int64_t)(r % a.P) * a.slot_bytes;
 }
 
-// Stores token t's k and v of the kHeads heads from h0 on as row `row` of request n: half of the wave has the key, half the
-// value, a lane 4 columns.
-template <bool kInt8, int kHeads>
-__device__ __forceinline__ void store_row(const PoolArgs& a, int n, int row, int t, int h0) {
+// Stores k and v of kItems (token, head) pairs as rows of request n, whose loads are under way together: token t's heads from h0
+// on as row `row` (kOf == kHeads), or head h0 of the tokens t, t + kWaves, ... below `end` as the rows row, row + kWaves, ...
+// Half of the wave has the key, half the value, a lane 4 columns.
+enum Items { kHeads, kTokens };
+template <bool kInt8, Items kOf, int kItems>
+__device__ __forceinline__ void store_rows(const PoolArgs& a, int n, int row, int t, int end, int h0) {
 #pragma clang fp contract(off)
   const int lane = lane_id(), c = lane & 31;
   const bool key = lane < 32, turn = a.rope.positions != nullptr;
-  const float* x = (key ? a.k_new : a.v_new) + (int64_t)t * a.in_stride + 4 * c;
-  f32x4 y[kHeads], pair[kHeads];  // the pair of column d is d +- 64
+  const float* x = (key ? a.k_new : a.v_new) + 4 * c;
+  f32x4 y[kItems], pair[kItems];  // the pair of column d is d +- 64
+  int pos[kItems];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int64_t at = (int64_t)min(h0 + i, a.heads - 1) * kD;
+  for (int i = 0; i < kItems; ++i) {
+    const int ti = kOf == kHeads ? t : min(t + i * kWaves, end - 1), h = kOf == kHeads ? min(h0 + i, a.heads - 1) : h0;
+    const int64_t at = (int64_t)ti * a.in_stride + (int64_t)h * kD;
     y[i] = *(const UOCR_GLOBAL f32x4*)(x + at);
-    if (turn) pair[i] = *(const UOCR_GLOBAL f32x4*)(x + at + (c < 16 ? 64 : -64));
+    if (turn) {
+      pair[i] = *(const UOCR_GLOBAL f32x4*)(x + at + (c < 16 ? 64 : -64));
+      pos[i] = kOf == kTokens || i == 0 ? min(max(ldg(a.rope.positions + ti), 0), a.rope.table_rows - 1) : pos[0];
+    }
   }
-  char* slot = slot_of(a, n, row) + (key ? 0 : a.kv_bytes);
-  if (turn) {
-    const int64_t at = (int64_t)min(max(ldg(a.rope.positions + t), 0), a.rope.table_rows - 1) * kD + 4 * c;
-    const f32x4 cs = *(const UOCR_GLOBAL f32x4*)(a.rope.cos_t + at), sn = *(const UOCR_GLOBAL f32x4*)(a.rope.sin_t + at);
+  char* slot[kItems];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i)
+  for (int i = 0; i < kItems; ++i)
+    slot[i] = kOf == kHeads && i > 0 ? slot[0]
+                                     : slot_of(a, n, kOf == kHeads ? row : min(row + i * kWaves, row + (end - 1 - t))) + (key ? 0 : a.kv_bytes);
+  if (turn) {
+    f32x4 cs[kItems], sn[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int64_t at = (int64_t)pos[i] * kD + 4 * c;
+      cs[i] = kOf == kHeads && i > 0 ? cs[0] : *(const UOCR_GLOBAL f32x4*)(a.rope.cos_t + at);
+      sn[i] = kOf == kHeads && i > 0 ? sn[0] : *(const UOCR_GLOBAL f32x4*)(a.rope.sin_t + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float turned = y[i][e] * cs[e] + (c < 16 ? -pair[i][e] : pair[i][e]) * sn[e];
+        const float turned = y[i][e] * cs[i][e] + (c < 16 ? -pair[i][e] : pair[i][e]) * sn[i][e];
         y[i][e] = key ? turned : y[i][e];
       }
   }
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    if (h >= a.heads) break;
+  for (int i = 0; i < kItems; ++i) {
+    const int h = kOf == kHeads ? h0 + i : h0;
+    if (kOf == kHeads ? h >= a.heads : t + i * kWaves >= end) break;
     if constexpr (kInt8) {
       uint32_t most = max(max(abs_bits(y[i].x), abs_bits(y[i].y)), max(abs_bits(y[i].z), abs_bits(y[i].w)));
 #pragma unroll
       for (int off = 1; off <= 8; off *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, off, kWave));
       const float scale = row_scale(max(most, other<16>(most)));
       const uint32_t q = to_int8x4(y[i].x, y[i].y, y[i].z, y[i].w, scale);
-      stg((uint32_t*)(slot + h * kD) + c, q);
-      if (c == 0) stg((float*)(slot + a.heads * kD) + h, scale);
+      stg((uint32_t*)(slot[i] + h * kD) + c, q);
+      if (c == 0) stg((float*)(slot[i] + a.heads * kD) + h, scale);
     } else {
-      *(UOCR_GLOBAL f32x4*)((float*)slot + h * kD + 4 * c) = y[i];
+      *(UOCR_GLOBAL f32x4*)((float*)slot[i] + h * kD + 4 * c) = y[i];
     }
   }
 }
@@ -129,7 +145,7 @@ __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
   Chunk c;
   if (!chunk_of(a, t, c)) return;
   const int64_t row = (int64_t)c.cached + (t - c.first);
-  if (row < a.max_rows) store_row<kInt8, kStoreHeads>(a, c.n, (int)row, t, h0);  // else past what the lookup row addresses
+  if (row < a.max_rows) store_rows<kInt8, kHeads, kStoreHeads>(a, c.n, (int)row, t, t + 1, h0);  // else past what the lookup row addresses
 }
 
 // ------------------------------------------------------------------ which piece of the work a workgroup takes
@@ -547,13 +563,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_pool_attend(Attend p) {
     if (a.stores) {
       // The new rows that this workgroup reads, and of its tile's tokens those that none does.  (Workgroups that read the
       // same rows store the same bits.)
-      for (int r = max(w.begin, w.cached) + wave; r < stop; r += kWaves)
-        store_row<kInt8, 1>(a, w.n, r, w.first + (r - w.cached), head);
-      if (w.split == 0)
-        for (int t = w.t0 + wave; t <= w.t_last; t += kWaves) {
-          const int64_t r = (int64_t)w.cached + (t - w.first);
-          if (r >= unread && r < a.max_rows) store_row<kInt8, 1>(a, w.n, (int)r, t, head);
-        }
+      constexpr int kAtOnce = kInt8 ? 4 : 2;
+      const int behind = w.first - w.cached;  // of a row, its token
+      for (int r = max(w.begin, w.cached) + wave; r < stop; r += kAtOnce * kWaves)
+        store_rows<kInt8, kTokens, kAtOnce>(a, w.n, r, behind + r, behind + stop, head);
+      if (w.split == 0) {
+        // tokens of the tile whose rows no token attends
+        const int t0 = max(w.t0, behind + unread), end = (int)min((int64_t)w.t_last + 1, (int64_t)behind + a.max_rows);
+        for (int t = t0 + wave; t < end; t += kAtOnce * kWaves)
+          store_rows<kInt8, kTokens, kAtOnce>(a, w.n, t - behind, t, end, head);
+      }
       __syncthreads();
       if (first < stop && !early) {
         load_keys(k, a, from, head, stop - 1 - first, lane);
@@ -1288,7 +1307,7 @@ __global__ void __launch_bounds__(256) k_pool_join(Attend p, bool ways) {
 
 // How a call's rows are cut.
 namespace {
-constexpr int kCus = 256, kStoredByReaders = 64;
+constexpr int kCus = 256;
 // Rows of a decode's split at least: two rounds of a wave's 32 rows, four of 16 (one request over 4000 rows 14.5 us in splits
 // of 704, 18.4 of 1408, 26 of 2816, on the device with the join; but 24 over 1000 19 in two and 16 whole).  Equal shares of
 // all requests' rows instead, whose workgroups go from one request to the next: no faster (24 over 1445 to 4000 46 us both
@@ -1414,8 +1433,10 @@ hipError_t launch_pool_attention(const PoolAttention& p, hipStream_t s) {
   a.out = p.out;
   a.scale = p.scale;
   a.rope = Rope{p.positions, p.cos_table, p.sin_table, p.table_rows};
-  // Few new rows are stored by those that read them, which saves a launch; many would be stored again and again.
-  a.stores = p.tokens <= kStoredByReaders;  // (tiles have more tokens)
+  // Few new rows are stored by those that read them, which saves a launch; many would take a workgroup longer than that: 16
+  // a step (chunks of 8 over none, 16 of them, 8.1 us for 10.5; of 4 over 300 rows, 40, 16.2 for 18.5; but one of 100 over none
+  // 18.8 for 11.3).  Not each request's are known here, only all of them and their mean.
+  a.stores = p.tokens <= 128 && p.tokens <= 32 * p.requests;  // (tiles have more tokens)
   if (p.write_index != nullptr) return launch<true, kOne>(p, a, s);
   if (p.visible == nullptr) return launch<true, kCausal>(p, a, s);
   return p.int8 ? launch<true, kTree>(p, a, s) : launch<false, kTree>(p, a, s);
