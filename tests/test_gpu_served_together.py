@@ -360,3 +360,31 @@ def test_more_wrapper_refusals() -> None:
         u.accept_drafts(chunk, _on([-1, 0, 0, 0]), _on([1, 2, 3]), _on([1, 2, 3, 4]))
     with pytest.raises(ValueError, match="out must have 4 words"):
         u.draft_masks(_on([-1, 0, 0, 0]), _on([0, 4]), out=torch.zeros(3, dtype=torch.int64, device=DEV))
+
+
+def test_the_librarys_own_workspace(monkeypatch) -> None:
+    """Entries that are given no workspace take the library's: the results of calls with one."""
+    u = _uocr()
+    from uocr_moe import ops
+
+    g = torch.Generator().manual_seed(9)
+    calls = []
+    for tokens, cached in ((40, 3000), (600, 5000)):
+        cols = -(-(tokens + cached) // P)
+        pool = quantized(torch.randn(cols, 2, 1, P, HEADS, D, generator=g), 512)
+        qkv = torch.randn(tokens, 3, HEADS, D, generator=g).to(DEV)
+        for masks in (None, torch.full((tokens,), -1, dtype=torch.int64, device=DEV)):
+            calls.append(lambda pool=pool, qkv=qkv, masks=masks, tokens=tokens, cached=cached, cols=cols: u.paged_chunk_attention(
+                *qkv.unbind(1), layer_idx=0, scale=SCALE, kv=u.PagedChunk(
+                    kv_blocks=pool.to(DEV), lookup_table=_on([list(range(cols))]), cache_lengths=_on([cached]),
+                    chunk_offsets=_on([0, tokens]), attend_max=tokens + cached, visible=masks)))
+        calls.append(lambda pool=pool, qkv=qkv, cached=cached, cols=cols: u.paged_decode_attention(
+            *qkv[:1].unbind(1), layer_idx=0, scale=SCALE, kv=u.PagedKv(
+                kv_blocks=pool.to(DEV), lookup_table=_on([list(range(cols))]), attend_lengths=_on([cached]),
+                attend_max=cached + 1, write_index=_on([7]))))
+    logits = torch.randn(8, 5000, generator=g).to(DEV)
+    calls.append(lambda: torch.stack([x.float() for x in u.beam_select(logits, torch.zeros(8, device=DEV), beams=4, eos=0)[:4]]))
+    want = [call() for call in calls]
+    monkeypatch.setattr(ops, "_workspace", lambda *a: None)
+    for _ in range(2):
+        assert all(torch.equal(call(), x) for call, x in zip(calls, want))
