@@ -185,9 +185,9 @@ __device__ __forceinline__ Chunk request_at(const PoolArgs& a, int i) {
   c.cached = (int)min(ldg(a.cache_lengths + i), (uint32_t)a.max_rows);
   return c;
 }
-// Items go to the XCDs in stretches, a piece's heads side by side and the tiles that read the same rows next: the heads of a
-// row are neighbours in memory (an int8 pool's share the line of their scales), and their XCD reads the rows once.  (Pieces
-// that go round the XCDs: eight trees of 61 over 4000 rows 130 us for 110.)  Up to 64 requests every wave counts the pieces
+// Items go to the XCDs in stretches, the tiles that read the same rows of a head side by side and the heads next: their XCD
+// reads the rows once, and the heads of an int8 row share the line of their scales.  (Pieces that go round the XCDs: eight
+// trees of 61 over 4000 rows 130 us for 110.)  Up to 64 requests every wave counts the pieces
 // that there are, and cuts them so that the device is filled by them once: the host does not know the lengths (with splits
 // from the longest, eight trees over 1667 to 4000 rows 92 us for 81).  Of more requests, a piece is a slot, whose tile and
 // split may not exist.  most_rows: where the join finds the rows of a split.
@@ -223,13 +223,11 @@ __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c,
       if (row < (uint32_t)all) pieces += tiles - before(row, mine.cached), row += my_rows;
     const int upto = wave_scan_i(pieces), total = __builtin_amdgcn_readlane(upto, 63);
     if (c.splits > 1 && blockIdx.x == 0) stg(most_rows, (int)most);
-    const int per = (total * a.heads + 7) / 8, item = c.round ? turn : xcd * per + turn;
-    int left = c.by_heads(item);
-    p.head = item - left * a.heads;
-    if (c.round) left = left * 8 + xcd;
-    if (left >= total || (!c.round && turn >= per)) return false;
-    const int at = __popcll(__ballot(upto <= left));  // the request whose pieces reach past it
-    left -= __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(pieces, at);
+    const int per = (total * a.heads + 7) / 8;
+    const int turns = c.by_heads(turn), item = c.round ? turn + (7 * turns + xcd) * a.heads : xcd * per + turn;
+    if (item >= total * a.heads || (!c.round && turn >= per)) return false;
+    const int at = __popcll(__ballot(upto <= c.by_heads(item)));  // the request whose pieces reach past it
+    int left = item - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(pieces, at)) * a.heads;
     p.n = at;
     p.first = __builtin_amdgcn_readlane(mine.first, at);
     p.end = __builtin_amdgcn_readlane(mine.end, at);
@@ -237,12 +235,14 @@ __device__ __forceinline__ bool find_piece(const PoolArgs& a, const PoolCuts& c,
     rows = __builtin_amdgcn_readlane(my_rows, at);
     j = __builtin_amdgcn_readlane(tiles, at) - 1;
     p.split = 0;
+    int here;  // tiles that have the split
     for (uint32_t row = 0;; row += rows, ++p.split) {
-      const int here = j + 1 - before(row, p.cached);
-      if (left < here) break;
-      left -= here;
+      here = j + 1 - before(row, p.cached);
+      if (left < here * a.heads) break;
+      left -= here * a.heads;
     }
-    j -= left;
+    p.head = left / here;
+    j -= left - p.head * here;
   } else {
     const int item = xcd * (int)(gridDim.x / 8) + turn;
     const int cell = c.by_heads(item), slot = cell / c.splits;  // the splits of a tile one after the other
