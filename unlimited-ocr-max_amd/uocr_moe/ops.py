@@ -841,7 +841,7 @@ def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tenso
         raise ValueError(f"{op}: the chunks' metadata is not for {n} requests")
     if tokens.shape[0] != total or answers.shape[0] != total:
         raise ValueError(f"{op}: parents, tokens and answers must have one length")
-    counts, following, lengths, path = parents.new_empty(3 * n + total).split([n, n, n, total])
+    counts, following, lengths, path = parents.new_empty(3 * n + total).split_with_sizes([n, n, n, total])
     if cached.dtype is torch.uint32:
         lengths = lengths.view(torch.uint32)
     _on_device(op, "uocr_accept_drafts", blocks.data_ptr(), pages, layers, page_size, slot,
