@@ -464,6 +464,8 @@ def _pool_call(op: str, name: str, inputs: tuple, stride: int, heads: int, head_
     (lengths, offsets, visible or None) of the others."""
     like = inputs[0]
     tokens = like.shape[0]
+    if rope_at and rope_at[1].shape[1] != head_dim:  # the entries take tables of head_dim columns
+        raise ValueError(f"{op}: the cos/sin tables are {rope_at[1].shape[1]} wide, not head_dim {head_dim}")
     if blocks.dtype is torch.int8:
         pages, _, layers, page_size, slot = _int8_pool(op, blocks).shape
         slots = (slot,)
