@@ -69,3 +69,16 @@ def test_tables_of_another_width_are_refused(calls, form, width) -> None:
     assert calls == []
     _attend(form, qkv)
     assert len(calls) == 1
+
+
+@pytest.mark.parametrize("form", [*FORMS, "float32 chunk"])
+@pytest.mark.parametrize("stride", [0, 1, 3 * HEADS * D + 2, (1 << 25) + 1])
+def test_one_row_of_any_stride(calls, form, stride) -> None:
+    """A single row is contiguous whatever its stride is, and goes to the entries as one that is packed."""
+    width = 3 * HEADS * D
+    qkv = _on(torch.zeros(width).as_strided((1, width), (stride, 1)))
+    assert qkv.is_contiguous() and qkv.stride(0) == stride
+    _attend(form, qkv)
+    (name, args), = calls
+    passed = args[5 if name == "uocr_paged_chunk_attention_qkv" else 7]  # row_stride
+    assert passed >= (width if "qkv" in name else HEADS * D) and passed % 4 == 0 and passed < 1 << 25

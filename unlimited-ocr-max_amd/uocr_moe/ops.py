@@ -730,7 +730,7 @@ def _fused_rows(op: str, qkv, heads: int) -> torch.Tensor:
     if heads < 1 or width % (3 * heads):
         raise ValueError(f"{op}: qkv width {width} is not 3 x {heads} heads")
     if qkv.stride(1) != 1 or not width <= qkv.stride(0) < _CHUNK_STRIDE or qkv.stride(0) % 4 or qkv.data_ptr() % 16:
-        qkv = _packed(qkv)
+        qkv = _packed(qkv).view(-1).view(qkv.shape)  # (one row is contiguous whatever its stride says)
     return qkv
 
 
