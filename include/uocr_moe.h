@@ -348,7 +348,8 @@ int uocr_draft_masks(int64_t* masks, const int32_t* parents, int64_t tokens, con
  * behind them; next_tokens int32 [requests] the answer to the last (-1: an empty chunk);
  * cache_lengths_out uint32 [requests] = cache_lengths + counts.  The path's rows, k and v of all
  * layers, move to rows cached, cached + 1, ... of the request.  kv_blocks: a pool of either
- * kind, slot_bytes a multiple of 16 (fp32: heads * 512).  Outputs overlap nothing. */
+ * kind, slot_bytes a multiple of 16 (fp32: heads * 512).  Outputs overlap nothing.  With no
+ * requests nothing is written. */
 int uocr_accept_drafts(void* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes,
                        const uint32_t* lookup, int64_t requests, int64_t lookup_cols, const uint32_t* cache_lengths,
                        const int32_t* chunk_offsets, const int32_t* parents, const int32_t* drafted, const int32_t* answers,

@@ -82,3 +82,16 @@ def test_one_row_of_any_stride(calls, form, stride) -> None:
     (name, args), = calls
     passed = args[5 if name == "uocr_paged_chunk_attention_qkv" else 7]  # row_stride
     assert passed >= (width if "qkv" in name else HEADS * D) and passed % 4 == 0 and passed < 1 << 25
+
+
+def test_accepting_for_no_requests_leaves_no_word_unset(calls, monkeypatch) -> None:
+    """Tokens of no chunk have -1 in the path, where there is no request at all too."""
+    import uocr_moe as u
+
+    allocate = torch.Tensor.new_empty
+    monkeypatch.setattr(OnGpu, "new_empty", lambda self, *a, **kw: allocate(self, *a, **kw).fill_(77))
+    kv = u.PagedChunk(kv_blocks=_pool(True), lookup_table=_on(torch.zeros(0, 1, dtype=torch.int32)), cache_lengths=_i32(),
+                      chunk_offsets=_i32(0), attend_max=1)
+    counts, path, following, lengths = u.accept_drafts(kv, _i32(-1, 0, 1), _i32(5, 6, 7), _i32(6, 7, 8))
+    assert path.tolist() == [-1, -1, -1]
+    assert counts.shape == following.shape == lengths.shape == (0,)

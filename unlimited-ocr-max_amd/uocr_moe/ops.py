@@ -850,6 +850,8 @@ def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tenso
                lookup.data_ptr(), n, lookup.shape[1], cached.data_ptr(), offsets.data_ptr(), parents.data_ptr(),
                tokens.data_ptr(), answers.data_ptr(), total, counts.data_ptr(), path.data_ptr(), following.data_ptr(),
                lengths.data_ptr(), tensors=(blocks, lookup, cached, offsets, parents, tokens, answers))
+    if n == 0:  # the entry writes nothing
+        path.fill_(-1)
     return counts, path, following, lengths
 
 
