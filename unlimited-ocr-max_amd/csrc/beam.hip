@@ -22,9 +22,9 @@ typedef float f32x4_at_float __attribute__((ext_vector_type(4), aligned(4)));
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kList = 1024;  // candidates that are ranked against one another in LDS
 
-// A float's bits in the order of the floats.
+// A float's bits in the order of the floats, which has -0.0 and 0.0 as one.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.0f);
   return (int)b < 0 ? ~b : b | 0x80000000u;
 }
 // A border that at least `most` lanes of a wave reach with `mine`, and few more: the most-th largest, its last 12 bits cut.
