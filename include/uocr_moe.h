@@ -363,8 +363,9 @@ int uocr_accept_drafts(void* kv_blocks, int64_t pages, int64_t layers, int64_t p
  *   [rows], may be NULL) not 0 has one candidate, eos with key = scores[b].
  *   rank = key, or, given lengths (int32 [rows]), key / length^alpha, the length being
  *   lengths[b] + 1, of an ended beam lengths[b].
- * Keys and ranks are in 64 bits, ties go to the lower (row, token).  Candidates without a finite rank come
- * last and get the score -inf.  Outputs, row by row: the token, the parent row, the key as fp32, whether it has
+ * Keys and ranks are in 64 bits, log sum exp within 2e-12; ties go to the lower (row, token).
+ * Candidates without a finite rank come last and get the score -inf.  Outputs, row by row: the
+ * token, the parent row, the key as fp32, whether it has
  * ended (its parent had, or the token is eos), the length, and the history (int32 [rows,
  * width]): the parent's, of a live one without its first id and with the token at the end.
  * lengths and history have an output each, or both are NULL.  workspace:

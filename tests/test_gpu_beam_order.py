@@ -1,6 +1,14 @@
-"""GPU tests of the order that ``beam_select`` puts candidates in."""
+"""GPU tests of the order that ``beam_select`` puts candidates in: ties, and candidates of different beams that are near one
+another.
+
+All is decided in 64 bits, the exponentials too: each is off by 1.1e-12 of itself, and so is their sum (its roundings add a few
+2^-53 each), whose logarithm is then off by less than 2e-12.  A key near -1 adds its own roundings, 2^-53 each.  The nearest
+candidates here are 1e-10 apart.
+"""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -44,3 +52,57 @@ def test_scores_of_either_zero_are_equal() -> None:
     ended = torch.ones(4, dtype=torch.int32)
     for scores in ([-0.0, 0.0, -0.0, 0.0], [0.0, -0.0, 0.0, 0.0]):
         assert _select(torch.randn(4, 50), torch.tensor(scores), 4, ended)[1] == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize(("requests", "beams", "vocab"), [(1, 8, 129280), (3, 8, 2500), (64, 8, 9001)])
+@pytest.mark.parametrize("gap", [1e-10, 1e-9, 1e-8, 1e-7, 1e-6])
+def test_near_candidates_of_different_beams(requests, beams, vocab, gap) -> None:
+    """Every beam has one likely token; the beams' scores put them `gap` apart, in an order of their own."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = requests * beams
+    logits = (2.5 * torch.randn(rows, vocab, generator=g)).clamp(max=7.0)  # log probabilities below -3
+    top = torch.randint(0, vocab, (rows,), generator=g)
+    at = torch.arange(rows)
+    logits[at, top] = -INF
+    rest = torch.cat([torch.logsumexp(x.double(), dim=1) for x in logits.split(64)])
+    logits[at, top] = (rest - 1.0 - math.log1p(-math.exp(-1.0))).float()  # a log probability near -1
+    best = logits[at, top].double()
+    lse = rest + torch.log1p((best - rest).exp())
+    order = torch.stack([torch.randperm(beams, generator=g) for _ in range(requests)])  # the place of each beam
+    scores = (-1.0 - gap * order.flatten().double() - (best - lse)).float()
+    keys = (scores.double() + (best - lse)).view(requests, beams)
+    want = torch.sort(keys, dim=1, descending=True).indices
+    assert torch.equal(want.argsort(dim=1), order)
+    apart = keys.gather(1, want).diff(dim=1)
+    assert bool((apart < -gap / 2).all()) and bool((keys > -1.5).all())
+    tokens, parents = _select(logits, scores, beams)
+    want = (want + beams * torch.arange(requests)[:, None]).flatten()
+    assert parents == want.tolist() and tokens == top[want].tolist()
+
+
+@pytest.mark.parametrize("top", [3e9, 2.0 ** 60, 3.4e38])
+def test_large_logits(top) -> None:
+    """Beside such a logit the next ones have no weight, however near they are for its size: the beams' scores decide."""
+    logits = torch.full((4, 5000), top)
+    logits *= 1.0 - torch.rand(4, 5000, generator=torch.Generator().manual_seed(5)) / 100 - 1e-5
+    best = [7, 4000, 2100, 12]
+    logits[range(4), best] = top
+    scores = torch.tensor([-3.0, -1.0, -4.0, -2.0])
+    tokens, parents = _select(logits, scores, 4)
+    assert parents == [1, 3, 0, 2] and tokens == [4000, 12, 7, 2100]
+
+
+def test_rows_without_a_finite_sum_come_last() -> None:
+    """A NaN anywhere in a row, of either sign, and infinite logits."""
+    logits = torch.randn(8, 5000, generator=torch.Generator().manual_seed(6))
+    logits[0, 4999] = float("nan")
+    logits[1, 2] = -float("nan")
+    logits[2, 2047] = INF
+    logits[3] = -INF
+    logits[4] = float("nan")
+    logits[5, 2048:] = -INF  # finite
+    logits[6, 17] = 30.0
+    logits[7, 18] = 40.0
+    _, parents = _select(logits, torch.zeros(8), 8)
+    assert parents[:2] == [6, 7] or parents[:2] == [7, 6]
+    assert set(parents) == {5, 6, 7}

@@ -6,8 +6,9 @@
 //   key(b, eos) = score_b, no other token                                    an ended one
 //   rank = key / length^alpha, the length with the new token                 (given lengths; else rank = key)
 //
-// The K best of a request's K beams by rank, ties to the lower (beam, token).  Keys and ranks are in 64 bits: which
-// of two near candidates wins decides what a request says.  A candidate whose rank is not finite (a token at -inf, a beam
+// The K best of a request's K beams by rank, ties to the lower (beam, token).  Keys and ranks are in 64 bits, the
+// exponentials and their sum too (a sum's logarithm is off by 2e-12 at most): which of two near candidates wins decides what a
+// request says.  A candidate whose rank is not finite (a token at -inf, a beam
 // whose score or sum is not finite) comes after all others, as -inf; of a beam without a finite sum it is the first
 // tokens that do.
 #include "uocr_device.h"
@@ -27,6 +28,10 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return (int)b < 0 ? ~b : b | 0x80000000u;
 }
+// The float whose bits come there; of what lies below all of them, -inf.
+__device__ __forceinline__ float of_ordered(uint32_t u) {
+  return u <= 0x007fffffu ? -kInf : __uint_as_float((int)u < 0 ? u ^ 0x80000000u : ~u);
+}
 // A border that at least `most` lanes of a wave reach with `mine`, and few more: the most-th largest, its last 12 bits cut.
 __device__ __forceinline__ uint32_t border_of(uint32_t mine, int most) {
   uint32_t t = 0;
@@ -39,8 +44,8 @@ __device__ __forceinline__ uint32_t border_of(uint32_t mine, int most) {
 }
 
 // Of the candidates that the threads of a workgroup hold, the first `most` (at most 32) by value (descending) and id
-// (ascending).  each(f) calls f(value, id) for a thread's candidates, put(rank, value, id) takes a chosen one; returns
-// their number.
+// (ascending).  `mine` is the thread's largest value (-inf: it has none); each(least, f) calls f(value, id) for its candidates
+// that are no smaller than the float `least`, put(rank, value, id) takes a chosen one; returns their number.
 //
 // At least `most` candidates are no smaller than the most-th largest of a wave's lanes' largest ones (as floats, whose
 // rounding keeps the order), and few are as large: those of the highest such border are listed, and ranked by counting.
@@ -53,12 +58,10 @@ struct Best {
   int listed;
 };
 template <typename V, typename Id, int kThreads, typename Each, typename Put>
-__device__ __forceinline__ int choose(Best<V, Id, kThreads>& b, int most, Each each, Put put) {
+__device__ __forceinline__ int choose(Best<V, Id, kThreads>& b, int most, V mine, Each each, Put put) {
   const int tid = (int)threadIdx.x;
   static_assert(kThreads <= kList, "a thread has a place in the list");
   const V none = -(V)__builtin_huge_val();
-  V mine = none;
-  each([&](V v, Id) { mine = v > mine ? v : mine; });
   const uint32_t own_border = border_of(ordered((float)mine), most);
   if (lane_id() == 0) b.border[tid / kWave] = own_border;
   if (tid == 0) b.listed = 0;
@@ -66,14 +69,13 @@ __device__ __forceinline__ int choose(Best<V, Id, kThreads>& b, int most, Each e
   uint32_t border = 0;
 #pragma unroll
   for (int i = 0; i < kThreads / kWave; ++i) border = max(border, b.border[i]);
-  if (ordered((float)mine) >= border)
-    each([&](V v, Id id) {
-      if (ordered((float)v) >= border) {
-        const int at = atomicAdd(&b.listed, 1);
-        if (at < kList) {
-          b.value[at] = v;
-          b.id[at] = id;
-        }
+  const float least = of_ordered(border);
+  if ((float)mine >= least)
+    each(least, [&](V v, Id id) {
+      const int at = atomicAdd(&b.listed, 1);
+      if (at < kList) {
+        b.value[at] = v;
+        b.id[at] = id;
       }
     });
   __syncthreads();
@@ -94,7 +96,7 @@ __device__ __forceinline__ int choose(Best<V, Id, kThreads>& b, int most, Each e
   for (int k = 0; k < most; ++k) {
     V v = none;
     Id at = -1;
-    each([&](V x, Id id) {
+    each(-kInf, [&](V x, Id id) {
       const bool after = k == 0 || x < last || (x == last && id > last_id);
       if (after && (at < 0 || x > v || (x == v && id < at))) {
         v = x;
@@ -123,22 +125,56 @@ __device__ __forceinline__ int choose(Best<V, Id, kThreads>& b, int most, Each e
 
 constexpr int kRowThreads = 256, kJoinThreads = 512;
 
-struct BeamWork {  // of each row's pieces: the largest logit and the sum, the best tokens
+struct BeamWork {  // of each row's pieces: the sum and the largest logit, the best tokens
   int pieces;
   Divide by_beam;  // candidates of a beam
+  double* sums;
   float* tops;
   float* values;
   int* ids;
 };
 
+// max(a, b, c), NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// The sum of e^x of four -700 <= x <= 0, each off by 1.1e-12 of itself: 2^(x log2 e), whose whole part is what stays of it
+// beside 1.5 2^52, in the sum's lower word, and the rest, a half at most, a polynomial (2^f by its values at nine Chebyshev
+// nodes; eleven would be 3e-16 off and take 3 us more of 57).  Four side by side: a step of one waits for the step before.
+__device__ __forceinline__ double exp_sum4(const double (&x)[4]) {
+  constexpr double kLog2E = 0x1.71547652b82fep+0, kWhole = 0x1.8p+52;
+  constexpr double kPoly[] = {0x1.00dc4a532fb8ep-16, 0x1.4308ac85aa947p-13, 0x1.5d8745a728441p-10, 0x1.3b2ab7181b755p-7,
+                              0x1.c6b08dd6fd234p-5, 0x1.ebfbdff823cedp-3, 0x1.62e42fef84cf0p-1, 0x1.0000000000000p+0};
+  double u[4], f[4], y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) u[e] = __builtin_fma(x[e], kLog2E, kWhole);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = u[e] - kWhole;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = __builtin_fma(x[e], kLog2E, -f[e]), y[e] = 0x1.63d136366db24p-20;
+#pragma unroll
+  for (double c : kPoly) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __builtin_fma(y[e], f[e], c);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexp(y[e], __double2loint(u[e]));
+  return (y[0] + y[1]) + (y[2] + y[3]);
+}
+
 // A workgroup has a piece of a row: its largest logit, its sum of exponentials, and its best K tokens.  Rows begin at any
-// float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.  Bound by memory where
-// rows are many (512 of 129280: 45 us, 5.9 TB/s), else by its trip there and the two passes over a thread's tokens (4 rows:
-// 5.6 us).
+// float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.  Where rows are many (512
+// of 129280: 57 us, 4.6 TB/s) the vector units have two thirds of the time, most of it for the exponentials, beside memory's
+// 45; few rows (4: 5.5 us) wait for their trip there.  (Exponentials and sums in 32 bits took 44, and candidates of different
+// beams nearer than 1e-6 could change places.)
 template <int kPer>
 __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWork w) {
   __shared__ Best<float, int, kRowThreads> best;
   __shared__ float parts[kRowThreads / kWave];
+  __shared__ double part_sums[kRowThreads / kWave];
   const int row = (int)blockIdx.y, piece = (int)blockIdx.x, tid = (int)threadIdx.x;
   if (p.ended != nullptr && ldg(p.ended + row) != 0) return;
   const int begin = piece * kRowThreads * kPer;
@@ -161,33 +197,51 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWor
     v[i + 2] = y.z;
     v[i + 3] = y.w;
   }
-  float m = v[0];
+  constexpr int kGroup = 8;  // tokens that are looked at together
+  float largest[kPer / kGroup], mine = -kInf;
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
-  m = tree_max(m);
+  for (int g = 0; g < kPer / kGroup; ++g) {
+    const float* x = v + g * kGroup;
+    largest[g] = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[7]);
+    mine = max3(mine, largest[g], largest[g]);
+  }
+  float m = tree_max(mine);  // (of the lanes without a NaN)
   if (lane_id() == 0) parts[tid / kWave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
-  __syncthreads();
-  float l = 0.0f;
-  const float off = m == -kInf ? 0.0f : m;
+  // Terms and sum are in 64 bits: the sums of two rows decide between their candidates.  What is further below the largest than
+  // 700 (e^-700 = 1e-304) counts as that far.
+  double l = 0.0;
+  const double off = m == -kInf ? 0.0 : (double)m;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) l += __builtin_amdgcn_exp2f((v[i] - off) * 1.44269504f);
-  l = tree_sum(l);
-  if (lane_id() == 0) parts[tid / kWave] = l;
+  for (int i = 0; i < kPer; i += 4) {
+    double x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmax((double)v[i + e] - off, -700.0);
+    l += exp_sum4(x);
+  }
+  if (m == -kInf) l = 0.0;
+  if (m == kInf || mine != mine) l = __builtin_nan("");
+  for (int j = 32; j >= 1; j /= 2) l += __shfl_xor(l, j, kWave);
+  if (lane_id() == 0) part_sums[tid / kWave] = l;
   __syncthreads();
   const int64_t at = (int64_t)row * w.pieces + piece;
   if (tid == 0) {
-    w.tops[2 * at] = m;
-    w.tops[2 * at + 1] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
+    w.tops[at] = m;
+    w.sums[at] = (part_sums[0] + part_sums[1]) + (part_sums[2] + part_sums[3]);
   }
   float* values = w.values + at * p.beams;
   int* ids = w.ids + at * p.beams;
-  const int found = choose(best, p.beams,
-                           [&](auto f) {
+  // (of a row with a NaN nothing counts)
+  const int found = choose(best, p.beams, mine,
+                           [&](float least, auto f) {
 #pragma unroll
-                             for (int i = 0; i < kPer; ++i)
-                               if (v[i] > -kInf) f(v[i], token(i));
+                             for (int g = 0; g < kPer / kGroup; ++g)
+                               if (largest[g] >= least) {
+#pragma unroll
+                                 for (int i = g * kGroup; i < (g + 1) * kGroup; ++i)
+                                   if (v[i] >= least && v[i] > -kInf) f(v[i], token(i));
+                               }
                            },
                            [&](int rank, float value, int id) {
                              values[rank] = value;
@@ -221,18 +275,20 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   }
   for (int b = wave; b < K; b += kJoinThreads / kWave) {
     const int64_t row = row0 + b;
-    const float* tops = w.tops + 2 * row * w.pieces;  // (an ended beam's are nobody's)
+    const float* tops = w.tops + row * w.pieces;  // (an ended beam's are nobody's)
+    const double* part_sums = w.sums + row * w.pieces;
     const bool ended = p.ended != nullptr && ldg(p.ended + row) != 0;
     const double score = ldg(p.scores + row);
     const int length = p.lengths != nullptr ? ldg(p.lengths + row) + (ended ? 0 : 1) : 0;
     const bool some = lane < w.pieces;
-    const float m0 = some ? ldg(tops + 2 * lane) : -kInf, l0 = some ? ldg(tops + 2 * lane + 1) : 0.0f;
+    const float m0 = some ? ldg(tops + lane) : -kInf;
+    const double l0 = some ? ldg(part_sums + lane) : 0.0;
     float m = m0;
-    for (int i = lane + kWave; i < w.pieces; i += kWave) m = fmaxf(m, ldg(tops + 2 * i));
+    for (int i = lane + kWave; i < w.pieces; i += kWave) m = fmaxf(m, ldg(tops + i));
     m = tree_max(m);
-    const auto at_most = [&](float mi, float li) { return li == 0.0f ? 0.0 : (double)li * full_exp((double)mi - (double)m); };
+    const auto at_most = [&](float mi, double li) { return li == 0.0 ? 0.0 : li * full_exp((double)mi - (double)m); };
     double l = at_most(m0, l0);
-    for (int i = lane + kWave; i < w.pieces; i += kWave) l += at_most(ldg(tops + 2 * i), ldg(tops + 2 * i + 1));
+    for (int i = lane + kWave; i < w.pieces; i += kWave) l += at_most(ldg(tops + i), ldg(part_sums + i));
     for (int off = 32; off >= 1; off /= 2) l += __shfl_xor(l, off, kWave);
     // (pow's code alone takes as long to fetch as all else here: length^-alpha by the logarithm, in the lane next to the sum's)
     const double logs = log(lane == 1 ? (double)length : l);
@@ -260,14 +316,19 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
       offer(f, b, scores[b], p.eos);
     }
   };
-  const auto each = [&](auto f) {
+  const auto each = [&](float least, auto f) {
+    const auto some = [&](double rank, int64_t id) {
+      if ((float)rank >= least) f(rank, id);
+    };
 #pragma unroll
     for (int u = 0; u < kHeld; ++u)
-      if (tid + u * kJoinThreads < candidates) one(f, tid + u * kJoinThreads, held[u], held_id[u]);
+      if (tid + u * kJoinThreads < candidates) one(some, tid + u * kJoinThreads, held[u], held_id[u]);
     for (int i = tid + kHeld * kJoinThreads; i < candidates; i += kJoinThreads)
-      one(f, i, ldg(w.values + first + i), ldg(w.ids + first + i));
+      one(some, i, ldg(w.values + first + i), ldg(w.ids + first + i));
   };
-  const int found = choose(best, K, each, [&](int rank, double, int64_t id) {
+  double mine = -__builtin_huge_val();
+  each(-kInf, [&](double rank, int64_t) { mine = rank > mine ? rank : mine; });
+  const int found = choose(best, K, mine, each, [&](int rank, double, int64_t id) {
     const int b = (int)(id / p.vocab);
     parents[rank] = b;
     tokens[rank] = (int)(id - (int64_t)b * p.vocab);
@@ -320,7 +381,7 @@ int pieces_of(int64_t rows, int vocab) {
 }  // namespace
 
 size_t beam_workspace_bytes(int64_t rows, int beams, int vocab) {
-  return (size_t)rows * pieces_of(rows, vocab) * (2 + 2 * (size_t)beams) * 4;
+  return (size_t)rows * pieces_of(rows, vocab) * (3 + 2 * (size_t)beams) * 4;
 }
 
 hipError_t launch_beam_select(const BeamSelect& p, int64_t rows, void* workspace, hipStream_t s) {
@@ -329,8 +390,9 @@ hipError_t launch_beam_select(const BeamSelect& p, int64_t rows, void* workspace
   w.pieces = pieces_of(rows, p.vocab);
   w.by_beam = divide_by(w.pieces * p.beams);
   const int64_t n = rows * w.pieces;
-  w.tops = (float*)workspace;
-  w.values = w.tops + 2 * n;
+  w.sums = (double*)workspace;
+  w.tops = (float*)(w.sums + n);
+  w.values = w.tops + n;
   w.ids = (int*)(w.values + n * p.beams);
   const dim3 grid((unsigned)w.pieces, (unsigned)rows), block(kRowThreads);
   const auto kernel = per_thread(rows, p.vocab) == 8 ? k_beam_rows<8> : k_beam_rows<32>;
