@@ -1,5 +1,5 @@
-"""GPU tests of the order that ``beam_select`` puts candidates in: ties, and candidates of different beams that are near one
-another.
+"""GPU tests of the order that ``beam_select`` puts candidates in: ties, candidates of different beams that are near one
+another, and lengths whose penalties make equal ranks.
 
 All is decided in 64 bits, the exponentials too: each is off by 1.1e-12 of itself, and so is their sum (its roundings add a few
 2^-53 each), whose logarithm is then off by less than 2e-12.  A key near -1 adds its own roundings, 2^-53 each.  The nearest
@@ -106,3 +106,27 @@ def test_rows_without_a_finite_sum_come_last() -> None:
     _, parents = _select(logits, torch.zeros(8), 8)
     assert parents[:2] == [6, 7] or parents[:2] == [7, 6]
     assert set(parents) == {5, 6, 7}
+
+
+@pytest.mark.parametrize("alpha", [1.0, 2.0, 0.5, -1.0])
+def test_equal_ranks_of_different_lengths(alpha) -> None:
+    """Scores in proportion to length^alpha, whole numbers all: every rank is one number, so the rows keep their order."""
+    g = torch.Generator().manual_seed(7)
+    beams, requests = 8, 64
+    rows = beams * requests
+    if alpha == 0.5:
+        root = torch.randint(1, 40, (rows,), generator=g)
+        lengths, power = root * root, root.double()
+    elif alpha == -1.0:
+        of = torch.tensor([n for n in range(1, 841) if 840 % n == 0])
+        lengths = of[torch.randint(0, len(of), (rows,), generator=g)]
+        power = 840.0 / lengths.double()
+    else:
+        lengths = torch.randint(1, 300, (rows,), generator=g)
+        power = lengths.double() ** alpha
+    times = torch.randint(1, 50, (requests,), generator=g).repeat_interleave(beams)
+    scores = (-times * power).float()
+    assert torch.equal(scores.double(), -times * power)
+    ended = torch.ones(rows, dtype=torch.int32)
+    _, parents = _select(torch.zeros(rows, beams), scores, beams, ended, lengths.int(), alpha)
+    assert parents == list(range(rows))

@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   __shared__ int lengths[kBeamsMost], state[kBeamsMost];  // 0: live, 1: ended, 2: no finite sum
   __shared__ int tokens[kBeamsMost], parents[kBeamsMost];
   const int K = p.beams, tid = (int)threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const bool penalised = p.lengths != nullptr && p.alpha != 0.0;
   const int64_t row0 = (int64_t)blockIdx.x * K;
   // The first candidates are asked for before the sums, which they wait for: of a request they lie one after another.
   constexpr int kHeld = 4;
@@ -290,14 +291,18 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
     double l = at_most(m0, l0);
     for (int i = lane + kWave; i < w.pieces; i += kWave) l += at_most(ldg(tops + i), ldg(part_sums + i));
     for (int off = 32; off >= 1; off /= 2) l += __shfl_xor(l, off, kWave);
-    // (pow's code alone takes as long to fetch as all else here: length^-alpha by the logarithm, in the lane next to the sum's)
+    // (pow's code alone takes as long to fetch as all else here: length^|alpha| by the logarithm, in the lane next to the sum's.
+    // Off by 2^-46 of itself at most, so that powers that near to a whole number count as that: beams of different lengths may
+    // have equal ranks where their powers are whole.)
     const double logs = log(lane == 1 ? (double)length : l);
     const double lse = (double)m + __shfl(logs, 0, kWave);
-    const double factor = p.lengths != nullptr && p.alpha != 0.0 ? full_exp(-p.alpha * __shfl(logs, 1, kWave)) : 1.0;
+    double power = penalised ? full_exp(__builtin_fabs(p.alpha) * __shfl(logs, 1, kWave)) : 1.0;
+    const double whole = __builtin_rint(power);
+    power = __builtin_fabs(power - whole) <= 0x1p-46 * power ? whole : power;
     if (lane == 0) {
       sums[b] = lse;
       scores[b] = score;
-      by[b] = factor;
+      by[b] = power;
       lengths[b] = length;
       state[b] = ended ? 1 : score - score == 0.0 && lse - lse == 0.0 ? 0 : 2;
     }
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   __syncthreads();
   const auto key_of = [&](int b, float logit) { return state[b] == 1 ? scores[b] : scores[b] + ((double)logit - sums[b]); };
   const auto offer = [&](auto f, int b, double key, int token) {
-    const double rank = key * by[b];
+    const double rank = !penalised ? key : p.alpha < 0.0 ? key * by[b] : key / by[b];
     if (rank - rank == 0.0) f(rank, (int64_t)b * p.vocab + token);
   };
   const auto one = [&](auto f, int i, float logit, int id) {
