@@ -130,3 +130,18 @@ def test_equal_ranks_of_different_lengths(alpha) -> None:
     ended = torch.ones(rows, dtype=torch.int32)
     _, parents = _select(torch.zeros(rows, beams), scores, beams, ended, lengths.int(), alpha)
     assert parents == list(range(rows))
+
+
+@pytest.mark.parametrize("score", [-1e20, torch.finfo(torch.float32).min, 1e18])
+def test_a_beams_tokens_go_by_their_logits(score) -> None:
+    """Beside such a score the keys of one beam are equal in 64 bits; its tokens' logits are not."""
+    logits = torch.randn(4, 5000, generator=torch.Generator().manual_seed(3))
+    logits[0, 4500] = 20.0
+    logits[0, 30] = logits[0, 4400] = 19.0
+    logits[0, 2500] = 18.0
+    scores = torch.full((4,), -INF)
+    scores[0] = score
+    assert _select(logits, scores, 4) == ([4500, 30, 4400, 2500], [0] * 4)
+    scores[1] = score  # of two beams the lower row comes first
+    logits[1, 7] = 40.0
+    assert _select(logits, scores, 4) == ([4500, 30, 4400, 2500], [0] * 4)

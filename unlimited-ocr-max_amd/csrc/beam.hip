@@ -6,7 +6,8 @@
 //   key(b, eos) = score_b, no other token                                    an ended one
 //   rank = key / length^alpha, the length with the new token                 (given lengths; else rank = key)
 //
-// The K best of a request's K beams by rank, ties to the lower (beam, token).  Keys and ranks are in 64 bits, the
+// The K best of a request's K beams by rank, ties to the lower beam, of a beam to the larger logit, then to the lower token
+// (beside a score of some size 64 bits do not tell the keys of a beam's tokens apart, and their logits do).  Keys and ranks are in 64 bits, the
 // exponentials and their sum too (a sum's logarithm is off by 2e-12 at most): which of two near candidates wins decides what a
 // request says.  A candidate whose rank is not finite (a token at -inf, a beam
 // whose score or sum is not finite) comes after all others, as -inf; of a beam without a finite sum it is the first
@@ -259,6 +260,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   __shared__ double sums[kBeamsMost], scores[kBeamsMost], by[kBeamsMost];
   __shared__ int lengths[kBeamsMost], state[kBeamsMost];  // 0: live, 1: ended, 2: no finite sum
   __shared__ int tokens[kBeamsMost], parents[kBeamsMost];
+  __shared__ float logits[kBeamsMost];
   const int K = p.beams, tid = (int)threadIdx.x, wave = tid / kWave, lane = lane_id();
   const bool penalised = p.lengths != nullptr && p.alpha != 0.0;
   const int64_t row0 = (int64_t)blockIdx.x * K;
@@ -309,16 +311,19 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   }
   __syncthreads();
   const auto key_of = [&](int b, float logit) { return state[b] == 1 ? scores[b] : scores[b] + ((double)logit - sums[b]); };
-  const auto offer = [&](auto f, int b, double key, int token) {
+  // A candidate's id is in the order of ties: 5 bits of its beam, 32 of its logit (the larger first), 26 of its place among the
+  // beam's (a row's pieces and what each has found are in the order of their tokens where logits are equal).
+  constexpr int kPlaceBits = 26, kBeamAt = kPlaceBits + 32;
+  const auto offer = [&](auto f, int b, double key, float logit, int place) {
     const double rank = !penalised ? key : p.alpha < 0.0 ? key * by[b] : key / by[b];
-    if (rank - rank == 0.0) f(rank, (int64_t)b * p.vocab + token);
+    if (rank - rank == 0.0) f(rank, (int64_t)b << kBeamAt | (int64_t)~ordered(logit) << kPlaceBits | place);
   };
   const auto one = [&](auto f, int i, float logit, int id) {
     const int b = w.by_beam(i);
     if (state[b] == 0) {
-      if (id >= 0) offer(f, b, key_of(b, logit), id);
+      if (id >= 0) offer(f, b, key_of(b, logit), logit, i - b * per);
     } else if (state[b] == 1 && i == b * per) {
-      offer(f, b, scores[b], p.eos);
+      offer(f, b, scores[b], 0.0f, 0);
     }
   };
   const auto each = [&](float least, auto f) {
@@ -334,9 +339,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   double mine = -__builtin_huge_val();
   each(-kInf, [&](double rank, int64_t) { mine = rank > mine ? rank : mine; });
   const int found = choose(best, K, mine, each, [&](int rank, double, int64_t id) {
-    const int b = (int)(id / p.vocab);
+    const int b = (int)(id >> kBeamAt), place = (int)id & ((1 << kPlaceBits) - 1);
     parents[rank] = b;
-    tokens[rank] = (int)(id - (int64_t)b * p.vocab);
+    tokens[rank] = state[b] == 1 ? p.eos : ldg(w.ids + first + (b * per + place));
+    logits[rank] = of_ordered(~(uint32_t)(id >> kPlaceBits));
   });
   __syncthreads();
   if (tid == 0)  // fewer with a finite rank than beams: the others in order
@@ -357,13 +363,11 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWo
   if (tid < K) {
     const int b = parents[tid], token = tokens[tid];
     const int64_t row = row0 + tid;
-    const double key = state[b] == 2 ? -__builtin_huge_val()
-                                     : key_of(b, state[b] == 1 ? 0.0f : ldg(p.logits + (row0 + b) * p.vocab + token));
     const bool counts = tid < found;  // others come after all, as -inf
     const bool ended = p.ended != nullptr && ldg(p.ended + row0 + b) != 0;
     stg(p.tokens_out + row, token);
     stg(p.parents_out + row, (int)(row0 + b));
-    stg(p.scores_out + row, counts ? (float)key : -kInf);
+    stg(p.scores_out + row, counts ? (float)key_of(b, logits[tid]) : -kInf);
     stg(p.ended_out + row, (int)(ended || token == p.eos));
     if (p.lengths != nullptr) stg(p.lengths_out + row, lengths[b]);
   }

@@ -880,7 +880,8 @@ def beam_select(logits, scores, *, beams: int, eos: int, ended=None, lengths=Non
     A candidate's key is ``scores[b] + logits[b, v] - logsumexp(logits[b])``; a beam whose ``ended`` (int32 ``[rows]``)
     is set has one candidate, ``eos`` at its score.  They rank by key, or, given ``lengths`` (int32 ``[rows]``, the
     tokens of each beam), by ``key / length ** alpha`` with the new token counted.  Keys and ranks are in 64 bits; ties go to
-    the lower (row, token); candidates without a finite rank come last, with score ``-inf``.
+    the lower row, of a row to the larger logit, then to the lower token; candidates without a finite rank come last, with
+    score ``-inf``.
 
     ``history`` int32 ``[rows, width]`` (:func:`ngram_block`'s) follows its beam: without its first id, and with the token
     at the end (an ended beam's as it is).  ``parents`` are rows of ``logits``, for :func:`fork_pages` with the rows
