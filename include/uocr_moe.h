@@ -336,7 +336,7 @@ int uocr_dequantize_pages(const int8_t* kv_int8, int64_t int8_pages, float* kv_b
 /* draft_masks -- the words `visible` of trees.  A request's chunk is its tree: token 0 the
  * root, parents int32 [tokens] the place in the chunk of each one's parent, which comes
  * before it (any other value: it has none).  masks int64 [tokens]: bits of a token's
- * ancestors and its own. */
+ * ancestors and its own; words of tokens that no chunk holds are not written. */
 int uocr_draft_masks(int64_t* masks, const int32_t* parents, int64_t tokens, const int32_t* chunk_offsets, int64_t requests,
                      void* stream, char* err, size_t errlen);
 
@@ -347,7 +347,9 @@ int uocr_draft_masks(int64_t* masks, const int32_t* parents, int64_t tokens, con
  * int32 [tokens] its tokens' places in the chunk, at the front of the chunk's words, -1
  * behind them; next_tokens int32 [requests] the answer to the last (-1: an empty chunk);
  * cache_lengths_out uint32 [requests] = cache_lengths + counts.  The path's rows, k and v of all
- * layers, move to rows cached, cached + 1, ... of the request.  kv_blocks: a pool of either
+ * layers, move to rows cached, cached + 1, ... of the request; rows at or past lookup_cols *
+ * page_size exist nowhere, are not moved and are counted all the same: a chunk whose rows the
+ * table addresses has none.  kv_blocks: a pool of either
  * kind, slot_bytes a multiple of 16 (fp32: heads * 512).  Outputs overlap nothing.  With no
  * requests nothing is written. */
 int uocr_accept_drafts(void* kv_blocks, int64_t pages, int64_t layers, int64_t page_size, int64_t slot_bytes,

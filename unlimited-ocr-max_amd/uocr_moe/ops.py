@@ -799,7 +799,8 @@ def dequantize_pages(kv_int8, src, kv_blocks, dst, *, rows=None) -> torch.Tensor
 def draft_masks(parents, chunk_offsets, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The words :attr:`PagedChunk.visible` of trees of drafted tokens: int64 ``[tokens]``, the bits of each token's
     ancestors and its own.  A request's chunk is its tree, token 0 the root; ``parents`` int32 ``[tokens]`` is the place
-    in the chunk of each one's parent, which comes before it (any other value: it has none)."""
+    in the chunk of each one's parent, which comes before it (any other value: it has none).  Words of tokens that no chunk
+    holds are not written: those of ``out`` keep what they held, those of a new result are not set."""
     op = "draft_masks"
     parents = _gpu(op, "parents", parents, torch.int32, 1)
     offsets = _gpu(op, "chunk_offsets", chunk_offsets, torch.int32, 1)
@@ -823,7 +824,8 @@ def accept_drafts(kv: PagedChunk, parents, tokens, answers) -> tuple[torch.Tenso
     either kind, written in place), move together behind the cached ones.  Returns ``(counts, path, next_tokens,
     cache_lengths)``: int32 ``[N]`` the paths' lengths (0: an empty chunk); int32 ``[tokens]`` their tokens' places in the
     chunk, at the front of its words, -1 behind; int32 ``[N]`` the answer to the last (-1: an empty chunk); the cached rows
-    now, as ``kv.cache_lengths``.  Of a chunk the first 64 tokens count."""
+    now, as ``kv.cache_lengths``.  Of a chunk the first 64 tokens count.  The lookup table has to address the chunk's rows:
+    rows past it exist nowhere, do not move, and are counted in the lengths all the same."""
     op = "accept_drafts"
     if isinstance(kv.kv_blocks, torch.Tensor) and kv.kv_blocks.dtype is torch.int8:
         blocks = _int8_pool(op, kv.kv_blocks)
