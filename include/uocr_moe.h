@@ -280,7 +280,8 @@ int uocr_compact_pages(float* kv_blocks, int64_t pages, int64_t layers, int64_t 
  *   q, k_new, v_new: fp32 [tokens, heads, 128] whose rows are row_stride floats apart;
  *   with `positions` (int32 [tokens], else NULL) q and k_new come before RoPE and are
  *   rotated as uocr_rope does (tables fp32 [table_rows, 128], 16-byte aligned).
- *   New rows are stored first; what is attended is what the pool then holds.
+ *   New rows are stored first; what is attended is what the pool then holds.  Values below
+ *   2^-100 lose lower bits in the sum over the rows.
  *   Lookup, lengths, offsets and attend_max as for the fp32 entries; tokens * heads at most
  *   2^25.  workspace: uocr_paged_pool_workspace_bytes(tokens, requests, heads, attend_max,
  *   form) bytes, 16-byte aligned, or NULL (the library's own); form 0: the decode entry, 1: chunks,

@@ -15,8 +15,11 @@
 // results do not depend on how it was cut.
 //
 // Products: the matrix instruction of bf16, fp32 sums.  An fp32 operand is held as three bf16 numbers whose sum it is
-// (24 bits, of its own exponent: no scale is shared, and nothing is out of range); an int8 one is a bf16 number.  So a
-// product with an int8 operand is exact in three, and one of two fp32 operands leaves out 2^-24 of itself in six.
+// (24 bits, of its own exponent: no scale is shared, and nothing is too large); an int8 one is a bf16 number.  So a
+// product with an int8 operand is exact in three, and six of the nine of two fp32 operands leave out 2^-21 of the product
+// where the lower bits of both are ones, some 2^-24 on average, always towards zero as the terms are cut off: what the sums
+// round is about as much (outputs are within 1e-6 of 64 bits' either way), and two products more would be a third more of
+// the matrix instructions.  bf16 ends at 2^-133: of values below 2^-100 the lower bits are lost.
 // The scores are S^T = K Q^T and the results O^T = V^T P^T: a lane owns a query, and its 16 scores of a block of 32 rows
 // come in the order in which the second product wants the weights.
 #include <algorithm>
