@@ -168,9 +168,9 @@ __device__ __forceinline__ double exp_sum4(const double (&x)[4]) {
 
 // A workgroup has a piece of a row: its largest logit, its sum of exponentials, and its best K tokens.  Rows begin at any
 // float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.  Where rows are many (512
-// of 129280: 57 us, 4.6 TB/s) the vector units have two thirds of the time, most of it for the exponentials, beside memory's
-// 45; few rows (4: 5.5 us) wait for their trip there.  (Exponentials and sums in 32 bits took 44, and candidates of different
-// beams nearer than 1e-6 could change places.)
+// of 129280, a fifth of them ended: 56 us, 3.8 TB/s) the vector units are busy for two thirds of the time, most of it with the
+// exponentials, and overlap the loads in part; few rows (4: 5.5 us) wait for their trip to memory.  (Exponentials and sums in
+// 32 bits took 44, at memory's rate, and candidates of different beams nearer than 1e-6 could change places.)
 template <int kPer>
 __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWork w) {
   __shared__ Best<float, int, kRowThreads> best;

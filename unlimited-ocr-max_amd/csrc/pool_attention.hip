@@ -136,8 +136,8 @@ __device__ __forceinline__ void store_rows(const PoolArgs& a, int n, int row, in
   }
 }
 
-// One wave per (token, 4 heads), which waits for the request's words once.  Bound by memory: 2900 tokens of ten heads in 10 us,
-// 3.6 TB/s.  Queries that come before RoPE are rotated where they are read.
+// One wave per (token, 4 heads), which waits for the request's words once.  Bound by memory: 2900 tokens of ten heads in 11 us,
+// 3.4 TB/s.  Queries that come before RoPE are rotated where they are read.
 constexpr int kStoreHeads = 4;
 template <bool kInt8>
 __global__ void __launch_bounds__(256) k_pool_store(PoolArgs a) {
@@ -956,9 +956,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_pool_tiles(Attend p) {
 // are fp32 multiply-adds on converted bytes, two instructions a byte, which at 64 lanes a clock is 32 bytes a clock of a
 // CU, three times what memory brings.  8 lanes have a row, 16 columns each, of the keys as of the values, so a row's weight
 // is where its values are: every group of 8 lanes has a softmax of its own, and nothing crosses lanes in the loop but a
-// score's three sums.  Bound by the trips to memory where rows are few (one request of 640 rows: 11 us), and by how many
-// loads a CU has under way where they are many (24 of 1445 to 4000: 46 us, 3.8 TB/s).  A row's scale is 4 bytes of a line of
-// its own: with one head a wave the lines cost a fifth of the time, so two heads share them where workgroups are many.
+// score's three sums.  Bound by the trips to memory where rows are few (one request of 640 rows: 11 us, where the fp32
+// pool's kernel, which cuts at 128 rows, takes 7).  Where they are many (24 of 1445 to 4000: 45 us, 3.8 TB/s) nothing is near
+// its limit all the time: 240 workgroups of unlike lengths, one a CU, are there for 69 % of it, the L1s wait for misses for
+// 46 %, the vector units are busy for 24 %.  A row's scale is 4 bytes of a line of its own, a third of the requests to L2: with
+// one head a wave the lines cost a fifth of the time, so two heads share them where workgroups are many.
 constexpr int kOneWaves = 12;  // as many as have their registers on a CU
 constexpr int kOneParts = 16;  // columns of a lane
 
