@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWor
 __device__ __attribute__((noinline)) double full_exp(double x) { return exp(x); }
 
 // A workgroup has a request: its beams' sums, their candidates, and the states of the chosen ones.  Bound by its dependent steps
-// (sums, candidates, chosen, states): 6.7 us for one request of 4 beams, 11 for 64 of 8.
+// (sums, candidates, chosen, states): 7 us for one request of 4 beams, 11.5 for 64 of 8.
 __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWork w) {
   __shared__ Best<double, int64_t, kJoinThreads> best;
   __shared__ double sums[kBeamsMost], scores[kBeamsMost], by[kBeamsMost];
