@@ -366,8 +366,8 @@ int uocr_accept_drafts(void* kv_blocks, int64_t pages, int64_t layers, int64_t p
  *   [rows], may be NULL) not 0 has one candidate, eos with key = scores[b].
  *   rank = key, or, given lengths (int32 [rows]), key / length^alpha, the length being
  *   lengths[b] + 1, of an ended beam lengths[b].
- * Keys and ranks are in 64 bits, log sum exp within 2e-12; ties go to the lower row, of a row to
- * the larger logit, then to the lower token.
+ * Keys and ranks are in 64 bits, log sum exp within 2e-12 and 2^-53 of itself; ties go to the
+ * lower row, of a row to the larger logit, then to the lower token.
  * Candidates without a finite rank come last and get the score -inf.  Outputs, row by row: the
  * token, the parent row, the key as fp32, whether it has
  * ended (its parent had, or the token is eos), the length, and the history (int32 [rows,
