@@ -7,11 +7,10 @@
 //   rank = key / length^alpha, the length with the new token                 (given lengths; else rank = key)
 //
 // The K best of a request's K beams by rank, ties to the lower beam, of a beam to the larger logit, then to the lower token
-// (beside a score of some size 64 bits do not tell the keys of a beam's tokens apart, and their logits do).  Keys and ranks are in 64 bits, the
-// exponentials and their sum too (a sum's logarithm is off by 2e-12 at most): which of two near candidates wins decides what a
-// request says.  A candidate whose rank is not finite (a token at -inf, a beam
-// whose score or sum is not finite) comes after all others, as -inf; of a beam without a finite sum it is the first
-// tokens that do.
+// (beside a score of some size 64 bits do not tell the keys of a beam's tokens apart, and their logits do).  Keys and ranks
+// are in 64 bits, the exponentials and their sum too (a sum's logarithm is off by 2e-12 at most): which of two near candidates
+// wins decides what a request says.  A candidate whose rank is not finite (a token at -inf, a beam whose score or sum is not
+// finite) comes after all others, as -inf; of a beam without a finite sum it is the first tokens that do.
 #include "uocr_device.h"
 #include "uocr_kernels.h"
 
@@ -143,7 +142,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // The sum of e^x of four -700 <= x <= 0, each off by 1.1e-12 of itself: 2^(x log2 e), whose whole part is what stays of it
 // beside 1.5 2^52, in the sum's lower word, and the rest, a half at most, a polynomial (2^f by its values at nine Chebyshev
-// nodes; eleven would be 3e-16 off and take 3 us more of 57).  Four side by side: a step of one waits for the step before.
+// nodes; eleven would be 3e-16 off and take 3 us more).  Four side by side: a step of one waits for the step before.
 __device__ __forceinline__ double exp_sum4(const double (&x)[4]) {
   constexpr double kLog2E = 0x1.71547652b82fep+0, kWhole = 0x1.8p+52;
   constexpr double kPoly[] = {0x1.00dc4a532fb8ep-16, 0x1.4308ac85aa947p-13, 0x1.5d8745a728441p-10, 0x1.3b2ab7181b755p-7,
@@ -167,12 +166,12 @@ __device__ __forceinline__ double exp_sum4(const double (&x)[4]) {
 }
 
 // A workgroup has a piece of a row: its largest logit, its sum of exponentials, and its best K tokens.  Rows begin at any
-// float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.  Where rows are many (512
-// of 129280, a fifth of them ended: 56 us, 3.8 TB/s) the vector units are busy for two thirds of the time, most of it with the
-// exponentials, and overlap the loads in part; few rows (4: 5.5 us) wait for their trip to memory.  (Exponentials and sums in
-// 32 bits took 44, at memory's rate, and candidates of different beams nearer than 1e-6 could change places.)
+// float (a load of 16 bytes wants 4-byte boundaries only), and a row's results do not depend on where.  Where rows are many
+// (512 of 129280, a fifth of them ended: 51 us, 4.2 TB/s) bound by the vector units (busy 83 % of the time), most of whose
+// work is the exponentials; few rows (4: 5.1 us) wait for their trip to memory.  (Exponentials and sums in 32 bits took 44, at
+// memory's rate, and candidates of different beams nearer than 1e-6 could change places.)
 template <int kPer>
-__global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWork w) {
+__global__ void __launch_bounds__(kRowThreads, 7) k_beam_rows(BeamSelect p, BeamWork w) {
   __shared__ Best<float, int, kRowThreads> best;
   __shared__ float parts[kRowThreads / kWave];
   __shared__ double part_sums[kRowThreads / kWave];
@@ -182,22 +181,35 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWor
   const float* x = p.logits + (int64_t)row * p.vocab;
   float v[kPer];
   const auto token = [&](int i) { return begin + (i / 4 * kRowThreads + tid) * 4 + i % 4; };
+  // Loads go before what other waves compute, and what is read once does not take the caches (512 rows 59 us without either, 56
+  // with the latter, 55 with both; whole pieces then without their ends in mind 52, and seven waves a SIMD 51).
+  __builtin_amdgcn_s_setprio(3);
+  const auto put = [&](int i, f32x4 y) {
 #pragma unroll
-  for (int i = 0; i < kPer; i += 4) {
-    const int at = token(i);
-    f32x4 y = {-kInf, -kInf, -kInf, -kInf};
-    if (at + 3 < p.vocab) {
-      y = *(const UOCR_GLOBAL f32x4_at_float*)(x + at);
-    } else {
+    for (int e = 0; e < 4; ++e) v[i + e] = y[e];
+  };
+  if (begin + kRowThreads * kPer <= p.vocab) {
+    const float* from = x + begin;
 #pragma unroll
-      for (int e = 0; e < 3; ++e)
-        if (at + e < p.vocab) y[e] = ldg(x + at + e);
+    for (int i = 0; i < kPer; i += 4)
+      put(i, __builtin_nontemporal_load((const UOCR_GLOBAL f32x4_at_float*)(from + i * kRowThreads + (uint32_t)tid * 4)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      const int at = token(i);
+      f32x4 y = {-kInf, -kInf, -kInf, -kInf};
+      if (at + 3 < p.vocab) {
+        y = __builtin_nontemporal_load((const UOCR_GLOBAL f32x4_at_float*)(x + at));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (at + e < p.vocab) y[e] = ldg(x + at + e);
+      }
+      put(i, y);
     }
-    v[i] = y.x;
-    v[i + 1] = y.y;
-    v[i + 2] = y.z;
-    v[i + 3] = y.w;
   }
+  __builtin_amdgcn_s_setprio(0);
+  __builtin_amdgcn_sched_barrier(0);
   constexpr int kGroup = 8;  // tokens that are looked at together
   float largest[kPer / kGroup], mine = -kInf;
 #pragma unroll
@@ -254,7 +266,7 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_rows(BeamSelect p, BeamWor
 __device__ __attribute__((noinline)) double full_exp(double x) { return exp(x); }
 
 // A workgroup has a request: its beams' sums, their candidates, and the states of the chosen ones.  Bound by its dependent steps
-// (sums, candidates, chosen, states): 7 us for one request of 4 beams, 11.5 for 64 of 8.
+// (sums, candidates, chosen, states): 7 us for one request of 4 beams, 10.5 for 64 of 8.
 __global__ void __launch_bounds__(kJoinThreads) k_beam_join(BeamSelect p, BeamWork w) {
   __shared__ Best<double, int64_t, kJoinThreads> best;
   __shared__ double sums[kBeamsMost], scores[kBeamsMost], by[kBeamsMost];
